@@ -48,6 +48,15 @@ class FcChunk(Structure):
                 ("n_out", c_int32), ("logits", c_void_p), ("logits_stride", c_int64), ("flags", c_int32)]
 
 
+class FcPages(Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_stride", c_int64), ("v_stride", c_int64),
+                ("n_pages", c_int32), ("n_kv_head", c_int32), ("page", c_int32), ("head_dim", c_int32),
+                ("dtype", c_int32)]
+
+
+FC_PAGED_ZERO_TAIL = 1  # fc_paged_attention flags: tokens past the last row become 0
+
+
 class FcRowstat(Structure):
     _fields_ = [("mx", c_float), ("sum", c_float), ("tau", c_float), ("tie_idx", c_int32),
                 ("argmax", c_int32), ("pad", c_int32 * 3)]
@@ -70,7 +79,8 @@ EXPORTS = ["fc_last_error", "fc_version", "fc_forward_workspace_bytes", "fc_forw
            "fc_attn_prologue", "fc_attn_qkv_workspace_bytes", "fc_attn_qkv", "fc_row_stats", "fc_row_stats_fields",
            "fc_spec_workspace_bytes",
            "fc_spec_round", "fc_spec_accept", "fc_spec_part_bytes", "fc_fast_sample", "fc_engine_sample",
-           "fc_cross_entropy", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe", "fc_gemm_walk_probe",
+           "fc_cross_entropy", "fc_page_tables", "fc_page_append", "fc_paged_attention",
+           "fc_paged_attention_workspace_bytes", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe", "fc_gemm_walk_probe",
            "fc_gemm_walk_probe_words", "fc_graph_begin", "fc_graph_end", "fc_graph_launch", "fc_graph_destroy"]
 
 _lib = None
@@ -123,6 +133,15 @@ def _declare(L):
     L.fc_engine_sample.restype = i32
     L.fc_cross_entropy.argtypes = [vp, i64, vp, i32, i32, vp, vp]
     L.fc_cross_entropy.restype = i32
+    L.fc_page_tables.argtypes = [vp] * 11 + [i32] * 6 + [vp]
+    L.fc_page_tables.restype = i32
+    L.fc_page_append.argtypes = [POINTER(FcPages), vp, vp, i64, i64, i64, i64, i32, vp, i32, vp]
+    L.fc_page_append.restype = i32
+    L.fc_paged_attention_workspace_bytes.argtypes = [POINTER(FcPages)] + [i32] * 7
+    L.fc_paged_attention_workspace_bytes.restype = i64
+    L.fc_paged_attention.argtypes = [POINTER(FcPages), vp, i64, i64, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, i32,
+                                     i32, i32, vp, i64, vp]
+    L.fc_paged_attention.restype = i32
     L.fc_read_probe.argtypes = [vp, i64, vp, i32, vp]
     L.fc_read_probe.restype = i32
     L.fc_l2_read_probe.argtypes = [vp, i64, i64, vp, i32, vp]

@@ -36,6 +36,21 @@ DeviceModel) and everything they write as tensors, declared mutated:
   spec_round(target, draft, t_k, t_v, t_hist, d_k, d_v, d_hist, buffers, batch, k, max_tokens,
              gen_cap, vocab, temperature, top_k, seed, workspace)
                                      one whole speculative round (engine.py:484-606)
+
+The paged KV cache (one layer; k_pages [n_pages][n_kv_head][page][head_dim]
+and v_pages [n_pages][n_kv_head][page / 32][head_dim][32] in the caches' block
+order, whose pages may be strided, as those of one layer of a pool of all
+layers are; every index tensor int32):
+  page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots,
+              page, prefix_len=0)
+                                     block tables, packed chunk and slot map of a step from the rows'
+                                     lengths, on the GPU (fc_page_tables); all but length and n_new mutated
+  page_append(k, v, slots, k_pages, v_pages)
+                                     new K and V [tokens][n_kv_head][head_dim], strided views of a fused
+                                     projection included, into their slots (engine.py:119-126)
+  paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None,
+                  prefix_len=0)      attention over the pages, the shared prefix computed once for all rows
+                                     (engine.py:128-156) -> [tokens][n_head * head_dim]; inference only
 `buffers` is the speculative state's device arrays in fc_spec_state order
 (`SPEC_BUFFERS`: t_len .. p_stats, then the partials buffer `part`).
 """
@@ -48,7 +63,8 @@ from . import _lib
 from ._lib import check, lib
 
 __all__ = ["pack_operand", "linear", "attention", "cross_entropy", "frag_to_rows", "forward", "attn_prologue",
-           "attn_qkv", "row_stats", "spec_accept", "spec_round", "SPEC_BUFFERS"]
+           "attn_qkv", "row_stats", "spec_accept", "spec_round", "SPEC_BUFFERS", "page_tables", "page_append",
+           "paged_attention"]
 
 NS = "flaxchat_mi355x"
 
@@ -441,3 +457,182 @@ def spec_round(target: int, draft: int, t_k: torch.Tensor, t_v: torch.Tensor, t_
 def _(target, draft, t_k, t_v, t_hist, d_k, d_v, d_hist, buffers, batch, k, max_tokens, gen_cap, vocab, temperature,
       top_k, seed, workspace):
     return None
+
+
+# ---------------------------------------------------------------- paged KV cache
+# Registered below custom_op, which costs about 12 us a call: a decode step's kernels take less.
+from typing import Optional  # noqa: E402
+
+_PAGED = torch.library.Library(NS, "FRAGMENT")
+
+
+def _op(schema: str):
+    """Defines operator `schema` with the decorated function as its implementation on every device (which
+    itself refuses tensors off the GPU)."""
+    def deco(fn):
+        _PAGED.define(schema)
+        _PAGED.impl(schema[:schema.index("(")], fn, "CompositeExplicitAutograd")
+        return fn
+    return deco
+
+
+def _on_gpu(name: str, first: torch.Tensor, *rest: torch.Tensor) -> int:
+    """The index of the CUDA device that all tensors are on."""
+    d = first.get_device()
+    if d < 0:
+        raise ValueError(f"{name}: tensors live on a CUDA device (got {first.device})")
+    for t in rest:
+        if t.get_device() != d:
+            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+    return d
+
+
+def _launch(name: str, device: int, fn, *args):
+    """fn(*args, stream) on `device`'s current stream, with that device current."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        check(rc, name)
+
+
+def _inner_contiguous(t: torch.Tensor) -> bool:
+    """Whether t[0] is contiguous."""
+    want = 1
+    for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and st != want:
+            return False
+        want *= n
+    return True
+
+
+def _pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> _lib.FcPages:
+    if k_pages.dim() != 4:
+        raise ValueError(f"{name}: k_pages [n_pages][n_kv_head][page][head_dim] (got {tuple(k_pages.shape)})")
+    N, G, page, hd = k_pages.shape
+    if page == 0 or page % 32 != 0:
+        raise ValueError(f"{name}: page must be a multiple of 32 (got {page})")
+    if N < 1 or G < 1 or not 1 <= hd <= 256:
+        raise ValueError(f"{name}: n_pages, n_kv_head and head_dim (at most 256) must be positive")
+    if tuple(v_pages.shape) != (N, G, page // 32, hd, 32):
+        raise ValueError(f"{name}: v_pages {[N, G, page // 32, hd, 32]} (got {tuple(v_pages.shape)})")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"{name}: k_pages and v_pages share one dtype")
+    code, elems = _dtype_code(k_pages), G * page * hd
+    ks, vs = (elems, elems) if N == 1 else (k_pages.stride(0), v_pages.stride(0))
+    if ks < elems or vs < elems or not (_inner_contiguous(k_pages) and _inner_contiguous(v_pages)):
+        raise ValueError(f"{name}: each page must be contiguous, and pages must not overlap")
+    return _lib.FcPages(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, N, G, page, hd, code)
+
+
+def _index(name: str, what: str, t: torch.Tensor, n: int):
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: {what} is a contiguous int32 tensor of {n} entries "
+                         f"(got {t.dtype}, {tuple(t.shape)})")
+
+
+@_op("page_tables(Tensor(a!) tables, Tensor(b!) held, Tensor(c!) free_pages, Tensor(d!) n_free, Tensor length, "
+     "Tensor n_new, Tensor(e!) row_off, Tensor(f!) start, Tensor(g!) tok_row, Tensor(h!) tok_pos, Tensor(i!) slots, "
+     "int page, int prefix_len=0) -> ()")
+def page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots, page,
+                prefix_len=0):
+    if tables.dim() != 2:
+        raise ValueError(f"page_tables: tables [batch][width] (got {tuple(tables.shape)})")
+    B, W = tables.shape
+    T, F = slots.numel(), free_pages.numel()
+    if not 1 <= B <= 4096 or W < 1 or not 1 <= T < 1 << 30 or not 1 <= F < 1 << 30:
+        raise ValueError("page_tables: batch in [1, 4096], width, tokens and the free stack not empty")
+    if page < 32 or page % 32 != 0 or prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
+        raise ValueError("page_tables: page a multiple of 32, prefix_len >= 0, positions below 2^31")
+    for what, t, n in (("tables", tables, B * W), ("held", held, B), ("free_pages", free_pages, F),
+                       ("n_free", n_free, 1), ("length", length, B), ("n_new", n_new, B), ("row_off", row_off, B + 1),
+                       ("start", start, B), ("tok_row", tok_row, T), ("tok_pos", tok_pos, T), ("slots", slots, T)):
+        _index("page_tables", what, t, n)
+    d = _on_gpu("page_tables", tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots)
+    _launch("fc_page_tables", d, lib().fc_page_tables, tables.data_ptr(), held.data_ptr(), free_pages.data_ptr(),
+            n_free.data_ptr(), length.data_ptr(), n_new.data_ptr(), row_off.data_ptr(), start.data_ptr(),
+            tok_row.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), B, W, F, T, page, prefix_len)
+
+
+@_op("page_append(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_pages, Tensor(b!) v_pages) -> ()")
+def page_append(k, v, slots, k_pages, v_pages):
+    p = _pages("page_append", k_pages, v_pages)
+    if k.dim() != 3 or k.shape[1:] != (p.n_kv_head, p.head_dim) or v.shape != k.shape:
+        raise ValueError(f"page_append: k and v [tokens][{p.n_kv_head}][{p.head_dim}] "
+                         f"(got {tuple(k.shape)} and {tuple(v.shape)})")
+    if k.dtype != v.dtype or (k.dtype != k_pages.dtype and k.dtype != torch.float32):
+        raise ValueError(f"page_append: k and v in the pages' dtype or fp32 (got {k.dtype} and {v.dtype})")
+    M = k.shape[0]
+    _index("page_append", "slots", slots, M)
+    d = _on_gpu("page_append", k_pages, v_pages, k, v, slots)
+    if M == 0:
+        return
+    if p.head_dim != 1:
+        k = k if k.stride(2) == 1 else k.contiguous()
+        v = v if v.stride(2) == 1 else v.contiguous()
+    _launch("fc_page_append", d, lib().fc_page_append, p, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+            v.stride(0), v.stride(1), _dtype_code(k), slots.data_ptr(), M)
+
+
+@_op("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor tables, Tensor row_off, Tensor start, "
+     "int max_per_row, int window, Tensor? prefix_pages=None, int prefix_len=0) -> Tensor")
+def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None,
+                    prefix_len=0):
+    p = _pages("paged_attention", k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != p.head_dim or q.shape[1] == 0 or q.shape[1] % p.n_kv_head != 0:
+        raise ValueError(f"paged_attention: q [tokens][n_head][{p.head_dim}], n_head a multiple of {p.n_kv_head} "
+                         f"(got {tuple(q.shape)})")
+    if q.dtype != k_pages.dtype:
+        raise ValueError("paged_attention: q and the pages share one dtype")
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise ValueError("paged_attention has no backward pass")
+    if tables.dim() != 2:
+        raise ValueError(f"paged_attention: tables [batch][width] (got {tuple(tables.shape)})")
+    B, W = tables.shape
+    T, H, hd = q.shape
+    if not 1 <= B <= 4096 or W < 1 or H > 65535 or max_per_row < 1 or window < 0:
+        raise ValueError("paged_attention: batch in [1, 4096], width, max_per_row >= 1, window >= 0")
+    if prefix_len < 0 or W * p.page + prefix_len > 0x7fffffff:
+        raise ValueError("paged_attention: prefix_len >= 0, positions below 2^31")
+    if max_per_row > 0x7fffffff or window > 0x7fffffff:
+        raise ValueError("paged_attention: max_per_row and window below 2^31")
+    _index("paged_attention", "tables", tables, B * W)
+    _index("paged_attention", "row_off", row_off, B + 1)
+    _index("paged_attention", "start", start, B)
+    pre = 0
+    if prefix_len > 0:
+        if prefix_pages is None or prefix_pages.numel() * p.page < prefix_len:
+            raise ValueError(f"paged_attention: prefix_pages holds the pages of {prefix_len} positions")
+        _index("paged_attention", "prefix_pages", prefix_pages, prefix_pages.numel())
+        pre = prefix_pages.data_ptr()
+        d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start, prefix_pages)
+    else:
+        d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start)
+    y = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+    if T == 0:
+        return y
+    if hd != 1 and q.stride(2) != 1:
+        q = q.contiguous()
+    nb = lib().fc_paged_attention_workspace_bytes(p, B, T, max_per_row, H, W, prefix_len, window)
+    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=q.device)
+    _launch("fc_paged_attention", d, lib().fc_paged_attention, p, q.data_ptr(), q.stride(0), q.stride(1),
+            y.data_ptr(), B, T, max_per_row, H, tables.data_ptr(), W, row_off.data_ptr(), start.data_ptr(), pre,
+            prefix_len, window, _lib.FC_PAGED_ZERO_TAIL, ws.data_ptr(), ws.numel())
+    return y
+
+
+@torch.library.register_fake(f"{NS}::page_tables", lib=_PAGED)
+def _(tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots, page, prefix_len=0):
+    return None
+
+
+@torch.library.register_fake(f"{NS}::page_append", lib=_PAGED)
+def _(k, v, slots, k_pages, v_pages):
+    return None
+
+
+@torch.library.register_fake(f"{NS}::paged_attention", lib=_PAGED)
+def _(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None, prefix_len=0):
+    return q.new_empty((q.shape[0], q.shape[1] * q.shape[2]))

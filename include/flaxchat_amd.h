@@ -326,6 +326,76 @@ int32_t fc_engine_sample(const float* logits, int32_t batch, int32_t V, float te
 int32_t fc_cross_entropy(const float* logits, int64_t row_stride, const int32_t* targets, int32_t rows,
                          int32_t V, float* loss, void* stream);
 
+/* One layer of a paged KV cache: n_pages pages of `page` positions (a
+ * multiple of 32) of every KV head. Page i starts at element i * k_stride of
+ * k and holds [kv_head][page][head_dim] in the K cache's block order; at
+ * element i * v_stride of v, [kv_head][page / 32][head_dim][32]. A layer of
+ * an fc_cache is such a pool: its rows are pages of `cap` positions. No
+ * counterpart in the reference, whose caches are contiguous rows
+ * (flaxchat/engine.py:26-48); head_dim <= 256. */
+typedef struct fc_pages {
+  void* k;
+  void* v;
+  int64_t k_stride, v_stride;  /* elements from one page to the next            */
+  int32_t n_pages, n_kv_head, page, head_dim, dtype;
+} fc_pages;
+
+/* The pages of one step, from the rows' lengths, on the device (all arrays
+ * int32 device memory). State, updated in place: tables[batch][width] (page
+ * ids), held[batch] (pages of each row), free_pages[free_cap] and n_free[1]
+ * (a stack; entries at n_free and above are scratch). Per row: length[b]
+ * positions held (counted behind the shared prefix of prefix_len positions),
+ * n_new[b] to be added; n_new < 0 ends the row: its pages go onto the stack,
+ * in row order, and held[b] becomes 0. A row with n_new > 0 asks if
+ * ceil(length / page) <= held <= width and length + n_new <= width * page; it
+ * needs the pages past held that its new positions reach. It is taken in if
+ * it needs none, or if its pages and those of all rows before it that ask fit
+ * the stack, and if its tokens and those of the rows before it that fit do
+ * not pass max_tokens. Pages come off the top of the stack. A row not taken
+ * in feeds nothing and keeps what it has. Writes the packed chunk: row_off
+ * [batch+1], start[batch] (prefix_len + length), and for each of max_tokens
+ * tokens its row, position and slot (page id * page + place in the page), -1
+ * past the end (slot also where the table's entry is no page id). length is
+ * left to the caller (a rollback lowers it; pages stay): the same call again
+ * changes nothing. batch <= 4096. */
+int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_pages, int32_t* n_free, const int32_t* length,
+                       const int32_t* n_new, int32_t* row_off, int32_t* start, int32_t* tok_row, int32_t* tok_pos,
+                       int32_t* slots, int32_t batch, int32_t width, int32_t free_cap, int32_t max_tokens,
+                       int32_t page, int32_t prefix_len, void* stream);
+
+/* K and V of M tokens into their slots (the cache append of
+ * flaxchat/engine.py:119-126 for pages): k and v [M][n_kv_head][head_dim]
+ * with the given token and head strides (elements; dims contiguous), in the
+ * pages' dtype or fp32, which is rounded to it. Slots outside the pool (-1)
+ * keep nothing; a slot may occur once. */
+int32_t fc_page_append(const fc_pages* pages, const void* k, const void* v, int64_t k_token_stride,
+                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t src_dtype,
+                       const int32_t* slots, int32_t M, void* stream);
+
+/* Attention over a paged cache whose rows share a prefix (the mathematics of
+ * flaxchat/engine.py:128-156: GQA, causal, inclusive window). Row b's queries
+ * are tokens row_off[b] .. row_off[b+1]-1 (packed, as in fc_chunk) at
+ * positions start[b] ..; position p < prefix_len is in the shared pages
+ * prefix_pages[p / page], from there on in tables[b][(p - prefix_len) / page]
+ * (place (p - prefix_len) % page). The prefix is read once for all rows. An
+ * entry outside [0, n_pages), and a position past the table, holds no key; a
+ * query that sees no key gets 0. What lies in slots that a query does not see
+ * does not reach its result, finite or not.
+ * q: [max_tokens][n_head][head_dim] with the given strides, y [max_tokens]
+ * [n_head * head_dim] row-major, both in the pages' dtype. Tokens past
+ * row_off[batch] are left as they are, or set to 0 with FC_PAGED_ZERO_TAIL; a
+ * row whose tokens run past max_tokens or number more than max_per_row is
+ * treated as empty. batch <= 4096. */
+#define FC_PAGED_ZERO_TAIL 1
+int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
+                                           int32_t max_per_row, int32_t n_head, int32_t width, int32_t prefix_len,
+                                           int32_t window);
+int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           void* y, int32_t batch, int32_t max_tokens, int32_t max_per_row, int32_t n_head,
+                           const int32_t* tables, int32_t width, const int32_t* row_off, const int32_t* start,
+                           const int32_t* prefix_pages, int32_t prefix_len, int32_t window, int32_t flags,
+                           void* work, int64_t work_bytes, void* stream);
+
 /* Streaming read of `bytes` (a multiple of 16) from device memory by
  * `workgroups` workgroups of 256 threads, each streaming one contiguous
  * share with 16-byte non-temporal loads; out receives 4 * workgroups

@@ -13,6 +13,11 @@
 #include "fc_common.h"
 #include "fc_internal.h"
 
+// K and V of a row's own pages are read once a call: non-temporal loads keep
+// them from displacing lines that are read again.
+typedef uint32_t kv_u32x4 __attribute__((ext_vector_type(4)));
+#define KV_LD(p) __builtin_bit_cast(uint4, __builtin_nontemporal_load((const kv_u32x4*)(p)))
+
 // Smallest b in [0, n) with off[b + 1] > t; n if there is none. Ends for any
 // contents of off.
 __device__ __forceinline__ int row_of(const int* off, int n, int t) {
@@ -326,6 +331,12 @@ struct PagedChunk {
   int B, H, W, P, window, max_per_row, Mcap, flags;
   int64_t qst, qsh;  // query strides (elements): token, head
   float scale;
+  // key splits: their number over a row's own keys and over the prefix, keys per prefix split, workgroups that
+  // the own keys are to be spread over
+  int S_own, S_pre, pre_chunk, target;
+  // partials of split s (the own ones first): po[(s Mcap + token) H + head][hd] unnormalised, pml (max, sum)
+  float* po;
+  float2* pml;
 };
 
 // Any head size, type and alignment: one workgroup per (token, head), keys in
@@ -389,10 +400,810 @@ __global__ __launch_bounds__(256) void k_paged_any(PagedChunk c, const T* __rest
   if (tid < hd) st<T>(yo, tid, l == 0.f ? 0.f : o / l);  // 0: no key
 }
 
+// Table entries are read through the constant address space: scalar loads,
+// whose result can be a scalar base of the direct LDS loads below.
+typedef const __attribute__((address_space(4))) int* const_ints;
+#define CONST_INTS(p) ((const_ints)(uint64_t)(p))
+
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                  0, 0);
+}
+__device__ __forceinline__ float exp2a(float x) { return __builtin_amdgcn_exp2f(x); }
+// Two keys' worth of a V operand word: all ones where the key is in [lo, hi].
+__device__ __forceinline__ uint32_t key_mask(int key, int lo, int hi) {
+  return (key >= lo && key <= hi ? 0xffffu : 0u) | (key + 1 >= lo && key + 1 <= hi ? 0xffff0000u : 0u);
+}
+// whether a pair of bf16 holds an infinity or NaN
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+template <int N>
+__device__ __forceinline__ int lanes_min(int v) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, WAVE));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+template <int N>
+__device__ __forceinline__ int lanes_max(int v) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, WAVE));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Keys of a job are counted from 0: the prefix's positions, or a row's own
+// ones (position - P, which is their place in the row's table).
+// The keys [lo, hi] that a query at position `pos` sees; hi < lo: none.
+__device__ __forceinline__ void key_range(const PagedChunk& c, int64_t pos, bool pre, int& lo, int& hi) {
+  const int64_t off = pre ? 0 : c.P, last = pre ? (int64_t)c.P - 1 : (int64_t)c.W * c.pv.page - 1;
+  hi = (int)max((int64_t)-1, min(pos - off, last));
+  lo = c.window > 0 ? (int)max((int64_t)0, min(pos - c.window - off, (int64_t)0x7fffffff)) : 0;
+}
+
+// Keys per split of the rows' own keys: what spreads all rows' keys over about
+// c.target workgroups (rows are of unequal length: a fixed number of splits
+// per row would leave the longest row's for last), at least 128 (a tile for
+// each of four waves), and no more splits of the longest row than c.S_own.
+// Every wave reads all rows' lengths; the result is the same in all of them.
+__device__ __forceinline__ int own_chunk(const PagedChunk& c, int units_per_row) {
+  float total = 0.f;
+  int longest = 1;
+  for (int r = threadIdx.x & 63; r < c.B; r += 64) {
+    const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
+    if (sp.n == 0) continue;
+    int lo, hi, lo1, hi1;
+    key_range(c, c.start[r], false, lo, hi);
+    key_range(c, (int64_t)c.start[r] + sp.n - 1, false, lo1, hi1);
+    const int len = hi1 < lo ? 0 : hi1 + 1 - (lo & ~31);
+    total += (float)len;
+    longest = max(longest, len);
+  }
+  total = wave_sum(total);
+  longest = lanes_max<64>(longest);
+  const float share = ceilf(total * (float)units_per_row / (float)c.target);
+  int chunk = max((int)fminf(share, 1e9f), max(128, (longest + c.S_own - 1) / c.S_own));
+  return __builtin_amdgcn_readfirstlane((chunk + 63) & ~63);
+}
+
+// Tokens past the last row: set to 0 by the launch's workgroups in turn.
+__device__ __forceinline__ void zero_tail(const PagedChunk& c, bf16_t* y, int wg, int nwg) {
+  const int n8 = c.H * c.pv.hd / 8;
+  for (int64_t t = max(0, c.row_off[c.B]) + (int64_t)wg; t < c.Mcap; t += nwg)
+    for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)(y + t * n8 * 8))[i] = uint4{0u, 0u, 0u, 0u};
+}
+
+// One 32-key tile of one wave for 16 query columns: S^T = K Q^T, the running
+// softmax, O^T += V^T P^T, as in fc_attn.hip's attn_tile. MASK: some column
+// does not see all 32 keys. vf then holds 0 for keys that none sees; `odd`:
+// it holds an infinity or NaN that some column does not see. Its product with
+// that column's weight 0 would be NaN, so the columns take turns, each with
+// the keys it sees.
+template <int HD, bool MASK>
+__device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint4 (&vf)[HD / 16],
+                                       const uint4 (&qf)[HD / 32], int kb, int g4, int lo, int hi, bool odd,
+                                       float scale_log2, float& m_run, float& l_run, f32x4 (&O)[HD / 16]) {
+  f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc) sc[cc] = mfma16(kf[cc][s], qf[s], sc[cc]);
+  float p[8], mt = -INFINITY;
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj) {
+    p[jj] = sc[jj >> 2][jj & 3] * scale_log2;
+    if constexpr (MASK) {
+      const int key = kb + 8 * g4 + jj;
+      p[jj] = key >= lo && key <= hi ? p[jj] : -INFINITY;
+    }
+    mt = fmaxf(mt, p[jj]);
+  }
+  mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
+  mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+  const float m_new = fmaxf(m_run, mt);
+  if (__any(m_new > m_run)) {
+    const float alpha = exp2a(m_run - (m_new == -INFINITY ? 0.f : m_new));
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) O[db] *= alpha;
+    m_run = m_new;
+  }
+  const float mu = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj) {
+    p[jj] = exp2a(p[jj] - mu);
+    l_run += p[jj];
+  }
+  // the weights go into the product rounded to bf16 (half a step, 2^-8, of each); the sum keeps fp32
+  const uint4 pf = {pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])};
+  if (MASK && odd) {
+    for (int col = 0; col < 16; ++col) {
+      const int lc = __builtin_amdgcn_readlane(lo, col), hc = __builtin_amdgcn_readlane(hi, col);
+      const int k0 = kb + 8 * g4;
+      const uint32_t m0 = key_mask(k0, lc, hc), m1 = key_mask(k0 + 2, lc, hc), m2 = key_mask(k0 + 4, lc, hc),
+                     m3 = key_mask(k0 + 6, lc, hc);
+      const bool mine = (threadIdx.x & 15) == col;
+#pragma unroll
+      for (int db = 0; db < HD / 16; ++db) {
+        const uint4 v = {vf[db].x & m0, vf[db].y & m1, vf[db].z & m2, vf[db].w & m3};
+        const f32x4 t = mfma16(v, pf, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int x = 0; x < 4; ++x) O[db][x] = mine ? O[db][x] + t[x] : O[db][x];
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int db = 0; db < HD / 16; ++db) O[db] = mfma16(vf[db], pf, O[db]);
+}
+
+// Few query columns (token, head in group): at most 16 QB of a row and KV
+// group, or, for the prefix (`pre`), of all rows together. A workgroup takes
+// one key split; its four waves every fourth 32-key tile, straight from memory
+// into registers, each tile applied to all QB blocks of 16 columns, and are
+// merged in LDS. grid (row x group, or group; 1; split).
+template <int HD, int QB>
+__global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf16_t* __restrict__ q,
+                                                         const bf16_t* __restrict__ kp,
+                                                         const bf16_t* __restrict__ vp, bf16_t* __restrict__ y,
+                                                         int pre) {
+  constexpr int NW = 4, NT = 2 * HD;  // threads that own 8 dims of a column after the merge
+  __shared__ float sm[NW][16], sl[NW][16];
+  __shared__ float so[NW][16][HD + 4];
+  static_assert(sizeof(so) >= (PT_ROWS + 1) * 4, "the rows' offsets");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int cl = lane & 15, g4 = lane >> 4, rep = c.H / c.pv.G, split = blockIdx.z;
+  const int S = c.S_own + c.S_pre;
+  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
+  int b = 0, g, base = 0, ncol;
+  if (pre) {
+    g = blockIdx.x;
+    ncol = c.Mcap * rep;
+    int* off = (int*)so;
+    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+    __syncthreads();
+  } else {
+    b = blockIdx.x / c.pv.G;
+    g = blockIdx.x - b * c.pv.G;
+    const RowSpan sp = row_span(c.row_off, b, c.max_per_row, c.Mcap);
+    if (sp.n == 0) return;
+    base = sp.base;
+    ncol = sp.n * rep;
+  }
+  // this lane's columns
+  uint4 qf[QB][HD / 32];
+  int lo[QB], hi[QB];
+  int w_lo = 0x7fffffff, w_hi = -1, f_lo = 0, f_hi = 0x7fffffff;
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+    const int col = 16 * u + cl;
+    bool ok = col < ncol;
+    const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
+    int64_t pos = 0;
+    if (pre) {
+      const int* off = (const int*)so;
+      const int r = row_of(off, c.B, j);
+      RowSpan sp{0, 0};
+      if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
+      ok = ok && j >= sp.base && j < sp.base + sp.n;
+      pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+    } else {
+      pos = (int64_t)c.start[b] + j;
+    }
+    key_range(c, pos, pre, lo[u], hi[u]);
+    if (!ok) lo[u] = 0x7fffffff, hi[u] = -1;
+    const bool some = lo[u] <= hi[u];  // columns that see nothing do not widen the range
+    w_lo = min(w_lo, some ? lo[u] : 0x7fffffff);
+    w_hi = max(w_hi, some ? hi[u] : -1);
+    f_lo = max(f_lo, ok ? lo[u] : 0);
+    f_hi = min(f_hi, ok ? hi[u] : 0x7fffffff);
+    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh + 8 * g4;
+    const uint32_t keep = ok ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s) {
+      const uint4 v = *(const uint4*)(qr + 32 * s);
+      qf[u][s] = uint4{v.x & keep, v.y & keep, v.z & keep, v.w & keep};
+    }
+  }
+  w_lo = lanes_min<16>(w_lo);
+  w_hi = lanes_max<16>(w_hi);
+  f_lo = lanes_max<16>(f_lo);
+  f_hi = lanes_min<16>(f_hi);
+  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G) : 0x7fffffe0;
+  const int64_t kbeg = (int64_t)(w_lo & ~31) + (int64_t)split * chunk;
+  const int64_t kend = min((int64_t)w_hi + 1, kbeg + chunk);
+  const int sg = pre ? c.S_own + split : split;
+  if (kbeg >= kend && S > 1) {
+    if (threadIdx.x < 16 * QB && threadIdx.x < ncol) {
+      const int j = threadIdx.x / rep, head = g * rep + threadIdx.x - j * rep;
+      c.pml[((int64_t)sg * c.Mcap + base + j) * c.H + head] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+
+  float m_run[QB], l_run[QB];
+  f32x4 O[QB][HD / 16];
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+    m_run[u] = -INFINITY;
+    l_run[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) O[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  const int tpp = c.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
+  int tile = (int)(min(kbeg, (int64_t)w_hi + 1) >> 5) + wave;
+  int pg = tile / tpp, r = tile - pg * tpp;
+  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
+  int id = tile < tend ? list[pg] : -1;
+  const int64_t gofs = (int64_t)g * c.pv.page * HD;
+  const int krow = 8 * (cl >> 2) + (cl & 3);  // the key of operand row cl (+ 4 cc)
+  while (tile < tend) {
+    const int kb = 32 * tile, id0 = id, r0 = r;
+    // the next tile's page, ahead of this one's work
+    tile += NW;
+    r += NW;
+    while (r >= tpp) r -= tpp, ++pg;
+    id = tile < tend ? list[pg] : -1;
+    if ((unsigned)id0 >= (unsigned)c.pv.N) continue;
+    uint4 kf[2][HD / 32], vf[HD / 16];
+    const bf16_t* kt = kp + (int64_t)id0 * c.pv.ks + gofs + r0 * (32 * HD);
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int s = 0; s < HD / 32; ++s)
+        kf[cc][s] = KV_LD((const uint4*)(HD == 128 ? kt + lane * 8 + (s * 2 + cc) * 512
+                                                   : kt + (krow + 4 * cc) * HD + 32 * s + 8 * g4));
+    const bf16_t* vt = vp + (int64_t)id0 * c.pv.vs + gofs + r0 * (32 * HD) + cl * 32 + 8 * g4;
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) vf[db] = KV_LD((const uint4*)(vt + db * 512));
+    if (kb >= f_lo && kb + 31 <= f_hi) {
+#pragma unroll
+      for (int u = 0; u < QB; ++u)
+        tile16<HD, false>(kf, vf, qf[u], kb, g4, 0, 0, false, scale_log2, m_run[u], l_run[u], O[u]);
+    } else {
+      const int k0 = kb + 8 * g4;
+      const uint32_t m0 = key_mask(k0, w_lo, w_hi), m1 = key_mask(k0 + 2, w_lo, w_hi),
+                     m2 = key_mask(k0 + 4, w_lo, w_hi), m3 = key_mask(k0 + 6, w_lo, w_hi);
+      bool odd = false;
+#pragma unroll
+      for (int db = 0; db < HD / 16; ++db) {
+        vf[db] = uint4{vf[db].x & m0, vf[db].y & m1, vf[db].z & m2, vf[db].w & m3};
+        odd |= odd_pair(vf[db].x) || odd_pair(vf[db].y) || odd_pair(vf[db].z) || odd_pair(vf[db].w);
+      }
+      odd = __any(odd);
+#pragma unroll
+      for (int u = 0; u < QB; ++u)
+        tile16<HD, true>(kf, vf, qf[u], kb, g4, lo[u], hi[u], odd, scale_log2, m_run[u], l_run[u], O[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+    if (16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
+      l_run[u] += __shfl_xor(l_run[u], 16, WAVE);
+      l_run[u] += __shfl_xor(l_run[u], 32, WAVE);
+      if (u > 0 || pre) __syncthreads();  // the readers of the LDS are done with it
+      if (g4 == 0) {
+        sm[wave][cl] = m_run[u];
+        sl[wave][cl] = l_run[u];
+      }
+#pragma unroll
+      for (int db = 0; db < HD / 16; ++db) *(f32x4*)&so[wave][cl][16 * db + 4 * g4] = O[u][db];
+      __syncthreads();
+      const int qc = threadIdx.x / (HD / 8), d0 = (threadIdx.x % (HD / 8)) * 8, col = 16 * u + qc;
+      if (threadIdx.x < NT && col < ncol) {
+        float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][qc]);
+        const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float a = exp2a(sm[w][qc] - mu);
+          L += a * sl[w][qc];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] += a * so[w][qc][d0 + i];
+        }
+        const int j = col / rep, head = g * rep + col - j * rep;
+        if (S == 1) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          *(uint4*)(y + ((int64_t)(base + j) * c.H + head) * HD + d0) =
+              uint4{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv),
+                    pack2bf(o[4] * inv, o[5] * inv), pack2bf(o[6] * inv, o[7] * inv)};
+        } else {
+          const int64_t at = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
+          float4* po = (float4*)(c.po + at * HD + d0);
+          po[0] = make_float4(o[0], o[1], o[2], o[3]);
+          po[1] = make_float4(o[4], o[5], o[6], o[7]);
+          if (d0 == 0) c.pml[at] = make_float2(M, L);
+        }
+      }
+    }
+  }
+}
+
+// Merge of the key splits of one (token, head), HD / 8 threads with 8
+// dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
+// first CB splits' loads are under way before the token's row is looked up.
+template <int HD, int CB>
+__global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, bf16_t* __restrict__ y) {
+  __shared__ int off[PT_ROWS + 1];
+  constexpr int TP = HD / 8;
+  const int64_t pair = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP, pairs = (int64_t)c.Mcap * c.H;
+  const int d0 = (threadIdx.x % TP) * 8, S = c.S_own + c.S_pre;
+  const int64_t at = min(pair, pairs - 1);
+  float2 e[CB];
+  float4 u[CB][2];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < CB; ++k) {
+      const int64_t i = (int64_t)min(s0 + k, S - 1) * pairs + at;
+      e[k] = c.pml[i];
+      u[k][0] = *(const float4*)(c.po + i * HD + d0);
+      u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
+    }
+  };
+  load(0);
+  for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+  float M = -INFINITY;
+  for (int s = threadIdx.x % TP; s < S; s += TP) M = fmaxf(M, c.pml[(int64_t)s * pairs + at].x);
+#pragma unroll
+  for (int o = TP / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, WAVE));
+  __syncthreads();
+  if (pair >= pairs) return;
+  const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
+  RowSpan sp{0, 0};
+  if (b < c.B) sp = row_span(off, b, c.max_per_row, c.Mcap);
+  bf16_t* yo = y + pair * HD + d0;
+  if (t < sp.base || t >= sp.base + sp.n) {
+    if ((c.flags & FC_PAGED_ZERO_TAIL) && t >= off[c.B]) *(uint4*)yo = uint4{0u, 0u, 0u, 0u};
+    return;
+  }
+  const float mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < S; s0 += CB) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int k = 0; k < CB; ++k) {
+      // a split without keys holds (-inf, 0) and no output
+      if (s0 + k >= S || (e[k].x == -INFINITY && e[k].y == 0.f)) continue;
+      const float a = exp2a(e[k].x - mu);
+      L += a * e[k].y;
+      o[0] += a * u[k][0].x; o[1] += a * u[k][0].y; o[2] += a * u[k][0].z; o[3] += a * u[k][0].w;
+      o[4] += a * u[k][1].x; o[5] += a * u[k][1].y; o[6] += a * u[k][1].z; o[7] += a * u[k][1].w;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *(uint4*)yo = uint4{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv),
+                      pack2bf(o[4] * inv, o[5] * inv), pack2bf(o[6] * inv, o[7] * inv)};
+}
+
+// Many query columns: 128 per workgroup, 32 per wave, on the 32x32x16 MFMA, of
+// one row and KV group, or, for the prefix (`pre`), of all rows' tokens side by
+// side, so that its keys are read once per 128 columns whatever rows they
+// belong to. The walk, the operand order in LDS and the softmax are those of
+// fc_attn.hip's prefill kernel: 64 keys a step through two LDS stages filled
+// by direct loads, scores and outputs in registers.
+//
+// Workgroups: unit = (row x group, or group) x key split; all column blocks of
+// a unit on one XCD, whose L2 then holds its keys.
+template <int HD>
+struct WideStage {
+  uint4 k[2][HD / 16][64];  // [32-key tile][16-dim slice][lane]
+  uint4 v[2][HD / 16][64];  // [32-key tile][2 (dim / 32) + key half][lane]
+};
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_t* __restrict__ q,
+                                                       const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
+                                                       bf16_t* __restrict__ y, int pre, int nunit, int nblk) {
+  constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
+  __shared__ WideStage<HD> stg[2];
+  __shared__ int rng[4][4];
+  static_assert(sizeof(stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
+  const int S = c.S_own + c.S_pre;
+  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
+  const int nul = (nunit + 7) >> 3, jj = blockIdx.x >> 3;
+  const int unit = (jj % nul) * 8 + (blockIdx.x & 7);
+  if (unit >= nunit) return;
+  const int c0 = (nblk - 1 - jj / nul) * 128, Sj = pre ? c.S_pre : c.S_own;  // a row's last columns see the most keys
+  const int ug = unit / Sj, split = unit - ug * Sj;
+  const int rep = c.H / c.pv.G;
+  int b = 0, g = ug, base = 0, ncol;
+  if (pre) {
+    const int used = min(max(c.row_off[c.B], 0), c.Mcap);
+    ncol = used * rep;
+    if (c0 >= ncol) return;
+    int* off = (int*)stg;
+    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+    __syncthreads();
+  } else {
+    b = ug / c.pv.G;
+    g = ug - b * c.pv.G;
+    const RowSpan sp = row_span(c.row_off, b, c.max_per_row, c.Mcap);
+    base = sp.base;
+    ncol = sp.n * rep;
+    if (c0 >= ncol) return;
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hl = lane >> 5, kk = lane & 31;
+  // this lane's column
+  const int col = c0 + 32 * wave + kk;
+  bool ok = col < ncol;
+  const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
+  int64_t pos = 0;
+  if (pre) {
+    const int* off = (const int*)stg;
+    const int r = row_of(off, c.B, j);
+    RowSpan sp{0, 0};
+    if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
+    ok = ok && j >= sp.base && j < sp.base + sp.n;
+    pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+  } else {
+    pos = (int64_t)c.start[b] + j;
+  }
+  v4u qf[DS];  // dims 16 h + 8 hl .. +7 of this lane's query
+  {
+    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh + 8 * hl;
+    const uint32_t keep = ok ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int h = 0; h < DS; ++h) qf[h] = *(const v4u*)(qr + 16 * h) & keep;
+  }
+  int lo_c, hi_c;
+  key_range(c, pos, pre, lo_c, hi_c);
+  if (!ok) lo_c = 0x7fffffff, hi_c = -1;
+  // the keys that some / every column of the wave sees, and of the workgroup
+  const bool some = lo_c <= hi_c;
+  const int w_lo = lanes_min<32>(some ? lo_c : 0x7fffffff), w_hi = lanes_max<32>(some ? hi_c : -1);
+  const int f_lo = lanes_max<32>(ok ? lo_c : 0), f_hi = lanes_min<32>(ok ? hi_c : 0x7fffffff);
+  if (lane == 0) {
+    rng[wave][0] = w_lo;
+    rng[wave][1] = w_hi;
+  }
+  __syncthreads();
+  int g_lo = 0x7fffffff, g_hi = -1;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    g_lo = min(g_lo, rng[w][0]);
+    g_hi = max(g_hi, rng[w][1]);
+  }
+  g_lo = __builtin_amdgcn_readfirstlane(g_lo);
+  g_hi = __builtin_amdgcn_readfirstlane(g_hi);
+  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G * nblk) : 0x7fffffc0;
+  // (a row's splits are counted from its first column's first key in every one of its blocks)
+  int row_lo = g_lo, unused;
+  if (!pre && c.window > 0 && Sj > 1) key_range(c, c.start[b], false, row_lo, unused);
+  const int64_t s_beg = (int64_t)(row_lo & ~31) + (int64_t)split * chunk;
+  const int64_t kend64 = min((int64_t)g_hi + 1, s_beg + chunk), kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
+  const int sg = pre ? c.S_own + split : split;
+  const bool none = kbeg64 >= kend64;
+  if (none && S > 1) {
+    if (threadIdx.x < 128 && c0 + threadIdx.x < ncol) {
+      const int cx = c0 + threadIdx.x, jx = cx / rep;
+      c.pml[((int64_t)sg * c.Mcap + base + jx) * c.H + g * rep + cx - jx * rep] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  const int t0 = none ? 0 : (int)kbeg64, kend = none ? 0 : (int)kend64;
+  const int ntiles = (kend - t0 + 31) >> 5, nstep = (ntiles + 1) >> 1;
+  const int hi_k = min(hi_c, kend - 1), w_hik = min(w_hi, kend - 1);  // behind kend a step repeats its last tile
+  // byte offsets of this lane's 16 bytes of the operands: K row kk is key
+  // 16 (kk / 16) + 8 ((kk / 4) % 2) + 4 ((kk / 8) % 2) + kk % 4 of the tile, V row kk is dim kk of 32
+  const int key = ((kk >> 4) << 4) | (((kk >> 2) & 1) << 3) | (((kk >> 3) & 1) << 2) | (kk & 3);
+  const uint32_t koff = HD == 128 ? 16u * (uint32_t)((((key >> 2) & 1) << 6) + ((key >> 3) << 2) + (key & 3) + 16 * hl)
+                                  : (uint32_t)(key * (2 * HD) + 16 * hl);
+  const uint32_t voff = 16u * (uint32_t)(4 * kk + hl);
+  const int64_t gofs = (int64_t)g * c.pv.page * HD;
+  f32x16 O[DD];
+#pragma unroll
+  for (int dd = 0; dd < DD; ++dd)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) O[dd][x] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  // the walk over the pages, one tile at a time; the next page's entry is under way a page ahead
+  const int tpp = c.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1;
+  int tile = t0 >> 5, pg = tile / tpp, tr = tile - pg * tpp;
+  const int pg_last = tlast / tpp;
+  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
+  int id = ntiles > 0 ? list[pg] : -1, id_next = ntiles > 0 ? list[min(pg + 1, pg_last)] : -1;
+  bool there[2][2];  // [stage][tile]: its page is one of the pool's
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  // each wave's loads of a tile: a quarter of K's slices and of V's dims
+#define WIDE_ISSUE(S_, st_)                                                                                  \
+  _Pragma("unroll") for (int u = 0; u < 2; ++u) {                                                            \
+    there[st_][u] = (unsigned)id < (unsigned)c.pv.N;                                                         \
+    const int64_t pid = there[st_][u] ? id : 0; /* no page: page 0's place is read and masked */             \
+    const bf16_t* kt = kp + pid * c.pv.ks + gofs + tr * (32 * HD);                                           \
+    const bf16_t* vt = vp + pid * c.pv.vs + gofs + tr * (32 * HD);                                           \
+    if constexpr (HD == 128) {                                                                               \
+      const uint32_t lk = LDS_ADDR(S_.k[u][0]) + 2048 * wave, lv = LDS_ADDR(S_.v[u][0]) + 2048 * wave;       \
+      lds_load_1k(kt + 1024 * wave, koff, lk);                                                               \
+      lds_load_1k(kt + 1024 * wave + 256, koff, lk + 1024);                                                  \
+      lds_load_1k(vt + 1024 * wave, voff, lv);                                                               \
+      lds_load_1k(vt + 1024 * wave + 16, voff, lv + 1024);                                                   \
+    } else {                                                                                                 \
+      lds_load_1k(kt + 16 * wave, koff, LDS_ADDR(S_.k[u][0]) + 1024 * wave);                                 \
+      lds_load_1k(vt + 1024 * (wave >> 1) + 16 * (wave & 1), voff, LDS_ADDR(S_.v[u][0]) + 1024 * wave);      \
+    }                                                                                                        \
+    if (tile < tlast) {                                                                                      \
+      ++tile;                                                                                                \
+      if (++tr == tpp) {                                                                                     \
+        tr = 0;                                                                                              \
+        id = id_next;                                                                                        \
+        ++pg;                                                                                                \
+        id_next = list[min(pg + 1, pg_last)];                                                                \
+      }                                                                                                      \
+    }                                                                                                        \
+  }
+#define WIDE_SYNC()                                                                                          \
+  {                                                                                                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                       \
+    __builtin_amdgcn_s_waitcnt(0); /* this step's loads, issued a step ago, and this wave's LDS reads */     \
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);                                                                 \
+    __builtin_amdgcn_sched_barrier(0);                                                                       \
+    __builtin_amdgcn_s_barrier();                                                                            \
+    __builtin_amdgcn_sched_barrier(0);                                                                       \
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);                                                                 \
+  }
+  auto step = [&](const WideStage<HD>& S_, const bool (&in)[2], int i) {
+    const int kb = t0 + 64 * i;
+    if (!(kb <= w_hik && kb + 63 >= w_lo)) return;
+    f32x16 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
+    v4u kf[DS][2], vf[2][DS];
+#pragma unroll
+    for (int h = 0; h < DS; ++h)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) kf[h][u] = __builtin_bit_cast(v4u, S_.k[u][h][lane]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int h = 0; h < DS; ++h)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sc[u] = mfma32(kf[h][u], qf[h], sc[u]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u][f][lane]);
+    __builtin_amdgcn_sched_barrier(0);
+    bool odd = false;
+    if (!(kb >= f_lo && kb + 63 <= min(f_hi, kend - 1) && in[0] && in[1])) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int kx = kb + 32 * u + 16 * (x >> 3) + 8 * hl + (x & 7);
+          if (!(kx >= lo_c && kx <= hi_k && in[u])) sc[u][x] = -INFINITY;
+        }
+        // keys that no column of the wave sees: their weights are 0, and so have their V to be, which may be
+        // anything; then whether any is left that is not finite
+        const int zlo = in[u] ? w_lo : 0x7fffffff;
+#pragma unroll
+        for (int f = 0; f < DS; ++f) {
+          const int k0 = kb + 32 * u + 16 * (f & 1) + 8 * hl;
+          v4u v = vf[u][f];
+          v.x &= key_mask(k0, zlo, w_hik);
+          v.y &= key_mask(k0 + 2, zlo, w_hik);
+          v.z &= key_mask(k0 + 4, zlo, w_hik);
+          v.w &= key_mask(k0 + 6, zlo, w_hik);
+          odd |= odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w);
+          vf[u][f] = v;
+        }
+      }
+      odd = __any(odd);
+    }
+    float m4[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) m4[x] = fmaxf(sc[0][x], sc[1][x]);
+#pragma unroll
+    for (int x = 4; x < 16; ++x) m4[x & 3] = fmaxf(m4[x & 3], fmaxf(sc[0][x], sc[1][x]));
+    float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    {
+      const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+      mt = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // lanes l and l ^ 32: the column's two key halves
+    }
+    const float m_new = fmaxf(m_run, mt * scale_log2);
+    if (__any(m_new > m_run)) {
+      const float alpha = exp2a(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd) O[dd] *= alpha;
+      m_run = m_new;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
+    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+    // 8 keys of the column as the P operand (rounded to bf16, the sum is not)
+    auto weights = [&](int u, int kh) {
+      float pv[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        pv[x] = exp2a(fmaf(sc[u][8 * kh + x], scale_log2, -m_use));
+        ps[x & 3] += pv[x];
+      }
+      return v4u{pack2bf(pv[0], pv[1]), pack2bf(pv[2], pv[3]), pack2bf(pv[4], pv[5]), pack2bf(pv[6], pv[7])};
+    };
+    if (!odd) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          const v4u pb = weights(u, kh);
+#pragma unroll
+          for (int dd = 0; dd < DD; ++dd) O[dd] = mfma32(vf[u][2 * dd + kh], pb, O[dd]);
+        }
+    } else {  // the columns in turn, each with the keys it sees (see tile16)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          const v4u pb = weights(u, kh);
+          const int k0 = kb + 32 * u + 16 * kh + 8 * hl;
+          for (int cx = 0; cx < 32; ++cx) {
+            const int lc = __builtin_amdgcn_readlane(lo_c, cx), hc = __builtin_amdgcn_readlane(hi_k, cx);
+            const v4u m = {key_mask(k0, lc, hc), key_mask(k0 + 2, lc, hc), key_mask(k0 + 4, lc, hc),
+                           key_mask(k0 + 6, lc, hc)};
+#pragma unroll
+            for (int dd = 0; dd < DD; ++dd) {
+              f32x16 z;
+#pragma unroll
+              for (int x = 0; x < 16; ++x) z[x] = 0.f;
+              z = mfma32(vf[u][2 * dd + kh] & m, pb, z);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) O[dd][x] = kk == cx ? O[dd][x] + z[x] : O[dd][x];
+            }
+          }
+        }
+    }
+    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+  };
+  __syncthreads();  // the rows' offsets in the stages have been read
+  if (ntiles > 0) WIDE_ISSUE(stg[0], 0);
+  for (int i = 0; i < nstep; i += 2) {
+    WIDE_SYNC();
+    WIDE_ISSUE(stg[1], 1);
+    step(stg[0], there[0], i);
+    if (i + 1 < nstep) {
+      WIDE_SYNC();
+      WIDE_ISSUE(stg[0], 0);
+      step(stg[1], there[1], i + 1);
+    }
+  }
+#undef WIDE_SYNC
+#undef WIDE_ISSUE
+  __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
+  __syncthreads();                // the stages become scratch
+  const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
+  // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
+  if (S > 1) {
+    if (ok) {
+      const int64_t at = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
+      float* po = c.po + at * HD + 4 * hl;
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          *(float4*)(po + 32 * dd + 8 * i4) =
+              make_float4(O[dd][4 * i4], O[dd][4 * i4 + 1], O[dd][4 * i4 + 2], O[dd][4 * i4 + 3]);
+      if (hl == 0) c.pml[at] = make_float2(m_run, l_tot);
+    }
+    return;
+  }
+  // through LDS, so that a lane writes 8 dims of a column
+  const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+  constexpr int LD = HD + 8;
+  bf16_t* T = (bf16_t*)&stg[wave >> 1] + (wave & 1) * 32 * LD;
+  static_assert(sizeof(WideStage<HD>) >= 2 * 32 * LD * 2, "two waves' scratch");
+#pragma unroll
+  for (int dd = 0; dd < DD; ++dd)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      uint2 pk;
+      pk.x = pack2bf(O[dd][4 * i4] * inv, O[dd][4 * i4 + 1] * inv);
+      pk.y = pack2bf(O[dd][4 * i4 + 2] * inv, O[dd][4 * i4 + 3] * inv);
+      *(uint2*)(T + kk * LD + 32 * dd + 8 * i4 + 4 * hl) = pk;
+    }
+  __builtin_amdgcn_wave_barrier();
+  constexpr int TP = HD / 8, CP = 64 / TP;  // lanes per column, columns per pass
+#pragma unroll
+  for (int it = 0; it < 32 / CP; ++it) {
+    const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * wave + cc, jo = co / rep;
+    const uint4 val = *(const uint4*)(T + cc * LD + d0);
+    if (co < ncol) *(uint4*)(y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+namespace {
+constexpr int64_t kPartMax = 256ll << 20;  // bytes of partials a call may ask for
+// How a call is cut: the kernels of the rows' own keys and of the prefix
+// (query blocks of 16 columns for the streaming kernel, 0: the wide one), the
+// wide one's column blocks, and the key splits.
+struct PagedPlan {
+  bool mfma;
+  int own_qb, own_blk, pre_qb, pre_blk;
+  int S_own, S_pre, pre_chunk, target;
+  int64_t part_bytes, ml_bytes;
+};
+PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, int W, int P, int window) {
+  PagedPlan a{};
+  a.mfma = p->dtype == FC_BF16 && (p->head_dim == 64 || p->head_dim == 128);
+  if (!a.mfma) return a;
+  const int G = p->n_kv_head, rep = H / G;
+  auto kernel = [](int64_t ncol, int& qb, int& blk) {
+    qb = ncol <= 16 ? 1 : ncol <= 32 ? 2 : 0;
+    blk = qb ? 1 : (int)((ncol + 127) / 128);
+  };
+  kernel((int64_t)std::min(max_per_row, T) * rep, a.own_qb, a.own_blk);
+  kernel((int64_t)T * rep, a.pre_qb, a.pre_blk);
+  // own keys
+  const int64_t width = (int64_t)W * p->page;
+  const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
+  const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
+  const int64_t room = std::max<int64_t>(1, kPartMax / one);
+  a.target = a.own_qb ? 1024 : 512;
+  a.S_own = (int)std::min({(longest + 127) / 128, std::max<int64_t>(1, 4 * a.target / units), room, (int64_t)128});
+  // the prefix
+  if (P > 0) {
+    const int64_t u = (int64_t)G * a.pre_blk;
+    const int64_t want = std::max<int64_t>(1, 512 / u);
+    a.S_pre = (int)std::min({want, (int64_t)(P + 127) / 128, room, (int64_t)128});
+    a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
+    a.S_pre = (P + a.pre_chunk - 1) / a.pre_chunk;
+  }
+  if (a.S_own + a.S_pre > 1) {
+    const int64_t pairs = (int64_t)T * H * (a.S_own + a.S_pre);
+    a.part_bytes = fc_align(pairs * p->head_dim * 4);
+    a.ml_bytes = fc_align(pairs * 8);
+  }
+  return a;
+}
+
+template <int HD>
+void launch_part(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, int pre,
+                 hipStream_t s) {
+  const int qb = pre ? a.pre_qb : a.own_qb, blk = pre ? a.pre_blk : a.own_blk, S = pre ? a.S_pre : a.S_own;
+  const int ug = pre ? c.pv.G : c.B * c.pv.G;
+  const bf16_t *qq = (const bf16_t*)q, *k = (const bf16_t*)p->k, *v = (const bf16_t*)p->v;
+  if (qb == 1)
+    hipLaunchKernelGGL((k_paged_stream<HD, 1>), dim3(ug, 1, S), dim3(256), 0, s, c, qq, k, v, (bf16_t*)y, pre);
+  else if (qb == 2)
+    hipLaunchKernelGGL((k_paged_stream<HD, 2>), dim3(ug, 1, S), dim3(256), 0, s, c, qq, k, v, (bf16_t*)y, pre);
+  else
+    hipLaunchKernelGGL(k_paged_wide<HD>, dim3((unsigned)(8 * ((ug * S + 7) / 8) * blk)), dim3(256), 0, s, c, qq, k, v,
+                       (bf16_t*)y, pre, ug * S, blk);
+}
+
+template <int HD>
+int launch_mfma(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, hipStream_t s) {
+  if (a.S_pre > 0) {
+    launch_part<HD>(c, a, p, q, y, 1, s);
+    FC_LAUNCH_CHECK();
+  }
+  launch_part<HD>(c, a, p, q, y, 0, s);
+  FC_LAUNCH_CHECK();
+  const int S = a.S_own + a.S_pre;
+  if (S > 1) {
+    const int64_t threads = (int64_t)c.Mcap * c.H * (HD / 8);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (S <= 2) hipLaunchKernelGGL((k_paged_merge<HD, 2>), grid, dim3(256), 0, s, c, (bf16_t*)y);
+    else if (S <= 4) hipLaunchKernelGGL((k_paged_merge<HD, 4>), grid, dim3(256), 0, s, c, (bf16_t*)y);
+    else hipLaunchKernelGGL((k_paged_merge<HD, 8>), grid, dim3(256), 0, s, c, (bf16_t*)y);
+    FC_LAUNCH_CHECK();
+  }
+  return FC_OK;
+}
+}  // namespace
+
 extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
                                                       int32_t max_per_row, int32_t n_head, int32_t width,
                                                       int32_t prefix_len, int32_t window) {
-  return 0;
+  if (check_pages(pages) != FC_OK) return FC_ERR_ARG;
+  FC_CHECK_ARG(batch > 0 && max_tokens > 0 && max_per_row > 0 && n_head > 0 && n_head % pages->n_kv_head == 0 &&
+                   width > 0 && prefix_len >= 0 && window >= 0, "sizes");
+  const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  return a.part_bytes + a.ml_bytes;
 }
 
 extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,
@@ -410,10 +1221,18 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   FC_CHECK_ARG(n_head <= 65535, "n_head must be <= 65535");
   FC_CHECK_ARG(window >= 0 && prefix_len >= 0 && (prefix_len == 0 || prefix_pages), "window, prefix");
   FC_CHECK_ARG(width > 0 && (int64_t)width * pages->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
+  const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  FC_CHECK_ARG(a.part_bytes == 0 || (work && work_bytes >= a.part_bytes + a.ml_bytes), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
-               1.f / sqrtf((float)pages->head_dim)};
+               1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, (float*)work,
+               (float2*)((char*)work + a.part_bytes)};
   const hipStream_t s = (hipStream_t)stream;
+  // the matrix-core kernels load 16 bytes at a time
+  const bool vec = (((uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)y | (uintptr_t)work) & 15) ==
+                       0 && ((q_token_stride | q_head_stride | pages->k_stride | pages->v_stride) & 7) == 0;
+  if (a.mfma && vec)
+    return pages->head_dim == 128 ? launch_mfma<128>(c, a, pages, q, y, s) : launch_mfma<64>(c, a, pages, q, y, s);
   if (pages->dtype == FC_BF16)
     hipLaunchKernelGGL(k_paged_any<bf16_t>, dim3(max_tokens, n_head), dim3(256), 0, s, c, (const bf16_t*)q,
                        (const bf16_t*)pages->k, (const bf16_t*)pages->v, (bf16_t*)y);

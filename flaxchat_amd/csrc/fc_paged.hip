@@ -411,13 +411,19 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
 }
 __device__ __forceinline__ float exp2a(float x) { return __builtin_amdgcn_exp2f(x); }
 // Two keys' worth of a V operand word: all ones where the key is in [lo, hi].
+// (Keys are compared as constants with bounds relative to the lane's first
+// key: the other way round the sums, one per key, are kept in registers
+// through the whole walk.)
 __device__ __forceinline__ uint32_t key_mask(int key, int lo, int hi) {
   return (key >= lo && key <= hi ? 0xffffu : 0u) | (key + 1 >= lo && key + 1 <= hi ? 0xffff0000u : 0u);
 }
-// whether a pair of bf16 holds an infinity or NaN
-__device__ __forceinline__ bool odd_pair(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+// The larger magnitudes of two pairs of bf16, as 15-bit numbers: an infinity
+// or NaN is one of 0x7f80 and more.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 max_magnitude(u16x2 a, uint32_t w) {
+  return __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
 }
+__device__ __forceinline__ bool any_odd(u16x2 m) { return __any(m.x >= 0x7f80 || m.y >= 0x7f80); }
 template <int N>
 __device__ __forceinline__ int lanes_min(int v) {
 #pragma unroll
@@ -472,15 +478,78 @@ __device__ __forceinline__ void zero_tail(const PagedChunk& c, bf16_t* y, int wg
     for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)(y + t * n8 * 8))[i] = uint4{0u, 0u, 0u, 0u};
 }
 
+// The matrix product multiplies a key's V by the weight 0 of a column that
+// does not see the key: NaN if V is not finite. Both kernels clear the keys
+// that no column of theirs sees, look for such values among the rest where the
+// columns differ (`odd`) and, if there are any, hand the workgroup's columns
+// [c_lo, c_hi) over to this plain form, one wave per column, over the keys
+// [kbeg, kend). (Anything done about them in the walk itself costs every call
+// registers, and spills.)
+template <int HD>
+__device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* q, const bf16_t* kp, const bf16_t* vp,
+                                             bf16_t* y, bool pre, int b, int g, int base, int c_lo, int c_hi, int kbeg,
+                                             int kend, int sg, int wave) {
+  const int lane = threadIdx.x & 63, rep = c.H / c.pv.G;
+  const int* list = pre ? c.pre : c.tables + (int64_t)b * c.W;
+  for (int col = c_lo + wave; col < c_hi; col += 4) {
+    const int j = col / rep, head = g * rep + col - j * rep;
+    int64_t pos = pre ? 0 : (int64_t)c.start[b] + j;
+    if (pre) {
+      const int r = row_of(c.row_off, c.B, j);
+      if (r >= c.B) continue;
+      const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
+      if (j < sp.base || j >= sp.base + sp.n) continue;
+      pos = (int64_t)c.start[r] + (j - sp.base);
+    }
+    int lo, hi;
+    key_range(c, pos, pre, lo, hi);
+    lo = max(lo, kbeg);
+    hi = min(hi, kend - 1);
+    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh;
+    float m = -INFINITY, l = 0.f, o[HD / 64] = {};
+    for (int k0 = lo; k0 <= hi; k0 += 64) {
+      const int key = k0 + lane, pg = min(key, hi) / c.pv.page, at = min(key, hi) - pg * c.pv.page;
+      const int id = list[pg];
+      const bool ok = key <= hi && (unsigned)id < (unsigned)c.pv.N;
+      float s = -INFINITY;
+      if (ok) {
+        float a = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < HD; ++d) a += bf2f(qr[d]) * bf2f(kp[k_elem(c.pv, id, g, at, d)]);
+        s = a * c.scale * 1.4426950408889634f;
+      }
+      const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
+      const float p = ok ? exp2a(s - mu) : 0.f, alpha = exp2a(m - mu);
+      l = l * alpha + wave_sum(p);
+      m = mn;
+#pragma unroll
+      for (int t = 0; t < HD / 64; ++t) o[t] *= alpha;
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i) {
+        const int idi = __shfl(ok ? id : -1, i, WAVE), ati = __shfl(at, i, WAVE);
+        const float w = __shfl(p, i, WAVE);
+        if (idi < 0) continue;
+#pragma unroll
+        for (int t = 0; t < HD / 64; ++t) o[t] += w * bf2f(vp[v_elem(c.pv, idi, g, ati, lane + 64 * t)]);
+      }
+    }
+    const int64_t pair = (int64_t)(base + j) * c.H + head;
+    if (c.S_own + c.S_pre == 1) {
+      for (int t = 0; t < HD / 64; ++t) y[pair * HD + lane + 64 * t] = f2bf(l == 0.f ? 0.f : o[t] / l);
+    } else {
+      const int64_t at = (int64_t)sg * c.Mcap * c.H + pair;
+      for (int t = 0; t < HD / 64; ++t) c.po[at * HD + lane + 64 * t] = o[t];
+      if (lane == 0) c.pml[at] = make_float2(m, l);
+    }
+  }
+}
+
 // One 32-key tile of one wave for 16 query columns: S^T = K Q^T, the running
-// softmax, O^T += V^T P^T, as in fc_attn.hip's attn_tile. MASK: some column
-// does not see all 32 keys. vf then holds 0 for keys that none sees; `odd`:
-// it holds an infinity or NaN that some column does not see. Its product with
-// that column's weight 0 would be NaN, so the columns take turns, each with
-// the keys it sees.
-template <int HD, bool MASK>
+// softmax, O^T += V^T P^T, as in fc_attn.hip's attn_tile. lo, hi: the keys that
+// this lane's column sees; vf holds 0 for those that none sees.
+template <int HD>
 __device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint4 (&vf)[HD / 16],
-                                       const uint4 (&qf)[HD / 32], int kb, int g4, int lo, int hi, bool odd,
+                                       const uint4 (&qf)[HD / 32], int kb, int g4, int lo, int hi,
                                        float scale_log2, float& m_run, float& l_run, f32x4 (&O)[HD / 16]) {
   f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -490,11 +559,7 @@ __device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint
   float p[8], mt = -INFINITY;
 #pragma unroll
   for (int jj = 0; jj < 8; ++jj) {
-    p[jj] = sc[jj >> 2][jj & 3] * scale_log2;
-    if constexpr (MASK) {
-      const int key = kb + 8 * g4 + jj;
-      p[jj] = key >= lo && key <= hi ? p[jj] : -INFINITY;
-    }
+    p[jj] = jj >= lo - kb - 8 * g4 && jj <= hi - kb - 8 * g4 ? sc[jj >> 2][jj & 3] * scale_log2 : -INFINITY;
     mt = fmaxf(mt, p[jj]);
   }
   mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
@@ -515,23 +580,6 @@ __device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint
   }
   // the weights go into the product rounded to bf16 (half a step, 2^-8, of each); the sum keeps fp32
   const uint4 pf = {pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])};
-  if (MASK && odd) {
-    for (int col = 0; col < 16; ++col) {
-      const int lc = __builtin_amdgcn_readlane(lo, col), hc = __builtin_amdgcn_readlane(hi, col);
-      const int k0 = kb + 8 * g4;
-      const uint32_t m0 = key_mask(k0, lc, hc), m1 = key_mask(k0 + 2, lc, hc), m2 = key_mask(k0 + 4, lc, hc),
-                     m3 = key_mask(k0 + 6, lc, hc);
-      const bool mine = (threadIdx.x & 15) == col;
-#pragma unroll
-      for (int db = 0; db < HD / 16; ++db) {
-        const uint4 v = {vf[db].x & m0, vf[db].y & m1, vf[db].z & m2, vf[db].w & m3};
-        const f32x4 t = mfma16(v, pf, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-        for (int x = 0; x < 4; ++x) O[db][x] = mine ? O[db][x] + t[x] : O[db][x];
-      }
-    }
-    return;
-  }
 #pragma unroll
   for (int db = 0; db < HD / 16; ++db) O[db] = mfma16(vf[db], pf, O[db]);
 }
@@ -620,6 +668,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
     return;
   }
 
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  const int tpp = c.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
+  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
+  const int64_t gofs = (int64_t)g * c.pv.page * HD;
+  const int krow = 8 * (cl >> 2) + (cl & 3);  // the key of operand row cl (+ 4 cc)
+  int tile = (int)(min(kbeg, (int64_t)w_hi + 1) >> 5) + wave;
+  int pg = tile / tpp, r = tile - pg * tpp;
   float m_run[QB], l_run[QB];
   f32x4 O[QB][HD / 16];
 #pragma unroll
@@ -629,14 +684,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) O[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float scale_log2 = c.scale * 1.4426950408889634f;
-  const int tpp = c.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
-  int tile = (int)(min(kbeg, (int64_t)w_hi + 1) >> 5) + wave;
-  int pg = tile / tpp, r = tile - pg * tpp;
-  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
   int id = tile < tend ? list[pg] : -1;
-  const int64_t gofs = (int64_t)g * c.pv.page * HD;
-  const int krow = 8 * (cl >> 2) + (cl & 3);  // the key of operand row cl (+ 4 cc)
+  bool odd = false;
   while (tile < tend) {
     const int kb = 32 * tile, id0 = id, r0 = r;
     // the next tile's page, ahead of this one's work
@@ -656,32 +705,33 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
     const bf16_t* vt = vp + (int64_t)id0 * c.pv.vs + gofs + r0 * (32 * HD) + cl * 32 + 8 * g4;
 #pragma unroll
     for (int db = 0; db < HD / 16; ++db) vf[db] = KV_LD((const uint4*)(vt + db * 512));
-    if (kb >= f_lo && kb + 31 <= f_hi) {
-#pragma unroll
-      for (int u = 0; u < QB; ++u)
-        tile16<HD, false>(kf, vf, qf[u], kb, g4, 0, 0, false, scale_log2, m_run[u], l_run[u], O[u]);
-    } else {
-      const int k0 = kb + 8 * g4;
-      const uint32_t m0 = key_mask(k0, w_lo, w_hi), m1 = key_mask(k0 + 2, w_lo, w_hi),
-                     m2 = key_mask(k0 + 4, w_lo, w_hi), m3 = key_mask(k0 + 6, w_lo, w_hi);
-      bool odd = false;
+    if (!(kb >= f_lo && kb + 31 <= f_hi)) {
+      const int zl = w_lo - kb - 8 * g4, zh = w_hi - kb - 8 * g4;
+      const uint32_t m0 = key_mask(0, zl, zh), m1 = key_mask(2, zl, zh), m2 = key_mask(4, zl, zh),
+                     m3 = key_mask(6, zl, zh);
+      u16x2 mag = {0, 0};
 #pragma unroll
       for (int db = 0; db < HD / 16; ++db) {
         vf[db] = uint4{vf[db].x & m0, vf[db].y & m1, vf[db].z & m2, vf[db].w & m3};
-        odd |= odd_pair(vf[db].x) || odd_pair(vf[db].y) || odd_pair(vf[db].z) || odd_pair(vf[db].w);
+        mag = max_magnitude(max_magnitude(mag, vf[db].x), vf[db].y);
+        mag = max_magnitude(max_magnitude(mag, vf[db].z), vf[db].w);
       }
-      odd = __any(odd);
-#pragma unroll
-      for (int u = 0; u < QB; ++u)
-        tile16<HD, true>(kf, vf, qf[u], kb, g4, lo[u], hi[u], odd, scale_log2, m_run[u], l_run[u], O[u]);
+      odd |= any_odd(mag);
     }
+#pragma unroll
+    for (int u = 0; u < QB; ++u)
+      tile16<HD>(kf, vf, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
+  }
+  if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
+    redo_columns<HD>(c, q, kp, vp, y, pre, b, g, base, 0, ncol, (int)min(kbeg, kend), (int)kend, sg, wave);
+    return;
   }
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     if (16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
       l_run[u] += __shfl_xor(l_run[u], 16, WAVE);
       l_run[u] += __shfl_xor(l_run[u], 32, WAVE);
-      if (u > 0 || pre) __syncthreads();  // the readers of the LDS are done with it
+      if (u > 0) __syncthreads();  // the readers of the LDS are done with it
       if (g4 == 0) {
         sm[wave][cl] = m_run[u];
         sl[wave][cl] = l_run[u];
@@ -849,10 +899,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
   int lo_c, hi_c;
   key_range(c, pos, pre, lo_c, hi_c);
   if (!ok) lo_c = 0x7fffffff, hi_c = -1;
-  // the keys that some / every column of the wave sees, and of the workgroup
-  const bool some = lo_c <= hi_c;
-  const int w_lo = lanes_min<32>(some ? lo_c : 0x7fffffff), w_hi = lanes_max<32>(some ? hi_c : -1);
-  const int f_lo = lanes_max<32>(ok ? lo_c : 0), f_hi = lanes_min<32>(ok ? hi_c : 0x7fffffff);
+  // the keys that some column of the workgroup sees
+  const int w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
+  int w_hi = lanes_max<32>(lo_c <= hi_c ? hi_c : -1);
   if (lane == 0) {
     rng[wave][0] = w_lo;
     rng[wave][1] = w_hi;
@@ -883,7 +932,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
   }
   const int t0 = none ? 0 : (int)kbeg64, kend = none ? 0 : (int)kend64;
   const int ntiles = (kend - t0 + 31) >> 5, nstep = (ntiles + 1) >> 1;
-  const int hi_k = min(hi_c, kend - 1), w_hik = min(w_hi, kend - 1);  // behind kend a step repeats its last tile
+  hi_c = min(hi_c, kend - 1);  // behind kend a step repeats its last tile
+  w_hi = min(w_hi, kend - 1);
+  const int f_lo = lanes_max<32>(ok ? lo_c : 0), f_hi = lanes_min<32>(ok ? hi_c : 0x7fffffff);  // seen by all
   // byte offsets of this lane's 16 bytes of the operands: K row kk is key
   // 16 (kk / 16) + 8 ((kk / 4) % 2) + 4 ((kk / 8) % 2) + kk % 4 of the tile, V row kk is dim kk of 32
   const int key = ((kk >> 4) << 4) | (((kk >> 2) & 1) << 3) | (((kk >> 3) & 1) << 2) | (kk & 3);
@@ -891,6 +942,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
                                   : (uint32_t)(key * (2 * HD) + 16 * hl);
   const uint32_t voff = 16u * (uint32_t)(4 * kk + hl);
   const int64_t gofs = (int64_t)g * c.pv.page * HD;
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  const int tpp = c.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
+  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
   f32x16 O[DD];
 #pragma unroll
   for (int dd = 0; dd < DD; ++dd)
@@ -898,18 +952,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
     for (int x = 0; x < 16; ++x) O[dd][x] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
   // the walk over the pages, one tile at a time; the next page's entry is under way a page ahead
-  const int tpp = c.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1;
-  int tile = t0 >> 5, pg = tile / tpp, tr = tile - pg * tpp;
-  const int pg_last = tlast / tpp;
-  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
+  int tile = t0 >> 5, pg = pg0, tr = tile - pg * tpp;
   int id = ntiles > 0 ? list[pg] : -1, id_next = ntiles > 0 ? list[min(pg + 1, pg_last)] : -1;
-  bool there[2][2];  // [stage][tile]: its page is one of the pool's
-  const float scale_log2 = c.scale * 1.4426950408889634f;
+  int now = 0, next = 0;  // bit u: the page of tile u of the step is one of the pool's
+  bool odd = false;
   // each wave's loads of a tile: a quarter of K's slices and of V's dims
-#define WIDE_ISSUE(S_, st_)                                                                                  \
+#define WIDE_ISSUE(S_)                                                                                       \
+  next = 0;                                                                                                  \
   _Pragma("unroll") for (int u = 0; u < 2; ++u) {                                                            \
-    there[st_][u] = (unsigned)id < (unsigned)c.pv.N;                                                         \
-    const int64_t pid = there[st_][u] ? id : 0; /* no page: page 0's place is read and masked */             \
+    const bool is = (unsigned)id < (unsigned)c.pv.N;                                                         \
+    next |= (int)is << u;                                                                                    \
+    const int64_t pid = is ? id : 0; /* no page: page 0's place is read and masked */                        \
     const bf16_t* kt = kp + pid * c.pv.ks + gofs + tr * (32 * HD);                                           \
     const bf16_t* vt = vp + pid * c.pv.vs + gofs + tr * (32 * HD);                                           \
     if constexpr (HD == 128) {                                                                               \
@@ -942,9 +995,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
     __builtin_amdgcn_sched_barrier(0);                                                                       \
     __atomic_signal_fence(__ATOMIC_SEQ_CST);                                                                 \
   }
-  auto step = [&](const WideStage<HD>& S_, const bool (&in)[2], int i) {
+  auto step = [&](const WideStage<HD>& S_, int in, int i) {
     const int kb = t0 + 64 * i;
-    if (!(kb <= w_hik && kb + 63 >= w_lo)) return;
+    if (!(kb <= w_hi && kb + 63 >= w_lo)) return;
     f32x16 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -966,31 +1019,35 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
 #pragma unroll
       for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u][f][lane]);
     __builtin_amdgcn_sched_barrier(0);
-    bool odd = false;
-    if (!(kb >= f_lo && kb + 63 <= min(f_hi, kend - 1) && in[0] && in[1])) {
+    if (!(kb >= f_lo && kb + 63 <= f_hi && in == 3)) {
+      u16x2 mag = {0, 0};
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        const bool there = (in >> u) & 1;
+        const int k0 = kb + 32 * u + 8 * hl;
+        const int lr = there ? lo_c - k0 : 64, hr = hi_c - k0;
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const int kx = kb + 32 * u + 16 * (x >> 3) + 8 * hl + (x & 7);
-          if (!(kx >= lo_c && kx <= hi_k && in[u])) sc[u][x] = -INFINITY;
+          const int kx = 16 * (x >> 3) + (x & 7);
+          if (!(kx >= lr && kx <= hr)) sc[u][x] = -INFINITY;
         }
         // keys that no column of the wave sees: their weights are 0, and so have their V to be, which may be
         // anything; then whether any is left that is not finite
-        const int zlo = in[u] ? w_lo : 0x7fffffff;
+        const int zl = there ? w_lo - k0 : 64, zh = w_hi - k0;
 #pragma unroll
         for (int f = 0; f < DS; ++f) {
-          const int k0 = kb + 32 * u + 16 * (f & 1) + 8 * hl;
+          const int kx = 16 * (f & 1);
           v4u v = vf[u][f];
-          v.x &= key_mask(k0, zlo, w_hik);
-          v.y &= key_mask(k0 + 2, zlo, w_hik);
-          v.z &= key_mask(k0 + 4, zlo, w_hik);
-          v.w &= key_mask(k0 + 6, zlo, w_hik);
-          odd |= odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w);
+          v.x &= key_mask(kx, zl, zh);
+          v.y &= key_mask(kx + 2, zl, zh);
+          v.z &= key_mask(kx + 4, zl, zh);
+          v.w &= key_mask(kx + 6, zl, zh);
+          mag = max_magnitude(max_magnitude(mag, v.x), v.y);
+          mag = max_magnitude(max_magnitude(mag, v.z), v.w);
           vf[u][f] = v;
         }
       }
-      odd = __any(odd);
+      odd |= any_odd(mag);
     }
     float m4[4];
 #pragma unroll
@@ -1012,66 +1069,39 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
-    // 8 keys of the column as the P operand (rounded to bf16, the sum is not)
-    auto weights = [&](int u, int kh) {
-      float pv[8];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        pv[x] = exp2a(fmaf(sc[u][8 * kh + x], scale_log2, -m_use));
-        ps[x & 3] += pv[x];
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh) {
+        float pv[8];  // rounded to bf16 for the product, not in the sum
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          pv[x] = exp2a(fmaf(sc[u][8 * kh + x], scale_log2, -m_use));
+          ps[x & 3] += pv[x];
+        }
+        const v4u pb = v4u{pack2bf(pv[0], pv[1]), pack2bf(pv[2], pv[3]), pack2bf(pv[4], pv[5]), pack2bf(pv[6], pv[7])};
+#pragma unroll
+        for (int dd = 0; dd < DD; ++dd) O[dd] = mfma32(vf[u][2 * dd + kh], pb, O[dd]);
       }
-      return v4u{pack2bf(pv[0], pv[1]), pack2bf(pv[2], pv[3]), pack2bf(pv[4], pv[5]), pack2bf(pv[6], pv[7])};
-    };
-    if (!odd) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          const v4u pb = weights(u, kh);
-#pragma unroll
-          for (int dd = 0; dd < DD; ++dd) O[dd] = mfma32(vf[u][2 * dd + kh], pb, O[dd]);
-        }
-    } else {  // the columns in turn, each with the keys it sees (see tile16)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          const v4u pb = weights(u, kh);
-          const int k0 = kb + 32 * u + 16 * kh + 8 * hl;
-          for (int cx = 0; cx < 32; ++cx) {
-            const int lc = __builtin_amdgcn_readlane(lo_c, cx), hc = __builtin_amdgcn_readlane(hi_k, cx);
-            const v4u m = {key_mask(k0, lc, hc), key_mask(k0 + 2, lc, hc), key_mask(k0 + 4, lc, hc),
-                           key_mask(k0 + 6, lc, hc)};
-#pragma unroll
-            for (int dd = 0; dd < DD; ++dd) {
-              f32x16 z;
-#pragma unroll
-              for (int x = 0; x < 16; ++x) z[x] = 0.f;
-              z = mfma32(vf[u][2 * dd + kh] & m, pb, z);
-#pragma unroll
-              for (int x = 0; x < 16; ++x) O[dd][x] = kk == cx ? O[dd][x] + z[x] : O[dd][x];
-            }
-          }
-        }
-    }
     l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   };
   __syncthreads();  // the rows' offsets in the stages have been read
-  if (ntiles > 0) WIDE_ISSUE(stg[0], 0);
-  for (int i = 0; i < nstep; i += 2) {
+  if (ntiles > 0) {
+    WIDE_ISSUE(stg[0]);
+  }
+  for (int i = 0; i < nstep; ++i) {
+    now = next;
     WIDE_SYNC();
-    WIDE_ISSUE(stg[1], 1);
-    step(stg[0], there[0], i);
-    if (i + 1 < nstep) {
-      WIDE_SYNC();
-      WIDE_ISSUE(stg[0], 0);
-      step(stg[1], there[1], i + 1);
-    }
+    WIDE_ISSUE(stg[(i + 1) & 1]);
+    step(stg[i & 1], now, i);
   }
 #undef WIDE_SYNC
 #undef WIDE_ISSUE
   __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
-  __syncthreads();                // the stages become scratch
+  if (__syncthreads_or(odd)) {    // (also: the stages become scratch)
+    redo_columns<HD>(c, q, kp, vp, y, pre, b, g, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
+    return;
+  }
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
   // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
   if (S > 1) {
@@ -1086,29 +1116,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
               make_float4(O[dd][4 * i4], O[dd][4 * i4 + 1], O[dd][4 * i4 + 2], O[dd][4 * i4 + 3]);
       if (hl == 0) c.pml[at] = make_float2(m_run, l_tot);
     }
-    return;
-  }
-  // through LDS, so that a lane writes 8 dims of a column
-  const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
-  constexpr int LD = HD + 8;
-  bf16_t* T = (bf16_t*)&stg[wave >> 1] + (wave & 1) * 32 * LD;
-  static_assert(sizeof(WideStage<HD>) >= 2 * 32 * LD * 2, "two waves' scratch");
+  } else {
+    // through LDS, so that a lane writes 8 dims of a column
+    const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+    constexpr int LD = HD + 8;
+    bf16_t* T = (bf16_t*)&stg[wave >> 1] + (wave & 1) * 32 * LD;
+    static_assert(sizeof(WideStage<HD>) >= 2 * 32 * LD * 2, "two waves' scratch");
 #pragma unroll
-  for (int dd = 0; dd < DD; ++dd)
+    for (int dd = 0; dd < DD; ++dd)
 #pragma unroll
-    for (int i4 = 0; i4 < 4; ++i4) {
-      uint2 pk;
-      pk.x = pack2bf(O[dd][4 * i4] * inv, O[dd][4 * i4 + 1] * inv);
-      pk.y = pack2bf(O[dd][4 * i4 + 2] * inv, O[dd][4 * i4 + 3] * inv);
-      *(uint2*)(T + kk * LD + 32 * dd + 8 * i4 + 4 * hl) = pk;
+      for (int i4 = 0; i4 < 4; ++i4) {
+        uint2 pk;
+        pk.x = pack2bf(O[dd][4 * i4] * inv, O[dd][4 * i4 + 1] * inv);
+        pk.y = pack2bf(O[dd][4 * i4 + 2] * inv, O[dd][4 * i4 + 3] * inv);
+        *(uint2*)(T + kk * LD + 32 * dd + 8 * i4 + 4 * hl) = pk;
+      }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int TP = HD / 8, CP = 64 / TP;  // lanes per column, columns per pass
+#pragma unroll
+    for (int it = 0; it < 32 / CP; ++it) {
+      const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * wave + cc, jo = co / rep;
+      const uint4 val = *(const uint4*)(T + cc * LD + d0);
+      if (co < ncol) *(uint4*)(y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
     }
-  __builtin_amdgcn_wave_barrier();
-  constexpr int TP = HD / 8, CP = 64 / TP;  // lanes per column, columns per pass
-#pragma unroll
-  for (int it = 0; it < 32 / CP; ++it) {
-    const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * wave + cc, jo = co / rep;
-    const uint4 val = *(const uint4*)(T + cc * LD + d0);
-    if (co < ncol) *(uint4*)(y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
   }
 }
 
@@ -1126,6 +1156,21 @@ struct PagedPlan {
   int S_own, S_pre, pre_chunk, target;
   int64_t part_bytes, ml_bytes;
 };
+// Key splits of the prefix: the time of the workgroups on their XCD (a unit's
+// column blocks share one; 64 run at once there, two a CU), a step of 64 keys
+// taking 2 us of two workgroups on a CU and 1.2 us of one, six steps' time for a
+// workgroup's start and end, and 4 TB/s for the partials (written and read).
+int pre_splits(int P, int G, int blk, int64_t part_bytes, int most) {
+  int best = 1;
+  double least = 1e30;
+  for (int S = 1; S <= std::min(most, (P + 127) / 128); ++S) {
+    const int64_t on = (int64_t)((G * S + 7) / 8) * blk, rounds = (on + 63) / 64;
+    const double steps = (P / S + 63) / 64 + 6;
+    const double t = rounds * steps * (on > 32 ? 2.0 : 1.2) + S * (double)part_bytes * 2 / 4e6;
+    if (t < least) least = t, best = S;
+  }
+  return best;
+}
 PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, int W, int P, int window) {
   PagedPlan a{};
   a.mfma = p->dtype == FC_BF16 && (p->head_dim == 64 || p->head_dim == 128);
@@ -1143,12 +1188,9 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
   a.target = a.own_qb ? 1024 : 512;
-  a.S_own = (int)std::min({(longest + 127) / 128, std::max<int64_t>(1, 4 * a.target / units), room, (int64_t)128});
-  // the prefix
+  a.S_own = (int)std::min({(longest + 127) / 128, std::max<int64_t>(1, (a.own_qb ? 4 : 2) * a.target / units), room, (int64_t)128});
   if (P > 0) {
-    const int64_t u = (int64_t)G * a.pre_blk;
-    const int64_t want = std::max<int64_t>(1, 512 / u);
-    a.S_pre = (int)std::min({want, (int64_t)(P + 127) / 128, room, (int64_t)128});
+    a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128));
     a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
     a.S_pre = (P + a.pre_chunk - 1) / a.pre_chunk;
   }

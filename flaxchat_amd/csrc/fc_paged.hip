@@ -472,10 +472,11 @@ __device__ __forceinline__ int own_chunk(const PagedChunk& c, int units_per_row)
 }
 
 // Tokens past the last row: set to 0 by the launch's workgroups in turn.
-__device__ __forceinline__ void zero_tail(const PagedChunk& c, bf16_t* y, int wg, int nwg) {
-  const int n8 = c.H * c.pv.hd / 8;
+template <typename T>
+__device__ __forceinline__ void zero_tail(const PagedChunk& c, T* y, int wg, int nwg) {
+  const int n8 = c.H * c.pv.hd * (int)sizeof(T) / 16;
   for (int64_t t = max(0, c.row_off[c.B]) + (int64_t)wg; t < c.Mcap; t += nwg)
-    for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)(y + t * n8 * 8))[i] = uint4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)y)[t * n8 + i] = uint4{0u, 0u, 0u, 0u};
 }
 
 // The matrix product multiplies a key's V by the weight 0 of a column that
@@ -485,9 +486,9 @@ __device__ __forceinline__ void zero_tail(const PagedChunk& c, bf16_t* y, int wg
 // [c_lo, c_hi) over to this plain form, one wave per column, over the keys
 // [kbeg, kend). (Anything done about them in the walk itself costs every call
 // registers, and spills.)
-template <int HD>
-__device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* q, const bf16_t* kp, const bf16_t* vp,
-                                             bf16_t* y, bool pre, int b, int g, int base, int c_lo, int c_hi, int kbeg,
+template <typename T, int HD>
+__device__ __forceinline__ void redo_columns(const PagedChunk& c, const T* q, const T* kp, const T* vp, T* y,
+                                              bool pre, int b, int g, int base, int c_lo, int c_hi, int kbeg,
                                              int kend, int sg, int wave) {
   const int lane = threadIdx.x & 63, rep = c.H / c.pv.G;
   const int* list = pre ? c.pre : c.tables + (int64_t)b * c.W;
@@ -505,7 +506,7 @@ __device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* 
     key_range(c, pos, pre, lo, hi);
     lo = max(lo, kbeg);
     hi = min(hi, kend - 1);
-    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh;
+    const T* qr = q + (base + j) * c.qst + head * c.qsh;
     float m = -INFINITY, l = 0.f, o[HD / 64] = {};
     for (int k0 = lo; k0 <= hi; k0 += 64) {
       const int key = k0 + lane, pg = min(key, hi) / c.pv.page, at = min(key, hi) - pg * c.pv.page;
@@ -515,7 +516,7 @@ __device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* 
       if (ok) {
         float a = 0.f;
 #pragma unroll 1
-        for (int d = 0; d < HD; ++d) a += bf2f(qr[d]) * bf2f(kp[k_elem(c.pv, id, g, at, d)]);
+        for (int d = 0; d < HD; ++d) a += ld<T>(qr, d) * ld<T>(kp, k_elem(c.pv, id, g, at, d));
         s = a * c.scale * 1.4426950408889634f;
       }
       const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
@@ -530,12 +531,12 @@ __device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* 
         const float w = __shfl(p, i, WAVE);
         if (idi < 0) continue;
 #pragma unroll
-        for (int t = 0; t < HD / 64; ++t) o[t] += w * bf2f(vp[v_elem(c.pv, idi, g, ati, lane + 64 * t)]);
+        for (int t = 0; t < HD / 64; ++t) o[t] += w * ld<T>(vp, v_elem(c.pv, idi, g, ati, lane + 64 * t));
       }
     }
     const int64_t pair = (int64_t)(base + j) * c.H + head;
     if (c.S_own + c.S_pre == 1) {
-      for (int t = 0; t < HD / 64; ++t) y[pair * HD + lane + 64 * t] = f2bf(l == 0.f ? 0.f : o[t] / l);
+      for (int t = 0; t < HD / 64; ++t) st<T>(y, pair * HD + lane + 64 * t, l == 0.f ? 0.f : o[t] / l);
     } else {
       const int64_t at = (int64_t)sg * c.Mcap * c.H + pair;
       for (int t = 0; t < HD / 64; ++t) c.po[at * HD + lane + 64 * t] = o[t];
@@ -544,18 +545,130 @@ __device__ __forceinline__ void redo_columns(const PagedChunk& c, const bf16_t* 
   }
 }
 
-// One 32-key tile of one wave for 16 query columns: S^T = K Q^T, the running
-// softmax, O^T += V^T P^T, as in fc_attn.hip's attn_tile. lo, hi: the keys that
-// this lane's column sees; vf holds 0 for those that none sees.
+// The matrix operands of one 32-key tile and 16 query columns, in registers:
+// lane l = cl + 16 g4 holds operand row cl. K row cl of half cc is key
+// 8 (cl / 4) + cl % 4 + 4 cc, so that the scores leave a lane with keys 8 g4 ..
+// +7 of its column: the P operand as they stand.
+__device__ __forceinline__ f32x4 mfma16f(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+template <typename T, int HD>
+struct Tile;
+// bf16: 16x16x32 products, 8 values of k a lane
 template <int HD>
-__device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint4 (&vf)[HD / 16],
-                                       const uint4 (&qf)[HD / 32], int kb, int g4, int lo, int hi,
-                                       float scale_log2, float& m_run, float& l_run, f32x4 (&O)[HD / 16]) {
+struct Tile<bf16_t, HD> {
+  uint4 k[2][HD / 32], v[HD / 16];
+  struct Q {
+    uint4 q[HD / 32];
+    __device__ __forceinline__ void load(const bf16_t* row, int g4, bool ok) {
+      const uint32_t keep = ok ? 0xffffffffu : 0u;  // (a select of the address would make these flat loads)
+#pragma unroll
+      for (int s = 0; s < HD / 32; ++s) {
+        const uint4 x = *(const uint4*)(row + 32 * s + 8 * g4);
+        q[s] = uint4{x.x & keep, x.y & keep, x.z & keep, x.w & keep};
+      }
+    }
+  };
+  __device__ __forceinline__ void load(const bf16_t* kt, const bf16_t* vt, int lane) {
+    const int cl = lane & 15, g4 = lane >> 4;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int s = 0; s < HD / 32; ++s)
+        k[cc][s] = KV_LD((const uint4*)(HD == 128 ? kt + lane * 8 + (s * 2 + cc) * 512
+                                                  : kt + (8 * (cl >> 2) + (cl & 3) + 4 * cc) * HD + 32 * s + 8 * g4));
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) v[db] = KV_LD((const uint4*)(vt + cl * 32 + 8 * g4 + db * 512));
+  }
+  // V = 0 for keys outside [zl, zh] (counted from the lane's first); whether any other value is not finite
+  __device__ __forceinline__ bool clear(int zl, int zh) {
+    const uint32_t m0 = key_mask(0, zl, zh), m1 = key_mask(2, zl, zh), m2 = key_mask(4, zl, zh),
+                   m3 = key_mask(6, zl, zh);
+    u16x2 mag = {0, 0};
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) {
+      v[db] = uint4{v[db].x & m0, v[db].y & m1, v[db].z & m2, v[db].w & m3};
+      mag = max_magnitude(max_magnitude(mag, v[db].x), v[db].y);
+      mag = max_magnitude(max_magnitude(mag, v[db].z), v[db].w);
+    }
+    return any_odd(mag);
+  }
+  __device__ __forceinline__ void scores(const Q& q, f32x4 (&sc)[2]) const {
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc) sc[cc] = mfma16(k[cc][s], q.q[s], sc[cc]);
+  }
+  // the weights go into the product rounded to bf16 (half a step, 2^-8, of each); their sum keeps fp32
+  __device__ __forceinline__ void add(const float (&p)[8], f32x4 (&O)[HD / 16]) const {
+    const uint4 pf = {pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])};
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) O[db] = mfma16(v[db], pf, O[db]);
+  }
+};
+// fp32: 16x16x4 products, one value of k a lane; 16-byte loads give it four products' worth
+template <int HD>
+struct Tile<float, HD> {
+  f32x4 k[2][HD / 16], v[HD / 16][2];
+  struct Q {
+    f32x4 q[HD / 16];
+    __device__ __forceinline__ void load(const float* row, int g4, bool ok) {
+#pragma unroll
+      for (int s = 0; s < HD / 16; ++s) {
+        const f32x4 x = *(const f32x4*)(row + 16 * s + 4 * g4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[s][i] = ok ? x[i] : 0.f;
+      }
+    }
+  };
+  __device__ __forceinline__ void load(const float* kt, const float* vt, int lane) {
+    const int cl = lane & 15, g4 = lane >> 4;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int s = 0; s < HD / 16; ++s)
+        k[cc][s] = *(const f32x4*)(kt + (8 * (cl >> 2) + (cl & 3) + 4 * cc) * HD + 16 * s + 4 * g4);
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[db][h] = *(const f32x4*)(vt + db * 512 + cl * 32 + 8 * g4 + 4 * h);
+  }
+  __device__ __forceinline__ bool clear(int zl, int zh) {
+    uint32_t mag = 0;
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = i >= zl && i <= zh ? v[db][i >> 2][i & 3] : 0.f;
+        mag = max(mag, __float_as_uint(x) & 0x7fffffffu);
+        v[db][i >> 2][i & 3] = x;
+      }
+    return __any(mag >= 0x7f800000u);
+  }
+  __device__ __forceinline__ void scores(const Q& q, f32x4 (&sc)[2]) const {
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) sc[cc] = mfma16f(k[cc][s][i], q.q[s][i], sc[cc]);
+  }
+  __device__ __forceinline__ void add(const float (&p)[8], f32x4 (&O)[HD / 16]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int db = 0; db < HD / 16; ++db) O[db] = mfma16f(v[db][i >> 2][i & 3], p[i], O[db]);
+  }
+};
+
+// One tile of one wave for 16 query columns: S^T = K Q^T, the running softmax,
+// O^T += V^T P^T. lo, hi: the keys that this lane's column sees; the tile's V is
+// 0 for those that none sees.
+template <typename T, int HD>
+__device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile<T, HD>::Q& q, int kb, int g4, int lo,
+                                       int hi, float scale_log2, float& m_run, float& l_run, f32x4 (&O)[HD / 16]) {
   f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-  for (int s = 0; s < HD / 32; ++s)
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc) sc[cc] = mfma16(kf[cc][s], qf[s], sc[cc]);
+  t.scores(q, sc);
   float p[8], mt = -INFINITY;
 #pragma unroll
   for (int jj = 0; jj < 8; ++jj) {
@@ -578,34 +691,42 @@ __device__ __forceinline__ void tile16(const uint4 (&kf)[2][HD / 32], const uint
     p[jj] = exp2a(p[jj] - mu);
     l_run += p[jj];
   }
-  // the weights go into the product rounded to bf16 (half a step, 2^-8, of each); the sum keeps fp32
-  const uint4 pf = {pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])};
-#pragma unroll
-  for (int db = 0; db < HD / 16; ++db) O[db] = mfma16(vf[db], pf, O[db]);
+  t.add(p, O);
 }
 
-// Few query columns (token, head in group): at most 16 QB of a row and KV
-// group, or, for the prefix (`pre`), of all rows together. A workgroup takes
-// one key split; its four waves every fourth 32-key tile, straight from memory
-// into registers, each tile applied to all QB blocks of 16 columns, and are
-// merged in LDS. grid (row x group, or group; 1; split).
-template <int HD, int QB>
-__global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf16_t* __restrict__ q,
-                                                         const bf16_t* __restrict__ kp,
-                                                         const bf16_t* __restrict__ vp, bf16_t* __restrict__ y,
-                                                         int pre) {
+// 8 results of a row
+__device__ __forceinline__ void store8(bf16_t* y, const float (&o)[8], float f) {
+  *(uint4*)y = uint4{pack2bf(o[0] * f, o[1] * f), pack2bf(o[2] * f, o[3] * f), pack2bf(o[4] * f, o[5] * f),
+                     pack2bf(o[6] * f, o[7] * f)};
+}
+__device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
+  ((float4*)y)[0] = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+  ((float4*)y)[1] = make_float4(o[4] * f, o[5] * f, o[6] * f, o[7] * f);
+}
+
+// Few query columns (token, head in group), or fp32: a workgroup takes 16 QB of
+// a row and KV group, or, for the prefix (`pre`), of all rows together, and one
+// key split; its four waves every fourth 32-key tile, straight from memory into
+// registers, each tile applied to all QB blocks of 16 columns, and are merged in
+// LDS. grid (row x group, or group; column block; split).
+template <typename T, int HD, int QB>
+__global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* __restrict__ q,
+                                                         const T* __restrict__ kp, const T* __restrict__ vp,
+                                                         T* __restrict__ y, int pre) {
   constexpr int NW = 4, NT = 2 * HD;  // threads that own 8 dims of a column after the merge
   __shared__ float sm[NW][16], sl[NW][16];
   __shared__ float so[NW][16][HD + 4];
   static_assert(sizeof(so) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cl = lane & 15, g4 = lane >> 4, rep = c.H / c.pv.G, split = blockIdx.z;
+  const int col0 = blockIdx.y * 16 * QB;
   const int S = c.S_own + c.S_pre;
-  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
+  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
   int b = 0, g, base = 0, ncol;
   if (pre) {
     g = blockIdx.x;
-    ncol = c.Mcap * rep;
+    ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
+    if (col0 >= ncol) return;
     int* off = (int*)so;
     for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
     __syncthreads();
@@ -613,17 +734,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
     b = blockIdx.x / c.pv.G;
     g = blockIdx.x - b * c.pv.G;
     const RowSpan sp = row_span(c.row_off, b, c.max_per_row, c.Mcap);
-    if (sp.n == 0) return;
     base = sp.base;
     ncol = sp.n * rep;
+    if (col0 >= ncol) return;
   }
   // this lane's columns
-  uint4 qf[QB][HD / 32];
+  typename Tile<T, HD>::Q qf[QB];
   int lo[QB], hi[QB];
   int w_lo = 0x7fffffff, w_hi = -1, f_lo = 0, f_hi = 0x7fffffff;
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
-    const int col = 16 * u + cl;
+    const int col = col0 + 16 * u + cl;
     bool ok = col < ncol;
     const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
     int64_t pos = 0;
@@ -644,25 +765,23 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
     w_hi = max(w_hi, some ? hi[u] : -1);
     f_lo = max(f_lo, ok ? lo[u] : 0);
     f_hi = min(f_hi, ok ? hi[u] : 0x7fffffff);
-    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh + 8 * g4;
-    const uint32_t keep = ok ? 0xffffffffu : 0u;
-#pragma unroll
-    for (int s = 0; s < HD / 32; ++s) {
-      const uint4 v = *(const uint4*)(qr + 32 * s);
-      qf[u][s] = uint4{v.x & keep, v.y & keep, v.z & keep, v.w & keep};
-    }
+    qf[u].load(q + (base + j) * c.qst + head * c.qsh, g4, ok);
   }
   w_lo = lanes_min<16>(w_lo);
   w_hi = lanes_max<16>(w_hi);
   f_lo = lanes_max<16>(f_lo);
   f_hi = lanes_min<16>(f_hi);
-  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G) : 0x7fffffe0;
-  const int64_t kbeg = (int64_t)(w_lo & ~31) + (int64_t)split * chunk;
-  const int64_t kend = min((int64_t)w_hi + 1, kbeg + chunk);
+  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G * gridDim.y) : 0x7fffffe0;
+  // (a row's splits are counted from its first column's first key in every one of its blocks)
+  int from = w_lo, unused;
+  if (!pre && c.window > 0 && c.S_own > 1) key_range(c, c.start[b], false, from, unused);
+  const int64_t s_beg = (int64_t)(from & ~31) + (int64_t)split * chunk;
+  const int64_t kbeg = max(s_beg, (int64_t)(w_lo & ~31)), kend = min((int64_t)w_hi + 1, s_beg + chunk);
   const int sg = pre ? c.S_own + split : split;
   if (kbeg >= kend && S > 1) {
-    if (threadIdx.x < 16 * QB && threadIdx.x < ncol) {
-      const int j = threadIdx.x / rep, head = g * rep + threadIdx.x - j * rep;
+    const int col = col0 + threadIdx.x;
+    if (threadIdx.x < 16 * QB && col < ncol) {
+      const int j = col / rep, head = g * rep + col - j * rep;
       c.pml[((int64_t)sg * c.Mcap + base + j) * c.H + head] = make_float2(-INFINITY, 0.f);
     }
     return;
@@ -672,7 +791,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
   const int tpp = c.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
   const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
   const int64_t gofs = (int64_t)g * c.pv.page * HD;
-  const int krow = 8 * (cl >> 2) + (cl & 3);  // the key of operand row cl (+ 4 cc)
   int tile = (int)(min(kbeg, (int64_t)w_hi + 1) >> 5) + wave;
   int pg = tile / tpp, r = tile - pg * tpp;
   float m_run[QB], l_run[QB];
@@ -694,41 +812,20 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
     while (r >= tpp) r -= tpp, ++pg;
     id = tile < tend ? list[pg] : -1;
     if ((unsigned)id0 >= (unsigned)c.pv.N) continue;
-    uint4 kf[2][HD / 32], vf[HD / 16];
-    const bf16_t* kt = kp + (int64_t)id0 * c.pv.ks + gofs + r0 * (32 * HD);
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-      for (int s = 0; s < HD / 32; ++s)
-        kf[cc][s] = KV_LD((const uint4*)(HD == 128 ? kt + lane * 8 + (s * 2 + cc) * 512
-                                                   : kt + (krow + 4 * cc) * HD + 32 * s + 8 * g4));
-    const bf16_t* vt = vp + (int64_t)id0 * c.pv.vs + gofs + r0 * (32 * HD) + cl * 32 + 8 * g4;
-#pragma unroll
-    for (int db = 0; db < HD / 16; ++db) vf[db] = KV_LD((const uint4*)(vt + db * 512));
-    if (!(kb >= f_lo && kb + 31 <= f_hi)) {
-      const int zl = w_lo - kb - 8 * g4, zh = w_hi - kb - 8 * g4;
-      const uint32_t m0 = key_mask(0, zl, zh), m1 = key_mask(2, zl, zh), m2 = key_mask(4, zl, zh),
-                     m3 = key_mask(6, zl, zh);
-      u16x2 mag = {0, 0};
-#pragma unroll
-      for (int db = 0; db < HD / 16; ++db) {
-        vf[db] = uint4{vf[db].x & m0, vf[db].y & m1, vf[db].z & m2, vf[db].w & m3};
-        mag = max_magnitude(max_magnitude(mag, vf[db].x), vf[db].y);
-        mag = max_magnitude(max_magnitude(mag, vf[db].z), vf[db].w);
-      }
-      odd |= any_odd(mag);
-    }
+    Tile<T, HD> t;
+    t.load(kp + (int64_t)id0 * c.pv.ks + gofs + r0 * (32 * HD), vp + (int64_t)id0 * c.pv.vs + gofs + r0 * (32 * HD), lane);
+    if (!(kb >= f_lo && kb + 31 <= f_hi)) odd |= t.clear(w_lo - kb - 8 * g4, w_hi - kb - 8 * g4);
 #pragma unroll
     for (int u = 0; u < QB; ++u)
-      tile16<HD>(kf, vf, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
+      tile16<T, HD>(t, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
   }
   if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
-    redo_columns<HD>(c, q, kp, vp, y, pre, b, g, base, 0, ncol, (int)min(kbeg, kend), (int)kend, sg, wave);
+    redo_columns<T, HD>(c, q, kp, vp, y, pre, b, g, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend), (int)kend, sg, wave);
     return;
   }
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
-    if (16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
+    if (col0 + 16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
       l_run[u] += __shfl_xor(l_run[u], 16, WAVE);
       l_run[u] += __shfl_xor(l_run[u], 32, WAVE);
       if (u > 0) __syncthreads();  // the readers of the LDS are done with it
@@ -739,7 +836,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
 #pragma unroll
       for (int db = 0; db < HD / 16; ++db) *(f32x4*)&so[wave][cl][16 * db + 4 * g4] = O[u][db];
       __syncthreads();
-      const int qc = threadIdx.x / (HD / 8), d0 = (threadIdx.x % (HD / 8)) * 8, col = 16 * u + qc;
+      const int qc = threadIdx.x / (HD / 8), d0 = (threadIdx.x % (HD / 8)) * 8, col = col0 + 16 * u + qc;
       if (threadIdx.x < NT && col < ncol) {
         float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -754,10 +851,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
         }
         const int j = col / rep, head = g * rep + col - j * rep;
         if (S == 1) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          *(uint4*)(y + ((int64_t)(base + j) * c.H + head) * HD + d0) =
-              uint4{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv),
-                    pack2bf(o[4] * inv, o[5] * inv), pack2bf(o[6] * inv, o[7] * inv)};
+          store8(y + ((int64_t)(base + j) * c.H + head) * HD + d0, o, L == 0.f ? 0.f : 1.f / L);
         } else {
           const int64_t at = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
           float4* po = (float4*)(c.po + at * HD + d0);
@@ -773,8 +867,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const bf1
 // Merge of the key splits of one (token, head), HD / 8 threads with 8
 // dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
 // first CB splits' loads are under way before the token's row is looked up.
-template <int HD, int CB>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, bf16_t* __restrict__ y) {
+template <typename T, int HD, int CB>
+__global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict__ y) {
   __shared__ int off[PT_ROWS + 1];
   constexpr int TP = HD / 8;
   const int64_t pair = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP, pairs = (int64_t)c.Mcap * c.H;
@@ -802,9 +896,10 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, bf16_t* __res
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
   RowSpan sp{0, 0};
   if (b < c.B) sp = row_span(off, b, c.max_per_row, c.Mcap);
-  bf16_t* yo = y + pair * HD + d0;
+  T* yo = y + pair * HD + d0;
   if (t < sp.base || t >= sp.base + sp.n) {
-    if ((c.flags & FC_PAGED_ZERO_TAIL) && t >= off[c.B]) *(uint4*)yo = uint4{0u, 0u, 0u, 0u};
+    if ((c.flags & FC_PAGED_ZERO_TAIL) && t >= off[c.B])
+      store8(yo, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, 1.f);
     return;
   }
   const float mu = M == -INFINITY ? 0.f : M;
@@ -821,9 +916,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, bf16_t* __res
       o[4] += a * u[k][1].x; o[5] += a * u[k][1].y; o[6] += a * u[k][1].z; o[7] += a * u[k][1].w;
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  *(uint4*)yo = uint4{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv),
-                      pack2bf(o[4] * inv, o[5] * inv), pack2bf(o[6] * inv, o[7] * inv)};
+  store8(yo, o, L == 0.f ? 0.f : 1.f / L);
 }
 
 // Many query columns: 128 per workgroup, 32 per wave, on the 32x32x16 MFMA, of
@@ -1099,7 +1192,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
 #undef WIDE_ISSUE
   __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
   if (__syncthreads_or(odd)) {    // (also: the stages become scratch)
-    redo_columns<HD>(c, q, kp, vp, y, pre, b, g, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
+    redo_columns<bf16_t, HD>(c, q, kp, vp, y, pre, b, g, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
     return;
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
@@ -1147,9 +1240,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
 // ---------------------------------------------------------------------------
 namespace {
 constexpr int64_t kPartMax = 256ll << 20;  // bytes of partials a call may ask for
-// How a call is cut: the kernels of the rows' own keys and of the prefix
-// (query blocks of 16 columns for the streaming kernel, 0: the wide one), the
-// wide one's column blocks, and the key splits.
+// How a call is cut: the kernels of the rows' own keys and of the prefix (query
+// blocks of 16 columns in a workgroup of the streaming kernel, 0: the wide one),
+// their column blocks, and the key splits.
 struct PagedPlan {
   bool mfma;
   int own_qb, own_blk, pre_qb, pre_blk;
@@ -1173,15 +1266,17 @@ int pre_splits(int P, int G, int blk, int64_t part_bytes, int most) {
 }
 PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, int W, int P, int window) {
   PagedPlan a{};
-  a.mfma = p->dtype == FC_BF16 && (p->head_dim == 64 || p->head_dim == 128);
+  a.mfma = p->head_dim == 64 || p->head_dim == 128;
   if (!a.mfma) return a;
   const int G = p->n_kv_head, rep = H / G;
-  auto kernel = [](int64_t ncol, int& qb, int& blk) {
-    qb = ncol <= 16 ? 1 : ncol <= 32 ? 2 : 0;
-    blk = qb ? 1 : (int)((ncol + 127) / 128);
+  auto kernel = [&](int64_t ncol, int& qb, int& blk) {
+    qb = ncol <= 16 || p->dtype == FC_F32 ? 1 : ncol <= 32 ? 2 : 0;
+    blk = (int)(qb ? (ncol + 16 * qb - 1) / (16 * qb) : (ncol + 127) / 128);
   };
   kernel((int64_t)std::min(max_per_row, T) * rep, a.own_qb, a.own_blk);
   kernel((int64_t)T * rep, a.pre_qb, a.pre_blk);
+  a.mfma = (!a.own_qb || a.own_blk <= 65535) && (!a.pre_qb || a.pre_blk <= 65535);
+  if (!a.mfma) return a;
   // own keys
   const int64_t width = (int64_t)W * p->page;
   const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
@@ -1202,36 +1297,38 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   return a;
 }
 
-template <int HD>
+template <typename T, int HD>
 void launch_part(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, int pre,
                  hipStream_t s) {
   const int qb = pre ? a.pre_qb : a.own_qb, blk = pre ? a.pre_blk : a.own_blk, S = pre ? a.S_pre : a.S_own;
   const int ug = pre ? c.pv.G : c.B * c.pv.G;
-  const bf16_t *qq = (const bf16_t*)q, *k = (const bf16_t*)p->k, *v = (const bf16_t*)p->v;
+  const T *qq = (const T*)q, *k = (const T*)p->k, *v = (const T*)p->v;
+  if constexpr (sizeof(T) == 2) {
+    if (qb == 2)
+      hipLaunchKernelGGL((k_paged_stream<T, HD, 2>), dim3(ug, blk, S), dim3(256), 0, s, c, qq, k, v, (T*)y, pre);
+    if (qb == 0)
+      hipLaunchKernelGGL(k_paged_wide<HD>, dim3((unsigned)(8 * ((ug * S + 7) / 8) * blk)), dim3(256), 0, s, c, qq, k,
+                         v, (T*)y, pre, ug * S, blk);
+  }
   if (qb == 1)
-    hipLaunchKernelGGL((k_paged_stream<HD, 1>), dim3(ug, 1, S), dim3(256), 0, s, c, qq, k, v, (bf16_t*)y, pre);
-  else if (qb == 2)
-    hipLaunchKernelGGL((k_paged_stream<HD, 2>), dim3(ug, 1, S), dim3(256), 0, s, c, qq, k, v, (bf16_t*)y, pre);
-  else
-    hipLaunchKernelGGL(k_paged_wide<HD>, dim3((unsigned)(8 * ((ug * S + 7) / 8) * blk)), dim3(256), 0, s, c, qq, k, v,
-                       (bf16_t*)y, pre, ug * S, blk);
+    hipLaunchKernelGGL((k_paged_stream<T, HD, 1>), dim3(ug, blk, S), dim3(256), 0, s, c, qq, k, v, (T*)y, pre);
 }
 
-template <int HD>
+template <typename T, int HD>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, hipStream_t s) {
   if (a.S_pre > 0) {
-    launch_part<HD>(c, a, p, q, y, 1, s);
+    launch_part<T, HD>(c, a, p, q, y, 1, s);
     FC_LAUNCH_CHECK();
   }
-  launch_part<HD>(c, a, p, q, y, 0, s);
+  launch_part<T, HD>(c, a, p, q, y, 0, s);
   FC_LAUNCH_CHECK();
   const int S = a.S_own + a.S_pre;
   if (S > 1) {
     const int64_t threads = (int64_t)c.Mcap * c.H * (HD / 8);
     const dim3 grid((unsigned)((threads + 255) / 256));
-    if (S <= 2) hipLaunchKernelGGL((k_paged_merge<HD, 2>), grid, dim3(256), 0, s, c, (bf16_t*)y);
-    else if (S <= 4) hipLaunchKernelGGL((k_paged_merge<HD, 4>), grid, dim3(256), 0, s, c, (bf16_t*)y);
-    else hipLaunchKernelGGL((k_paged_merge<HD, 8>), grid, dim3(256), 0, s, c, (bf16_t*)y);
+    if (S <= 2) hipLaunchKernelGGL((k_paged_merge<T, HD, 2>), grid, dim3(256), 0, s, c, (T*)y);
+    else if (S <= 4) hipLaunchKernelGGL((k_paged_merge<T, HD, 4>), grid, dim3(256), 0, s, c, (T*)y);
+    else hipLaunchKernelGGL((k_paged_merge<T, HD, 8>), grid, dim3(256), 0, s, c, (T*)y);
     FC_LAUNCH_CHECK();
   }
   return FC_OK;
@@ -1264,6 +1361,11 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   FC_CHECK_ARG(window >= 0 && prefix_len >= 0 && (prefix_len == 0 || prefix_pages), "window, prefix");
   FC_CHECK_ARG(width > 0 && (int64_t)width * pages->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  // a launch's threads are counted in 32 bits along x, its workgroups in 16 along y
+  const int64_t own = (int64_t)batch * pages->n_kv_head * std::max(a.S_own, 1) * std::max(a.own_blk, 1);
+  const int64_t pre = (int64_t)pages->n_kv_head * std::max(a.S_pre, 1) * std::max(a.pre_blk, 1);
+  const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
+  FC_CHECK_ARG(std::max({own, pre, merge, (int64_t)max_tokens}) < (1 << 24) - 16, "too many tokens, rows or heads");
   FC_CHECK_ARG(a.part_bytes == 0 || (work && work_bytes >= a.part_bytes + a.ml_bytes), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
@@ -1271,10 +1373,16 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
                (float2*)((char*)work + a.part_bytes)};
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
+  const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;
   const bool vec = (((uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)y | (uintptr_t)work) & 15) ==
-                       0 && ((q_token_stride | q_head_stride | pages->k_stride | pages->v_stride) & 7) == 0;
-  if (a.mfma && vec)
-    return pages->head_dim == 128 ? launch_mfma<128>(c, a, pages, q, y, s) : launch_mfma<64>(c, a, pages, q, y, s);
+                       0 && (strides & (pages->dtype == FC_BF16 ? 7 : 3)) == 0;
+  if (a.mfma && vec) {
+    if (pages->dtype == FC_BF16)
+      return pages->head_dim == 128 ? launch_mfma<bf16_t, 128>(c, a, pages, q, y, s)
+                                    : launch_mfma<bf16_t, 64>(c, a, pages, q, y, s);
+    return pages->head_dim == 128 ? launch_mfma<float, 128>(c, a, pages, q, y, s)
+                                  : launch_mfma<float, 64>(c, a, pages, q, y, s);
+  }
   if (pages->dtype == FC_BF16)
     hipLaunchKernelGGL(k_paged_any<bf16_t>, dim3(max_tokens, n_head), dim3(256), 0, s, c, (const bf16_t*)q,
                        (const bf16_t*)pages->k, (const bf16_t*)pages->v, (bf16_t*)y);

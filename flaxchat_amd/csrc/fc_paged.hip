@@ -12,6 +12,7 @@
 // row's table. An entry outside [0, n_pages) holds no keys.
 #include "fc_common.h"
 #include "fc_internal.h"
+#include <type_traits>
 
 // K and V of a row's own pages are read once a call: non-temporal loads keep
 // them from displacing lines that are read again.
@@ -424,17 +425,58 @@ __device__ __forceinline__ u16x2 max_magnitude(u16x2 a, uint32_t w) {
   return __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
 }
 __device__ __forceinline__ bool any_odd(u16x2 m) { return __any(m.x >= 0x7f80 || m.y >= 0x7f80); }
+// Reductions over the lanes of a wave in registers (rotations within 16 lanes,
+// swaps of rows and halves): the shuffles through LDS take ~5 times as long, and
+// a workgroup's first loads wait for these.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+}
+template <int N, typename F>
+__device__ __forceinline__ int lanes_reduce(int v, F f) {  // over groups of N = 16, 32 or 64 lanes, in every lane
+  v = f(v, dpp<0x128>(v));
+  v = f(v, dpp<0x124>(v));
+  v = f(v, dpp<0x122>(v));
+  v = f(v, dpp<0x121>(v));
+  if constexpr (N > 16) {
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = f((int)h[0], (int)h[1]);
+  }
+  if constexpr (N > 32) {
+    const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = f((int)h[0], (int)h[1]);
+  }
+  return v;
+}
 template <int N>
 __device__ __forceinline__ int lanes_min(int v) {
-#pragma unroll
-  for (int o = N / 2; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, WAVE));
-  return __builtin_amdgcn_readfirstlane(v);
+  return __builtin_amdgcn_readfirstlane(lanes_reduce<N>(v, [](int a, int b) { return min(a, b); }));
 }
 template <int N>
 __device__ __forceinline__ int lanes_max(int v) {
-#pragma unroll
-  for (int o = N / 2; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, WAVE));
-  return __builtin_amdgcn_readfirstlane(v);
+  return __builtin_amdgcn_readfirstlane(lanes_reduce<N>(v, [](int a, int b) { return max(a, b); }));
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+  return __uint_as_float(lanes_reduce<64>(__float_as_uint(v), [](int a, int b) {
+    return (int)__float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+// maximum over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float rows_max(float v) {
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const auto g = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(g[0]), __uint_as_float(g[1]));
+}
+// inclusive sum over the lanes up to this one (up to 2^31)
+__device__ __forceinline__ int lanes_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // a row's last lane onto the next row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the lower half's onto the upper
+  return v;
 }
 
 // Keys of a job are counted from 0: the prefix's positions, or a row's own
@@ -446,29 +488,79 @@ __device__ __forceinline__ void key_range(const PagedChunk& c, int64_t pos, bool
   lo = c.window > 0 ? (int)max((int64_t)0, min(pos - c.window - off, (int64_t)0x7fffffff)) : 0;
 }
 
-// Keys per split of the rows' own keys: what spreads all rows' keys over about
-// c.target workgroups (rows are of unequal length: a fixed number of splits
-// per row would leave the longest row's for last), at least 128 (a tile for
-// each of four waves), and no more splits of the longest row than c.S_own.
-// Every wave reads all rows' lengths; the result is the same in all of them.
-__device__ __forceinline__ int own_chunk(const PagedChunk& c, int units_per_row) {
+// The rows' own keys as a list of work items (row, column block, key split, KV
+// group), which every workgroup looks its own one up in, by its number: a row
+// has as many blocks of CB columns as its queries fill and as many splits as it
+// has chunks of keys. The chunk is what spreads all rows' keys over about
+// c.target items (rows are of unequal length: with a number of splits for all,
+// the longest row's would be left for last and the short rows' have nothing to
+// do), at least 128 keys (a tile for each of four waves), no more than
+// CHUNK_MAX (items of equal length, several rounds of them) and at least what
+// makes c.S_own splits of the longest row. Every wave reads all rows' lengths; the
+// list is the same in all of them.
+#define CHUNK_MAX 4096
+struct Item {
+  int b, blk, split, nsplit, g, chunk;
+};
+// keys of row r's walk, from the 32-key block of its first query's first key; -1: no query
+__device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
+  const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
+  ncol = sp.n * (c.H / c.pv.G);
+  if (sp.n == 0) return -1;
+  int lo, hi, lo1, hi1;
+  key_range(c, c.start[r], false, lo, hi);
+  key_range(c, (int64_t)c.start[r] + sp.n - 1, false, lo1, hi1);
+  return hi1 < lo ? 0 : hi1 + 1 - (lo & ~31);
+}
+template <int CB>
+__device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
+  const int lane = threadIdx.x & 63;
+  int len = -1, ncol = 0;  // of this lane's row of the 64 looked at last
   float total = 0.f;
   int longest = 1;
-  for (int r = threadIdx.x & 63; r < c.B; r += 64) {
-    const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
-    if (sp.n == 0) continue;
-    int lo, hi, lo1, hi1;
-    key_range(c, c.start[r], false, lo, hi);
-    key_range(c, (int64_t)c.start[r] + sp.n - 1, false, lo1, hi1);
-    const int len = hi1 < lo ? 0 : hi1 + 1 - (lo & ~31);
-    total += (float)len;
+  for (int r0 = 0; r0 < c.B; r0 += 64) {
+    len = r0 + lane < c.B ? row_keys(c, r0 + lane, ncol) : -1;
+    if (len < 0) ncol = 0;
+    total += (float)max(len, 0) * (float)((ncol + CB - 1) / CB);
     longest = max(longest, len);
   }
-  total = wave_sum(total);
+  total = lanes_sum(total);
   longest = lanes_max<64>(longest);
-  const float share = ceilf(total * (float)units_per_row / (float)c.target);
-  int chunk = max((int)fminf(share, 1e9f), max(128, (longest + c.S_own - 1) / c.S_own));
-  return __builtin_amdgcn_readfirstlane((chunk + 63) & ~63);
+  const float share = ceilf(total * (float)c.pv.G / (float)c.target);
+  const int least = max(128, (longest + c.S_own - 1) / c.S_own);
+  it.chunk = __builtin_amdgcn_readfirstlane((max((int)fminf(share, (float)CHUNK_MAX), least) + 63) & ~63);
+  const float per = 1.f / (float)it.chunk;
+  for (int r0 = 0; r0 < c.B; r0 += 64) {
+    if (c.B > 64) {
+      len = r0 + lane < c.B ? row_keys(c, r0 + lane, ncol) : -1;
+      if (len < 0) ncol = 0;
+    }
+    int ns = (int)((float)max(len, 0) * per);  // len / chunk, one off at most
+    ns += ns * it.chunk < len;
+    ns = max(1, ns - ((ns - 1) * it.chunk >= len));
+    const int nb = (ncol + CB - 1) / CB, mine = len < 0 ? 0 : ns * nb * c.pv.G;
+    const int upto = lanes_scan(mine);
+    const uint64_t past = __ballot(upto > at);
+    if (past == 0) {
+      at -= __builtin_amdgcn_readlane(upto, 63);
+      continue;
+    }
+    const int l = __builtin_ctzll(past);
+    at -= __builtin_amdgcn_readlane(upto - mine, l);
+    it.b = r0 + l;
+    it.nsplit = __builtin_amdgcn_readlane(ns, l);
+    it.g = at % c.pv.G;
+    at /= c.pv.G;
+    it.split = at % it.nsplit;
+    it.blk = at / it.nsplit;
+    return true;
+  }
+  return false;
+}
+// The partials of a row's column that no split writes: the item of its last split marks them.
+__device__ __forceinline__ void mark_unused(const PagedChunk& c, const Item& it, int64_t pair) {
+  if (it.split == it.nsplit - 1)
+    for (int s = it.nsplit; s < c.S_own; ++s) c.pml[(int64_t)s * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
 }
 
 // Tokens past the last row: set to 0 by the launch's workgroups in turn.
@@ -488,9 +580,9 @@ __device__ __forceinline__ void zero_tail(const PagedChunk& c, T* y, int wg, int
 // registers, and spills.)
 template <typename T, int HD>
 __device__ __forceinline__ void redo_columns(const PagedChunk& c, const T* q, const T* kp, const T* vp, T* y,
-                                              bool pre, int b, int g, int base, int c_lo, int c_hi, int kbeg,
+                                              bool pre, const Item& it, int base, int c_lo, int c_hi, int kbeg,
                                              int kend, int sg, int wave) {
-  const int lane = threadIdx.x & 63, rep = c.H / c.pv.G;
+  const int lane = threadIdx.x & 63, rep = c.H / c.pv.G, b = it.b, g = it.g;
   const int* list = pre ? c.pre : c.tables + (int64_t)b * c.W;
   for (int col = c_lo + wave; col < c_hi; col += 4) {
     const int j = col / rep, head = g * rep + col - j * rep;
@@ -540,7 +632,10 @@ __device__ __forceinline__ void redo_columns(const PagedChunk& c, const T* q, co
     } else {
       const int64_t at = (int64_t)sg * c.Mcap * c.H + pair;
       for (int t = 0; t < HD / 64; ++t) c.po[at * HD + lane + 64 * t] = o[t];
-      if (lane == 0) c.pml[at] = make_float2(m, l);
+      if (lane == 0) {
+        c.pml[at] = make_float2(m, l);
+        if (!pre) mark_unused(c, it, pair);
+      }
     }
   }
 }
@@ -675,9 +770,7 @@ __device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile
     p[jj] = jj >= lo - kb - 8 * g4 && jj <= hi - kb - 8 * g4 ? sc[jj >> 2][jj & 3] * scale_log2 : -INFINITY;
     mt = fmaxf(mt, p[jj]);
   }
-  mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
-  mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-  const float m_new = fmaxf(m_run, mt);
+  const float m_new = fmaxf(m_run, rows_max(mt));
   if (__any(m_new > m_run)) {
     const float alpha = exp2a(m_run - (m_new == -INFINITY ? 0.f : m_new));
     l_run *= alpha;
@@ -708,36 +801,41 @@ __device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
 // a row and KV group, or, for the prefix (`pre`), of all rows together, and one
 // key split; its four waves every fourth 32-key tile, straight from memory into
 // registers, each tile applied to all QB blocks of 16 columns, and are merged in
-// LDS. grid (row x group, or group; column block; split).
-template <typename T, int HD, int QB>
-__global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* __restrict__ q,
-                                                         const T* __restrict__ kp, const T* __restrict__ vp,
-                                                         T* __restrict__ y, int pre) {
+// LDS. `at`: its number among the list's items, or the prefix's (group, split,
+// block).
+template <int HD>
+struct StreamLds {
+  float o[4][16][HD + 4];
+  float m[4][16], l[4][16];
+};
+template <typename T, int HD, int QB, bool pre>
+__device__ __forceinline__ void stream_keys(const PagedChunk& c, const T* __restrict__ q, const T* __restrict__ kp,
+                                            const T* __restrict__ vp, T* __restrict__ y, StreamLds<HD>& lds, int at) {
   constexpr int NW = 4, NT = 2 * HD;  // threads that own 8 dims of a column after the merge
-  __shared__ float sm[NW][16], sl[NW][16];
-  __shared__ float so[NW][16][HD + 4];
-  static_assert(sizeof(so) >= (PT_ROWS + 1) * 4, "the rows' offsets");
+  static_assert(sizeof(lds) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int cl = lane & 15, g4 = lane >> 4, rep = c.H / c.pv.G, split = blockIdx.z;
-  const int col0 = blockIdx.y * 16 * QB;
+  const int cl = lane & 15, g4 = lane >> 4, rep = c.H / c.pv.G;
   const int S = c.S_own + c.S_pre;
-  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
-  int b = 0, g, base = 0, ncol;
-  if (pre) {
-    g = blockIdx.x;
+  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
+  Item it{0, 0, 0, 1, 0, c.pre_chunk};
+  int base = 0, ncol;
+  if constexpr (pre) {
+    it.g = at % c.pv.G;
+    at /= c.pv.G;
+    it.split = at % c.S_pre;
+    it.blk = at / c.S_pre;
     ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
-    if (col0 >= ncol) return;
-    int* off = (int*)so;
+    if (it.blk * 16 * QB >= ncol) return;
+    int* off = (int*)&lds;
     for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
     __syncthreads();
   } else {
-    b = blockIdx.x / c.pv.G;
-    g = blockIdx.x - b * c.pv.G;
-    const RowSpan sp = row_span(c.row_off, b, c.max_per_row, c.Mcap);
+    if (!find_item<16 * QB>(c, at, it)) return;
+    const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
     base = sp.base;
     ncol = sp.n * rep;
-    if (col0 >= ncol) return;
   }
+  const int b = it.b, g = it.g, col0 = it.blk * 16 * QB;
   // this lane's columns
   typename Tile<T, HD>::Q qf[QB];
   int lo[QB], hi[QB];
@@ -749,7 +847,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* 
     const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
     int64_t pos = 0;
     if (pre) {
-      const int* off = (const int*)so;
+      const int* off = (const int*)&lds;
       const int r = row_of(off, c.B, j);
       RowSpan sp{0, 0};
       if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
@@ -771,18 +869,19 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* 
   w_hi = lanes_max<16>(w_hi);
   f_lo = lanes_max<16>(f_lo);
   f_hi = lanes_min<16>(f_hi);
-  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G * gridDim.y) : 0x7fffffe0;
   // (a row's splits are counted from its first column's first key in every one of its blocks)
   int from = w_lo, unused;
-  if (!pre && c.window > 0 && c.S_own > 1) key_range(c, c.start[b], false, from, unused);
-  const int64_t s_beg = (int64_t)(from & ~31) + (int64_t)split * chunk;
-  const int64_t kbeg = max(s_beg, (int64_t)(w_lo & ~31)), kend = min((int64_t)w_hi + 1, s_beg + chunk);
-  const int sg = pre ? c.S_own + split : split;
+  if (!pre && c.window > 0) key_range(c, c.start[b], false, from, unused);
+  const int64_t s_beg = (int64_t)(from & ~31) + (int64_t)it.split * it.chunk;
+  const int64_t kbeg = max(s_beg, (int64_t)(w_lo & ~31)), kend = min((int64_t)w_hi + 1, s_beg + it.chunk);
+  const int sg = pre ? c.S_own + it.split : it.split;
   if (kbeg >= kend && S > 1) {
     const int col = col0 + threadIdx.x;
     if (threadIdx.x < 16 * QB && col < ncol) {
       const int j = col / rep, head = g * rep + col - j * rep;
-      c.pml[((int64_t)sg * c.Mcap + base + j) * c.H + head] = make_float2(-INFINITY, 0.f);
+      const int64_t pair = (int64_t)(base + j) * c.H + head;
+      c.pml[(int64_t)sg * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
+      if (!pre) mark_unused(c, it, pair);
     }
     return;
   }
@@ -820,7 +919,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* 
       tile16<T, HD>(t, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
   }
   if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
-    redo_columns<T, HD>(c, q, kp, vp, y, pre, b, g, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend), (int)kend, sg, wave);
+    redo_columns<T, HD>(c, q, kp, vp, y, pre, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend),
+                        (int)kend, sg, wave);
     return;
   }
 #pragma unroll
@@ -830,34 +930,37 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* 
       l_run[u] += __shfl_xor(l_run[u], 32, WAVE);
       if (u > 0) __syncthreads();  // the readers of the LDS are done with it
       if (g4 == 0) {
-        sm[wave][cl] = m_run[u];
-        sl[wave][cl] = l_run[u];
+        lds.m[wave][cl] = m_run[u];
+        lds.l[wave][cl] = l_run[u];
       }
 #pragma unroll
-      for (int db = 0; db < HD / 16; ++db) *(f32x4*)&so[wave][cl][16 * db + 4 * g4] = O[u][db];
+      for (int db = 0; db < HD / 16; ++db) *(f32x4*)&lds.o[wave][cl][16 * db + 4 * g4] = O[u][db];
       __syncthreads();
       const int qc = threadIdx.x / (HD / 8), d0 = (threadIdx.x % (HD / 8)) * 8, col = col0 + 16 * u + qc;
       if (threadIdx.x < NT && col < ncol) {
         float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][qc]);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, lds.m[w][qc]);
         const float mu = M == -INFINITY ? 0.f : M;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          const float a = exp2a(sm[w][qc] - mu);
-          L += a * sl[w][qc];
+          const float a = exp2a(lds.m[w][qc] - mu);
+          L += a * lds.l[w][qc];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] += a * so[w][qc][d0 + i];
+          for (int i = 0; i < 8; ++i) o[i] += a * lds.o[w][qc][d0 + i];
         }
         const int j = col / rep, head = g * rep + col - j * rep;
         if (S == 1) {
           store8(y + ((int64_t)(base + j) * c.H + head) * HD + d0, o, L == 0.f ? 0.f : 1.f / L);
         } else {
-          const int64_t at = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
-          float4* po = (float4*)(c.po + at * HD + d0);
+          const int64_t slot = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
+          float4* po = (float4*)(c.po + slot * HD + d0);
           po[0] = make_float4(o[0], o[1], o[2], o[3]);
           po[1] = make_float4(o[4], o[5], o[6], o[7]);
-          if (d0 == 0) c.pml[at] = make_float2(M, L);
+          if (d0 == 0) {
+            c.pml[slot] = make_float2(M, L);
+            if (!pre) mark_unused(c, it, (int64_t)(base + j) * c.H + head);
+          }
         }
       }
     }
@@ -866,31 +969,28 @@ __global__ __launch_bounds__(256, 2) void k_paged_stream(PagedChunk c, const T* 
 
 // Merge of the key splits of one (token, head), HD / 8 threads with 8
 // dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
-// first CB splits' loads are under way before the token's row is looked up.
+// splits' (max, sum) are read side by side, ahead of the token's row; then the
+// outputs of those that hold keys, CB at a time.
 template <typename T, int HD, int CB>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict__ y) {
   __shared__ int off[PT_ROWS + 1];
   constexpr int TP = HD / 8;
   const int64_t pair = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP, pairs = (int64_t)c.Mcap * c.H;
-  const int d0 = (threadIdx.x % TP) * 8, S = c.S_own + c.S_pre;
+  const int tp = threadIdx.x % TP, d0 = tp * 8, S = c.S_own + c.S_pre, own = c.S_own;
   const int64_t at = min(pair, pairs - 1);
-  float2 e[CB];
-  float4 u[CB][2];
-  auto load = [&](int s0) {
-#pragma unroll
-    for (int k = 0; k < CB; ++k) {
-      const int64_t i = (int64_t)min(s0 + k, S - 1) * pairs + at;
-      e[k] = c.pml[i];
-      u[k][0] = *(const float4*)(c.po + i * HD + d0);
-      u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
-    }
-  };
-  load(0);
-  for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
   float M = -INFINITY;
-  for (int s = threadIdx.x % TP; s < S; s += TP) M = fmaxf(M, c.pml[(int64_t)s * pairs + at].x);
+  int used = 0;  // own splits with keys: the first ones
+  for (int s = tp; s < S; s += TP) {
+    const float2 e = c.pml[(int64_t)s * pairs + at];
+    M = fmaxf(M, e.x);
+    if (s < own && (e.x != -INFINITY || e.y != 0.f)) used = s + 1;
+  }
+  for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
 #pragma unroll
-  for (int o = TP / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, WAVE));
+  for (int o = TP / 2; o > 0; o >>= 1) {
+    M = fmaxf(M, __shfl_xor(M, o, WAVE));
+    used = max(used, __shfl_xor(used, o, WAVE));
+  }
   __syncthreads();
   if (pair >= pairs) return;
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
@@ -904,12 +1004,22 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict
   }
   const float mu = M == -INFINITY ? 0.f : M;
   float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < S; s0 += CB) {
-    if (s0 > 0) load(s0);
+  const int n = used + c.S_pre;
+  for (int s0 = 0; s0 < n; s0 += CB) {
+    float2 e[CB];
+    float4 u[CB][2];
+#pragma unroll
+    for (int k = 0; k < CB; ++k) {
+      const int s = min(s0 + k, n - 1);
+      const int64_t i = (int64_t)(s < used ? s : s - used + own) * pairs + at;
+      e[k] = c.pml[i];
+      u[k][0] = *(const float4*)(c.po + i * HD + d0);
+      u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
+    }
 #pragma unroll
     for (int k = 0; k < CB; ++k) {
       // a split without keys holds (-inf, 0) and no output
-      if (s0 + k >= S || (e[k].x == -INFINITY && e[k].y == 0.f)) continue;
+      if (s0 + k >= n || (e[k].x == -INFINITY && e[k].y == 0.f)) continue;
       const float a = exp2a(e[k].x - mu);
       L += a * e[k].y;
       o[0] += a * u[k][0].x; o[1] += a * u[k][0].y; o[2] += a * u[k][0].z; o[3] += a * u[k][0].w;
@@ -926,45 +1036,49 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict
 // fc_attn.hip's prefill kernel: 64 keys a step through two LDS stages filled
 // by direct loads, scores and outputs in registers.
 //
-// Workgroups: unit = (row x group, or group) x key split; all column blocks of
-// a unit on one XCD, whose L2 then holds its keys.
+// Workgroups: the items of the list, or, for the prefix, group x key split x
+// column block, all blocks of a split on one XCD, whose L2 then holds its keys.
 template <int HD>
 struct WideStage {
   uint4 k[2][HD / 16][64];  // [32-key tile][16-dim slice][lane]
   uint4 v[2][HD / 16][64];  // [32-key tile][2 (dim / 32) + key half][lane]
 };
 template <int HD>
-__global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_t* __restrict__ q,
-                                                       const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
-                                                       bf16_t* __restrict__ y, int pre, int nunit, int nblk) {
+struct WideLds {
+  WideStage<HD> stg[2];
+  int rng[4][2];
+};
+template <int HD, bool pre>
+__device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __restrict__ q,
+                                          const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
+                                          bf16_t* __restrict__ y, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
-  __shared__ WideStage<HD> stg[2];
-  __shared__ int rng[4][4];
-  static_assert(sizeof(stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
+  WideStage<HD>(&stg)[2] = lds.stg;
+  static_assert(sizeof(lds.stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int S = c.S_own + c.S_pre;
   if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
-  const int nul = (nunit + 7) >> 3, jj = blockIdx.x >> 3;
-  const int unit = (jj % nul) * 8 + (blockIdx.x & 7);
-  if (unit >= nunit) return;
-  const int c0 = (nblk - 1 - jj / nul) * 128, Sj = pre ? c.S_pre : c.S_own;  // a row's last columns see the most keys
-  const int ug = unit / Sj, split = unit - ug * Sj;
   const int rep = c.H / c.pv.G;
-  int b = 0, g = ug, base = 0, ncol;
-  if (pre) {
-    const int used = min(max(c.row_off[c.B], 0), c.Mcap);
-    ncol = used * rep;
-    if (c0 >= ncol) return;
+  Item it{0, 0, 0, 1, 0, c.pre_chunk};
+  int base = 0, ncol;
+  if constexpr (pre) {
+    const int nunit = c.pv.G * c.S_pre, nul = (nunit + 7) >> 3, jj = at >> 3;
+    const int unit = (jj % nul) * 8 + (at & 7);
+    if (unit >= nunit) return;
+    it.blk = jj / nul;
+    it.g = unit / c.S_pre;
+    it.split = unit - it.g * c.S_pre;
+    ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
+    if (it.blk * 128 >= ncol) return;
     int* off = (int*)stg;
     for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
     __syncthreads();
   } else {
-    b = ug / c.pv.G;
-    g = ug - b * c.pv.G;
-    const RowSpan sp = row_span(c.row_off, b, c.max_per_row, c.Mcap);
+    if (!find_item<128>(c, at, it)) return;
+    const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
     base = sp.base;
     ncol = sp.n * rep;
-    if (c0 >= ncol) return;
   }
+  const int b = it.b, g = it.g, c0 = it.blk * 128;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, kk = lane & 31;
   // this lane's column
@@ -996,30 +1110,31 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
   const int w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
   int w_hi = lanes_max<32>(lo_c <= hi_c ? hi_c : -1);
   if (lane == 0) {
-    rng[wave][0] = w_lo;
-    rng[wave][1] = w_hi;
+    lds.rng[wave][0] = w_lo;
+    lds.rng[wave][1] = w_hi;
   }
   __syncthreads();
   int g_lo = 0x7fffffff, g_hi = -1;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    g_lo = min(g_lo, rng[w][0]);
-    g_hi = max(g_hi, rng[w][1]);
+    g_lo = min(g_lo, lds.rng[w][0]);
+    g_hi = max(g_hi, lds.rng[w][1]);
   }
   g_lo = __builtin_amdgcn_readfirstlane(g_lo);
   g_hi = __builtin_amdgcn_readfirstlane(g_hi);
-  const int chunk = pre ? c.pre_chunk : c.S_own > 1 ? own_chunk(c, c.pv.G * nblk) : 0x7fffffc0;
   // (a row's splits are counted from its first column's first key in every one of its blocks)
   int row_lo = g_lo, unused;
-  if (!pre && c.window > 0 && Sj > 1) key_range(c, c.start[b], false, row_lo, unused);
-  const int64_t s_beg = (int64_t)(row_lo & ~31) + (int64_t)split * chunk;
-  const int64_t kend64 = min((int64_t)g_hi + 1, s_beg + chunk), kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
-  const int sg = pre ? c.S_own + split : split;
+  if (!pre && c.window > 0) key_range(c, c.start[b], false, row_lo, unused);
+  const int64_t s_beg = (int64_t)(row_lo & ~31) + (int64_t)it.split * it.chunk;
+  const int64_t kend64 = min((int64_t)g_hi + 1, s_beg + it.chunk), kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
+  const int sg = pre ? c.S_own + it.split : it.split;
   const bool none = kbeg64 >= kend64;
   if (none && S > 1) {
     if (threadIdx.x < 128 && c0 + threadIdx.x < ncol) {
       const int cx = c0 + threadIdx.x, jx = cx / rep;
-      c.pml[((int64_t)sg * c.Mcap + base + jx) * c.H + g * rep + cx - jx * rep] = make_float2(-INFINITY, 0.f);
+      const int64_t pair = (int64_t)(base + jx) * c.H + g * rep + cx - jx * rep;
+      c.pml[(int64_t)sg * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
+      if (!pre) mark_unused(c, it, pair);
     }
     return;
   }
@@ -1192,22 +1307,25 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
 #undef WIDE_ISSUE
   __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
   if (__syncthreads_or(odd)) {    // (also: the stages become scratch)
-    redo_columns<bf16_t, HD>(c, q, kp, vp, y, pre, b, g, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
+    redo_columns<bf16_t, HD>(c, q, kp, vp, y, pre, it, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
     return;
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
   // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
   if (S > 1) {
     if (ok) {
-      const int64_t at = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
-      float* po = c.po + at * HD + 4 * hl;
+      const int64_t slot = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
+      float* po = c.po + slot * HD + 4 * hl;
 #pragma unroll
       for (int dd = 0; dd < DD; ++dd)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
           *(float4*)(po + 32 * dd + 8 * i4) =
               make_float4(O[dd][4 * i4], O[dd][4 * i4 + 1], O[dd][4 * i4 + 2], O[dd][4 * i4 + 3]);
-      if (hl == 0) c.pml[at] = make_float2(m_run, l_tot);
+      if (hl == 0) {
+        c.pml[slot] = make_float2(m_run, l_tot);
+        if (!pre) mark_unused(c, it, (int64_t)(base + j) * c.H + head);
+      }
     }
   } else {
     // through LDS, so that a lane writes 8 dims of a column
@@ -1235,6 +1353,43 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedChunk c, const bf16_
   }
 }
 
+// The prefix (PRE: 16-column blocks of the streaming kernel, 0: the wide one,
+// -1: no prefix) and the rows' own keys in one launch: the first is bound by
+// the matrix cores where many rows share it, the second by memory, and each
+// hides the other's start and end. 256 workgroups of either in turn, so that a CU
+// holds one of each.
+template <typename T, int HD, int PRE, int OWN>
+__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedChunk c, const T* __restrict__ q,
+                                                       const T* __restrict__ kp, const T* __restrict__ vp,
+                                                       T* __restrict__ y, int npre, int nown) {
+  union Lds {
+    StreamLds<HD> s;
+    std::conditional_t<PRE == 0 || OWN == 0, WideLds<HD>, char> w;
+  };
+  __shared__ Lds lds;
+  int at = blockIdx.x;
+  if constexpr (PRE >= 0) {
+    const int both = min((npre + 255) >> 8, (nown + 255) >> 8);
+    bool pre;
+    if ((at >> 8) < 2 * both) {
+      pre = !((at >> 8) & 1);
+      at = ((at >> 9) << 8) | (at & 255);
+    } else {
+      at -= both << 8;
+      pre = npre > nown;
+    }
+    if (pre) {
+      if (at >= npre) return;
+      if constexpr (PRE == 0) wide_keys<HD, true>(c, q, kp, vp, y, lds.w, at);
+      else stream_keys<T, HD, PRE, true>(c, q, kp, vp, y, lds.s, at);
+      return;
+    }
+    if (at >= nown) return;
+  }
+  if constexpr (OWN == 0) wide_keys<HD, false>(c, q, kp, vp, y, lds.w, at);
+  else stream_keys<T, HD, OWN, false>(c, q, kp, vp, y, lds.s, at);
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -1247,19 +1402,21 @@ struct PagedPlan {
   bool mfma;
   int own_qb, own_blk, pre_qb, pre_blk;
   int S_own, S_pre, pre_chunk, target;
+  int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short
   int64_t part_bytes, ml_bytes;
 };
 // Key splits of the prefix: the time of the workgroups on their XCD (a unit's
 // column blocks share one; 64 run at once there, two a CU), a step of 64 keys
 // taking 2 us of two workgroups on a CU and 1.2 us of one, six steps' time for a
-// workgroup's start and end, and 4 TB/s for the partials (written and read).
+// workgroup's start and end, and 10 TB/s for the partials (written and read, from the
+// last cache).
 int pre_splits(int P, int G, int blk, int64_t part_bytes, int most) {
   int best = 1;
   double least = 1e30;
   for (int S = 1; S <= std::min(most, (P + 127) / 128); ++S) {
     const int64_t on = (int64_t)((G * S + 7) / 8) * blk, rounds = (on + 63) / 64;
     const double steps = (P / S + 63) / 64 + 6;
-    const double t = rounds * steps * (on > 32 ? 2.0 : 1.2) + S * (double)part_bytes * 2 / 4e6;
+    const double t = rounds * steps * (on > 32 ? 2.0 : 1.2) + S * (double)part_bytes * 2 / 10e6;
     if (t < least) least = t, best = S;
   }
   return best;
@@ -1282,8 +1439,11 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
   const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
-  a.target = a.own_qb ? 1024 : 512;
-  a.S_own = (int)std::min({(longest + 127) / 128, std::max<int64_t>(1, (a.own_qb ? 4 : 2) * a.target / units), room, (int64_t)128});
+  a.target = a.own_qb ? 768 : 256;
+  a.S_own = (int)std::min({(longest + 127) / 128, room, (int64_t)64});
+  // one split, and no merge, where every workgroup that fits the card has a row of its own and rows are short
+  if (P == 0 && units >= 512 && longest <= 1024) a.S_own = 1;
+  a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, units * longest / CHUNK_MAX);
   if (P > 0) {
     a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128));
     a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
@@ -1298,29 +1458,32 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
 }
 
 template <typename T, int HD>
-void launch_part(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, int pre,
-                 hipStream_t s) {
-  const int qb = pre ? a.pre_qb : a.own_qb, blk = pre ? a.pre_blk : a.own_blk, S = pre ? a.S_pre : a.S_own;
-  const int ug = pre ? c.pv.G : c.B * c.pv.G;
-  const T *qq = (const T*)q, *k = (const T*)p->k, *v = (const T*)p->v;
-  if constexpr (sizeof(T) == 2) {
-    if (qb == 2)
-      hipLaunchKernelGGL((k_paged_stream<T, HD, 2>), dim3(ug, blk, S), dim3(256), 0, s, c, qq, k, v, (T*)y, pre);
-    if (qb == 0)
-      hipLaunchKernelGGL(k_paged_wide<HD>, dim3((unsigned)(8 * ((ug * S + 7) / 8) * blk)), dim3(256), 0, s, c, qq, k,
-                         v, (T*)y, pre, ug * S, blk);
-  }
-  if (qb == 1)
-    hipLaunchKernelGGL((k_paged_stream<T, HD, 1>), dim3(ug, blk, S), dim3(256), 0, s, c, qq, k, v, (T*)y, pre);
-}
-
-template <typename T, int HD>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, hipStream_t s) {
-  if (a.S_pre > 0) {
-    launch_part<T, HD>(c, a, p, q, y, 1, s);
-    FC_LAUNCH_CHECK();
+  const int nown = (int)a.items;
+  const int npre = a.S_pre == 0 ? 0 : a.pre_qb ? c.pv.G * a.S_pre * a.pre_blk
+                                               : 8 * ((c.pv.G * a.S_pre + 7) / 8) * a.pre_blk;
+  const dim3 grid(npre == 0 ? nown : 256 * ((npre + 255) / 256 + (nown + 255) / 256));
+  const T *qq = (const T*)q, *k = (const T*)p->k, *v = (const T*)p->v;
+#define PAGED(PRE, OWN)                                                                                             \
+  hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN>), grid, dim3(256), 0, s, c, qq, k, v, (T*)y, npre, nown)
+  if constexpr (sizeof(T) == 4) {
+    if (npre == 0) PAGED(-1, 1);
+    else PAGED(1, 1);
+  } else if (npre == 0) {
+    if (a.own_qb == 1) PAGED(-1, 1);
+    else if (a.own_qb == 2) PAGED(-1, 2);
+    else PAGED(-1, 0);
+  } else if (a.own_qb == 0) {
+    PAGED(0, 0);
+  } else if (a.own_qb == 2) {
+    if (a.pre_qb == 2) PAGED(2, 2);
+    else PAGED(0, 2);
+  } else {
+    if (a.pre_qb == 1) PAGED(1, 1);
+    else if (a.pre_qb == 2) PAGED(2, 1);
+    else PAGED(0, 1);
   }
-  launch_part<T, HD>(c, a, p, q, y, 0, s);
+#undef PAGED
   FC_LAUNCH_CHECK();
   const int S = a.S_own + a.S_pre;
   if (S > 1) {
@@ -1362,10 +1525,9 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   FC_CHECK_ARG(width > 0 && (int64_t)width * pages->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
   // a launch's threads are counted in 32 bits along x, its workgroups in 16 along y
-  const int64_t own = (int64_t)batch * pages->n_kv_head * std::max(a.S_own, 1) * std::max(a.own_blk, 1);
   const int64_t pre = (int64_t)pages->n_kv_head * std::max(a.S_pre, 1) * std::max(a.pre_blk, 1);
   const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
-  FC_CHECK_ARG(std::max({own, pre, merge, (int64_t)max_tokens}) < (1 << 24) - 16, "too many tokens, rows or heads");
+  FC_CHECK_ARG(std::max({a.items + pre, merge, (int64_t)max_tokens}) < (1 << 24) - 16, "too many tokens, rows or heads");
   FC_CHECK_ARG(a.part_bytes == 0 || (work && work_bytes >= a.part_bytes + a.ml_bytes), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,

@@ -281,11 +281,12 @@ __device__ __forceinline__ int64_t v_elem(const PageView& pv, int id, int g, int
   return (int64_t)id * pv.vs + (int64_t)g * pv.page * pv.hd + (int64_t)(at >> 5) * 32 * pv.hd + d * 32 + (at & 31);
 }
 
+// Any head size and alignment: an element per thread.
 template <typename T, typename S>
-__global__ __launch_bounds__(256) void k_page_append(PageView pv, T* __restrict__ kp, T* __restrict__ vp,
-                                                     const S* __restrict__ k, const S* __restrict__ v, int64_t kst,
-                                                     int64_t ksh, int64_t vst, int64_t vsh,
-                                                     const int* __restrict__ slots, int M) {
+__global__ __launch_bounds__(256) void k_page_append_any(PageView pv, T* __restrict__ kp, T* __restrict__ vp,
+                                                         const S* __restrict__ k, const S* __restrict__ v, int64_t kst,
+                                                         int64_t ksh, int64_t vst, int64_t vsh,
+                                                         const int* __restrict__ slots, int M) {
   const int64_t per = (int64_t)pv.G * pv.hd;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * per; i += (int64_t)gridDim.x * 256) {
     const int m = (int)(i / per), r = (int)(i - m * per), g = r / pv.hd, d = r - g * pv.hd;
@@ -294,6 +295,126 @@ __global__ __launch_bounds__(256) void k_page_append(PageView pv, T* __restrict_
     const int id = slot / pv.page, at = slot - id * pv.page;
     st<T>(kp, k_elem(pv, id, g, at, d), ld<S>(k, m * kst + g * ksh + d));
     st<T>(vp, v_elem(pv, id, g, at, d), ld<S>(v, m * vst + g * vsh + d));
+  }
+}
+
+// 8 consecutive values as fp32, and back (rounded to nearest even)
+__device__ __forceinline__ void load8(const bf16_t* p, float (&x)[8]) {
+  const uint4 u = *(const uint4*)p;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+// 8 results of a row, times f
+__device__ __forceinline__ void store8(bf16_t* y, const float (&o)[8], float f) {
+  *(uint4*)y = uint4{pack2bf(o[0] * f, o[1] * f), pack2bf(o[2] * f, o[3] * f), pack2bf(o[4] * f, o[5] * f),
+                     pack2bf(o[6] * f, o[7] * f)};
+}
+__device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
+  ((float4*)y)[0] = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+  ((float4*)y)[1] = make_float4(o[4] * f, o[5] * f, o[6] * f, o[7] * f);
+}
+
+// About 32 tokens of one KV head per workgroup, 16 bytes per load and store.
+// K: 8 dims of a position are 16 bytes of its block; lanes are dealt so that the
+// positions next to each other in it are next to each other in the wave. V is
+// stored dim by dim: through LDS, and where 8 tokens fill an aligned run of 8
+// positions (a prompt's, save its ends) they are one store, element by element
+// elsewhere (2-byte stores to rows 64 bytes apart take a cycle per lane). Hence a
+// workgroup's tokens begin where a run of 8 does, if one is near. Bound by the
+// copy of K and V.
+#define PA_TILE 32
+#define PA_MOST (PA_TILE + 7)
+// First token of tile i: the first one from 32 i on that begins a run of 8
+// positions, or does not follow the one before it.
+__device__ __forceinline__ int append_from(const int* __restrict__ slots, int M, int i) {
+  const int64_t t = (int64_t)PA_TILE * i;
+  if (i == 0 || t >= M) return (int)min(t, (int64_t)M);
+  const int k = threadIdx.x & 7;
+  const int a = t + k < M ? slots[t + k] : -1, b = t + k - 1 < M ? slots[t + k - 1] : -1;
+  const uint64_t cut = __ballot(a < 0 || (a & 7) == 0 || a != b + 1);
+  return (int)t + __builtin_ctzll(cut);  // of 8 that follow each other one begins a run
+}
+
+template <typename T, typename S, bool KBLK>
+__global__ __launch_bounds__(256) void k_page_append(PageView pv, T* __restrict__ kp, T* __restrict__ vp,
+                                                     const S* __restrict__ k, const S* __restrict__ v, int64_t kst,
+                                                     int64_t ksh, int64_t vst, int64_t vsh,
+                                                     const int* __restrict__ slots, int M) {
+  extern __shared__ char lds[];  // the tile's V, [token][hd + pad]
+  __shared__ int s_slot[64], s_run[8], s_one[64], s_n[2];
+  const int g = blockIdx.y, tid = threadIdx.x, n8 = pv.hd >> 3, ldv = pv.hd + 2;
+  T* tv = (T*)lds;
+  const int t0 = append_from(slots, M, blockIdx.x), n = append_from(slots, M, blockIdx.x + 1) - t0;
+  if (n <= 0) return;
+  if (tid < 64) {
+    int slot = tid < n ? slots[t0 + tid] : -1;
+    if (slot < 0 || slot / pv.page >= pv.N) slot = -1;
+    s_slot[tid] = slot;
+    // runs of 8 positions whose tokens are all here, and the tokens outside them
+    uint64_t run = __ballot(slot >= 0 && (slot & 7) == 0), ok = __ballot(slot >= 0);
+    const uint64_t next = __ballot(slot >= 0 && slot == __shfl_up(slot, 1, WAVE) + 1);  // follows the lane before
+#pragma unroll
+    for (int i = 1; i < 8; ++i) run &= next >> i;
+    uint64_t in = run;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) in |= run << i;
+    const uint64_t below = (1ull << tid) - 1, one = ok & ~in;
+    if ((run >> tid) & 1) s_run[__popcll(run & below)] = tid;
+    if ((one >> tid) & 1) s_one[__popcll(one & below)] = tid;
+    if (tid == 0) {
+      s_n[0] = __popcll(run);
+      s_n[1] = __popcll(one);
+    }
+  }
+  for (int i = tid; i < n * n8; i += 256) {
+    const int t = i / n8, d = 8 * (i - t * n8);
+    float x[8];
+    load8(v + (t0 + t) * vst + g * vsh + d, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) st<T>(tv, t * ldv + d + e, x[e]);
+  }
+  __syncthreads();
+  // K: chunk i is 8 dims of a token; in the matrix-core order 16 lanes take every token of a half block
+  const int chunks = KBLK ? ((n + 31) >> 5) * 512 : n * n8;
+  for (int i = tid; i < chunks; i += 256) {
+    int t, d;
+    if constexpr (KBLK) {
+      const int r = i & 15;
+      t = 32 * (i >> 9) + 8 * (r >> 2) + (r & 3) + 4 * ((i >> 6) & 1);
+      d = 32 * ((i >> 7) & 3) + 8 * ((i >> 4) & 3);
+    } else {
+      t = i / n8;
+      d = 8 * (i - t * n8);
+    }
+    const int slot = t < n ? s_slot[t] : -1;
+    if (slot < 0) continue;
+    float x[8];
+    load8(k + (t0 + t) * kst + g * ksh + d, x);
+    const int id = slot / pv.page;
+    store8(kp + k_elem(pv, id, g, slot - id * pv.page, d), x, 1.f);
+  }
+  // V: four runs of a block side by side are a row of 64 bytes
+  const int nr = s_n[0], no = s_n[1];
+  for (int i = tid; i < ((nr + 3) & ~3) * pv.hd; i += 256) {
+    const int q = (i & 3) + 4 * (i / (4 * pv.hd)), d = (i >> 2) % pv.hd;
+    if (q >= nr) continue;
+    const int t = s_run[q], slot = s_slot[t], id = slot / pv.page;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ld<T>(tv, (t + e) * ldv + d);
+    store8(vp + v_elem(pv, id, g, slot - id * pv.page, d), x, 1.f);
+  }
+  for (int i = tid; i < no * pv.hd; i += 256) {
+    const int q = i / pv.hd, d = i - q * pv.hd, t = s_one[q], slot = s_slot[t], id = slot / pv.page;
+    st<T>(vp, v_elem(pv, id, g, slot - id * pv.page, d), ld<T>(tv, t * ldv + d));
   }
 }
 
@@ -309,14 +430,37 @@ extern "C" int32_t fc_page_append(const fc_pages* pages, const void* k, const vo
   FC_CHECK_ARG(k && v && slots, "null pointer");
   const PageView pv = page_view(pages);
   const hipStream_t s = (hipStream_t)stream;
+  const int per = src_dtype == FC_BF16 ? 8 : 4, per_page = pages->dtype == FC_BF16 ? 8 : 4;
+  const uintptr_t at = (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)k | (uintptr_t)v;
+  const int64_t strides = k_token_stride | k_head_stride | v_token_stride | v_head_stride;
+  const bool vec = (at & 15) == 0 && strides % per == 0 && (pages->k_stride | pages->v_stride) % per_page == 0 &&
+                   pv.hd % 8 == 0 && pv.G <= 65535;
+  const int tiles = (M + PA_TILE - 1) / PA_TILE;
   const int64_t n = (int64_t)M * pv.G * pv.hd;
-  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 65536));
-#define APPEND(T, S)                                                                                                 \
-  hipLaunchKernelGGL((k_page_append<T, S>), grid, dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, (const S*)k,      \
-                     (const S*)v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, M)
-  if (pages->dtype == FC_F32) APPEND(float, float);
-  else if (src_dtype == FC_F32) APPEND(bf16_t, float);
-  else APPEND(bf16_t, bf16_t);
+#define APPEND(T, S, KBLK)                                                                                           \
+  if (vec)                                                                                                           \
+    hipLaunchKernelGGL((k_page_append<T, S, KBLK>), dim3(tiles, pv.G), dim3(256), PA_MOST * (pv.hd + 2) * sizeof(T), \
+                       s, pv, (T*)pages->k, (T*)pages->v, (const S*)k, (const S*)v, k_token_stride, k_head_stride,   \
+                       v_token_stride, v_head_stride, slots, M);                                                     \
+  else                                                                                                               \
+    hipLaunchKernelGGL((k_page_append_any<T, S>), dim3((unsigned)std::min<int64_t>((n + 255) / 256, 65536)),         \
+                       dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, (const S*)k, (const S*)v, k_token_stride,    \
+                       k_head_stride, v_token_stride, v_head_stride, slots, M)
+  if (pages->dtype == FC_F32) {
+    APPEND(float, float, false);
+  } else if (src_dtype == FC_F32) {
+    if (pv.kblk) {
+      APPEND(bf16_t, float, true);
+    } else {
+      APPEND(bf16_t, float, false);
+    }
+  } else {
+    if (pv.kblk) {
+      APPEND(bf16_t, bf16_t, true);
+    } else {
+      APPEND(bf16_t, bf16_t, false);
+    }
+  }
 #undef APPEND
   FC_LAUNCH_CHECK();
   return FC_OK;
@@ -785,16 +929,6 @@ __device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile
     l_run += p[jj];
   }
   t.add(p, O);
-}
-
-// 8 results of a row
-__device__ __forceinline__ void store8(bf16_t* y, const float (&o)[8], float f) {
-  *(uint4*)y = uint4{pack2bf(o[0] * f, o[1] * f), pack2bf(o[2] * f, o[3] * f), pack2bf(o[4] * f, o[5] * f),
-                     pack2bf(o[6] * f, o[7] * f)};
-}
-__device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
-  ((float4*)y)[0] = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
-  ((float4*)y)[1] = make_float4(o[4] * f, o[5] * f, o[6] * f, o[7] * f);
 }
 
 // Few query columns (token, head in group), or fp32: a workgroup takes 16 QB of

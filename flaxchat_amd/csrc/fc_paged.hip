@@ -476,20 +476,50 @@ struct PagedChunk {
   int B, H, W, P, window, max_per_row, Mcap, flags;
   int64_t qst, qsh;  // query strides (elements): token, head
   float scale;
-  // key splits: their number over a row's own keys and over the prefix, keys per prefix split, workgroups that
-  // the own keys are to be spread over
+  // key splits: most of a row's own keys, of the prefix, keys of each of these; workgroups that the own keys are to
+  // be spread over
   int S_own, S_pre, pre_chunk, target;
   // partials of split s (the own ones first): po[(s Mcap + token) H + head][hd] unnormalised, pml (max, sum)
   float* po;
   float2* pml;
+  const void *q, *kp, *vp;
+  void* y;
 };
+
+// The chunk, read from the kernel's arguments (its first) at this point and not
+// kept from earlier. What is kept of it through a whole walk, with the constants
+// that the compiler makes of it for its divisions, is more than the scalar
+// registers hold, and a spill of theirs is not to be had here: a part of one came
+// back wrong (the lower half of a pointer), so the walks' kernels are to have none.
+template <typename P>
+__device__ __forceinline__ P* in_global(P* p) {
+  return (P*)(__attribute__((address_space(1))) P*)p;
+}
+__device__ __forceinline__ PagedChunk chunk_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  PagedChunk c;
+  __builtin_memcpy(&c, (const void*)p, sizeof(c));
+  c.tables = in_global(c.tables);
+  c.row_off = in_global(c.row_off);
+  c.start = in_global(c.start);
+  c.pre = in_global(c.pre);
+  c.po = in_global(c.po);
+  c.pml = in_global(c.pml);
+  c.q = in_global(c.q);
+  c.kp = in_global(c.kp);
+  c.vp = in_global(c.vp);
+  c.y = in_global(c.y);
+  return c;
+}
 
 // Any head size, type and alignment: one workgroup per (token, head), keys in
 // blocks of 256 (a thread scores one key, then sums one dimension), with the
 // running maximum and sum of the softmax.
 template <typename T>
-__global__ __launch_bounds__(256) void k_paged_any(PagedChunk c, const T* __restrict__ q, const T* __restrict__ kp,
-                                                   const T* __restrict__ vp, T* __restrict__ y) {
+__global__ __launch_bounds__(256) void k_paged_any(PagedChunk c) {
+  const T *q = (const T*)c.q, *kp = (const T*)c.kp, *vp = (const T*)c.vp;
+  T* y = (T*)c.y;
   __shared__ float qs[256], ps[256], red[16];
   const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, hd = c.pv.hd;
   T* yo = y + ((int64_t)t * c.H + h) * hd;
@@ -632,19 +662,12 @@ __device__ __forceinline__ void key_range(const PagedChunk& c, int64_t pos, bool
   lo = c.window > 0 ? (int)max((int64_t)0, min(pos - c.window - off, (int64_t)0x7fffffff)) : 0;
 }
 
-// The rows' own keys as a list of work items (row, column block, key split, KV
-// group), which every workgroup looks its own one up in, by its number: a row
-// has as many blocks of CB columns as its queries fill and as many splits as it
-// has chunks of keys. The chunk is what spreads all rows' keys over about
-// c.target items (rows are of unequal length: with a number of splits for all,
-// the longest row's would be left for last and the short rows' have nothing to
-// do), at least 128 keys (a tile for each of four waves), no more than
-// CHUNK_MAX (items of equal length, several rounds of them) and at least what
-// makes c.S_own splits of the longest row. Every wave reads all rows' lengths; the
-// list is the same in all of them.
-#define CHUNK_MAX 4096
+// A piece of work: a column block of row b (or, for the prefix, of all tokens)
+// and KV group g against `len` keys from `skip` keys on behind the 32-key block
+// of the row's first key; the `split`th of the block's nsplit pieces.
 struct Item {
-  int b, blk, split, nsplit, g, chunk;
+  int b, blk, g, split, nsplit, len;
+  int64_t skip;
 };
 // keys of row r's walk, from the 32-key block of its first query's first key; -1: no query
 __device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
@@ -656,6 +679,19 @@ __device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
   key_range(c, (int64_t)c.start[r] + sp.n - 1, false, lo1, hi1);
   return hi1 < lo ? 0 : hi1 + 1 - (lo & ~31);
 }
+
+// Rows are of unequal length: with a number of key splits for all, the longest
+// row's would be left for last and the short rows' have nothing to do. So the
+// rows' own keys are a list of items (row, column block, key split, KV group), cut
+// by one chunk length for all rows, and every workgroup looks its own one up, by
+// its number, from all rows' lengths (each wave reads them all; the result is the
+// same everywhere). The chunk is what spreads the keys over about c.target items,
+// at least 128 (a tile for each of four waves), no more than CHUNK_MAX (several
+// rounds of items: their times differ then) and at least what makes c.S_own
+// splits of the longest row. (One share of all keys for each workgroup that fits
+// the card, whatever rows it crosses, took 10-15% longer: a workgroup then waits
+// at every border, where two on a CU hide each other's.)
+#define CHUNK_MAX 4096
 template <int CB>
 __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
   const int lane = threadIdx.x & 63;
@@ -672,16 +708,16 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
   longest = lanes_max<64>(longest);
   const float share = ceilf(total * (float)c.pv.G / (float)c.target);
   const int least = max(128, (longest + c.S_own - 1) / c.S_own);
-  it.chunk = __builtin_amdgcn_readfirstlane((max((int)fminf(share, (float)CHUNK_MAX), least) + 63) & ~63);
-  const float per = 1.f / (float)it.chunk;
+  it.len = __builtin_amdgcn_readfirstlane((max((int)fminf(share, (float)CHUNK_MAX), least) + 63) & ~63);
+  const float per = 1.f / (float)it.len;
   for (int r0 = 0; r0 < c.B; r0 += 64) {
     if (c.B > 64) {
       len = r0 + lane < c.B ? row_keys(c, r0 + lane, ncol) : -1;
       if (len < 0) ncol = 0;
     }
-    int ns = (int)((float)max(len, 0) * per);  // len / chunk, one off at most
-    ns += ns * it.chunk < len;
-    ns = max(1, ns - ((ns - 1) * it.chunk >= len));
+    int ns = (int)((float)max(len, 0) * per);  // len / it.len, one off at most
+    ns += ns * it.len < len;
+    ns = max(1, ns - ((ns - 1) * it.len >= len));
     const int nb = (ncol + CB - 1) / CB, mine = len < 0 ? 0 : ns * nb * c.pv.G;
     const int upto = lanes_scan(mine);
     const uint64_t past = __ballot(upto > at);
@@ -697,6 +733,7 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
     at /= c.pv.G;
     it.split = at % it.nsplit;
     it.blk = at / it.nsplit;
+    it.skip = (int64_t)it.split * it.len;
     return true;
   }
   return false;
@@ -709,10 +746,12 @@ __device__ __forceinline__ void mark_unused(const PagedChunk& c, const Item& it,
 
 // Tokens past the last row: set to 0 by the launch's workgroups in turn.
 template <typename T>
-__device__ __forceinline__ void zero_tail(const PagedChunk& c, T* y, int wg, int nwg) {
+__device__ __forceinline__ void zero_tail(int wg, int nwg) {
+  const PagedChunk c = chunk_args();
+  if (c.S_own + c.S_pre > 1 || !(c.flags & FC_PAGED_ZERO_TAIL)) return;
   const int n8 = c.H * c.pv.hd * (int)sizeof(T) / 16;
   for (int64_t t = max(0, c.row_off[c.B]) + (int64_t)wg; t < c.Mcap; t += nwg)
-    for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)y)[t * n8 + i] = uint4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < n8; i += blockDim.x) ((uint4*)c.y)[t * n8 + i] = uint4{0u, 0u, 0u, 0u};
 }
 
 // The matrix product multiplies a key's V by the weight 0 of a column that
@@ -723,9 +762,12 @@ __device__ __forceinline__ void zero_tail(const PagedChunk& c, T* y, int wg, int
 // [kbeg, kend). (Anything done about them in the walk itself costs every call
 // registers, and spills.)
 template <typename T, int HD>
-__device__ __forceinline__ void redo_columns(const PagedChunk& c, const T* q, const T* kp, const T* vp, T* y,
-                                              bool pre, const Item& it, int base, int c_lo, int c_hi, int kbeg,
-                                             int kend, int sg, int wave) {
+__device__ __forceinline__ void redo_columns(bool pre, const Item& it, int base, int c_lo, int c_hi, int kbeg, int kend,
+                                             int wave) {
+  const PagedChunk c = chunk_args();
+  const T *q = (const T*)c.q, *kp = (const T*)c.kp, *vp = (const T*)c.vp;
+  T* y = (T*)c.y;
+  const int sg = pre ? c.S_own + it.split : it.split;
   const int lane = threadIdx.x & 63, rep = c.H / c.pv.G, b = it.b, g = it.g;
   const int* list = pre ? c.pre : c.tables + (int64_t)b * c.W;
   for (int col = c_lo + wave; col < c_hi; col += 4) {
@@ -935,95 +977,77 @@ __device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile
 // a row and KV group, or, for the prefix (`pre`), of all rows together, and one
 // key split; its four waves every fourth 32-key tile, straight from memory into
 // registers, each tile applied to all QB blocks of 16 columns, and are merged in
-// LDS. `at`: its number among the list's items, or the prefix's (group, split,
-// block).
+// LDS.
 template <int HD>
 struct StreamLds {
   float o[4][16][HD + 4];
   float m[4][16], l[4][16];
 };
 template <typename T, int HD, int QB, bool pre>
-__device__ __forceinline__ void stream_keys(const PagedChunk& c, const T* __restrict__ q, const T* __restrict__ kp,
-                                            const T* __restrict__ vp, T* __restrict__ y, StreamLds<HD>& lds, int at) {
+__device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& lds, const Item& it, int base,
+                                            int ncol) {
   constexpr int NW = 4, NT = 2 * HD;  // threads that own 8 dims of a column after the merge
-  static_assert(sizeof(lds) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int cl = lane & 15, g4 = lane >> 4, rep = c.H / c.pv.G;
-  const int S = c.S_own + c.S_pre;
-  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
-  Item it{0, 0, 0, 1, 0, c.pre_chunk};
-  int base = 0, ncol;
-  if constexpr (pre) {
-    it.g = at % c.pv.G;
-    at /= c.pv.G;
-    it.split = at % c.S_pre;
-    it.blk = at / c.S_pre;
-    ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
-    if (it.blk * 16 * QB >= ncol) return;
-    int* off = (int*)&lds;
-    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
-    __syncthreads();
-  } else {
-    if (!find_item<16 * QB>(c, at, it)) return;
-    const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
-    base = sp.base;
-    ncol = sp.n * rep;
-  }
+  const int cl = lane & 15, g4 = lane >> 4;
   const int b = it.b, g = it.g, col0 = it.blk * 16 * QB;
-  // this lane's columns
   typename Tile<T, HD>::Q qf[QB];
   int lo[QB], hi[QB];
   int w_lo = 0x7fffffff, w_hi = -1, f_lo = 0, f_hi = 0x7fffffff;
+  int64_t kbeg, kend;
+  {
+    const PagedChunk& c = w;
+    const int rep = c.H / c.pv.G;
+    // this lane's columns
 #pragma unroll
-  for (int u = 0; u < QB; ++u) {
-    const int col = col0 + 16 * u + cl;
-    bool ok = col < ncol;
-    const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
-    int64_t pos = 0;
-    if (pre) {
-      const int* off = (const int*)&lds;
-      const int r = row_of(off, c.B, j);
-      RowSpan sp{0, 0};
-      if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
-      ok = ok && j >= sp.base && j < sp.base + sp.n;
-      pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
-    } else {
-      pos = (int64_t)c.start[b] + j;
+    for (int u = 0; u < QB; ++u) {
+      const int col = col0 + 16 * u + cl;
+      bool ok = col < ncol;
+      const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
+      int64_t pos = 0;
+      if (pre) {
+        const int* off = (const int*)&lds;
+        const int r = row_of(off, c.B, j);
+        RowSpan sp{0, 0};
+        if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
+        ok = ok && j >= sp.base && j < sp.base + sp.n;
+        pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+      } else {
+        pos = (int64_t)c.start[b] + j;
+      }
+      key_range(c, pos, pre, lo[u], hi[u]);
+      if (!ok) lo[u] = 0x7fffffff, hi[u] = -1;
+      const bool some = lo[u] <= hi[u];  // columns that see nothing do not widen the range
+      w_lo = min(w_lo, some ? lo[u] : 0x7fffffff);
+      w_hi = max(w_hi, some ? hi[u] : -1);
+      f_lo = max(f_lo, ok ? lo[u] : 0);
+      f_hi = min(f_hi, ok ? hi[u] : 0x7fffffff);
+      qf[u].load((const T*)c.q + (base + j) * c.qst + head * c.qsh, g4, ok);
     }
-    key_range(c, pos, pre, lo[u], hi[u]);
-    if (!ok) lo[u] = 0x7fffffff, hi[u] = -1;
-    const bool some = lo[u] <= hi[u];  // columns that see nothing do not widen the range
-    w_lo = min(w_lo, some ? lo[u] : 0x7fffffff);
-    w_hi = max(w_hi, some ? hi[u] : -1);
-    f_lo = max(f_lo, ok ? lo[u] : 0);
-    f_hi = min(f_hi, ok ? hi[u] : 0x7fffffff);
-    qf[u].load(q + (base + j) * c.qst + head * c.qsh, g4, ok);
+    w_lo = lanes_min<16>(w_lo);
+    w_hi = lanes_max<16>(w_hi);
+    f_lo = lanes_max<16>(f_lo);
+    f_hi = lanes_min<16>(f_hi);
+    // (a row's splits are counted from its first column's first key in every one of its blocks)
+    int from = w_lo, unused;
+    if (!pre && c.window > 0) key_range(c, c.start[b], false, from, unused);
+    const int64_t s_beg = (int64_t)(from & ~31) + it.skip;
+    kbeg = max(s_beg, (int64_t)(w_lo & ~31));
+    kend = min((int64_t)w_hi + 1, s_beg + it.len);
   }
-  w_lo = lanes_min<16>(w_lo);
-  w_hi = lanes_max<16>(w_hi);
-  f_lo = lanes_max<16>(f_lo);
-  f_hi = lanes_min<16>(f_hi);
-  // (a row's splits are counted from its first column's first key in every one of its blocks)
-  int from = w_lo, unused;
-  if (!pre && c.window > 0) key_range(c, c.start[b], false, from, unused);
-  const int64_t s_beg = (int64_t)(from & ~31) + (int64_t)it.split * it.chunk;
-  const int64_t kbeg = max(s_beg, (int64_t)(w_lo & ~31)), kend = min((int64_t)w_hi + 1, s_beg + it.chunk);
-  const int sg = pre ? c.S_own + it.split : it.split;
-  if (kbeg >= kend && S > 1) {
-    const int col = col0 + threadIdx.x;
+  if (kbeg >= kend && w.S_own + w.S_pre > 1) {
+    const int col = col0 + threadIdx.x, rep = w.H / w.pv.G;
     if (threadIdx.x < 16 * QB && col < ncol) {
-      const int j = col / rep, head = g * rep + col - j * rep;
-      const int64_t pair = (int64_t)(base + j) * c.H + head;
-      c.pml[(int64_t)sg * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
-      if (!pre) mark_unused(c, it, pair);
+      const int j = col / rep;
+      const int64_t pair = (int64_t)(base + j) * w.H + g * rep + col - j * rep;
+      w.pml[(int64_t)(pre ? w.S_own + it.split : it.split) * w.Mcap * w.H + pair] = make_float2(-INFINITY, 0.f);
+      if (!pre) mark_unused(w, it, pair);
     }
     return;
   }
-
-  const float scale_log2 = c.scale * 1.4426950408889634f;
-  const int tpp = c.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
-  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
-  const int64_t gofs = (int64_t)g * c.pv.page * HD;
+  const float scale_log2 = w.scale * 1.4426950408889634f;
+  const int tpp = w.pv.page >> 5, tend = kbeg >= kend ? 0 : (int)((kend + 31) >> 5);
+  const const_ints list = CONST_INTS(pre ? w.pre : w.tables + (int64_t)b * w.W);
+  const int64_t gofs = (int64_t)g * w.pv.page * HD;
   int tile = (int)(min(kbeg, (int64_t)w_hi + 1) >> 5) + wave;
   int pg = tile / tpp, r = tile - pg * tpp;
   float m_run[QB], l_run[QB];
@@ -1044,19 +1068,20 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, const T* __rest
     r += NW;
     while (r >= tpp) r -= tpp, ++pg;
     id = tile < tend ? list[pg] : -1;
-    if ((unsigned)id0 >= (unsigned)c.pv.N) continue;
+    if ((unsigned)id0 >= (unsigned)w.pv.N) continue;
     Tile<T, HD> t;
-    t.load(kp + (int64_t)id0 * c.pv.ks + gofs + r0 * (32 * HD), vp + (int64_t)id0 * c.pv.vs + gofs + r0 * (32 * HD), lane);
+    t.load((const T*)w.kp + (int64_t)id0 * w.pv.ks + gofs + r0 * (32 * HD), (const T*)w.vp + (int64_t)id0 * w.pv.vs + gofs + r0 * (32 * HD), lane);
     if (!(kb >= f_lo && kb + 31 <= f_hi)) odd |= t.clear(w_lo - kb - 8 * g4, w_hi - kb - 8 * g4);
 #pragma unroll
     for (int u = 0; u < QB; ++u)
       tile16<T, HD>(t, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
   }
   if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
-    redo_columns<T, HD>(c, q, kp, vp, y, pre, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend),
-                        (int)kend, sg, wave);
+    redo_columns<T, HD>(pre, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend), (int)kend, wave);
     return;
   }
+  const PagedChunk c = chunk_args();
+  const int rep = c.H / c.pv.G, S = c.S_own + c.S_pre, sg = pre ? c.S_own + it.split : it.split;
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     if (col0 + 16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
@@ -1085,7 +1110,7 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, const T* __rest
         }
         const int j = col / rep, head = g * rep + col - j * rep;
         if (S == 1) {
-          store8(y + ((int64_t)(base + j) * c.H + head) * HD + d0, o, L == 0.f ? 0.f : 1.f / L);
+          store8((T*)c.y + ((int64_t)(base + j) * c.H + head) * HD + d0, o, L == 0.f ? 0.f : 1.f / L);
         } else {
           const int64_t slot = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
           float4* po = (float4*)(c.po + slot * HD + d0);
@@ -1101,12 +1126,38 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, const T* __rest
   }
 }
 
+// The workgroup numbered `at`: an item of the list, or a split of the prefix.
+template <typename T, int HD, int QB, bool pre>
+__device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& lds, int at) {
+  Item it;
+  int base = 0, ncol;
+  if constexpr (pre) {
+    static_assert(sizeof(lds) >= (PT_ROWS + 1) * 4, "the rows' offsets");
+    it = Item{0, 0, at % c.pv.G, 0, 1, c.pre_chunk, 0};
+    at /= c.pv.G;
+    it.split = at % c.S_pre;
+    it.blk = at / c.S_pre;
+    it.skip = (int64_t)it.split * it.len;
+    ncol = min(max(c.row_off[c.B], 0), c.Mcap) * (c.H / c.pv.G);
+    if (it.blk * 16 * QB >= ncol) return;
+    int* off = (int*)&lds;
+    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+    __syncthreads();
+  } else {
+    if (!find_item<16 * QB>(c, at, it)) return;
+    const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
+    base = sp.base;
+    ncol = sp.n * (c.H / c.pv.G);
+  }
+  stream_item<T, HD, QB, pre>(c, lds, it, base, ncol);
+}
+
 // Merge of the key splits of one (token, head), HD / 8 threads with 8
 // dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
 // splits' (max, sum) are read side by side, ahead of the token's row; then the
 // outputs of those that hold keys, CB at a time.
 template <typename T, int HD, int CB>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict__ y) {
+__global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
   __shared__ int off[PT_ROWS + 1];
   constexpr int TP = HD / 8;
   const int64_t pair = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP, pairs = (int64_t)c.Mcap * c.H;
@@ -1130,7 +1181,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c, T* __restrict
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
   RowSpan sp{0, 0};
   if (b < c.B) sp = row_span(off, b, c.max_per_row, c.Mcap);
-  T* yo = y + pair * HD + d0;
+  T* yo = (T*)c.y + pair * HD + d0;
   if (t < sp.base || t >= sp.base + sp.n) {
     if ((c.flags & FC_PAGED_ZERO_TAIL) && t >= off[c.B])
       store8(yo, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, 1.f);
@@ -1183,92 +1234,96 @@ struct WideLds {
   int rng[4][2];
 };
 template <int HD, bool pre>
-__device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __restrict__ q,
-                                          const bf16_t* __restrict__ kp, const bf16_t* __restrict__ vp,
-                                          bf16_t* __restrict__ y, WideLds<HD>& lds, int at) {
+__device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
   WideStage<HD>(&stg)[2] = lds.stg;
   static_assert(sizeof(lds.stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
-  const int S = c.S_own + c.S_pre;
-  if (S == 1 && (c.flags & FC_PAGED_ZERO_TAIL)) zero_tail(c, y, blockIdx.x, gridDim.x);
-  const int rep = c.H / c.pv.G;
-  Item it{0, 0, 0, 1, 0, c.pre_chunk};
-  int base = 0, ncol;
-  if constexpr (pre) {
-    const int nunit = c.pv.G * c.S_pre, nul = (nunit + 7) >> 3, jj = at >> 3;
-    const int unit = (jj % nul) * 8 + (at & 7);
-    if (unit >= nunit) return;
-    it.blk = jj / nul;
-    it.g = unit / c.S_pre;
-    it.split = unit - it.g * c.S_pre;
-    ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
-    if (it.blk * 128 >= ncol) return;
-    int* off = (int*)stg;
-    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
-    __syncthreads();
-  } else {
-    if (!find_item<128>(c, at, it)) return;
-    const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
-    base = sp.base;
-    ncol = sp.n * rep;
-  }
-  const int b = it.b, g = it.g, c0 = it.blk * 128;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, kk = lane & 31;
-  // this lane's column
-  const int col = c0 + 32 * wave + kk;
-  bool ok = col < ncol;
-  const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
-  int64_t pos = 0;
-  if (pre) {
-    const int* off = (const int*)stg;
-    const int r = row_of(off, c.B, j);
-    RowSpan sp{0, 0};
-    if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
-    ok = ok && j >= sp.base && j < sp.base + sp.n;
-    pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
-  } else {
-    pos = (int64_t)c.start[b] + j;
-  }
+  Item it;
+  int base = 0, ncol, lo_c, hi_c, w_lo, w_hi;
+  int64_t kbeg64, kend64;
+  bool ok;
   v4u qf[DS];  // dims 16 h + 8 hl .. +7 of this lane's query
   {
-    const bf16_t* qr = q + (base + j) * c.qst + head * c.qsh + 8 * hl;
-    const uint32_t keep = ok ? 0xffffffffu : 0u;
+    const PagedChunk& c = w;
+    const int rep = c.H / c.pv.G;
+    it = Item{0, 0, 0, 0, 1, c.pre_chunk, 0};
+    if constexpr (pre) {
+      const int nunit = c.pv.G * c.S_pre, nul = (nunit + 7) >> 3, jj = at >> 3;
+      const int unit = (jj % nul) * 8 + (at & 7);
+      if (unit >= nunit) return;
+      it.blk = jj / nul;
+      it.g = unit / c.S_pre;
+      it.split = unit - it.g * c.S_pre;
+      it.skip = (int64_t)it.split * it.len;
+      ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
+      if (it.blk * 128 >= ncol) return;
+      int* off = (int*)stg;
+      for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+      __syncthreads();
+    } else {
+      if (!find_item<128>(c, at, it)) return;
+      const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
+      base = sp.base;
+      ncol = sp.n * rep;
+    }
+    const int c0 = it.blk * 128;
+    // this lane's column
+    const int col = c0 + 32 * wave + kk;
+    ok = col < ncol;
+    const int j = ok ? col / rep : 0, head = it.g * rep + (ok ? col - j * rep : 0);
+    int64_t pos = 0;
+    if (pre) {
+      const int* off = (const int*)stg;
+      const int r = row_of(off, c.B, j);
+      RowSpan sp{0, 0};
+      if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
+      ok = ok && j >= sp.base && j < sp.base + sp.n;
+      pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+    } else {
+      pos = (int64_t)c.start[it.b] + j;
+    }
+    {
+      const bf16_t* qr = (const bf16_t*)c.q + (base + j) * c.qst + head * c.qsh + 8 * hl;
+      const uint32_t keep = ok ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int h = 0; h < DS; ++h) qf[h] = *(const v4u*)(qr + 16 * h) & keep;
-  }
-  int lo_c, hi_c;
-  key_range(c, pos, pre, lo_c, hi_c);
-  if (!ok) lo_c = 0x7fffffff, hi_c = -1;
-  // the keys that some column of the workgroup sees
-  const int w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
-  int w_hi = lanes_max<32>(lo_c <= hi_c ? hi_c : -1);
-  if (lane == 0) {
-    lds.rng[wave][0] = w_lo;
-    lds.rng[wave][1] = w_hi;
-  }
-  __syncthreads();
-  int g_lo = 0x7fffffff, g_hi = -1;
+      for (int h = 0; h < DS; ++h) qf[h] = *(const v4u*)(qr + 16 * h) & keep;
+    }
+    key_range(c, pos, pre, lo_c, hi_c);
+    if (!ok) lo_c = 0x7fffffff, hi_c = -1;
+    // the keys that some column of the workgroup sees
+    w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
+    w_hi = lanes_max<32>(lo_c <= hi_c ? hi_c : -1);
+    if (lane == 0) {
+      lds.rng[wave][0] = w_lo;
+      lds.rng[wave][1] = w_hi;
+    }
+    __syncthreads();
+    int g_lo = 0x7fffffff, g_hi = -1;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    g_lo = min(g_lo, lds.rng[w][0]);
-    g_hi = max(g_hi, lds.rng[w][1]);
+    for (int w = 0; w < 4; ++w) {
+      g_lo = min(g_lo, lds.rng[w][0]);
+      g_hi = max(g_hi, lds.rng[w][1]);
+    }
+    g_lo = __builtin_amdgcn_readfirstlane(g_lo);
+    g_hi = __builtin_amdgcn_readfirstlane(g_hi);
+    // (a row's splits are counted from its first column's first key in every one of its blocks)
+    int row_lo = g_lo, unused;
+    if (!pre && c.window > 0) key_range(c, c.start[it.b], false, row_lo, unused);
+    const int64_t s_beg = (int64_t)(row_lo & ~31) + it.skip;
+    kend64 = min((int64_t)g_hi + 1, s_beg + it.len);
+    kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
   }
-  g_lo = __builtin_amdgcn_readfirstlane(g_lo);
-  g_hi = __builtin_amdgcn_readfirstlane(g_hi);
-  // (a row's splits are counted from its first column's first key in every one of its blocks)
-  int row_lo = g_lo, unused;
-  if (!pre && c.window > 0) key_range(c, c.start[b], false, row_lo, unused);
-  const int64_t s_beg = (int64_t)(row_lo & ~31) + (int64_t)it.split * it.chunk;
-  const int64_t kend64 = min((int64_t)g_hi + 1, s_beg + it.chunk), kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
-  const int sg = pre ? c.S_own + it.split : it.split;
+  const int b = it.b, g = it.g, c0 = it.blk * 128;
   const bool none = kbeg64 >= kend64;
-  if (none && S > 1) {
-    if (threadIdx.x < 128 && c0 + threadIdx.x < ncol) {
-      const int cx = c0 + threadIdx.x, jx = cx / rep;
-      const int64_t pair = (int64_t)(base + jx) * c.H + g * rep + cx - jx * rep;
-      c.pml[(int64_t)sg * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
-      if (!pre) mark_unused(c, it, pair);
+  if (none && w.S_own + w.S_pre > 1) {
+    const int cx = c0 + threadIdx.x, rep = w.H / w.pv.G;
+    if (threadIdx.x < 128 && cx < ncol) {
+      const int jx = cx / rep;
+      const int64_t pair = (int64_t)(base + jx) * w.H + g * rep + cx - jx * rep;
+      w.pml[(int64_t)(pre ? w.S_own + it.split : it.split) * w.Mcap * w.H + pair] = make_float2(-INFINITY, 0.f);
+      if (!pre) mark_unused(w, it, pair);
     }
     return;
   }
@@ -1283,10 +1338,10 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __r
   const uint32_t koff = HD == 128 ? 16u * (uint32_t)((((key >> 2) & 1) << 6) + ((key >> 3) << 2) + (key & 3) + 16 * hl)
                                   : (uint32_t)(key * (2 * HD) + 16 * hl);
   const uint32_t voff = 16u * (uint32_t)(4 * kk + hl);
-  const int64_t gofs = (int64_t)g * c.pv.page * HD;
-  const float scale_log2 = c.scale * 1.4426950408889634f;
-  const int tpp = c.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
-  const const_ints list = CONST_INTS(pre ? c.pre : c.tables + (int64_t)b * c.W);
+  const int64_t gofs = (int64_t)g * w.pv.page * HD;
+  const float scale_log2 = w.scale * 1.4426950408889634f;
+  const int tpp = w.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
+  const const_ints list = CONST_INTS(pre ? w.pre : w.tables + (int64_t)b * w.W);
   f32x16 O[DD];
 #pragma unroll
   for (int dd = 0; dd < DD; ++dd)
@@ -1302,11 +1357,11 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __r
 #define WIDE_ISSUE(S_)                                                                                       \
   next = 0;                                                                                                  \
   _Pragma("unroll") for (int u = 0; u < 2; ++u) {                                                            \
-    const bool is = (unsigned)id < (unsigned)c.pv.N;                                                         \
+    const bool is = (unsigned)id < (unsigned)w.pv.N;                                                         \
     next |= (int)is << u;                                                                                    \
     const int64_t pid = is ? id : 0; /* no page: page 0's place is read and masked */                        \
-    const bf16_t* kt = kp + pid * c.pv.ks + gofs + tr * (32 * HD);                                           \
-    const bf16_t* vt = vp + pid * c.pv.vs + gofs + tr * (32 * HD);                                           \
+    const bf16_t* kt = (const bf16_t*)w.kp + pid * w.pv.ks + gofs + tr * (32 * HD);                          \
+    const bf16_t* vt = (const bf16_t*)w.vp + pid * w.pv.vs + gofs + tr * (32 * HD);                          \
     if constexpr (HD == 128) {                                                                               \
       const uint32_t lk = LDS_ADDR(S_.k[u][0]) + 2048 * wave, lv = LDS_ADDR(S_.v[u][0]) + 2048 * wave;       \
       lds_load_1k(kt + 1024 * wave, koff, lk);                                                               \
@@ -1441,9 +1496,12 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __r
 #undef WIDE_ISSUE
   __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
   if (__syncthreads_or(odd)) {    // (also: the stages become scratch)
-    redo_columns<bf16_t, HD>(c, q, kp, vp, y, pre, it, base, c0, min(c0 + 128, ncol), t0, kend, sg, wave);
+    redo_columns<bf16_t, HD>(pre, it, base, c0, min(c0 + 128, ncol), t0, kend, wave);
     return;
   }
+  const PagedChunk c = chunk_args();
+  const int rep = c.H / c.pv.G, S = c.S_own + c.S_pre, sg = pre ? c.S_own + it.split : it.split;
+  const int col = c0 + 32 * wave + kk, j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
   // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
   if (S > 1) {
@@ -1482,7 +1540,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __r
     for (int it = 0; it < 32 / CP; ++it) {
       const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * wave + cc, jo = co / rep;
       const uint4 val = *(const uint4*)(T + cc * LD + d0);
-      if (co < ncol) *(uint4*)(y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
+      if (co < ncol) *(uint4*)((bf16_t*)c.y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
     }
   }
 }
@@ -1493,15 +1551,14 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& c, const bf16_t* __r
 // hides the other's start and end. 256 workgroups of either in turn, so that a CU
 // holds one of each.
 template <typename T, int HD, int PRE, int OWN>
-__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedChunk c, const T* __restrict__ q,
-                                                       const T* __restrict__ kp, const T* __restrict__ vp,
-                                                       T* __restrict__ y, int npre, int nown) {
+__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedChunk c, int npre, int nown) {
   union Lds {
     StreamLds<HD> s;
     std::conditional_t<PRE == 0 || OWN == 0, WideLds<HD>, char> w;
   };
   __shared__ Lds lds;
   int at = blockIdx.x;
+  if constexpr (PRE < 0) zero_tail<T>(blockIdx.x, gridDim.x);
   if constexpr (PRE >= 0) {
     const int both = min((npre + 255) >> 8, (nown + 255) >> 8);
     bool pre;
@@ -1514,14 +1571,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedChunk c, const T* __
     }
     if (pre) {
       if (at >= npre) return;
-      if constexpr (PRE == 0) wide_keys<HD, true>(c, q, kp, vp, y, lds.w, at);
-      else stream_keys<T, HD, PRE, true>(c, q, kp, vp, y, lds.s, at);
+      if constexpr (PRE == 0) wide_keys<HD, true>(c, lds.w, at);
+      else stream_keys<T, HD, PRE, true>(c, lds.s, at);
       return;
     }
     if (at >= nown) return;
   }
-  if constexpr (OWN == 0) wide_keys<HD, false>(c, q, kp, vp, y, lds.w, at);
-  else stream_keys<T, HD, OWN, false>(c, q, kp, vp, y, lds.s, at);
+  const PagedChunk o = PRE >= 0 ? chunk_args() : c;
+  if constexpr (OWN == 0) wide_keys<HD, false>(o, lds.w, at);
+  else stream_keys<T, HD, OWN, false>(o, lds.s, at);
 }
 
 // ---------------------------------------------------------------------------
@@ -1573,10 +1631,11 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
   const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
-  a.target = a.own_qb ? 768 : 256;
   a.S_own = (int)std::min({(longest + 127) / 128, room, (int64_t)64});
-  // one split, and no merge, where every workgroup that fits the card has a row of its own and rows are short
-  if (P == 0 && units >= 512 && longest <= 1024) a.S_own = 1;
+  // short rows without a prefix: one split, and no merge (one row of 640 keys, 6 heads: one launch of 10.6 us, or 6.8
+  // and 3.4 with the gap between them; 17 us or 21 from one call to the next)
+  if (P == 0 && longest <= 1024) a.S_own = 1;
+  a.target = a.own_qb ? 768 : 256;
   a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, units * longest / CHUNK_MAX);
   if (P > 0) {
     a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128));
@@ -1592,14 +1651,13 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
 }
 
 template <typename T, int HD>
-int launch_mfma(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, const void* q, void* y, hipStream_t s) {
+int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   const int nown = (int)a.items;
   const int npre = a.S_pre == 0 ? 0 : a.pre_qb ? c.pv.G * a.S_pre * a.pre_blk
                                                : 8 * ((c.pv.G * a.S_pre + 7) / 8) * a.pre_blk;
   const dim3 grid(npre == 0 ? nown : 256 * ((npre + 255) / 256 + (nown + 255) / 256));
-  const T *qq = (const T*)q, *k = (const T*)p->k, *v = (const T*)p->v;
 #define PAGED(PRE, OWN)                                                                                             \
-  hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN>), grid, dim3(256), 0, s, c, qq, k, v, (T*)y, npre, nown)
+  hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN>), grid, dim3(256), 0, s, c, npre, nown)
   if constexpr (sizeof(T) == 4) {
     if (npre == 0) PAGED(-1, 1);
     else PAGED(1, 1);
@@ -1623,9 +1681,9 @@ int launch_mfma(const PagedChunk& c, const PagedPlan& a, const fc_pages* p, cons
   if (S > 1) {
     const int64_t threads = (int64_t)c.Mcap * c.H * (HD / 8);
     const dim3 grid((unsigned)((threads + 255) / 256));
-    if (S <= 2) hipLaunchKernelGGL((k_paged_merge<T, HD, 2>), grid, dim3(256), 0, s, c, (T*)y);
-    else if (S <= 4) hipLaunchKernelGGL((k_paged_merge<T, HD, 4>), grid, dim3(256), 0, s, c, (T*)y);
-    else hipLaunchKernelGGL((k_paged_merge<T, HD, 8>), grid, dim3(256), 0, s, c, (T*)y);
+    if (S <= 2) hipLaunchKernelGGL((k_paged_merge<T, HD, 2>), grid, dim3(256), 0, s, c);
+    else if (S <= 4) hipLaunchKernelGGL((k_paged_merge<T, HD, 4>), grid, dim3(256), 0, s, c);
+    else hipLaunchKernelGGL((k_paged_merge<T, HD, 8>), grid, dim3(256), 0, s, c);
     FC_LAUNCH_CHECK();
   }
   return FC_OK;
@@ -1661,12 +1719,12 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   // a launch's threads are counted in 32 bits along x, its workgroups in 16 along y
   const int64_t pre = (int64_t)pages->n_kv_head * std::max(a.S_pre, 1) * std::max(a.pre_blk, 1);
   const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
-  FC_CHECK_ARG(std::max({a.items + pre, merge, (int64_t)max_tokens}) < (1 << 24) - 16, "too many tokens, rows or heads");
+  FC_CHECK_ARG(std::max({a.items + pre, merge, (int64_t)max_tokens}) < (1 << 24) - 1024, "too many tokens, rows or heads");
   FC_CHECK_ARG(a.part_bytes == 0 || (work && work_bytes >= a.part_bytes + a.ml_bytes), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
                1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, (float*)work,
-               (float2*)((char*)work + a.part_bytes)};
+               (float2*)((char*)work + a.part_bytes), q, pages->k, pages->v, y};
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;
@@ -1674,17 +1732,15 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
                        0 && (strides & (pages->dtype == FC_BF16 ? 7 : 3)) == 0;
   if (a.mfma && vec) {
     if (pages->dtype == FC_BF16)
-      return pages->head_dim == 128 ? launch_mfma<bf16_t, 128>(c, a, pages, q, y, s)
-                                    : launch_mfma<bf16_t, 64>(c, a, pages, q, y, s);
-    return pages->head_dim == 128 ? launch_mfma<float, 128>(c, a, pages, q, y, s)
-                                  : launch_mfma<float, 64>(c, a, pages, q, y, s);
+      return pages->head_dim == 128 ? launch_mfma<bf16_t, 128>(c, a, s)
+                                    : launch_mfma<bf16_t, 64>(c, a, s);
+    return pages->head_dim == 128 ? launch_mfma<float, 128>(c, a, s)
+                                  : launch_mfma<float, 64>(c, a, s);
   }
   if (pages->dtype == FC_BF16)
-    hipLaunchKernelGGL(k_paged_any<bf16_t>, dim3(max_tokens, n_head), dim3(256), 0, s, c, (const bf16_t*)q,
-                       (const bf16_t*)pages->k, (const bf16_t*)pages->v, (bf16_t*)y);
+    hipLaunchKernelGGL(k_paged_any<bf16_t>, dim3(max_tokens, n_head), dim3(256), 0, s, c);
   else
-    hipLaunchKernelGGL(k_paged_any<float>, dim3(max_tokens, n_head), dim3(256), 0, s, c, (const float*)q,
-                       (const float*)pages->k, (const float*)pages->v, (float*)y);
+    hipLaunchKernelGGL(k_paged_any<float>, dim3(max_tokens, n_head), dim3(256), 0, s, c);
   FC_LAUNCH_CHECK();
   return FC_OK;
 }

@@ -479,21 +479,25 @@ def _op(schema: str):
 def _on_gpu(name: str, first: torch.Tensor, *rest: torch.Tensor) -> int:
     """The index of the CUDA device that all tensors are on."""
     d = first.get_device()
-    if d < 0:
-        raise ValueError(f"{name}: tensors live on a CUDA device (got {first.device})")
     for t in rest:
         if t.get_device() != d:
             raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+    if d < 0:
+        raise ValueError(f"{name}: tensors live on a CUDA device (got {first.device})")
     return d
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone: a tenth of current_stream's time
 
 
 def _launch(name: str, device: int, fn, *args):
     """fn(*args, stream) on `device`'s current stream, with that device current."""
+    s = _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
     if device == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, s)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, s)
     if rc != 0:
         check(rc, name)
 
@@ -508,7 +512,8 @@ def _inner_contiguous(t: torch.Tensor) -> bool:
     return True
 
 
-def _pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> _lib.FcPages:
+def _pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """(fc_pages, n_kv_head, page, head_dim) of a pool."""
     if k_pages.dim() != 4:
         raise ValueError(f"{name}: k_pages [n_pages][n_kv_head][page][head_dim] (got {tuple(k_pages.shape)})")
     N, G, page, hd = k_pages.shape
@@ -516,15 +521,19 @@ def _pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> _lib.FcPa
         raise ValueError(f"{name}: page must be a multiple of 32 (got {page})")
     if N < 1 or G < 1 or not 1 <= hd <= 256:
         raise ValueError(f"{name}: n_pages, n_kv_head and head_dim (at most 256) must be positive")
-    if tuple(v_pages.shape) != (N, G, page // 32, hd, 32):
+    if v_pages.shape != (N, G, page // 32, hd, 32):
         raise ValueError(f"{name}: v_pages {[N, G, page // 32, hd, 32]} (got {tuple(v_pages.shape)})")
-    if k_pages.dtype != v_pages.dtype:
+    dt = k_pages.dtype
+    if v_pages.dtype != dt:
         raise ValueError(f"{name}: k_pages and v_pages share one dtype")
-    code, elems = _dtype_code(k_pages), G * page * hd
-    ks, vs = (elems, elems) if N == 1 else (k_pages.stride(0), v_pages.stride(0))
-    if ks < elems or vs < elems or not (_inner_contiguous(k_pages) and _inner_contiguous(v_pages)):
-        raise ValueError(f"{name}: each page must be contiguous, and pages must not overlap")
-    return _lib.FcPages(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, N, G, page, hd, code)
+    ks = vs = G * page * hd
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        if N > 1:
+            ks, vs = k_pages.stride(0), v_pages.stride(0)
+        if min(ks, vs) < G * page * hd or not (_inner_contiguous(k_pages) and _inner_contiguous(v_pages)):
+            raise ValueError(f"{name}: each page must be contiguous, and pages must not overlap")
+    code = _lib.FC_BF16 if dt == torch.bfloat16 else _dtype_code(k_pages)
+    return _lib.FcPages(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, N, G, page, hd, code), G, page, hd
 
 
 def _index(name: str, what: str, t: torch.Tensor, n: int):
@@ -546,22 +555,21 @@ def page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start,
         raise ValueError("page_tables: batch in [1, 4096], width, tokens and the free stack not empty")
     if page < 32 or page % 32 != 0 or prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
         raise ValueError("page_tables: page a multiple of 32, prefix_len >= 0, positions below 2^31")
-    for what, t, n in (("tables", tables, B * W), ("held", held, B), ("free_pages", free_pages, F),
-                       ("n_free", n_free, 1), ("length", length, B), ("n_new", n_new, B), ("row_off", row_off, B + 1),
-                       ("start", start, B), ("tok_row", tok_row, T), ("tok_pos", tok_pos, T), ("slots", slots, T)):
-        _index("page_tables", what, t, n)
-    d = _on_gpu("page_tables", tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots)
-    _launch("fc_page_tables", d, lib().fc_page_tables, tables.data_ptr(), held.data_ptr(), free_pages.data_ptr(),
-            n_free.data_ptr(), length.data_ptr(), n_new.data_ptr(), row_off.data_ptr(), start.data_ptr(),
-            tok_row.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), B, W, F, T, page, prefix_len)
+    ts = (tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots)
+    i32 = torch.int32
+    for i, (t, n) in enumerate(zip(ts, (B * W, B, F, 1, B, B, B + 1, B, T, T, T))):
+        if t.dtype is not i32 or t.numel() != n or not t.is_contiguous():
+            _index("page_tables", ("tables", "held", "free_pages", "n_free", "length", "n_new", "row_off", "start",
+                                   "tok_row", "tok_pos", "slots")[i], t, n)
+    d = _on_gpu("page_tables", *ts)
+    _launch("fc_page_tables", d, lib().fc_page_tables, *[t.data_ptr() for t in ts], B, W, F, T, page, prefix_len)
 
 
 @_op("page_append(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_pages, Tensor(b!) v_pages) -> ()")
 def page_append(k, v, slots, k_pages, v_pages):
-    p = _pages("page_append", k_pages, v_pages)
-    if k.dim() != 3 or k.shape[1:] != (p.n_kv_head, p.head_dim) or v.shape != k.shape:
-        raise ValueError(f"page_append: k and v [tokens][{p.n_kv_head}][{p.head_dim}] "
-                         f"(got {tuple(k.shape)} and {tuple(v.shape)})")
+    p, G, _, hd = _pages("page_append", k_pages, v_pages)
+    if k.dim() != 3 or k.shape[1:] != (G, hd) or v.shape != k.shape:
+        raise ValueError(f"page_append: k and v [tokens][{G}][{hd}] (got {tuple(k.shape)} and {tuple(v.shape)})")
     if k.dtype != v.dtype or (k.dtype != k_pages.dtype and k.dtype != torch.float32):
         raise ValueError(f"page_append: k and v in the pages' dtype or fp32 (got {k.dtype} and {v.dtype})")
     M = k.shape[0]
@@ -569,57 +577,64 @@ def page_append(k, v, slots, k_pages, v_pages):
     d = _on_gpu("page_append", k_pages, v_pages, k, v, slots)
     if M == 0:
         return
-    if p.head_dim != 1:
-        k = k if k.stride(2) == 1 else k.contiguous()
-        v = v if v.stride(2) == 1 else v.contiguous()
-    _launch("fc_page_append", d, lib().fc_page_append, p, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
-            v.stride(0), v.stride(1), _dtype_code(k), slots.data_ptr(), M)
+    kt, kh, kd = k.stride()
+    vt, vh, vd = v.stride()
+    if hd != 1 and (kd != 1 or vd != 1):
+        k, v = k.contiguous(), v.contiguous()
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+    _launch("fc_page_append", d, lib().fc_page_append, p, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, _dtype_code(k),
+            slots.data_ptr(), M)
 
 
 @_op("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor tables, Tensor row_off, Tensor start, "
      "int max_per_row, int window, Tensor? prefix_pages=None, int prefix_len=0) -> Tensor")
 def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None,
                     prefix_len=0):
-    p = _pages("paged_attention", k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != p.head_dim or q.shape[1] == 0 or q.shape[1] % p.n_kv_head != 0:
-        raise ValueError(f"paged_attention: q [tokens][n_head][{p.head_dim}], n_head a multiple of {p.n_kv_head} "
+    p, G, page, hd = _pages("paged_attention", k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != hd or q.shape[1] == 0 or q.shape[1] % G != 0:
+        raise ValueError(f"paged_attention: q [tokens][n_head][{hd}], n_head a multiple of {G} "
                          f"(got {tuple(q.shape)})")
     if q.dtype != k_pages.dtype:
         raise ValueError("paged_attention: q and the pages share one dtype")
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise ValueError("paged_attention has no backward pass")
     if tables.dim() != 2:
         raise ValueError(f"paged_attention: tables [batch][width] (got {tuple(tables.shape)})")
     B, W = tables.shape
-    T, H, hd = q.shape
-    if not 1 <= B <= 4096 or W < 1 or H > 65535 or max_per_row < 1 or window < 0:
-        raise ValueError("paged_attention: batch in [1, 4096], width, max_per_row >= 1, window >= 0")
-    if prefix_len < 0 or W * p.page + prefix_len > 0x7fffffff:
+    T, H, _ = q.shape
+    if not 1 <= B <= 4096 or W < 1 or H > 65535 or not 1 <= max_per_row <= 0x7fffffff:
+        raise ValueError("paged_attention: batch in [1, 4096], width and max_per_row at least 1 and below 2^31")
+    if not 0 <= window <= 0x7fffffff:
+        raise ValueError("paged_attention: window in [0, 2^31)")
+    if prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
         raise ValueError("paged_attention: prefix_len >= 0, positions below 2^31")
-    if max_per_row > 0x7fffffff or window > 0x7fffffff:
-        raise ValueError("paged_attention: max_per_row and window below 2^31")
     _index("paged_attention", "tables", tables, B * W)
     _index("paged_attention", "row_off", row_off, B + 1)
     _index("paged_attention", "start", start, B)
     pre = 0
     if prefix_len > 0:
-        if prefix_pages is None or prefix_pages.numel() * p.page < prefix_len:
+        if prefix_pages is None or prefix_pages.numel() * page < prefix_len:
             raise ValueError(f"paged_attention: prefix_pages holds the pages of {prefix_len} positions")
         _index("paged_attention", "prefix_pages", prefix_pages, prefix_pages.numel())
         pre = prefix_pages.data_ptr()
         d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start, prefix_pages)
     else:
         d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start)
-    y = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+    y = q.new_empty((T, H * hd))
     if T == 0:
         return y
-    if hd != 1 and q.stride(2) != 1:
+    qt, qh, qd = q.stride()
+    if hd != 1 and qd != 1:
         q = q.contiguous()
-    nb = lib().fc_paged_attention_workspace_bytes(p, B, T, max_per_row, H, W, prefix_len, window)
-    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=q.device)
-    _launch("fc_paged_attention", d, lib().fc_paged_attention, p, q.data_ptr(), q.stride(0), q.stride(1),
-            y.data_ptr(), B, T, max_per_row, H, tables.data_ptr(), W, row_off.data_ptr(), start.data_ptr(), pre,
-            prefix_len, window, _lib.FC_PAGED_ZERO_TAIL, ws.data_ptr(), ws.numel())
+        qt, qh, _ = q.stride()
+    L = lib()
+    nb = L.fc_paged_attention_workspace_bytes(p, B, T, max_per_row, H, W, prefix_len, window)
+    if nb < 0:
+        check(nb, "fc_paged_attention_workspace_bytes")
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None  # held until the launch is queued
+    _launch("fc_paged_attention", d, L.fc_paged_attention, p, q.data_ptr(), qt, qh, y.data_ptr(), B, T, max_per_row, H,
+            tables.data_ptr(), W, row_off.data_ptr(), start.data_ptr(), pre, prefix_len, window,
+            _lib.FC_PAGED_ZERO_TAIL, ws.data_ptr() if nb else 0, nb)
     return y
 
 

@@ -38,15 +38,16 @@ __device__ __forceinline__ int row_of(const int* off, int n, int t) {
 // rows (pages given back, pages needed, tokens), so one workgroup does it all,
 // in place: every row is read before the first is written. Sums saturate at
 // 2^30 (they are only compared with capacities below that), which keeps them
-// associative and in 32 bits whatever the arrays hold. Bound by latency: two
-// scans over 16 waves, four dependent passes over global memory.
+// associative and in 32 bits whatever the arrays hold. Bound by latency: four
+// dependent passes over global memory and two scans, hence no more waves than
+// there are rows or tokens for (64 rows with 16 waves: 7.8 us, with one: 6.5).
 #define PT_ROWS 4096     // rows a call may have: 4 per thread
 #define PT_SAT (1u << 30)
 __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, PT_SAT); }
 
-// Exclusive scan over the workgroup's 1024 threads of two values at once.
+// Exclusive scan over the workgroup's threads of two values at once.
 __device__ __forceinline__ void scan2(uint32_t& a, uint32_t& b, uint2* red, uint2& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   uint32_t x = a, y = b;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -61,7 +62,7 @@ __device__ __forceinline__ void scan2(uint32_t& a, uint32_t& b, uint2* red, uint
   if (lane == 0) xe = ye = 0;
   __syncthreads();
   uint32_t px = 0, py = 0, tx = 0, ty = 0;
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < nw; ++i) {
     const uint2 r = red[i];
     if (i < w) px = sat_add(px, r.x), py = sat_add(py, r.y);
     tx = sat_add(tx, r.x);
@@ -73,52 +74,67 @@ __device__ __forceinline__ void scan2(uint32_t& a, uint32_t& b, uint2* red, uint
   total = make_uint2(tx, ty);
 }
 
-// Row, position and slot of token t of the packed chunk; off: the rows'
-// offsets (batch + 1).
-__device__ __forceinline__ void slot_of(int t, const int* off, int batch, int W, int page, int prefix,
-                                        const int* tables, const int* __restrict__ length,
-                                        int* __restrict__ tok_row, int* __restrict__ tok_pos,
-                                        int* __restrict__ slots) {
-  int row = -1, pos = -1, slot = -1;
-  if (t < off[batch]) {
-    row = row_of(off, batch, t);
-    const int at = length[row] + t - off[row];
-    const int64_t id = tables[(int64_t)row * W + at / page];
-    pos = prefix + at;
-    if (id >= 0 && (id + 1) * page <= 0x7fffffff) slot = (int)id * page + at % page;
+// Rows, positions and slots of four tokens of the packed chunk, t0 + i * step;
+// off: the rows' offsets (batch + 1). Their searches and loads go side by side.
+__device__ __forceinline__ void slots_of(int t0, int step, int max_tokens, const int* off, int batch, int W, int page,
+                                         int prefix, const int* tables, const int* __restrict__ length,
+                                         int* __restrict__ tok_row, int* __restrict__ tok_pos,
+                                         int* __restrict__ slots) {
+  const int total = off[batch];
+  int row[4] = {0, 0, 0, 0}, at[4], id[4];
+  for (int s = 1 << (31 - __builtin_clz(batch)); s > 0; s >>= 1)  // the last row that begins at the token or before
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (row[i] + s < batch && off[row[i] + s] <= t0 + i * step) row[i] += s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t0 + i * step;
+    at[i] = t < total ? length[row[i]] + t - off[row[i]] : 0;
   }
-  tok_row[t] = row;
-  tok_pos[t] = pos;
-  slots[t] = slot;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) id[i] = t0 + i * step < total ? tables[(int64_t)row[i] * W + at[i] / page] : -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t0 + i * step;
+    if (t >= max_tokens) continue;
+    const bool in = t < total;
+    tok_row[t] = in ? row[i] : -1;
+    tok_pos[t] = in ? prefix + at[i] : -1;
+    slots[t] = id[i] >= 0 && ((int64_t)id[i] + 1) * page <= 0x7fffffff ? id[i] * page + at[i] % page : -1;
+  }
 }
 
-__global__ __launch_bounds__(1024) void k_page_tables(int batch, int W, int page, int prefix, int F, int max_tokens,
-                                                      int fill, int* tables, int* held, int* stack, int* n_free,
-                                                      const int* __restrict__ length, const int* __restrict__ n_new,
-                                                      int* __restrict__ row_off, int* __restrict__ start,
-                                                      int* __restrict__ tok_row, int* __restrict__ tok_pos,
-                                                      int* __restrict__ slots) {
-  __shared__ int s_off[PT_ROWS + 1], s_take[PT_ROWS + 1], s_give[PT_ROWS + 1];
+struct TableArgs {
+  int batch, W, page, prefix, F, max_tokens, fill;
+  int *tables, *held, *stack, *n_free;
+  const int *length, *n_new;
+  int *row_off, *start, *tok_row, *tok_pos, *slots;
+};
+__global__ __launch_bounds__(1024) void k_page_tables(TableArgs t) {
+  const int batch = t.batch, W = t.W, page = t.page, F = t.F, max_tokens = t.max_tokens;
+  int *tables = t.tables, *held = t.held, *stack = t.stack;
+  __shared__ int s_off[PT_ROWS + 1], s_take[PT_ROWS + 1], s_give[PT_ROWS];
   __shared__ uint2 red[16];
   const int tid = threadIdx.x, b0 = 4 * tid;
   const int64_t width = (int64_t)W * page;
   int hb[4], nb[4], lb[4];
-  uint32_t need[4], give[4];
-  bool asks[4];
+  uint32_t ask[4], need[4], give[4];  // tokens asked for, pages they need, pages given back
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = b0 + i < batch;
     hb[i] = in ? held[b0 + i] : 0;
-    nb[i] = in ? n_new[b0 + i] : 0;
-    lb[i] = in ? length[b0 + i] : 0;
+    nb[i] = in ? t.n_new[b0 + i] : 0;
+    lb[i] = in ? t.length[b0 + i] : 0;
   }
-  const int nf = min(max(n_free[0], 0), F);
+  const int nf = min(max(t.n_free[0], 0), F);
   uint32_t a = 0, b = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t end = (int64_t)lb[i] + nb[i];
-    asks[i] = nb[i] > 0 && lb[i] >= 0 && end <= width && hb[i] <= W && ((int64_t)lb[i] + page - 1) / page <= hb[i];
-    need[i] = asks[i] ? (uint32_t)max((int64_t)0, min((end + page - 1) / page - hb[i], (int64_t)PT_SAT)) : 0;
+    const bool asks =
+        nb[i] > 0 && lb[i] >= 0 && end <= width && hb[i] <= W && ((int64_t)lb[i] + page - 1) / page <= hb[i];
+    ask[i] = asks ? (uint32_t)nb[i] : 0;
+    need[i] = asks ? (uint32_t)max((int64_t)0, min((end + page - 1) / page - hb[i], (int64_t)PT_SAT)) : 0;
     give[i] = nb[i] < 0 ? (uint32_t)min(max(hb[i], 0), W) : 0;
     a = sat_add(a, need[i]);
     b = sat_add(b, give[i]);
@@ -129,32 +145,30 @@ __global__ __launch_bounds__(1024) void k_page_tables(int batch, int W, int page
   const int avail = nf + given;
   // rows whose pages fit the stack, then rows whose tokens fit the chunk
   uint32_t c = 0, d = 0;
-  bool fits[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     s_give[b0 + i] = (int)b;
     b = sat_add(b, give[i]);
     a = sat_add(a, need[i]);
-    fits[i] = asks[i] && (need[i] == 0 || a <= (uint32_t)avail);
-    c = sat_add(c, fits[i] ? (uint32_t)nb[i] : 0);
-    d = sat_add(d, fits[i] ? need[i] : 0);
+    if (need[i] > 0 && a > (uint32_t)avail) ask[i] = need[i] = 0;
+    c = sat_add(c, ask[i]);
+    d = sat_add(d, need[i]);
   }
   scan2(c, d, red, tot);
   // Past the first row whose tokens do not fit, none fit (the sum only grows), so the sums up to it are
   // those over the rows that are in.
-  bool in[4];
   uint32_t in_n = 0, in_p = 0;  // the sums after this thread's last row that is in
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t c0 = c, d0 = d;
-    c = sat_add(c, fits[i] ? (uint32_t)nb[i] : 0);
-    d = sat_add(d, fits[i] ? need[i] : 0);
-    in[i] = fits[i] && c <= (uint32_t)max_tokens;
-    if (in[i]) in_n = c, in_p = d;
-    s_off[b0 + i] = (int)min(c0, (uint32_t)max_tokens + 1);
-    s_take[b0 + i] = (int)d0;
+    s_off[b0 + i] = (int)min(c, (uint32_t)max_tokens + 1);
+    s_take[b0 + i] = (int)d;
+    c = sat_add(c, ask[i]);
+    d = sat_add(d, need[i]);
+    if (c > (uint32_t)max_tokens) need[i] = 0;
+    else if (ask[i] > 0) in_n = c, in_p = d;
   }
   // totals over the rows that are in
+  const int nw = blockDim.x >> 6, step = blockDim.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     in_n = max(in_n, __shfl_xor(in_n, o, WAVE));
@@ -162,7 +176,7 @@ __global__ __launch_bounds__(1024) void k_page_tables(int batch, int W, int page
   }
   if ((tid & 63) == 0) red[tid >> 6] = make_uint2(in_n, in_p);
   __syncthreads();
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < nw; ++i) {
     in_n = max(in_n, red[i].x);
     in_p = max(in_p, red[i].y);
   }
@@ -173,18 +187,17 @@ __global__ __launch_bounds__(1024) void k_page_tables(int batch, int W, int page
     s_take[b0 + i] = min(s_take[b0 + i], (int)in_p);
   }
   if (tid == 0) {
-    s_off[PT_ROWS] = (int)in_n;
-    s_take[PT_ROWS] = (int)in_p;
-    s_give[PT_ROWS] = (int)tot.y;
+    s_off[4 * step] = (int)in_n;
+    s_take[4 * step] = (int)in_p;
   }
   __syncthreads();
-  // rows past the batch give, take and feed nothing, so entry `batch` of each array is its total
-  for (int i = tid; i < given; i += 1024) {
-    const int r = row_of(s_give, batch - 1, i);  // (the last row needs no bound of its own)
+  // (the last row needs no bound of its own, hence batch - 1; rows past the batch give, take and feed nothing)
+  for (int i = tid; i < given; i += step) {
+    const int r = row_of(s_give, batch - 1, i);
     stack[nf + i] = tables[(int64_t)r * W + i - s_give[r]];
   }
   __syncthreads();
-  for (int i = tid; i < (int)in_p; i += 1024) {
+  for (int i = tid; i < (int)in_p; i += step) {
     const int r = row_of(s_take, batch - 1, i);
     tables[(int64_t)r * W + held[r] + i - s_take[r]] = stack[avail - 1 - i];
   }
@@ -192,21 +205,20 @@ __global__ __launch_bounds__(1024) void k_page_tables(int batch, int W, int page
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (b0 + i < batch) {
-      held[b0 + i] = nb[i] < 0 ? 0 : in[i] ? hb[i] + (int)need[i] : hb[i];
-      start[b0 + i] = prefix + (nb[i] < 0 ? 0 : lb[i]);
-      row_off[b0 + i] = s_off[b0 + i];
+      held[b0 + i] = nb[i] < 0 ? 0 : hb[i] + (int)need[i];
+      t.start[b0 + i] = t.prefix + (nb[i] < 0 ? 0 : lb[i]);
+      t.row_off[b0 + i] = s_off[b0 + i];
     }
   if (tid == 0) {
-    row_off[batch] = (int)in_n;
-    n_free[0] = avail - (int)in_p;
+    t.row_off[batch] = (int)in_n;
+    t.n_free[0] = avail - (int)in_p;
   }
-  if (!fill) return;
-  for (int t = tid; t < max_tokens; t += 1024)
-    slot_of(t, s_off, batch, W, page, prefix, tables, length, tok_row, tok_pos, slots);
+  if (!t.fill) return;
+  for (int k = tid; k < max_tokens; k += 4 * step)
+    slots_of(k, step, max_tokens, s_off, batch, W, page, t.prefix, tables, t.length, t.tok_row, t.tok_pos, t.slots);
 }
 
-// The tokens of a large chunk, once the rows are settled: one workgroup per
-// 1024 tokens.
+// The tokens of a large chunk, once the rows are settled: 1024 per workgroup.
 __global__ __launch_bounds__(256) void k_page_slots(int batch, int W, int page, int prefix, int max_tokens,
                                                     const int* __restrict__ tables, const int* __restrict__ length,
                                                     const int* __restrict__ row_off, int* __restrict__ tok_row,
@@ -214,15 +226,13 @@ __global__ __launch_bounds__(256) void k_page_slots(int batch, int W, int page, 
   __shared__ int s_off[PT_ROWS + 1];
   for (int i = threadIdx.x; i <= batch; i += 256) s_off[i] = row_off[i];
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = blockIdx.x * 1024 + 256 * i + threadIdx.x;
-    if (t < max_tokens) slot_of(t, s_off, batch, W, page, prefix, tables, length, tok_row, tok_pos, slots);
-  }
+  slots_of(blockIdx.x * 1024 + threadIdx.x, 256, max_tokens, s_off, batch, W, page, prefix, tables, length, tok_row,
+           tok_pos, slots);
 }
 
-// tokens up to which the settling workgroup writes them itself
-#define PT_INLINE 2048
+// Tokens up to which the settling workgroup writes them itself: 64 rows and their 64 tokens are 6.5 us that way and
+// 4.3 + 4 in two launches, 1000 rows with 7000 tokens 16.4 us or 6.1 + 7.2.
+#define PT_INLINE 512
 
 extern "C" int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_pages, int32_t* n_free,
                                   const int32_t* length, const int32_t* n_new, int32_t* row_off, int32_t* start,
@@ -239,8 +249,10 @@ extern "C" int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_
                "free_cap and max_tokens must be in [1, 2^30)");
   const hipStream_t s = (hipStream_t)stream;
   const int fill = max_tokens <= PT_INLINE;
-  hipLaunchKernelGGL(k_page_tables, dim3(1), dim3(1024), 0, s, batch, width, page, prefix_len, free_cap, max_tokens,
-                     fill, tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots);
+  const TableArgs t{batch, width, page, prefix_len, free_cap, max_tokens, fill, tables, held, free_pages, n_free,
+                    length, n_new, row_off, start, tok_row, tok_pos, slots};
+  const int threads = std::max((batch + 3) / 4, fill ? (max_tokens + 3) / 4 : 0);
+  hipLaunchKernelGGL(k_page_tables, dim3(1), dim3(std::min(1024, (threads + 63) / 64 * 64)), 0, s, t);
   FC_LAUNCH_CHECK();
   if (!fill) {
     hipLaunchKernelGGL(k_page_slots, dim3((max_tokens + 1023) / 1024), dim3(256), 0, s, batch, width, page, prefix_len,

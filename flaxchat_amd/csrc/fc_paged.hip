@@ -698,9 +698,11 @@ __device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
 // by one chunk length for all rows, and every workgroup looks its own one up, by
 // its number, from all rows' lengths (each wave reads them all; the result is the
 // same everywhere). The chunk is what spreads the keys over about c.target items,
-// at least 128 (a tile for each of four waves), no more than CHUNK_MAX (several
-// rounds of items: their times differ then) and at least what makes c.S_own
-// splits of the longest row. (One share of all keys for each workgroup that fits
+// at least 128 (a tile for each of four waves), in the streaming kernel no more
+// than CHUNK_MAX (several rounds of items: their times differ then; a cut column
+// block of the wide kernel costs more than that, 16 rows of 512 at 8000 keys 633 us
+// with the limit and 560 without) and at least what makes c.S_own splits of the
+// longest row. (One share of all keys for each workgroup that fits
 // the card, whatever rows it crosses, took 10-15% longer: a workgroup then waits
 // at every border, where two on a CU hide each other's.)
 #define CHUNK_MAX 4096
@@ -720,7 +722,7 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
   longest = lanes_max<64>(longest);
   const float share = ceilf(total * (float)c.pv.G / (float)c.target);
   const int least = max(128, (longest + c.S_own - 1) / c.S_own);
-  it.len = __builtin_amdgcn_readfirstlane((max((int)fminf(share, (float)CHUNK_MAX), least) + 63) & ~63);
+  it.len = __builtin_amdgcn_readfirstlane((max((int)fminf(share, CB == 128 ? 1e9f : (float)CHUNK_MAX), least) + 63) & ~63);
   const float per = 1.f / (float)it.len;
   for (int r0 = 0; r0 < c.B; r0 += 64) {
     if (c.B > 64) {
@@ -744,7 +746,7 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
     it.g = at % c.pv.G;
     at /= c.pv.G;
     it.split = at % it.nsplit;
-    it.blk = at / it.nsplit;
+    it.blk = __builtin_amdgcn_readlane(nb, l) - 1 - at / it.nsplit;  // (later queries see more keys: first)
     it.skip = (int64_t)it.split * it.len;
     return true;
   }
@@ -754,6 +756,15 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
 __device__ __forceinline__ void mark_unused(const PagedChunk& c, const Item& it, int64_t pair) {
   if (it.split == it.nsplit - 1)
     for (int s = it.nsplit; s < c.S_own; ++s) c.pml[(int64_t)s * c.Mcap * c.H + pair] = make_float2(-INFINITY, 0.f);
+}
+
+// An item that holds all of its columns' keys writes their outputs itself. Where other rows are split it says so in
+// place of the first partial's sum, which is never negative.
+__device__ __forceinline__ bool whole(const PagedChunk& c, const Item& it) {
+  return c.S_pre == 0 && it.nsplit == 1;
+}
+__device__ __forceinline__ void mark_whole(const PagedChunk& c, int64_t pair) {
+  if (c.S_own > 1) c.pml[pair] = make_float2(0.f, -1.f);
 }
 
 // Tokens past the last row: set to 0 by the launch's workgroups in turn.
@@ -825,7 +836,8 @@ __device__ __forceinline__ void redo_columns(bool pre, const Item& it, int base,
       }
     }
     const int64_t pair = (int64_t)(base + j) * c.H + head;
-    if (c.S_own + c.S_pre == 1) {
+    if (whole(c, it)) {
+      if (lane == 0) mark_whole(c, pair);
       for (int t = 0; t < HD / 64; ++t) st<T>(y, pair * HD + lane + 64 * t, l == 0.f ? 0.f : o[t] / l);
     } else {
       const int64_t at = (int64_t)sg * c.Mcap * c.H + pair;
@@ -1082,7 +1094,8 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
     id = tile < tend ? list[pg] : -1;
     if ((unsigned)id0 >= (unsigned)w.pv.N) continue;
     Tile<T, HD> t;
-    t.load((const T*)w.kp + (int64_t)id0 * w.pv.ks + gofs + r0 * (32 * HD), (const T*)w.vp + (int64_t)id0 * w.pv.vs + gofs + r0 * (32 * HD), lane);
+    const int64_t in = gofs + r0 * (32 * HD);
+    t.load((const T*)w.kp + (int64_t)id0 * w.pv.ks + in, (const T*)w.vp + (int64_t)id0 * w.pv.vs + in, lane);
     if (!(kb >= f_lo && kb + 31 <= f_hi)) odd |= t.clear(w_lo - kb - 8 * g4, w_hi - kb - 8 * g4);
 #pragma unroll
     for (int u = 0; u < QB; ++u)
@@ -1093,7 +1106,7 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
     return;
   }
   const PagedChunk c = chunk_args();
-  const int rep = c.H / c.pv.G, S = c.S_own + c.S_pre, sg = pre ? c.S_own + it.split : it.split;
+  const int rep = c.H / c.pv.G, sg = pre ? c.S_own + it.split : it.split;
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     if (col0 + 16 * u < ncol) {  // uniform; a guard, not a break, so that u stays a constant
@@ -1121,7 +1134,8 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
           for (int i = 0; i < 8; ++i) o[i] += a * lds.o[w][qc][d0 + i];
         }
         const int j = col / rep, head = g * rep + col - j * rep;
-        if (S == 1) {
+        if (!pre && whole(c, it)) {
+          if (d0 == 0) mark_whole(c, (int64_t)(base + j) * c.H + head);
           store8((T*)c.y + ((int64_t)(base + j) * c.H + head) * HD + d0, o, L == 0.f ? 0.f : 1.f / L);
         } else {
           const int64_t slot = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
@@ -1177,6 +1191,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
   const int64_t at = min(pair, pairs - 1);
   float M = -INFINITY;
   int used = 0;  // own splits with keys: the first ones
+  const bool done = c.pml[at].y < 0.f;  // by a whole item
   for (int s = tp; s < S; s += TP) {
     const float2 e = c.pml[(int64_t)s * pairs + at];
     M = fmaxf(M, e.x);
@@ -1199,6 +1214,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
       store8(yo, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, 1.f);
     return;
   }
+  if (done) return;
   const float mu = M == -INFINITY ? 0.f : M;
   float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int n = used + c.S_pre;
@@ -1512,11 +1528,11 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     return;
   }
   const PagedChunk c = chunk_args();
-  const int rep = c.H / c.pv.G, S = c.S_own + c.S_pre, sg = pre ? c.S_own + it.split : it.split;
+  const int rep = c.H / c.pv.G, sg = pre ? c.S_own + it.split : it.split;
   const int col = c0 + 32 * wave + kk, j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
   // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
-  if (S > 1) {
+  if (pre || !whole(c, it)) {
     if (ok) {
       const int64_t slot = ((int64_t)sg * c.Mcap + base + j) * c.H + head;
       float* po = c.po + slot * HD + 4 * hl;
@@ -1532,6 +1548,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       }
     }
   } else {
+    if (ok && hl == 0) mark_whole(c, (int64_t)(base + j) * c.H + head);
     // through LDS, so that a lane writes 8 dims of a column
     const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
     constexpr int LD = HD + 8;
@@ -1644,6 +1661,10 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
   a.S_own = (int)std::min({(longest + 127) / 128, room, (int64_t)64});
+  // In the wide kernel, whose column blocks mostly fill the card, no more than it takes to fill it or one for 1024
+  // keys: every (token, head) has a sum for each. (16 rows of up to 512 tokens at up to 2000 keys: 97 us without
+  // this rule and with partials of rows that are not split, 84 so.)
+  if (!a.own_qb) a.S_own = (int)std::min<int64_t>(a.S_own, std::max((longest + 1023) / 1024, (511 + units) / units));
   // short rows without a prefix: one split, and no merge (one row of 640 keys, 6 heads: one launch of 10.6 us, or 6.8
   // and 3.4 with the gap between them; 17 us or 21 from one call to the next)
   if (P == 0 && longest <= 1024) a.S_own = 1;

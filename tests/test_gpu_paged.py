@@ -503,3 +503,32 @@ def test_decode_loop(dtype):
         _check(got, ref, tol, f"step {step}")
         if back:
             hist[back[0]] = tuple(x[:-back[1]] for x in hist[back[0]])
+
+
+@pytest.mark.parametrize("hd,H,G", [(128, 4, 2), (64, 6, 2)])
+@pytest.mark.parametrize("P,window", [(0, 0), (0, 100), (1, 0), (33, 0), (96, 40), (500, 333), (1500, 1024)])
+@pytest.mark.parametrize("ctx,n", [
+    ([0, 5, 31, 200], [130, 1, 64, 0]),          # short rows: each one's keys are one piece
+    ([1500, 0, 700], [90, 20, 150]),             # pieces of long rows beside a short one's whole
+    ([40] * 40, [66, 0, 1, 130] * 10),           # more column blocks than workgroups at once
+])
+def test_prompts_behind_a_prefix(hd, H, G, P, window, ctx, n):
+    """Rows of many query columns: prefixes that end inside a block of 32 keys,
+    windows that reach back over their end, and rows that are cut into pieces
+    beside rows that are not."""
+    _say(f"paged_attention hd={hd} prefix {P} window {window}: rows of {n[:4]} tokens at {ctx[:4]}")
+    c = Paged(23, ctx, n, P, G, hd, 64, torch.bfloat16)
+    q = c.queries(H, tail=3)
+    got = _run(c, q, window)
+    ref, tol = c.reference(q, window)
+    _check(got, ref, tol)
+    assert torch.all(got[int(c.off[-1]):] == 0)
+    # a V that is not finite at a position that only the row's last two queries see
+    if window == 0:
+        b = int(np.argmax(c.n))
+        at = int(c.ctx[b] + c.n[b]) - 2
+        c.V[c.tables[b, at // 64], :, at % 64] = INF
+        got = _run(c, q, window)
+        keep = np.ones(len(q), bool)
+        keep[c.off[b + 1] - 2:c.off[b + 1]] = False
+        _check(got[keep], ref[keep], tol[keep], "a later position's V")

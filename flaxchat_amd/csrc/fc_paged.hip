@@ -702,7 +702,8 @@ __device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
 // than CHUNK_MAX (several rounds of items: their times differ then; a cut column
 // block of the wide kernel costs more than that, 16 rows of 512 at 8000 keys 633 us
 // with the limit and 560 without) and at least what makes c.S_own splits of the
-// longest row. (One share of all keys for each workgroup that fits
+// longest row; a row's pieces are then of one length (64 rows of 4800 keys, 12 heads:
+// 302 us, and 356 with 4096 and 704). (One share of all keys for each workgroup that fits
 // the card, whatever rows it crosses, took 10-15% longer: a workgroup then waits
 // at every border, where two on a CU hide each other's.)
 #define CHUNK_MAX 4096
@@ -743,6 +744,8 @@ __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it)
     at -= __builtin_amdgcn_readlane(upto - mine, l);
     it.b = r0 + l;
     it.nsplit = __builtin_amdgcn_readlane(ns, l);
+    // pieces of one length (no longer than the chunk, so none is empty)
+    if (it.nsplit > 1) it.len = ((__builtin_amdgcn_readlane(len, l) - 1) / it.nsplit + 64) & ~63;
     it.g = at % c.pv.G;
     at /= c.pv.G;
     it.split = at % it.nsplit;
@@ -1580,7 +1583,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 // hides the other's start and end. 256 workgroups of either in turn, so that a CU
 // holds one of each.
 template <typename T, int HD, int PRE, int OWN>
-__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedChunk c, int npre, int nown) {
+__global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2) void k_paged_attn(PagedChunk c, int npre, int nown) {
   union Lds {
     StreamLds<HD> s;
     std::conditional_t<PRE == 0 || OWN == 0, WideLds<HD>, char> w;
@@ -1626,18 +1629,21 @@ struct PagedPlan {
   int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short
   int64_t part_bytes, ml_bytes;
 };
-// Key splits of the prefix: the time of the workgroups on their XCD (a unit's
-// column blocks share one; 64 run at once there, two a CU), a step of 64 keys
-// taking 2 us of two workgroups on a CU and 1.2 us of one, six steps' time for a
-// workgroup's start and end, and 10 TB/s for the partials (written and read, from the
-// last cache).
-int pre_splits(int P, int G, int blk, int64_t part_bytes, int most) {
+// Key splits of the prefix. With S of them, in us: the time that their workgroups
+// take on the XCD with the most of them (a unit's column blocks share one; 64 run
+// at once there, two a CU), 2 us for a step of 64 keys, twice that in fp32, and six
+// steps for a workgroup's start and end; half of one workgroup's time alone (1.2 us a
+// step: the rows' own keys hide some of it); 5 TB/s for the partials, and 0.2 of
+// the merge. Against the best of S = 1 .. 40 its choice costs 5% or less in 10 of 13
+// measured shapes and 16% at most (prefixes of 1000 to 16000 keys under 1 to 4482
+// tokens: 18 to 212 us).
+int pre_splits(int P, int G, int blk, int64_t part_bytes, int most, bool fp32) {
   int best = 1;
   double least = 1e30;
   for (int S = 1; S <= std::min(most, (P + 127) / 128); ++S) {
-    const int64_t on = (int64_t)((G * S + 7) / 8) * blk, rounds = (on + 63) / 64;
-    const double steps = (P / S + 63) / 64 + 6;
-    const double t = rounds * steps * (on > 32 ? 2.0 : 1.2) + S * (double)part_bytes * 2 / 10e6;
+    const int64_t on = (int64_t)((G * S + 7) / 8) * blk;
+    const double steps = ((P + S - 1) / S + 63) / 64 * (fp32 ? 2 : 1) + 6;
+    const double t = on * steps * 2.0 / 64 + steps * 0.6 + S * (0.2 + (double)part_bytes * 2 / 5e6);
     if (t < least) least = t, best = S;
   }
   return best;
@@ -1671,7 +1677,7 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   a.target = a.own_qb ? 768 : 256;
   a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, units * longest / CHUNK_MAX);
   if (P > 0) {
-    a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128));
+    a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
     a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
     a.S_pre = (P + a.pre_chunk - 1) / a.pre_chunk;
   }

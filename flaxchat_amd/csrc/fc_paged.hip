@@ -494,6 +494,7 @@ struct PagedChunk {
   // partials of split s (the own ones first): po[(s Mcap + token) H + head][hd] unnormalised, pml (max, sum)
   float* po;
   float2* pml;
+  int* items;  // of more than ROWS_SCAN rows: the chunk's length, and every 64 rows' first item
   const void *q, *kp, *vp;
   void* y;
 };
@@ -507,6 +508,12 @@ template <typename P>
 __device__ __forceinline__ P* in_global(P* p) {
   return (P*)(__attribute__((address_space(1))) P*)p;
 }
+template <typename P>
+__device__ __forceinline__ P* scalar(P* p) {  // the same in every lane, and known to be
+  const uint64_t u = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return in_global((P*)((uint64_t)hi << 32 | lo));
+}
 __device__ __forceinline__ PagedChunk chunk_args() {
   auto p = __builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
@@ -518,6 +525,7 @@ __device__ __forceinline__ PagedChunk chunk_args() {
   c.pre = in_global(c.pre);
   c.po = in_global(c.po);
   c.pml = in_global(c.pml);
+  c.items = in_global(c.items);
   c.q = in_global(c.q);
   c.kp = in_global(c.kp);
   c.vp = in_global(c.vp);
@@ -681,15 +689,19 @@ struct Item {
   int b, blk, g, split, nsplit, len;
   int64_t skip;
 };
-// keys of row r's walk, from the 32-key block of its first query's first key; -1: no query
-__device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
-  const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
-  ncol = sp.n * (c.H / c.pv.G);
-  if (sp.n == 0) return -1;
+// keys of row r's walk, from the 32-key block of its first query's first key, and its column blocks; -1: no query
+struct RowKeys {
+  int len, blocks;
+};
+template <int CB>
+__device__ __forceinline__ RowKeys row_keys(const PagedChunk& c, int r) {
+  const int64_t at = c.start[min(r, c.B - 1)];  // (its load goes beside those of the offsets)
+  const RowSpan sp = row_span(c.row_off, min(r, c.B - 1), c.max_per_row, c.Mcap);
   int lo, hi, lo1, hi1;
-  key_range(c, c.start[r], false, lo, hi);
-  key_range(c, (int64_t)c.start[r] + sp.n - 1, false, lo1, hi1);
-  return hi1 < lo ? 0 : hi1 + 1 - (lo & ~31);
+  key_range(c, at, false, lo, hi);
+  key_range(c, at + sp.n - 1, false, lo1, hi1);
+  if (r >= c.B || sp.n == 0) return {-1, 0};
+  return {hi1 < lo ? 0 : hi1 + 1 - (lo & ~31), (sp.n * (c.H / c.pv.G) + CB - 1) / CB};
 }
 
 // Rows are of unequal length: with a number of key splits for all, the longest
@@ -706,54 +718,108 @@ __device__ __forceinline__ int row_keys(const PagedChunk& c, int r, int& ncol) {
 // 302 us, and 356 with 4096 and 704). (One share of all keys for each workgroup that fits
 // the card, whatever rows it crosses, took 10-15% longer: a workgroup then waits
 // at every border, where two on a CU hide each other's.)
+// Up to ROWS_SCAN rows every wave looks through all of them. With more the reading
+// of so many lengths would be most of a workgroup's time (4096 rows of up to 200
+// keys: 1448 us, 215 with the list): a kernel ahead of the walk finds the chunk and
+// where every 64 rows' items begin.
 #define CHUNK_MAX 4096
+#define ROWS_SCAN 256
 template <int CB>
-__device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
+__device__ __forceinline__ int chunk_length(const PagedChunk& c, float total, int longest) {
+  const float share = ceilf(total * (float)c.pv.G / (float)c.target);
+  const int least = max(128, (longest + c.S_own - 1) / c.S_own);
+  const float most = CB == 128 ? 1e9f : (float)CHUNK_MAX;
+  return __builtin_amdgcn_readfirstlane((max((int)fminf(share, most), least) + 63) & ~63);
+}
+// pieces of a row: its keys / chunk, at least one
+__device__ __forceinline__ int row_pieces(const RowKeys& r, int chunk) {
+  int ns = (int)((float)max(r.len, 0) * (1.f / (float)chunk));  // one off at most
+  ns += ns * chunk < r.len;
+  return max(1, ns - ((ns - 1) * chunk >= r.len));
+}
+// The item numbered `at` from the 64 rows' first on, lane l holding row r0 + l; false: it is behind them, and at less
+// by theirs.
+__device__ __forceinline__ bool item_of(const PagedChunk& c, int& at, int r0, const RowKeys& r, int chunk, Item& it) {
+  const int ns = row_pieces(r, chunk), mine = ns * r.blocks * c.pv.G, upto = lanes_scan(mine);
+  const uint64_t past = __ballot(upto > at);
+  if (past == 0) {
+    at -= __builtin_amdgcn_readlane(upto, 63);
+    return false;
+  }
+  const int l = __builtin_ctzll(past);
+  at -= __builtin_amdgcn_readlane(upto - mine, l);
+  // (the walk's addresses are scalar: said so here, since the compiler loses track of it where the ways here meet)
+  it.b = __builtin_amdgcn_readfirstlane(r0 + l);
+  it.nsplit = __builtin_amdgcn_readlane(ns, l);
+  // pieces of one length (no longer than the chunk, so none is empty)
+  it.len = it.nsplit > 1 ? ((__builtin_amdgcn_readlane(r.len, l) - 1) / it.nsplit + 64) & ~63 : chunk;
+  const int unit = __builtin_amdgcn_readfirstlane(at) / c.pv.G;
+  it.g = __builtin_amdgcn_readfirstlane(at) - unit * c.pv.G;
+  it.blk = __builtin_amdgcn_readlane(r.blocks, l) - 1 - unit / it.nsplit;  // (later queries see more keys: first)
+  it.split = unit % it.nsplit;
+  it.skip = (int64_t)it.split * it.len;
+  return true;
+}
+template <int CB, int N>
+__device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it) {
   const int lane = threadIdx.x & 63;
-  int len = -1, ncol = 0;  // of this lane's row of the 64 looked at last
+  RowKeys r[N];
   float total = 0.f;
   int longest = 1;
-  for (int r0 = 0; r0 < c.B; r0 += 64) {
-    len = r0 + lane < c.B ? row_keys(c, r0 + lane, ncol) : -1;
-    if (len < 0) ncol = 0;
-    total += (float)max(len, 0) * (float)((ncol + CB - 1) / CB);
-    longest = max(longest, len);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r[i] = row_keys<CB>(c, 64 * i + lane);
+    total += (float)max(r[i].len, 0) * (float)r[i].blocks;
+    longest = max(longest, r[i].len);
+  }
+  const int chunk = chunk_length<CB>(c, lanes_sum(total), lanes_max<64>(longest));
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (item_of(c, at, 64 * i, r[i], chunk, it)) return true;
+  return false;
+}
+template <int CB>
+__device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
+  if (c.B <= 64) return find_among<CB, 1>(c, at, it);
+  if (c.B <= ROWS_SCAN) return find_among<CB, ROWS_SCAN / 64>(c, at, it);
+  const int lane = threadIdx.x & 63, n = (c.B + 63) >> 6;
+  const int chunk = __builtin_amdgcn_readfirstlane(c.items[0]), first = c.items[1 + min(lane, n)];
+  const int k = __builtin_popcountll(__ballot(lane < n && first <= at)) - 1;
+  at -= __builtin_amdgcn_readlane(first, k);
+  return item_of(c, at, 64 * k, row_keys<CB>(c, 64 * k + lane), chunk, it);
+}
+template <int CB>
+__global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
+  constexpr int N = PT_ROWS / 1024;
+  __shared__ float s_total[16];
+  __shared__ int s_longest[16], s_items[64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  RowKeys r[N];
+  float total = 0.f;
+  int longest = 1;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r[i] = row_keys<CB>(c, 64 * (wave + 16 * i) + lane);
+    total += (float)max(r[i].len, 0) * (float)r[i].blocks;
+    longest = max(longest, r[i].len);
   }
   total = lanes_sum(total);
   longest = lanes_max<64>(longest);
-  const float share = ceilf(total * (float)c.pv.G / (float)c.target);
-  const int least = max(128, (longest + c.S_own - 1) / c.S_own);
-  it.len = __builtin_amdgcn_readfirstlane((max((int)fminf(share, CB == 128 ? 1e9f : (float)CHUNK_MAX), least) + 63) & ~63);
-  const float per = 1.f / (float)it.len;
-  for (int r0 = 0; r0 < c.B; r0 += 64) {
-    if (c.B > 64) {
-      len = r0 + lane < c.B ? row_keys(c, r0 + lane, ncol) : -1;
-      if (len < 0) ncol = 0;
-    }
-    int ns = (int)((float)max(len, 0) * per);  // len / it.len, one off at most
-    ns += ns * it.len < len;
-    ns = max(1, ns - ((ns - 1) * it.len >= len));
-    const int nb = (ncol + CB - 1) / CB, mine = len < 0 ? 0 : ns * nb * c.pv.G;
-    const int upto = lanes_scan(mine);
-    const uint64_t past = __ballot(upto > at);
-    if (past == 0) {
-      at -= __builtin_amdgcn_readlane(upto, 63);
-      continue;
-    }
-    const int l = __builtin_ctzll(past);
-    at -= __builtin_amdgcn_readlane(upto - mine, l);
-    it.b = r0 + l;
-    it.nsplit = __builtin_amdgcn_readlane(ns, l);
-    // pieces of one length (no longer than the chunk, so none is empty)
-    if (it.nsplit > 1) it.len = ((__builtin_amdgcn_readlane(len, l) - 1) / it.nsplit + 64) & ~63;
-    it.g = at % c.pv.G;
-    at /= c.pv.G;
-    it.split = at % it.nsplit;
-    it.blk = __builtin_amdgcn_readlane(nb, l) - 1 - at / it.nsplit;  // (later queries see more keys: first)
-    it.skip = (int64_t)it.split * it.len;
-    return true;
+  if (lane == 0) s_total[wave] = total, s_longest[wave] = longest;
+  __syncthreads();
+  total = 0.f;
+  for (int i = 0; i < 16; ++i) total += s_total[i], longest = max(longest, s_longest[i]);
+  const int chunk = chunk_length<CB>(c, total, longest);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int upto = lanes_scan(row_pieces(r[i], chunk) * r[i].blocks * c.pv.G);
+    if (lane == 63) s_items[wave + 16 * i] = upto;
   }
-  return false;
+  __syncthreads();
+  if (wave > 0) return;
+  const int mine = s_items[lane], n = (c.B + 63) >> 6;
+  if (lane < n) c.items[1 + lane] = lanes_scan(mine) - mine;
+  if (lane == 0) c.items[0] = chunk;
 }
 // The partials of a row's column that no split writes: the item of its last split marks them.
 __device__ __forceinline__ void mark_unused(const PagedChunk& c, const Item& it, int64_t pair) {
@@ -1371,6 +1437,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
   const uint32_t voff = 16u * (uint32_t)(4 * kk + hl);
   const int64_t gofs = (int64_t)g * w.pv.page * HD;
   const float scale_log2 = w.scale * 1.4426950408889634f;
+  const char *kp = (const char*)scalar(w.kp), *vp = (const char*)scalar(w.vp);
   const int tpp = w.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
   const const_ints list = CONST_INTS(pre ? w.pre : w.tables + (int64_t)b * w.W);
   f32x16 O[DD];
@@ -1391,8 +1458,8 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     const bool is = (unsigned)id < (unsigned)w.pv.N;                                                         \
     next |= (int)is << u;                                                                                    \
     const int64_t pid = is ? id : 0; /* no page: page 0's place is read and masked */                        \
-    const bf16_t* kt = (const bf16_t*)w.kp + pid * w.pv.ks + gofs + tr * (32 * HD);                          \
-    const bf16_t* vt = (const bf16_t*)w.vp + pid * w.pv.vs + gofs + tr * (32 * HD);                          \
+    const bf16_t* kt = (const bf16_t*)kp + pid * w.pv.ks + gofs + tr * (32 * HD);                          \
+    const bf16_t* vt = (const bf16_t*)vp + pid * w.pv.vs + gofs + tr * (32 * HD);                          \
     if constexpr (HD == 128) {                                                                               \
       const uint32_t lk = LDS_ADDR(S_.k[u][0]) + 2048 * wave, lv = LDS_ADDR(S_.v[u][0]) + 2048 * wave;       \
       lds_load_1k(kt + 1024 * wave, koff, lk);                                                               \
@@ -1583,7 +1650,8 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 // hides the other's start and end. 256 workgroups of either in turn, so that a CU
 // holds one of each.
 template <typename T, int HD, int PRE, int OWN>
-__global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2) void k_paged_attn(PagedChunk c, int npre, int nown) {
+__global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2) void k_paged_attn(PagedChunk c,
+                                                                                                int npre, int nown) {
   union Lds {
     StreamLds<HD> s;
     std::conditional_t<PRE == 0 || OWN == 0, WideLds<HD>, char> w;
@@ -1627,7 +1695,7 @@ struct PagedPlan {
   int own_qb, own_blk, pre_qb, pre_blk;
   int S_own, S_pre, pre_chunk, target;
   int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short
-  int64_t part_bytes, ml_bytes;
+  int64_t part_bytes, ml_bytes, item_bytes;
 };
 // Key splits of the prefix. With S of them, in us: the time that their workgroups
 // take on the XCD with the most of them (a unit's column blocks share one; 64 run
@@ -1664,13 +1732,17 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   // own keys
   const int64_t width = (int64_t)W * p->page;
   const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
-  const int64_t units = (int64_t)B * G * a.own_blk, one = (int64_t)T * H * (p->head_dim + 2) * 4;
+  // (a row's last block may be short, so the tokens make up to one more block a row than they would side by side)
+  const int cb = a.own_qb ? 16 * a.own_qb : 128;
+  const int64_t units = G * std::min((int64_t)B * a.own_blk, (int64_t)T * rep / cb + B);
+  const int64_t one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
   a.S_own = (int)std::min({(longest + 127) / 128, room, (int64_t)64});
-  // In the wide kernel, whose column blocks mostly fill the card, no more than it takes to fill it or one for 1024
-  // keys: every (token, head) has a sum for each. (16 rows of up to 512 tokens at up to 2000 keys: 97 us without
-  // this rule and with partials of rows that are not split, 84 so.)
-  if (!a.own_qb) a.S_own = (int)std::min<int64_t>(a.S_own, std::max((longest + 1023) / 1024, (511 + units) / units));
+  // Where the rows alone make several items for every workgroup, no more than it takes to cut the longest into pieces
+  // of 512 keys (1024 in the wide kernel): every (token, head) has a sum for each. (16 rows of up to 512 tokens at up
+  // to 2000 keys: 97 us without this rule and with partials of rows that are not split, 84 so.)
+  const int fill = a.own_qb ? 4 * 768 : 512, piece = a.own_qb ? 512 : 1024;
+  a.S_own = (int)std::min<int64_t>(a.S_own, std::max((longest + piece - 1) / piece, (fill - 1 + units) / units));
   // short rows without a prefix: one split, and no merge (one row of 640 keys, 6 heads: one launch of 10.6 us, or 6.8
   // and 3.4 with the gap between them; 17 us or 21 from one call to the next)
   if (P == 0 && longest <= 1024) a.S_own = 1;
@@ -1686,6 +1758,7 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
     a.part_bytes = fc_align(pairs * p->head_dim * 4);
     a.ml_bytes = fc_align(pairs * 8);
   }
+  if (B > ROWS_SCAN) a.item_bytes = fc_align((1 + PT_ROWS / 64) * 4);
   return a;
 }
 
@@ -1694,6 +1767,12 @@ int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   const int nown = (int)a.items;
   const int npre = a.S_pre == 0 ? 0 : a.pre_qb ? c.pv.G * a.S_pre * a.pre_blk
                                                : 8 * ((c.pv.G * a.S_pre + 7) / 8) * a.pre_blk;
+  if (c.B > ROWS_SCAN) {
+    if (a.own_qb == 0) hipLaunchKernelGGL(k_paged_items<128>, dim3(1), dim3(1024), 0, s, c);
+    else if (a.own_qb == 2) hipLaunchKernelGGL(k_paged_items<32>, dim3(1), dim3(1024), 0, s, c);
+    else hipLaunchKernelGGL(k_paged_items<16>, dim3(1), dim3(1024), 0, s, c);
+    FC_LAUNCH_CHECK();
+  }
   const dim3 grid(npre == 0 ? nown : 256 * ((npre + 255) / 256 + (nown + 255) / 256));
 #define PAGED(PRE, OWN)                                                                                             \
   hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN>), grid, dim3(256), 0, s, c, npre, nown)
@@ -1736,7 +1815,7 @@ extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int
   FC_CHECK_ARG(batch > 0 && max_tokens > 0 && max_per_row > 0 && n_head > 0 && n_head % pages->n_kv_head == 0 &&
                    width > 0 && prefix_len >= 0 && window >= 0, "sizes");
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
-  return a.part_bytes + a.ml_bytes;
+  return a.part_bytes + a.ml_bytes + a.item_bytes;
 }
 
 extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,
@@ -1759,11 +1838,13 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   const int64_t pre = (int64_t)pages->n_kv_head * std::max(a.S_pre, 1) * std::max(a.pre_blk, 1);
   const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
   FC_CHECK_ARG(std::max({a.items + pre, merge, (int64_t)max_tokens}) < (1 << 24) - 1024, "too many tokens, rows or heads");
-  FC_CHECK_ARG(a.part_bytes == 0 || (work && work_bytes >= a.part_bytes + a.ml_bytes), "workspace too small");
+  const int64_t need = a.part_bytes + a.ml_bytes + a.item_bytes;
+  FC_CHECK_ARG(need == 0 || (work && work_bytes >= need), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
                1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, (float*)work,
-               (float2*)((char*)work + a.part_bytes), q, pages->k, pages->v, y};
+               (float2*)((char*)work + a.part_bytes), (int*)((char*)work + a.part_bytes + a.ml_bytes),
+               q, pages->k, pages->v, y};
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;

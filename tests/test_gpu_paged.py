@@ -532,3 +532,24 @@ def test_prompts_behind_a_prefix(hd, H, G, P, window, ctx, n):
         keep = np.ones(len(q), bool)
         keep[c.off[b + 1] - 2:c.off[b + 1]] = False
         _check(got[keep], ref[keep], tol[keep], "a later position's V")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,most,P,window", [
+    (70, 3, 0, 0), (256, 9, 40, 0), (257, 3, 0, 0), (300, 20, 33, 0), (300, 70, 0, 25), (1030, 2, 10, 0),
+    (4096, 1, 0, 0),  # the most there may be
+])
+def test_many_rows(dtype, B, most, P, window):
+    """Rows by the hundred, a few of them long and many without a token, in
+    blocks of 16, 32 and 128 columns."""
+    _say(f"paged_attention {dtype}: {B} rows of up to {most} tokens, prefix {P}, window {window}")
+    r = np.random.default_rng(B)
+    ctx, n = r.integers(0, 40, B), r.integers(0, most + 1, B)
+    ctx[r.integers(0, B, 3)] = 700
+    n[[0, B - 1]] = most
+    c = Paged(29, ctx, n, P, 1, 128, 32, DT[dtype])
+    q = c.queries(2, tail=1)
+    got = _run(c, q, window)
+    ref, tol = c.reference(q, window)
+    _check(got, ref, tol)
+    assert torch.all(got[int(c.off[-1]):] == 0)

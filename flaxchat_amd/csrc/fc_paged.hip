@@ -341,7 +341,9 @@ __device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
 // positions (a prompt's, save its ends) they are one store, element by element
 // elsewhere (2-byte stores to rows 64 bytes apart take a cycle per lane). Hence a
 // workgroup's tokens begin where a run of 8 does, if one is near. Bound by the
-// copy of K and V.
+// copy of K and V in a prompt: 16000 tokens of 4 heads 21 us (3.1 TB/s moved, a plain
+// copy 4.9); 448 tokens in runs of up to 7, 12 heads, 11 us, of which most is the
+// waits for slots, values and LDS one after the other.
 #define PA_TILE 32
 #define PA_MOST (PA_TILE + 7)
 // First token of tile i: the first one from 32 i on that begins a run of 8
@@ -511,7 +513,8 @@ __device__ __forceinline__ P* in_global(P* p) {
 template <typename P>
 __device__ __forceinline__ P* scalar(P* p) {  // the same in every lane, and known to be
   const uint64_t u = (uint64_t)p;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
   return in_global((P*)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ PagedChunk chunk_args() {
@@ -535,7 +538,9 @@ __device__ __forceinline__ PagedChunk chunk_args() {
 
 // Any head size, type and alignment: one workgroup per (token, head), keys in
 // blocks of 256 (a thread scores one key, then sums one dimension), with the
-// running maximum and sum of the softmax.
+// running maximum and sum of the softmax. Without matrix instructions and with keys
+// read once per query head, it is for shapes that no model here has: 64 rows of 300
+// keys, 12 heads of 96, 175 us (12 of 128: 25).
 template <typename T>
 __global__ __launch_bounds__(256) void k_paged_any(PagedChunk c) {
   const T *q = (const T*)c.q, *kp = (const T*)c.kp, *vp = (const T*)c.vp;
@@ -1071,6 +1076,13 @@ __device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile
 // key split; its four waves every fourth 32-key tile, straight from memory into
 // registers, each tile applied to all QB blocks of 16 columns, and are merged in
 // LDS.
+//
+// Bound by the reading of K and V: 17 rows of about 114000 keys (8 KV heads of 128)
+// take 1.26 ms, 6.4 TB/s of the 7.1 that a plain read reaches, 64 rows of 2400 keys
+// (12 heads) 152 us, 6.2 TB/s. Short rows are bound by what a workgroup waits for
+// one after the other (the rows' offsets, the table, the keys): 64 rows of 300 keys
+// 25 us, 4.8 TB/s. fp32 takes four times the matrix instructions of bf16 for as
+// many keys: 8 rows of 5 tokens, 6 heads, behind 1000 keys 17 us.
 template <int HD>
 struct StreamLds {
   float o[4][16][HD + 4];
@@ -1250,7 +1262,9 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& 
 // Merge of the key splits of one (token, head), HD / 8 threads with 8
 // dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
 // splits' (max, sum) are read side by side, ahead of the token's row; then the
-// outputs of those that hold keys, CB at a time.
+// outputs of those that hold keys, CB at a time. Bound by the reading of the
+// partials: 4482 tokens of 12 heads with three of them 18 us, 5.4 TB/s; with few
+// tokens by the launch and three waits, 5 us.
 template <typename T, int HD, int CB>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
   __shared__ int off[PT_ROWS + 1];
@@ -1320,6 +1334,16 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
 //
 // Workgroups: the items of the list, or, for the prefix, group x key split x
 // column block, all blocks of a split on one XCD, whose L2 then holds its keys.
+//
+// Bound by the matrix cores and the softmax's arithmetic together: a step of a wave
+// is 1024 cycles of the first and about 1300 of the second, of which two waves a
+// SIMD hide a part (16 rows of 512 tokens behind 8000 shared keys 510 us, 0.81
+// PFLOP/s; a library matrix product reaches 1.23). With few steps a workgroup the
+// start and the end weigh in: behind 4001 keys, 4482 tokens of unequal rows, 205 us,
+// 0.61 PFLOP/s. Tried and slower: a row's prefix and own keys in one walk, which
+// saves the merge but cuts the work in pieces too large to fill the card evenly (275
+// us); the maximum left behind by up to 2^8, to scale the sums less often, gave 4% and
+// cost precision, as the largest weight is then no longer 1.
 template <int HD>
 struct WideStage {
   uint4 k[2][HD / 16][64];  // [32-key tile][16-dim slice][lane]
@@ -1648,7 +1672,10 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 // -1: no prefix) and the rows' own keys in one launch: the first is bound by
 // the matrix cores where many rows share it, the second by memory, and each
 // hides the other's start and end. 256 workgroups of either in turn, so that a CU
-// holds one of each.
+// holds one of each. (64 samples behind 5000 keys: 41 us with the merge, the rows' own
+// keys alone 29, the prefix alone 15.) Without a prefix the streaming kernel runs
+// three to a CU, which hides more of the waits at an item's start (64 rows of 300 keys
+// 25 us, two to a CU 30; rows of 100000 keys 1262 us, and 1243).
 template <typename T, int HD, int PRE, int OWN>
 __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2) void k_paged_attn(PagedChunk c,
                                                                                                 int npre, int nown) {
@@ -1762,11 +1789,15 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   return a;
 }
 
+// workgroups of the prefix: in the wide kernel's order its units go to the XCDs in turn
+int64_t prefix_groups(const PagedPlan& a, int G) {
+  const int units = G * a.S_pre;
+  return (int64_t)(a.pre_qb ? units : (units + 7) / 8 * 8) * a.pre_blk;
+}
+
 template <typename T, int HD>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
-  const int nown = (int)a.items;
-  const int npre = a.S_pre == 0 ? 0 : a.pre_qb ? c.pv.G * a.S_pre * a.pre_blk
-                                               : 8 * ((c.pv.G * a.S_pre + 7) / 8) * a.pre_blk;
+  const int nown = (int)a.items, npre = (int)prefix_groups(a, c.pv.G);
   if (c.B > ROWS_SCAN) {
     if (a.own_qb == 0) hipLaunchKernelGGL(k_paged_items<128>, dim3(1), dim3(1024), 0, s, c);
     else if (a.own_qb == 2) hipLaunchKernelGGL(k_paged_items<32>, dim3(1), dim3(1024), 0, s, c);
@@ -1835,9 +1866,9 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   FC_CHECK_ARG(width > 0 && (int64_t)width * pages->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
   // a launch's threads are counted in 32 bits along x, its workgroups in 16 along y
-  const int64_t pre = (int64_t)pages->n_kv_head * std::max(a.S_pre, 1) * std::max(a.pre_blk, 1);
   const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
-  FC_CHECK_ARG(std::max({a.items + pre, merge, (int64_t)max_tokens}) < (1 << 24) - 1024, "too many tokens, rows or heads");
+  FC_CHECK_ARG(std::max({a.items + prefix_groups(a, pages->n_kv_head), merge, (int64_t)max_tokens}) < (1 << 24) - 1024,
+               "too many tokens, rows or heads");
   const int64_t need = a.part_bytes + a.ml_bytes + a.item_bytes;
   FC_CHECK_ARG(need == 0 || (work && work_bytes >= need), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,

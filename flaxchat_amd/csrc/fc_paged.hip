@@ -1272,6 +1272,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
   const int64_t pair = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP, pairs = (int64_t)c.Mcap * c.H;
   const int tp = threadIdx.x % TP, d0 = tp * 8, S = c.S_own + c.S_pre, own = c.S_own;
   const int64_t at = min(pair, pairs - 1);
+  const int off0 = c.row_off[min((int)threadIdx.x, c.B)];  // its wait goes beside the next loads'
   float M = -INFINITY;
   int used = 0;  // own splits with keys: the first ones
   const bool done = c.pml[at].y < 0.f;  // by a whole item
@@ -1280,12 +1281,28 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
     M = fmaxf(M, e.x);
     if (s < own && (e.x != -INFINITY || e.y != 0.f)) used = s + 1;
   }
-  for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+  if ((int)threadIdx.x <= c.B) off[threadIdx.x] = off0;
+  for (int i = threadIdx.x + 256; i <= c.B; i += 256) off[i] = c.row_off[i];
 #pragma unroll
   for (int o = TP / 2; o > 0; o >>= 1) {
     M = fmaxf(M, __shfl_xor(M, o, WAVE));
     used = max(used, __shfl_xor(used, o, WAVE));
   }
+  // CB splits' partials, under way while the token's row is looked up
+  const int n = used + c.S_pre;
+  float2 e[CB];
+  float4 u[CB][2];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < CB; ++k) {
+      const int s = min(s0 + k, n - 1);
+      const int64_t i = (int64_t)(s < used ? s : s - used + own) * pairs + at;
+      e[k] = c.pml[i];
+      u[k][0] = *(const float4*)(c.po + i * HD + d0);
+      u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
+    }
+  };
+  load(0);
   __syncthreads();
   if (pair >= pairs) return;
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
@@ -1300,18 +1317,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
   if (done) return;
   const float mu = M == -INFINITY ? 0.f : M;
   float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const int n = used + c.S_pre;
   for (int s0 = 0; s0 < n; s0 += CB) {
-    float2 e[CB];
-    float4 u[CB][2];
-#pragma unroll
-    for (int k = 0; k < CB; ++k) {
-      const int s = min(s0 + k, n - 1);
-      const int64_t i = (int64_t)(s < used ? s : s - used + own) * pairs + at;
-      e[k] = c.pml[i];
-      u[k][0] = *(const float4*)(c.po + i * HD + d0);
-      u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
-    }
+    if (s0 > 0) load(s0);
 #pragma unroll
     for (int k = 0; k < CB; ++k) {
       // a split without keys holds (-inf, 0) and no output

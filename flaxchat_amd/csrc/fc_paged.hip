@@ -34,6 +34,18 @@ __device__ __forceinline__ int row_of(const int* off, int n, int t) {
 // ---------------------------------------------------------------------------
 // Page tables
 // ---------------------------------------------------------------------------
+// The rows' offsets into LDS, by 256 threads, four loads under way at once.
+__device__ __forceinline__ void stage_offsets(int* off, const int* __restrict__ row_off, int batch) {
+  for (int i0 = threadIdx.x; i0 <= batch; i0 += 1024) {
+    int x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = row_off[min(i0 + 256 * k, batch)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i0 + 256 * k <= batch) off[i0 + 256 * k] = x[k];
+  }
+}
+
 // What a batch's step does to its pages is a handful of prefix sums over the
 // rows (pages given back, pages needed, tokens), so one workgroup does it all,
 // in place: every row is read before the first is written. Sums saturate at
@@ -224,7 +236,7 @@ __global__ __launch_bounds__(256) void k_page_slots(int batch, int W, int page, 
                                                     const int* __restrict__ row_off, int* __restrict__ tok_row,
                                                     int* __restrict__ tok_pos, int* __restrict__ slots) {
   __shared__ int s_off[PT_ROWS + 1];
-  for (int i = threadIdx.x; i <= batch; i += 256) s_off[i] = row_off[i];
+  stage_offsets(s_off, row_off, batch);
   __syncthreads();
   slots_of(blockIdx.x * 1024 + threadIdx.x, 256, max_tokens, s_off, batch, W, page, prefix, tables, length, tok_row,
            tok_pos, slots);
@@ -1248,7 +1260,7 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& 
     ncol = min(max(c.row_off[c.B], 0), c.Mcap) * (c.H / c.pv.G);
     if (it.blk * 16 * QB >= ncol) return;
     int* off = (int*)&lds;
-    for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+    stage_offsets(off, c.row_off, c.B);
     __syncthreads();
   } else {
     if (!find_item<16 * QB>(c, at, it)) return;
@@ -1388,7 +1400,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       ncol = min(max(c.row_off[c.B], 0), c.Mcap) * rep;
       if (it.blk * 128 >= ncol) return;
       int* off = (int*)stg;
-      for (int i = threadIdx.x; i <= c.B; i += 256) off[i] = c.row_off[i];
+      stage_offsets(off, c.row_off, c.B);
       __syncthreads();
     } else {
       if (!find_item<128>(c, at, it)) return;

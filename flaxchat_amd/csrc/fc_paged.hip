@@ -740,19 +740,22 @@ __device__ __forceinline__ RowKeys row_keys(const PagedChunk& c, int r) {
 // keys: 1448 us, 215 with the list): a kernel ahead of the walk finds the chunk and
 // where every 64 rows' items begin.
 #define CHUNK_MAX 4096
+#define CHUNK_WIDE 1000000000
 #define ROWS_SCAN 256
 template <int CB>
 __device__ __forceinline__ int chunk_length(const PagedChunk& c, float total, int longest) {
   const float share = ceilf(total * (float)c.pv.G / (float)c.target);
-  const int least = max(128, (longest + c.S_own - 1) / c.S_own);
-  const float most = CB == 128 ? 1e9f : (float)CHUNK_MAX;
-  return __builtin_amdgcn_readfirstlane((max((int)fminf(share, most), least) + 63) & ~63);
+  // (unsigned: a row may have up to 2^31 - 32 keys)
+  const uint32_t least = max(128u, ((uint32_t)longest + c.S_own - 1) / c.S_own);
+  const uint32_t len = (max((uint32_t)fminf(share, (float)(CB == 128 ? CHUNK_WIDE : CHUNK_MAX)), least) + 63) & ~63u;
+  return __builtin_amdgcn_readfirstlane((int)min(len, 0x7fffffe0u));
 }
 // pieces of a row: its keys / chunk, at least one
 __device__ __forceinline__ int row_pieces(const RowKeys& r, int chunk) {
-  int ns = (int)((float)max(r.len, 0) * (1.f / (float)chunk));  // one off at most
-  ns += ns * chunk < r.len;
-  return max(1, ns - ((ns - 1) * chunk >= r.len));
+  const uint32_t len = max(r.len, 0), by = chunk;
+  uint32_t ns = (uint32_t)((float)len * (1.f / (float)chunk));  // one off at most
+  ns += ns * by < len;
+  return max(1, (int)(ns - (ns > 1 && (ns - 1) * by >= len)));
 }
 // The item numbered `at` from the 64 rows' first on, lane l holding row r0 + l; false: it is behind them, and at less
 // by theirs.
@@ -1314,7 +1317,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
       u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
     }
   };
-  load(0);
+  if (!done) load(0);
   __syncthreads();
   if (pair >= pairs) return;
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);
@@ -1793,7 +1796,8 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   // and 3.4 with the gap between them; 17 us or 21 from one call to the next)
   if (P == 0 && longest <= 1024) a.S_own = 1;
   a.target = a.own_qb ? 768 : 256;
-  a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, units * longest / CHUNK_MAX);
+  const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;
+  a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, cut);
   if (P > 0) {
     a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
     a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;

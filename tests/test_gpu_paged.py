@@ -553,3 +553,21 @@ def test_many_rows(dtype, B, most, P, window):
     ref, tol = c.reference(q, window)
     _check(got, ref, tol)
     assert torch.all(got[int(c.off[-1]):] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,window", [(3, 40), (3, 0), (45, 40)])
+def test_last_positions(dtype, n, window):
+    """A table of 2^31 - 32 positions, all but the last two pages without an
+    entry: the arithmetic of positions and pieces at the end of its range."""
+    _say(f"paged_attention {dtype}: {n} tokens at the last positions, window {window}")
+    W, N = 2 ** 26 - 1, 4
+    c = Paged(31, [64 - n], [n], 0, 2, 128, 32, DT[dtype], extra=2)  # 64 positions: the last two pages
+    assert c.N == N
+    a = c.device(dev())
+    tables = torch.full((1, W), -1, dtype=torch.int32, device=dev())
+    tables[0, -2:] = a["tables"][0]
+    q = c.queries(4)
+    got = _run(c, q, window, dict(a, tables=tables, start=up([32 * W - n])))
+    ref, tol = c.reference(q, window)
+    _check(got, ref, tol)

@@ -251,14 +251,14 @@ extern "C" int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_
                                   int32_t* tok_row, int32_t* tok_pos, int32_t* slots, int32_t batch, int32_t width,
                                   int32_t free_cap, int32_t max_tokens, int32_t page, int32_t prefix_len,
                                   void* stream) {
-  FC_CHECK_ARG(tables && held && free_pages && n_free && length && n_new && row_off && start && tok_row && tok_pos &&
+  FC_CHECK_ARG(tables && held && (free_pages || free_cap == 0) && n_free && length && n_new && row_off && start && tok_row && tok_pos &&
                    slots, "null pointer");
   FC_CHECK_ARG(batch > 0 && batch <= PT_ROWS, "batch must be in [1, 4096]");
   FC_CHECK_ARG(page > 0 && page % 32 == 0, "page must be a multiple of 32");
   FC_CHECK_ARG(width > 0 && prefix_len >= 0 && (int64_t)width * page + prefix_len <= 0x7fffffff,
                "positions must fit 31 bits");
-  FC_CHECK_ARG(free_cap > 0 && free_cap < (int32_t)PT_SAT && max_tokens > 0 && max_tokens < (int32_t)PT_SAT,
-               "free_cap and max_tokens must be in [1, 2^30)");
+  FC_CHECK_ARG(free_cap >= 0 && free_cap < (int32_t)PT_SAT && max_tokens > 0 && max_tokens < (int32_t)PT_SAT,
+               "free_cap must be in [0, 2^30), max_tokens in [1, 2^30)");
   const hipStream_t s = (hipStream_t)stream;
   const int fill = max_tokens <= PT_INLINE;
   const TableArgs t{batch, width, page, prefix_len, free_cap, max_tokens, fill, tables, held, free_pages, n_free,

@@ -551,8 +551,8 @@ def page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start,
         raise ValueError(f"page_tables: tables [batch][width] (got {tuple(tables.shape)})")
     B, W = tables.shape
     T, F = slots.numel(), free_pages.numel()
-    if not 1 <= B <= 4096 or W < 1 or not 1 <= T < 1 << 30 or not 1 <= F < 1 << 30:
-        raise ValueError("page_tables: batch in [1, 4096], width, tokens and the free stack not empty")
+    if not 1 <= B <= 4096 or W < 1 or not 1 <= T < 1 << 30 or F >= 1 << 30:
+        raise ValueError("page_tables: batch in [1, 4096], width and tokens not empty, both and free_pages below 2^30")
     if page < 32 or page % 32 != 0 or prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
         raise ValueError("page_tables: page a multiple of 32, prefix_len >= 0, positions below 2^31")
     ts = (tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots)

@@ -343,7 +343,7 @@ typedef struct fc_pages {
 /* The pages of one step, from the rows' lengths, on the device (all arrays
  * int32 device memory). State, updated in place: tables[batch][width] (page
  * ids), held[batch] (pages of each row), free_pages[free_cap] and n_free[1]
- * (a stack; entries at n_free and above are scratch). Per row: length[b]
+ * (a stack; entries at n_free and above are scratch; free_cap may be 0). Per row: length[b]
  * positions held (counted behind the shared prefix of prefix_len positions),
  * n_new[b] to be added; n_new < 0 ends the row: its pages go onto the stack,
  * in row order, and held[b] becomes 0. A row with n_new > 0 asks if

@@ -107,6 +107,21 @@ def test_page_tables_small_stack():
 
 
 # ---------------------------------------------------------------- page_append
+def test_page_tables_no_pages():
+    """A stack without room: rows that need no page are taken in, others not."""
+    _say("page_tables: an empty stack")
+    B, W, page, T = 4, 3, 32, 12
+    tables = np.array([[5, -1, -1], [6, 7, -1], [-1, -1, -1], [8, -1, -1]])
+    held, length, n_new = np.array([1, 2, 0, 1]), np.array([30, 40, 0, 32]), np.array([2, 5, 1, 1])
+    t = [tables, held, np.zeros(0), np.array([0]), length, n_new, np.zeros(B + 1), np.zeros(B)]
+    d = [up(x) for x in t + 3 * [np.zeros(T)]]
+    OPS.page_tables(*d, page, 10)
+    want = tables_reference(tables, held, np.zeros(0, np.int64), np.array([0]), length, n_new, page, 10, T)
+    for got, w in zip(d[6:], want):
+        assert np.array_equal(got.cpu().numpy(), w)
+    assert np.array_equal(d[0].cpu().numpy(), tables) and d[6].tolist() == [0, 2, 7, 7, 7] and d[3].item() == 0
+
+
 @pytest.mark.parametrize("dtype,src", [("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp32")])
 @pytest.mark.parametrize("G,hd,page,runs,strided", [
     (1, 128, 32, [1], False),

@@ -117,7 +117,8 @@ def test_append_refusals(kw, match):
     (dict(slots=i32(5)), "tok_row"),
     (dict(n_new=torch.zeros(3, dtype=torch.int64)), "int32"),
     (dict(length=i32(6)[::2]), "contiguous"),
-    (dict(free_pages=i32(0)), "free"),
+    (dict(free_pages=i32(0)), "CUDA"),  # a stack without room is none to refuse
+    (dict(free_pages=torch.zeros(9, dtype=torch.int64)), "free"),
 ])
 def test_tables_refusals(kw, match):
     with pytest.raises(ValueError, match=match):

@@ -251,8 +251,8 @@ extern "C" int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_
                                   int32_t* tok_row, int32_t* tok_pos, int32_t* slots, int32_t batch, int32_t width,
                                   int32_t free_cap, int32_t max_tokens, int32_t page, int32_t prefix_len,
                                   void* stream) {
-  FC_CHECK_ARG(tables && held && (free_pages || free_cap == 0) && n_free && length && n_new && row_off && start && tok_row && tok_pos &&
-                   slots, "null pointer");
+  FC_CHECK_ARG(tables && held && (free_pages || free_cap == 0) && n_free && length && n_new && row_off && start &&
+                   tok_row && tok_pos && slots, "null pointer");
   FC_CHECK_ARG(batch > 0 && batch <= PT_ROWS, "batch must be in [1, 4096]");
   FC_CHECK_ARG(page > 0 && page % 32 == 0, "page must be a multiple of 32");
   FC_CHECK_ARG(width > 0 && prefix_len >= 0 && (int64_t)width * page + prefix_len <= 0x7fffffff,
@@ -505,6 +505,7 @@ struct PagedChunk {
   // key splits: most of a row's own keys, of the prefix, keys of each of these; workgroups that the own keys are to
   // be spread over
   int S_own, S_pre, pre_chunk, target;
+  int joint;  // the rows' walks begin with the prefix, P rounded up to 32; 0: it is walked for itself, or there is none
   // partials of split s (the own ones first): po[(s Mcap + token) H + head][hd] unnormalised, pml (max, sum)
   float* po;
   float2* pml;
@@ -699,6 +700,23 @@ __device__ __forceinline__ void key_range(const PagedChunk& c, int64_t pos, bool
   lo = c.window > 0 ? (int)max((int64_t)0, min(pos - c.window - off, (int64_t)0x7fffffff)) : 0;
 }
 
+// How a workgroup walks: over a row's own keys, over the prefix for all rows, or
+// over a row's keys and, if c.joint, the prefix ahead of them. In the last, keys are
+// counted from the prefix's first, and own ones from c.joint: no key lies between.
+enum Walk { OWN_KEYS, PREFIX_KEYS, ROW_KEYS };
+template <int walk>
+__device__ __forceinline__ void walk_range(const PagedChunk& c, int64_t pos, int& lo, int& hi) {
+  key_range(c, pos, walk == PREFIX_KEYS, lo, hi);
+  if constexpr (walk == ROW_KEYS) {
+    int plo, phi;
+    key_range(c, pos, true, plo, phi);
+    if (c.joint > 0) {
+      lo = plo < c.P ? plo : (int)min((int64_t)lo + c.joint, (int64_t)0x7fffffff);
+      hi = hi >= 0 ? hi + c.joint : phi;
+    }
+  }
+}
+
 // A piece of work: a column block of row b (or, for the prefix, of all tokens)
 // and KV group g against `len` keys from `skip` keys on behind the 32-key block
 // of the row's first key; the `split`th of the block's nsplit pieces.
@@ -710,13 +728,13 @@ struct Item {
 struct RowKeys {
   int len, blocks;
 };
-template <int CB>
+template <int CB, int walk>
 __device__ __forceinline__ RowKeys row_keys(const PagedChunk& c, int r) {
   const int64_t at = c.start[min(r, c.B - 1)];  // (its load goes beside those of the offsets)
   const RowSpan sp = row_span(c.row_off, min(r, c.B - 1), c.max_per_row, c.Mcap);
   int lo, hi, lo1, hi1;
-  key_range(c, at, false, lo, hi);
-  key_range(c, at + sp.n - 1, false, lo1, hi1);
+  walk_range<walk>(c, at, lo, hi);
+  walk_range<walk>(c, at + sp.n - 1, lo1, hi1);
   if (r >= c.B || sp.n == 0) return {-1, 0};
   return {hi1 < lo ? 0 : hi1 + 1 - (lo & ~31), (sp.n * (c.H / c.pv.G) + CB - 1) / CB};
 }
@@ -780,7 +798,7 @@ __device__ __forceinline__ bool item_of(const PagedChunk& c, int& at, int r0, co
   it.skip = (int64_t)it.split * it.len;
   return true;
 }
-template <int CB, int N>
+template <int CB, int walk, int N>
 __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it) {
   const int lane = threadIdx.x & 63;
   RowKeys r[N];
@@ -788,7 +806,7 @@ __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it
   int longest = 1;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    r[i] = row_keys<CB>(c, 64 * i + lane);
+    r[i] = row_keys<CB, walk>(c, 64 * i + lane);
     total += (float)max(r[i].len, 0) * (float)r[i].blocks;
     longest = max(longest, r[i].len);
   }
@@ -798,17 +816,17 @@ __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it
     if (item_of(c, at, 64 * i, r[i], chunk, it)) return true;
   return false;
 }
-template <int CB>
+template <int CB, int walk>
 __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
-  if (c.B <= 64) return find_among<CB, 1>(c, at, it);
-  if (c.B <= ROWS_SCAN) return find_among<CB, ROWS_SCAN / 64>(c, at, it);
+  if (c.B <= 64) return find_among<CB, walk, 1>(c, at, it);
+  if (c.B <= ROWS_SCAN) return find_among<CB, walk, ROWS_SCAN / 64>(c, at, it);
   const int lane = threadIdx.x & 63, n = (c.B + 63) >> 6;
   const int chunk = __builtin_amdgcn_readfirstlane(c.items[0]), first = c.items[1 + min(lane, n)];
   const int k = __builtin_popcountll(__ballot(lane < n && first <= at)) - 1;
   at -= __builtin_amdgcn_readlane(first, k);
-  return item_of(c, at, 64 * k, row_keys<CB>(c, 64 * k + lane), chunk, it);
+  return item_of(c, at, 64 * k, row_keys<CB, walk>(c, 64 * k + lane), chunk, it);
 }
-template <int CB>
+template <int CB, int walk>
 __global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
   constexpr int N = PT_ROWS / 1024;
   __shared__ float s_total[16];
@@ -819,7 +837,7 @@ __global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
   int longest = 1;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    r[i] = row_keys<CB>(c, 64 * (wave + 16 * i) + lane);
+    r[i] = row_keys<CB, walk>(c, 64 * (wave + 16 * i) + lane);
     total += (float)max(r[i].len, 0) * (float)r[i].blocks;
     longest = max(longest, r[i].len);
   }
@@ -874,14 +892,14 @@ __device__ __forceinline__ void zero_tail(int wg, int nwg) {
 // [kbeg, kend). (Anything done about them in the walk itself costs every call
 // registers, and spills.)
 template <typename T, int HD>
-__device__ __forceinline__ void redo_columns(bool pre, const Item& it, int base, int c_lo, int c_hi, int kbeg, int kend,
+__device__ __forceinline__ void redo_columns(int walk, const Item& it, int base, int c_lo, int c_hi, int kbeg, int kend,
                                              int wave) {
   const PagedChunk c = chunk_args();
   const T *q = (const T*)c.q, *kp = (const T*)c.kp, *vp = (const T*)c.vp;
   T* y = (T*)c.y;
+  const bool pre = walk == PREFIX_KEYS;
   const int sg = pre ? c.S_own + it.split : it.split;
   const int lane = threadIdx.x & 63, rep = c.H / c.pv.G, b = it.b, g = it.g;
-  const int* list = pre ? c.pre : c.tables + (int64_t)b * c.W;
   for (int col = c_lo + wave; col < c_hi; col += 4) {
     const int j = col / rep, head = g * rep + col - j * rep;
     int64_t pos = pre ? 0 : (int64_t)c.start[b] + j;
@@ -892,36 +910,43 @@ __device__ __forceinline__ void redo_columns(bool pre, const Item& it, int base,
       if (j < sp.base || j >= sp.base + sp.n) continue;
       pos = (int64_t)c.start[r] + (j - sp.base);
     }
-    int lo, hi;
-    key_range(c, pos, pre, lo, hi);
-    lo = max(lo, kbeg);
-    hi = min(hi, kend - 1);
+    int v_lo, v_hi;
+    if (walk == ROW_KEYS) walk_range<ROW_KEYS>(c, pos, v_lo, v_hi);
+    else key_range(c, pos, pre, v_lo, v_hi);
+    v_lo = max(v_lo, kbeg);
+    v_hi = min(v_hi, kend - 1);
     const T* qr = q + (base + j) * c.qst + head * c.qsh;
     float m = -INFINITY, l = 0.f, o[HD / 64] = {};
-    for (int k0 = lo; k0 <= hi; k0 += 64) {
-      const int key = k0 + lane, pg = min(key, hi) / c.pv.page, at = min(key, hi) - pg * c.pv.page;
-      const int id = list[pg];
-      const bool ok = key <= hi && (unsigned)id < (unsigned)c.pv.N;
-      float s = -INFINITY;
-      if (ok) {
-        float a = 0.f;
 #pragma unroll 1
-        for (int d = 0; d < HD; ++d) a += ld<T>(qr, d) * ld<T>(kp, k_elem(c.pv, id, g, at, d));
-        s = a * c.scale * 1.4426950408889634f;
-      }
-      const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
-      const float p = ok ? exp2a(s - mu) : 0.f, alpha = exp2a(m - mu);
-      l = l * alpha + wave_sum(p);
-      m = mn;
-#pragma unroll
-      for (int t = 0; t < HD / 64; ++t) o[t] *= alpha;
+    for (int part = walk == ROW_KEYS && c.joint > 0 ? 0 : 1; part < 2; ++part) {  // the prefix, the row's own keys
+      const int from = part == 1 && walk == ROW_KEYS ? c.joint : 0;
+      const int lo = max(v_lo - from, 0), hi = part == 0 ? min(v_hi, c.P - 1) : v_hi - from;
+      const int* list = pre || part == 0 ? c.pre : c.tables + (int64_t)b * c.W;
+      for (int k0 = lo; k0 <= hi; k0 += 64) {
+        const int key = k0 + lane, pg = min(key, hi) / c.pv.page, at = min(key, hi) - pg * c.pv.page;
+        const int id = list[pg];
+        const bool ok = key <= hi && (unsigned)id < (unsigned)c.pv.N;
+        float s = -INFINITY;
+        if (ok) {
+          float a = 0.f;
 #pragma unroll 1
-      for (int i = 0; i < 64; ++i) {
-        const int idi = __shfl(ok ? id : -1, i, WAVE), ati = __shfl(at, i, WAVE);
-        const float w = __shfl(p, i, WAVE);
-        if (idi < 0) continue;
+          for (int d = 0; d < HD; ++d) a += ld<T>(qr, d) * ld<T>(kp, k_elem(c.pv, id, g, at, d));
+          s = a * c.scale * 1.4426950408889634f;
+        }
+        const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
+        const float p = ok ? exp2a(s - mu) : 0.f, alpha = exp2a(m - mu);
+        l = l * alpha + wave_sum(p);
+        m = mn;
 #pragma unroll
-        for (int t = 0; t < HD / 64; ++t) o[t] += w * ld<T>(vp, v_elem(c.pv, idi, g, ati, lane + 64 * t));
+        for (int t = 0; t < HD / 64; ++t) o[t] *= alpha;
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i) {
+          const int idi = __shfl(ok ? id : -1, i, WAVE), ati = __shfl(at, i, WAVE);
+          const float w = __shfl(p, i, WAVE);
+          if (idi < 0) continue;
+#pragma unroll
+          for (int t = 0; t < HD / 64; ++t) o[t] += w * ld<T>(vp, v_elem(c.pv, idi, g, ati, lane + 64 * t));
+        }
       }
     }
     const int64_t pair = (int64_t)(base + j) * c.H + head;
@@ -1198,7 +1223,8 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
       tile16<T, HD>(t, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
   }
   if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
-    redo_columns<T, HD>(pre, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend), (int)kend, wave);
+    redo_columns<T, HD>(pre ? PREFIX_KEYS : OWN_KEYS, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend),
+                        (int)kend, wave);
     return;
   }
   const PagedChunk c = chunk_args();
@@ -1266,7 +1292,7 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& 
     stage_offsets(off, c.row_off, c.B);
     __syncthreads();
   } else {
-    if (!find_item<16 * QB>(c, at, it)) return;
+    if (!find_item<16 * QB, OWN_KEYS>(c, at, it)) return;
     const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
     base = sp.base;
     ncol = sp.n * (c.H / c.pv.G);
@@ -1376,9 +1402,10 @@ struct WideLds {
   WideStage<HD> stg[2];
   int rng[4][2];
 };
-template <int HD, bool pre>
+template <int HD, int walk>
 __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
+  constexpr bool pre = walk == PREFIX_KEYS;
   WideStage<HD>(&stg)[2] = lds.stg;
   static_assert(sizeof(lds.stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1406,7 +1433,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       stage_offsets(off, c.row_off, c.B);
       __syncthreads();
     } else {
-      if (!find_item<128>(c, at, it)) return;
+      if (!find_item<128, walk>(c, at, it)) return;
       const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
       base = sp.base;
       ncol = sp.n * rep;
@@ -1433,7 +1460,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 #pragma unroll
       for (int h = 0; h < DS; ++h) qf[h] = *(const v4u*)(qr + 16 * h) & keep;
     }
-    key_range(c, pos, pre, lo_c, hi_c);
+    walk_range<walk>(c, pos, lo_c, hi_c);
     if (!ok) lo_c = 0x7fffffff, hi_c = -1;
     // the keys that some column of the workgroup sees
     w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
@@ -1453,7 +1480,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     g_hi = __builtin_amdgcn_readfirstlane(g_hi);
     // (a row's splits are counted from its first column's first key in every one of its blocks)
     int row_lo = g_lo, unused;
-    if (!pre && c.window > 0) key_range(c, c.start[it.b], false, row_lo, unused);
+    if (!pre && c.window > 0) walk_range<walk>(c, c.start[it.b], row_lo, unused);
     const int64_t s_beg = (int64_t)(row_lo & ~31) + it.skip;
     kend64 = min((int64_t)g_hi + 1, s_beg + it.len);
     kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
@@ -1470,11 +1497,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     }
     return;
   }
-  const int t0 = none ? 0 : (int)kbeg64, kend = none ? 0 : (int)kend64;
-  const int ntiles = (kend - t0 + 31) >> 5, nstep = (ntiles + 1) >> 1;
-  hi_c = min(hi_c, kend - 1);  // behind kend a step repeats its last tile
-  w_hi = min(w_hi, kend - 1);
-  const int f_lo = lanes_max<32>(ok ? lo_c : 0), f_hi = lanes_min<32>(ok ? hi_c : 0x7fffffff);  // seen by all
+  const int kbeg = none ? 0 : (int)kbeg64, kend = none ? 0 : (int)kend64;
   // byte offsets of this lane's 16 bytes of the operands: K row kk is key
   // 16 (kk / 16) + 8 ((kk / 4) % 2) + 4 ((kk / 8) % 2) + kk % 4 of the tile, V row kk is dim kk of 32
   const int key = ((kk >> 4) << 4) | (((kk >> 2) & 1) << 3) | (((kk >> 3) & 1) << 2) | (kk & 3);
@@ -1484,19 +1507,15 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
   const int64_t gofs = (int64_t)g * w.pv.page * HD;
   const float scale_log2 = w.scale * 1.4426950408889634f;
   const char *kp = (const char*)scalar(w.kp), *vp = (const char*)scalar(w.vp);
-  const int tpp = w.pv.page >> 5, tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
-  const const_ints list = CONST_INTS(pre ? w.pre : w.tables + (int64_t)b * w.W);
+  const int tpp = w.pv.page >> 5;
   f32x16 O[DD];
 #pragma unroll
   for (int dd = 0; dd < DD; ++dd)
 #pragma unroll
     for (int x = 0; x < 16; ++x) O[dd][x] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
-  // the walk over the pages, one tile at a time; the next page's entry is under way a page ahead
-  int tile = t0 >> 5, pg = pg0, tr = tile - pg * tpp;
-  int id = ntiles > 0 ? list[pg] : -1, id_next = ntiles > 0 ? list[min(pg + 1, pg_last)] : -1;
-  int now = 0, next = 0;  // bit u: the page of tile u of the step is one of the pool's
   bool odd = false;
+  __syncthreads();  // the rows' offsets in the stages have been read
   // each wave's loads of a tile: a quarter of K's slices and of V's dims
 #define WIDE_ISSUE(S_)                                                                                       \
   next = 0;                                                                                                  \
@@ -1536,111 +1555,126 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     __builtin_amdgcn_sched_barrier(0);                                                                       \
     __atomic_signal_fence(__ATOMIC_SEQ_CST);                                                                 \
   }
-  auto step = [&](const WideStage<HD>& S_, int in, int i) {
-    const int kb = t0 + 64 * i;
-    if (!(kb <= w_hi && kb + 63 >= w_lo)) return;
-    f32x16 sc[2];
+  // the prefix and then the row's own keys, or the one of them that this walk is over
+#pragma unroll 1
+  for (int part = walk == ROW_KEYS && w.joint > 0 ? 0 : 1; part < 2; ++part) {
+    const int from = part == 1 && walk == ROW_KEYS ? w.joint : 0;
+    const int t0 = max(kbeg - from, 0), t1 = part == 0 ? min(kend, w.P) : kend - from;
+    if (t0 >= t1) continue;
+    const int ntiles = (t1 - t0 + 31) >> 5, nstep = (ntiles + 1) >> 1;
+    const int tlast = (t0 >> 5) + ntiles - 1, pg0 = (t0 >> 5) / tpp, pg_last = tlast / tpp;
+    const const_ints list = CONST_INTS(pre || part == 0 ? w.pre : w.tables + (int64_t)b * w.W);
+    // keys that the column sees, that one of the wave does, that all of them do; behind t1 a step repeats its last tile
+    const int lo = lo_c - from, hi = min(hi_c - from, t1 - 1), a_lo = w_lo - from, a_hi = min(w_hi - from, t1 - 1);
+    const int f_lo = lanes_max<32>(ok ? lo : 0), f_hi = lanes_min<32>(ok ? hi : 0x7fffffff);
+    // the walk over the pages, one tile at a time; the next page's entry is under way a page ahead
+    int tile = t0 >> 5, pg = pg0, tr = tile - pg * tpp;
+    int id = list[pg], id_next = list[min(pg + 1, pg_last)];
+    int now = 0, next = 0;  // bit u: the page of tile u of the step is one of the pool's
+    auto step = [&](const WideStage<HD>& S_, int in, int i) {
+      const int kb = t0 + 64 * i;
+      if (!(kb <= a_hi && kb + 63 >= a_lo)) return;
+      f32x16 sc[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
-    v4u kf[DS][2], vf[2][DS];
+        for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
+      v4u kf[DS][2], vf[2][DS];
 #pragma unroll
-    for (int h = 0; h < DS; ++h)
+      for (int h = 0; h < DS; ++h)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) kf[h][u] = __builtin_bit_cast(v4u, S_.k[u][h][lane]);
-    __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < 2; ++u) kf[h][u] = __builtin_bit_cast(v4u, S_.k[u][h][lane]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int h = 0; h < DS; ++h)
+      for (int h = 0; h < DS; ++h)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) sc[u] = mfma32(kf[h][u], qf[h], sc[u]);
-    __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < 2; ++u) sc[u] = mfma32(kf[h][u], qf[h], sc[u]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u][f][lane]);
-    __builtin_amdgcn_sched_barrier(0);
-    if (!(kb >= f_lo && kb + 63 <= f_hi && in == 3)) {
-      u16x2 mag = {0, 0};
+        for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u][f][lane]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!(kb >= f_lo && kb + 63 <= f_hi && in == 3)) {
+        u16x2 mag = {0, 0};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bool there = (in >> u) & 1;
-        const int k0 = kb + 32 * u + 8 * hl;
-        const int lr = there ? lo_c - k0 : 64, hr = hi_c - k0;
+        for (int u = 0; u < 2; ++u) {
+          const bool there = (in >> u) & 1;
+          const int k0 = kb + 32 * u + 8 * hl;
+          const int lr = there ? lo - k0 : 64, hr = hi - k0;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int kx = 16 * (x >> 3) + (x & 7);
-          if (!(kx >= lr && kx <= hr)) sc[u][x] = -INFINITY;
+          for (int x = 0; x < 16; ++x) {
+            const int kx = 16 * (x >> 3) + (x & 7);
+            if (!(kx >= lr && kx <= hr)) sc[u][x] = -INFINITY;
+          }
+          // keys that no column of the wave sees: their weights are 0, and so have their V to be, which may be
+          // anything; then whether any is left that is not finite
+          const int zl = there ? a_lo - k0 : 64, zh = a_hi - k0;
+#pragma unroll
+          for (int f = 0; f < DS; ++f) {
+            const int kx = 16 * (f & 1);
+            v4u v = vf[u][f];
+            v.x &= key_mask(kx, zl, zh);
+            v.y &= key_mask(kx + 2, zl, zh);
+            v.z &= key_mask(kx + 4, zl, zh);
+            v.w &= key_mask(kx + 6, zl, zh);
+            mag = max_magnitude(max_magnitude(mag, v.x), v.y);
+            mag = max_magnitude(max_magnitude(mag, v.z), v.w);
+            vf[u][f] = v;
+          }
         }
-        // keys that no column of the wave sees: their weights are 0, and so have their V to be, which may be
-        // anything; then whether any is left that is not finite
-        const int zl = there ? w_lo - k0 : 64, zh = w_hi - k0;
-#pragma unroll
-        for (int f = 0; f < DS; ++f) {
-          const int kx = 16 * (f & 1);
-          v4u v = vf[u][f];
-          v.x &= key_mask(kx, zl, zh);
-          v.y &= key_mask(kx + 2, zl, zh);
-          v.z &= key_mask(kx + 4, zl, zh);
-          v.w &= key_mask(kx + 6, zl, zh);
-          mag = max_magnitude(max_magnitude(mag, v.x), v.y);
-          mag = max_magnitude(max_magnitude(mag, v.z), v.w);
-          vf[u][f] = v;
-        }
+        odd |= any_odd(mag);
       }
-      odd |= any_odd(mag);
-    }
-    float m4[4];
+      float m4[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) m4[x] = fmaxf(sc[0][x], sc[1][x]);
+      for (int x = 0; x < 4; ++x) m4[x] = fmaxf(sc[0][x], sc[1][x]);
 #pragma unroll
-    for (int x = 4; x < 16; ++x) m4[x & 3] = fmaxf(m4[x & 3], fmaxf(sc[0][x], sc[1][x]));
-    float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-    {
-      const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
-      mt = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // lanes l and l ^ 32: the column's two key halves
-    }
-    const float m_new = fmaxf(m_run, mt * scale_log2);
-    if (__any(m_new > m_run)) {
-      const float alpha = exp2a(m_run - (m_new == -INFINITY ? 0.f : m_new));
-      l_run *= alpha;
-#pragma unroll
-      for (int dd = 0; dd < DD; ++dd) O[dd] *= alpha;
-      m_run = m_new;
-    }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
-    float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
-        float pv[8];  // rounded to bf16 for the product, not in the sum
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          pv[x] = exp2a(fmaf(sc[u][8 * kh + x], scale_log2, -m_use));
-          ps[x & 3] += pv[x];
-        }
-        const v4u pb = v4u{pack2bf(pv[0], pv[1]), pack2bf(pv[2], pv[3]), pack2bf(pv[4], pv[5]), pack2bf(pv[6], pv[7])};
-#pragma unroll
-        for (int dd = 0; dd < DD; ++dd) O[dd] = mfma32(vf[u][2 * dd + kh], pb, O[dd]);
+      for (int x = 4; x < 16; ++x) m4[x & 3] = fmaxf(m4[x & 3], fmaxf(sc[0][x], sc[1][x]));
+      float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      {
+        const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        mt = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // lanes l and l ^ 32: the column's two key halves
       }
-    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-  };
-  __syncthreads();  // the rows' offsets in the stages have been read
-  if (ntiles > 0) {
+      const float m_new = fmaxf(m_run, mt * scale_log2);
+      if (__any(m_new > m_run)) {
+        const float alpha = exp2a(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        l_run *= alpha;
+#pragma unroll
+        for (int dd = 0; dd < DD; ++dd) O[dd] *= alpha;
+        m_run = m_new;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
+      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          float pv[8];  // rounded to bf16 for the product, not in the sum
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            pv[x] = exp2a(fmaf(sc[u][8 * kh + x], scale_log2, -m_use));
+            ps[x & 3] += pv[x];
+          }
+          const v4u pb =
+              v4u{pack2bf(pv[0], pv[1]), pack2bf(pv[2], pv[3]), pack2bf(pv[4], pv[5]), pack2bf(pv[6], pv[7])};
+#pragma unroll
+          for (int dd = 0; dd < DD; ++dd) O[dd] = mfma32(vf[u][2 * dd + kh], pb, O[dd]);
+        }
+      l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    };
     WIDE_ISSUE(stg[0]);
-  }
-  for (int i = 0; i < nstep; ++i) {
-    now = next;
-    WIDE_SYNC();
-    WIDE_ISSUE(stg[(i + 1) & 1]);
-    step(stg[i & 1], now, i);
+    for (int i = 0; i < nstep; ++i) {
+      now = next;
+      WIDE_SYNC();
+      WIDE_ISSUE(stg[(i + 1) & 1]);
+      step(stg[i & 1], now, i);
+    }
+    WIDE_SYNC();  // no direct load outlives its stage, no reader is left in the stages
   }
 #undef WIDE_SYNC
 #undef WIDE_ISSUE
-  __builtin_amdgcn_s_waitcnt(0);  // no direct load outlives its stage
-  if (__syncthreads_or(odd)) {    // (also: the stages become scratch)
-    redo_columns<bf16_t, HD>(pre, it, base, c0, min(c0 + 128, ncol), t0, kend, wave);
+  if (__syncthreads_or(odd)) {
+    redo_columns<bf16_t, HD>(walk, it, base, c0, min(c0 + 128, ncol), kbeg, kend, wave);
     return;
   }
   const PagedChunk c = chunk_args();
@@ -1720,14 +1754,14 @@ __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2)
     }
     if (pre) {
       if (at >= npre) return;
-      if constexpr (PRE == 0) wide_keys<HD, true>(c, lds.w, at);
+      if constexpr (PRE == 0) wide_keys<HD, PREFIX_KEYS>(c, lds.w, at);
       else stream_keys<T, HD, PRE, true>(c, lds.s, at);
       return;
     }
     if (at >= nown) return;
   }
   const PagedChunk o = PRE >= 0 ? chunk_args() : c;
-  if constexpr (OWN == 0) wide_keys<HD, false>(o, lds.w, at);
+  if constexpr (OWN == 0) wide_keys<HD, PRE < 0 ? ROW_KEYS : OWN_KEYS>(o, lds.w, at);
   else stream_keys<T, HD, OWN, false>(o, lds.s, at);
 }
 
@@ -1742,7 +1776,7 @@ constexpr int64_t kPartMax = 256ll << 20;  // bytes of partials a call may ask f
 struct PagedPlan {
   bool mfma;
   int own_qb, own_blk, pre_qb, pre_blk;
-  int S_own, S_pre, pre_chunk, target;
+  int S_own, S_pre, pre_chunk, target, joint;
   int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short
   int64_t part_bytes, ml_bytes, item_bytes;
 };
@@ -1778,12 +1812,23 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   kernel((int64_t)T * rep, a.pre_qb, a.pre_blk);
   a.mfma = (!a.own_qb || a.own_blk <= 65535) && (!a.pre_qb || a.pre_blk <= 65535);
   if (!a.mfma) return a;
-  // own keys
-  const int64_t width = (int64_t)W * p->page;
-  const int64_t longest = window > 0 ? std::min(width, (int64_t)window + max_per_row + 32) : width;
+  const int64_t width = (int64_t)W * p->page, pad = ((int64_t)P + 31) / 32 * 32;
   // (a row's last block may be short, so the tokens make up to one more block a row than they would side by side)
   const int cb = a.own_qb ? 16 * a.own_qb : 128;
   const int64_t units = G * std::min((int64_t)B * a.own_blk, (int64_t)T * rep / cb + B);
+  // Rows that fill column blocks of the wide kernel may walk the prefix themselves, which saves its partials and the
+  // merge, but cuts the work coarser and leaves the rows' last blocks part empty: done where they see little of it, or
+  // the blocks are several rounds of the card's 512 workgroups and not many more than the tokens fill. (92 rows of 490
+  // tokens, 8 heads on one, behind 7 keys: 167 us so, and 726 with the prefix walked for itself; 64 rows of up to 512,
+  // 12 heads, behind 2000: 441 and 542; but 16 such rows behind 4001, 516 blocks, 264 and 205, and 100 rows of up to
+  // 130 behind 8000 627 and 422.)
+  const int64_t cols = (int64_t)std::min(max_per_row, T) * rep, full = G * ((int64_t)T * rep / 128);
+  const bool rounds = units >= 3 * 512 && units <= full + full * 3 / 5;
+  const int seen = window > 0 ? std::min(P, window) : P;  // by tokens behind the prefix
+  if (P > 0 && !a.own_qb && cols >= 128 && (seen <= 1024 || rounds) && pad + width <= 0x7fffffff) a.joint = (int)pad;
+  // the rows' walks
+  const int64_t all = width + a.joint;
+  const int64_t longest = window > 0 ? std::min(all, (int64_t)window + max_per_row + 64) : all;
   const int64_t one = (int64_t)T * H * (p->head_dim + 2) * 4;
   const int64_t room = std::max<int64_t>(1, kPartMax / one);
   a.S_own = (int)std::min({(longest + 127) / 128, room, (int64_t)64});
@@ -1798,7 +1843,7 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   a.target = a.own_qb ? 768 : 256;
   const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;
   a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, cut);
-  if (P > 0) {
+  if (P > 0 && a.joint == 0) {
     a.S_pre = pre_splits(P, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
     a.pre_chunk = ((P + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
     a.S_pre = (P + a.pre_chunk - 1) / a.pre_chunk;
@@ -1822,9 +1867,9 @@ template <typename T, int HD>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   const int nown = (int)a.items, npre = (int)prefix_groups(a, c.pv.G);
   if (c.B > ROWS_SCAN) {
-    if (a.own_qb == 0) hipLaunchKernelGGL(k_paged_items<128>, dim3(1), dim3(1024), 0, s, c);
-    else if (a.own_qb == 2) hipLaunchKernelGGL(k_paged_items<32>, dim3(1), dim3(1024), 0, s, c);
-    else hipLaunchKernelGGL(k_paged_items<16>, dim3(1), dim3(1024), 0, s, c);
+    if (a.own_qb == 0) hipLaunchKernelGGL((k_paged_items<128, ROW_KEYS>), dim3(1), dim3(1024), 0, s, c);
+    else if (a.own_qb == 2) hipLaunchKernelGGL((k_paged_items<32, OWN_KEYS>), dim3(1), dim3(1024), 0, s, c);
+    else hipLaunchKernelGGL((k_paged_items<16, OWN_KEYS>), dim3(1), dim3(1024), 0, s, c);
     FC_LAUNCH_CHECK();
   }
   const dim3 grid(npre == 0 ? nown : 256 * ((npre + 255) / 256 + (nown + 255) / 256));
@@ -1896,7 +1941,7 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
   FC_CHECK_ARG(need == 0 || (work && work_bytes >= need), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
-               1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, (float*)work,
+               1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, a.joint, (float*)work,
                (float2*)((char*)work + a.part_bytes), (int*)((char*)work + a.part_bytes + a.ml_bytes),
                q, pages->k, pages->v, y};
   const hipStream_t s = (hipStream_t)stream;

@@ -586,3 +586,37 @@ def test_last_positions(dtype, n, window):
     got = _run(c, q, window, dict(a, tables=tables, start=up([32 * W - n])))
     ref, tol = c.reference(q, window)
     _check(got, ref, tol)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("window", [0, 30])
+def test_many_rows_and_a_long_one(hd, window):
+    """300 rows of few tokens and one of column blocks, behind 40 keys."""
+    _say(f"paged_attention hd={hd} window {window}: 300 rows, one long")
+    n = np.arange(300) % 4
+    n[150] = 130
+    c = Paged(37, np.arange(300) * 7 % 50, n, 40, 2, hd, 32, torch.bfloat16)
+    q = c.queries(2, tail=1)
+    ref, tol = c.reference(q, window)
+    _check(_run(c, q, window), ref, tol)
+
+
+@pytest.mark.parametrize("hd,window", [(128, 1000), (64, 0)])
+def test_many_blocks_behind_a_long_prefix(hd, window):
+    """Full column blocks for several rounds of workgroups, which then walk a
+    prefix past 1024 keys themselves."""
+    _say(f"paged_attention hd={hd} window {window}: many blocks behind 1100 keys")
+    n = [16] * 97
+    n[3], n[90] = 15, 0
+    c = Paged(41, np.arange(97) * 7 % 50, n, 1100, 16, hd, 32, torch.bfloat16)
+    q = c.queries(128, tail=1)
+    got = _run(c, q, window)
+    rows = [2, 3, 4, 90, 91, 96]  # of which the result is looked at
+    sub = Paged.__new__(Paged)
+    sub.__dict__.update(c.__dict__)
+    sub.n = np.where(np.isin(np.arange(97), rows), c.n, 0)
+    ref, tol = sub.reference(q, window)
+    at = np.concatenate([np.arange(c.off[b], c.off[b + 1]) for b in rows])
+    _check(got[at], ref[at], tol[at])
+    whole = got[:int(c.off[-1])]
+    assert torch.isfinite(whole).all() and (whole != 0).any(1).all()

@@ -1343,7 +1343,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
       u[k][1] = *(const float4*)(c.po + i * HD + d0 + 4);
     }
   };
-  if (!done) load(0);
+  if (!done && n > 0) load(0);  // (n = 0: no split holds a key, or a token of no row)
   __syncthreads();
   if (pair >= pairs) return;
   const int t = (int)(pair / c.H), b = row_of(off, c.B, t);

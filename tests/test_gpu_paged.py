@@ -620,3 +620,36 @@ def test_many_blocks_behind_a_long_prefix(hd, window):
     _check(got[at], ref[at], tol[at])
     whole = got[:int(c.off[-1])]
     assert torch.isfinite(whole).all() and (whole != 0).any(1).all()
+
+
+@pytest.mark.parametrize("fill", [(-INF, 0.0), (NAN, NAN), (0.0, -1.0)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("ctx,n,P", [([3000, 5, 700], [1, 3, 2], 0), ([3000, 5, 700], [1, 3, 2], 40),
+                                     ([2500, 5, 0], [140, 3, 20], 33)])
+def test_workspace_holds_anything(fill, dtype, ctx, n, P):
+    """What an earlier call left in the workspace (marks of pieces without
+    keys, of whole ones) decides nothing, for tokens behind the last row
+    either."""
+    from flaxchat_amd import _lib
+    _say(f"paged_attention {dtype}: workspace full of {fill}, prefix {P}")
+    c = Paged(43, ctx, n, P, 2, 128, 32, DT[dtype])
+    q = c.queries(4, tail=5)
+    ref, tol = c.reference(q, 0)
+    a, T, most = c.device(dev()), len(q), int(max(n))
+    qt = torch.from_numpy(q).to(dev(), c.dtype)
+    N, G, page, hd = a["k"].shape
+    p = _lib.FcPages(a["k"].data_ptr(), a["v"].data_ptr(), G * page * hd, G * page * hd, N, G, page, hd,
+                     1 if dtype == "bf16" else 0)
+    L = _lib.lib()
+    nb = L.fc_paged_attention_workspace_bytes(p, 3, T, most, 4, c.W, P, 0)
+    assert nb > 0
+    room = torch.tensor(fill, device=dev()).repeat(nb // 4 + 1024)  # the middle half is the call's
+    at = (room.numel() - nb // 4) // 2 // 64 * 64
+    ws = room[at:at + nb // 4]
+    y = torch.full((T, 4 * 128), 7.0, device=dev(), dtype=c.dtype)
+    _lib.check(L.fc_paged_attention(p, qt.data_ptr(), 512, 128, y.data_ptr(), 3, T, most, 4, a["tables"].data_ptr(),
+                                    c.W, a["row_off"].data_ptr(), a["start"].data_ptr(), a["pre"].data_ptr() or None,
+                                    P, 0, 1, ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    _check(y, ref, tol)
+    assert torch.all(y[int(c.off[-1]):] == 0)

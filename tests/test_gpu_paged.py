@@ -653,3 +653,17 @@ def test_workspace_holds_anything(fill, dtype, ctx, n, P):
     torch.cuda.synchronize()
     _check(y, ref, tol)
     assert torch.all(y[int(c.off[-1]):] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 45])
+@pytest.mark.parametrize("window", [70, 300])
+def test_windows_far_apart_in_the_prefix(dtype, n, window):
+    """Rows that begin within the prefix, a thousand positions from each
+    other: one column block's windows lie all over it."""
+    _say(f"paged_attention {dtype}: rows of {n} at 100, 1000, 1990 and 2050, window {window}")
+    c = Paged(47, [0, 0, 0, 50], [n] * 4, 2000, 2, 128, 32, DT[dtype])
+    c.start = np.array([100, 1000, 1990, 2050], np.int32)
+    q = c.queries(4)
+    ref, tol = c.reference(q, window)
+    _check(_run(c, q, window), ref, tol)

@@ -1389,10 +1389,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {
 // SIMD hide a part (16 rows of 512 tokens behind 8000 shared keys 510 us, 0.81
 // PFLOP/s; a library matrix product reaches 1.23). With few steps a workgroup the
 // start and the end weigh in: behind 4001 keys, 4482 tokens of unequal rows, 205 us,
-// 0.61 PFLOP/s. Tried and slower: a row's prefix and own keys in one walk, which
-// saves the merge but cuts the work in pieces too large to fill the card evenly (275
-// us); the maximum left behind by up to 2^8, to scale the sums less often, gave 4% and
-// cost precision, as the largest weight is then no longer 1.
+// 0.61 PFLOP/s. Tried: the maximum left behind by up to 2^8, to scale the sums less
+// often, gave 4% and cost precision, as the largest weight is then no longer 1.
 template <int HD>
 struct WideStage {
   uint4 k[2][HD / 16][64];  // [32-key tile][16-dim slice][lane]
@@ -1525,8 +1523,8 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     const bool is = (unsigned)id < (unsigned)w.pv.N;                                                         \
     next |= (int)is << u;                                                                                    \
     const int64_t pid = is ? id : 0; /* no page: page 0's place is read and masked */                        \
-    const bf16_t* kt = (const bf16_t*)kp + pid * w.pv.ks + gofs + tr * (32 * HD);                          \
-    const bf16_t* vt = (const bf16_t*)vp + pid * w.pv.vs + gofs + tr * (32 * HD);                          \
+    const bf16_t* kt = (const bf16_t*)kp + pid * w.pv.ks + gofs + tr * (32 * HD);                            \
+    const bf16_t* vt = (const bf16_t*)vp + pid * w.pv.vs + gofs + tr * (32 * HD);                            \
     if constexpr (HD == 128) {                                                                               \
       const uint32_t lk = LDS_ADDR(S_.k[u][0]) + 2048 * wave, lv = LDS_ADDR(S_.v[u][0]) + 2048 * wave;       \
       lds_load_1k(kt + 1024 * wave, koff, lk);                                                               \

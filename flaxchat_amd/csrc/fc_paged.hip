@@ -1305,7 +1305,7 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& 
 // dimensions each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. The
 // splits' (max, sum) are read side by side, ahead of the token's row; then the
 // outputs of those that hold keys, CB at a time. Bound by the reading of the
-// partials: 4482 tokens of 12 heads with three of them 18 us, 5.4 TB/s; with few
+// partials: 4482 tokens of 12 heads with three of them 17 us, 5.7 TB/s; with few
 // tokens by the launch and three waits, 5 us.
 template <typename T, int HD, int CB>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedChunk c) {

@@ -667,3 +667,37 @@ def test_windows_far_apart_in_the_prefix(dtype, n, window):
     q = c.queries(4)
     ref, tol = c.reference(q, window)
     _check(_run(c, q, window), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_two_calls_at_once_and_replays(dtype):
+    """A captured call over many rows replayed on one stream while others of
+    other shapes run on a second one: each as it is alone, bit for bit."""
+    _say(f"paged_attention {dtype}: two streams, a graph of 300 rows")
+    n = np.arange(300) % 4
+    n[150] = 130
+    big = Paged(37, np.arange(300) * 7 % 50, n, 40, 2, 128, 32, DT[dtype])
+    small = Paged(53, [3000, 5, 700], [1, 3, 2], 333, 2, 128, 32, DT[dtype])
+    calls = []
+    for c in (big, small):
+        a, q = c.device(dev()), torch.from_numpy(c.queries(4, tail=1)).to(dev(), c.dtype)
+        calls.append(lambda c=c, a=a, q=q: _run(c, None, 100, a, qt=q))
+    alone = [f().clone() for f in calls]
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(one):
+        calls[0]()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=one):
+        y = calls[0]()
+    for _ in range(4):
+        y.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            graph.replay()
+        with torch.cuda.stream(two):
+            got = [calls[1]() for _ in range(3)] + [calls[0]()]
+        torch.cuda.synchronize()
+        assert torch.equal(y, alone[0]) and torch.equal(got[3], alone[0])
+        assert all(torch.equal(g, alone[1]) for g in got[:3])

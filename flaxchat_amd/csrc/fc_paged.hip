@@ -1788,12 +1788,12 @@ struct PagedPlan {
 // the merge. Against the best of S = 1 .. 40 its choice costs 5% or less in 10 of 13
 // measured shapes and 16% at most (prefixes of 1000 to 16000 keys under 1 to 4482
 // tokens: 18 to 212 us).
-int pre_splits(int P, int G, int blk, int64_t part_bytes, int most, bool fp32) {
+int pre_splits(int64_t P, int G, int blk, int64_t part_bytes, int most, bool fp32) {
   int best = 1;
   double least = 1e30;
-  for (int S = 1; S <= std::min(most, (P + 127) / 128); ++S) {
+  for (int S = 1; S <= std::min<int64_t>(most, (P + 127) / 128); ++S) {
     const int64_t on = (int64_t)((G * S + 7) / 8) * blk;
-    const double steps = ((P + S - 1) / S + 63) / 64 * (fp32 ? 2 : 1) + 6;
+    const double steps = (double)(((P + S - 1) / S + 63) / 64 * (fp32 ? 2 : 1) + 6);
     const double t = on * steps * 2.0 / 64 + steps * 0.6 + S * (0.2 + (double)part_bytes * 2 / 5e6);
     if (t < least) least = t, best = S;
   }
@@ -1847,10 +1847,12 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
     // The splits are counted from the first key that a column block sees: all of the prefix, or, by tokens behind it,
     // the window's end. The last one takes what is left, for rows that begin within the prefix. (7 rows of 9 tokens, 8
     // heads on one, fp32, a window of 1024 over 12268 keys: 85 us with splits of the whole prefix, 25 so.)
-    const int over = window > 0 ? (int)std::min<int64_t>(P, (int64_t)window + 32) : P;
-    a.S_pre = pre_splits(over, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
-    a.pre_chunk = ((over + a.S_pre - 1) / a.S_pre + 63) / 64 * 64;
-    a.S_pre = (over + a.pre_chunk - 1) / a.pre_chunk;
+    // (in 64 bits: a prefix may have up to 2^31 - 33 positions)
+    const int64_t over = window > 0 ? std::min<int64_t>(P, (int64_t)window + 32) : P;
+    const int S = pre_splits(over, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
+    const int64_t chunk = ((over + S - 1) / S + 63) / 64 * 64;
+    a.S_pre = (int)((over + chunk - 1) / chunk);
+    a.pre_chunk = (int)std::min<int64_t>(chunk, 0x7fffffc0);  // (below the chunk with one split alone, which takes all)
   }
   if (a.S_own + a.S_pre > 1) {
     const int64_t pairs = (int64_t)T * H * (a.S_own + a.S_pre);
@@ -1911,12 +1913,28 @@ int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
 }
 }  // namespace
 
+// What the plan's arithmetic and the launches are made for. (A launch's threads are counted in 32 bits along x, its
+// workgroups in 16 along y.)
+static constexpr int64_t kMostGroups = (1 << 24) - 1024;
+static int check_sizes(const fc_pages* p, int32_t batch, int32_t max_tokens, int32_t max_per_row, int32_t n_head,
+                       int32_t width, int32_t prefix_len, int32_t window) {
+  FC_CHECK_ARG(batch > 0 && batch <= PT_ROWS, "batch must be in [1, 4096]");
+  FC_CHECK_ARG(max_tokens > 0 && max_per_row > 0 && n_head > 0 && n_head % p->n_kv_head == 0,
+               "max_tokens, max_per_row, n_head (a multiple of n_kv_head)");
+  FC_CHECK_ARG(n_head <= 65535, "n_head must be <= 65535");
+  FC_CHECK_ARG(window >= 0 && prefix_len >= 0, "window, prefix");
+  FC_CHECK_ARG(width > 0 && (int64_t)width * p->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
+  const int64_t merge = (int64_t)max_tokens * n_head * (p->head_dim / 8) / 256;
+  FC_CHECK_ARG(std::max<int64_t>(merge, max_tokens) < kMostGroups, "too many tokens or heads");
+  return FC_OK;
+}
+
 extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
                                                       int32_t max_per_row, int32_t n_head, int32_t width,
                                                       int32_t prefix_len, int32_t window) {
-  if (check_pages(pages) != FC_OK) return FC_ERR_ARG;
-  FC_CHECK_ARG(batch > 0 && max_tokens > 0 && max_per_row > 0 && n_head > 0 && n_head % pages->n_kv_head == 0 &&
-                   width > 0 && prefix_len >= 0 && window >= 0, "sizes");
+  if (check_pages(pages) != FC_OK ||
+      check_sizes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window) != FC_OK)
+    return FC_ERR_ARG;
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
   return a.part_bytes + a.ml_bytes + a.item_bytes;
 }
@@ -1927,20 +1945,14 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
                                       const int32_t* row_off, const int32_t* start, const int32_t* prefix_pages,
                                       int32_t prefix_len, int32_t window, int32_t flags, void* work,
                                       int64_t work_bytes, void* stream) {
-  const int rc = check_pages(pages);
+  int rc = check_pages(pages);
   if (rc != FC_OK) return rc;
   FC_CHECK_ARG(q && y && tables && row_off && start, "null pointer");
-  FC_CHECK_ARG(batch > 0 && batch <= PT_ROWS, "batch must be in [1, 4096]");
-  FC_CHECK_ARG(max_tokens > 0 && max_per_row > 0 && n_head > 0 && n_head % pages->n_kv_head == 0,
-               "max_tokens, max_per_row, n_head (a multiple of n_kv_head)");
-  FC_CHECK_ARG(n_head <= 65535, "n_head must be <= 65535");
-  FC_CHECK_ARG(window >= 0 && prefix_len >= 0 && (prefix_len == 0 || prefix_pages), "window, prefix");
-  FC_CHECK_ARG(width > 0 && (int64_t)width * pages->page + prefix_len <= 0x7fffffff, "positions must fit 31 bits");
+  rc = check_sizes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  if (rc != FC_OK) return rc;
+  FC_CHECK_ARG(prefix_len == 0 || prefix_pages, "window, prefix");
   const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
-  // a launch's threads are counted in 32 bits along x, its workgroups in 16 along y
-  const int64_t merge = (int64_t)max_tokens * n_head * (pages->head_dim / 8) / 256;
-  FC_CHECK_ARG(std::max({a.items + prefix_groups(a, pages->n_kv_head), merge, (int64_t)max_tokens}) < (1 << 24) - 1024,
-               "too many tokens, rows or heads");
+  FC_CHECK_ARG(a.items + prefix_groups(a, pages->n_kv_head) < kMostGroups, "too many tokens, rows or heads");
   const int64_t need = a.part_bytes + a.ml_bytes + a.item_bytes;
   FC_CHECK_ARG(need == 0 || (work && work_bytes >= need), "workspace too small");
   PagedChunk c{page_view(pages), tables, row_off, start, prefix_pages, batch, n_head, width, prefix_len, window,

@@ -1,0 +1,45 @@
+"""The paged-cache operators at the ends of what they accept, without a GPU:
+how a call is cut (its workspace) and what is refused. Nothing is launched."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from flaxchat_amd import _lib  # noqa: E402
+
+P_MOST = 2 ** 31 - 1 - 32  # with a table of one page of 32 positions: the longest prefix accepted
+
+
+def pages(G=1, hd=128, page=32, n_pages=4, dtype=_lib.FC_BF16):
+    each = G * page * hd
+    return _lib.FcPages(0x1000, 0x1000, each, each, n_pages, G, page, hd, dtype)
+
+
+def workspace(p, B, T, most, H, W, P, window=0):
+    return _lib.lib().fc_paged_attention_workspace_bytes(p, B, T, most, H, W, P, window)
+
+
+@pytest.mark.parametrize("dtype", [_lib.FC_BF16, _lib.FC_F32])
+@pytest.mark.parametrize("B,T,most,G,H,window", [
+    (1, 1, 1, 1, 1, 0), (1, 1, 1, 8, 8, 0), (64, 64, 1, 12, 12, 0), (40, 4096, 100, 12, 12, 0), (4, 8, 2, 2, 8, 0),
+    (1, 1, 1, 1, 1, 2 ** 31 - 1), (300, 4000, 40, 4, 12, 2 ** 31 - 40),
+])
+def test_workspace_of_long_prefixes(dtype, B, T, most, G, H, window):
+    """A prefix has at least one split, the own keys another: room for both
+    whatever the prefix's length, up to the last one accepted."""
+    p = pages(G, dtype=dtype)
+    two = 2 * T * H * (128 + 2) * 4
+    lengths = [1, 127, 128, 129, 10 ** 6, 1908874305, 2130836481, 2 ** 31 - 200, 2 ** 31 - 129, 2 ** 31 - 97, P_MOST - 1,
+               P_MOST]
+    lengths += range(2 ** 31 - 40 * 10 ** 6, P_MOST, 1234567)
+    for P in lengths:
+        nb = workspace(p, B, T, most, H, 1, P, window)
+        assert nb >= two, (P, nb)
+
+
+def test_workspace_refuses_what_the_call_does():
+    p = pages()
+    assert workspace(p, 1, 1, 1, 1, 1, P_MOST) > 0
+    for bad in (dict(P=P_MOST + 1), dict(W=2 ** 26), dict(B=4097), dict(H=65536), dict(T=1 << 24), dict(window=-1),
+                dict(T=1 << 22, H=60000)):
+        assert workspace(p, **{**dict(B=1, T=1, most=1, H=1, W=1, P=0), **bad}) < 0, bad

@@ -922,10 +922,12 @@ __device__ __forceinline__ void redo_columns(int walk, const Item& it, int base,
       const int from = part == 1 && walk == ROW_KEYS ? c.joint : 0;
       const int lo = max(v_lo - from, 0), hi = part == 0 ? min(v_hi, c.P - 1) : v_hi - from;
       const int* list = pre || part == 0 ? c.pre : c.tables + (int64_t)b * c.W;
-      for (int k0 = lo; k0 <= hi; k0 += 64) {
-        const int key = k0 + lane, pg = min(key, hi) / c.pv.page, at = min(key, hi) - pg * c.pv.page;
+      // (counted by what is left: a key behind hi may not fit 31 bits)
+      for (int left = hi - lo + 1; left > 0; left -= 64) {
+        const int key = hi + 1 - left + min(lane, left - 1), pg = key / c.pv.page, at = key - pg * c.pv.page;
         const int id = list[pg];
-        const bool ok = key <= hi && (unsigned)id < (unsigned)c.pv.N;
+        const bool ok = lane < left && (unsigned)id < (unsigned)c.pv.N;
+        if (!__any(ok)) continue;
         float s = -INFINITY;
         if (ok) {
           float a = 0.f;

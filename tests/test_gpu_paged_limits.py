@@ -1,0 +1,58 @@
+"""paged_attention at the ends of what it accepts, and where the tests of
+tests/test_gpu_paged.py cannot tell: against the softmax in 64 bits, and
+against whole numbers that one key more or less changes."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.paged_cases import Paged  # noqa: E402
+from tests.test_gpu_kernels import _say  # noqa: E402
+from tests.test_gpu_paged import DT, INF, OPS, _check, _run, dev, up  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,window", [(3, 20), (3, 90), (3, 0), (45, 5), (45, 20)])
+def test_last_positions_with_values_not_finite(dtype, n, window):
+    """The last positions of a table of 2^31 - 32, whose last two V are infinite: the
+    queries ahead of those go over their keys in the plain form, whose
+    arithmetic has to end at the last position."""
+    _say(f"paged_attention {dtype}: {n} tokens at the last positions, window {window}, V not finite")
+    W = 2 ** 26 - 1
+    c = Paged(31, [64 - n], [n], 0, 2, 128, 32, DT[dtype], extra=2)  # 64 positions: the last two pages
+    q = c.queries(4)
+    ref, tol = c.reference(q, window)
+    c.V[c.tables[0, 1], :, 30:] = INF
+    a = c.device(dev())
+    tables = torch.full((1, W), -1, dtype=torch.int32, device=dev())
+    tables[0, -2:] = a["tables"][0]
+    got = _run(c, q, window, dict(a, tables=tables, start=up([32 * W - n])))
+    _check(got[:n - 2], ref[:n - 2], tol[:n - 2])
+    assert not torch.isfinite(got[n - 2:]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,n", [(1, 3), (2, 9)])
+@pytest.mark.parametrize("inside,window", [(False, 0), (False, 40), (True, 0), (True, 17)])
+def test_longest_prefix(dtype, B, n, inside, window):
+    """A prefix of 2^31 - 33 positions, of which the last 63 are held: rows
+    behind it, and rows that begin in it ahead of a V that is infinite."""
+    P = 2 ** 31 - 33
+    _say(f"paged_attention {dtype}: {B} rows of {n} {'within' if inside else 'behind'} the longest prefix, {window}")
+    c = Paged(59, [10 + b for b in range(B)], [n] * B, 63, 2, 128, 32, DT[dtype])
+    c.start = np.array([63 - n if inside else 63 + 10 + b for b in range(B)], np.int32)
+    q = c.queries(4)
+    ref, tol = c.reference(q, window)
+    if inside:  # the last position is a row's last query's alone
+        c.V[c.pre_ids[1], :, 30] = INF
+    a = c.device(dev())
+    pre = torch.full((2 ** 26 - 1,), -1, dtype=torch.int32, device=dev())
+    pre[-2:] = a["pre"]
+    got = OPS.paged_attention(torch.from_numpy(q).to(dev(), c.dtype), a["k"], a["v"], a["tables"], a["row_off"],
+                              up(c.start.astype(np.int64) + (P - 63)), n, window, pre, P)
+    keep = np.arange(len(q)) % n < (n - 1 if inside else n)
+    _check(got[keep], ref[keep], tol[keep])
+    assert not torch.isfinite(got[~keep]).any()

@@ -40,7 +40,8 @@ DeviceModel) and everything they write as tensors, declared mutated:
 The paged KV cache (one layer; k_pages [n_pages][n_kv_head][page][head_dim]
 and v_pages [n_pages][n_kv_head][page / 32][head_dim][32] in the caches' block
 order, whose pages may be strided, as those of one layer of a pool of all
-layers are; every index tensor int32):
+layers are; every index tensor int32). None has a backward pass: tensors that require a gradient are refused
+where gradients are recorded, and what a call writes counts as modified in place:
   page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots,
               page, prefix_len=0)
                                      block tables, packed chunk and slot map of a step from the rows'
@@ -502,6 +503,10 @@ def _launch(name: str, device: int, fn, *args):
         check(rc, name)
 
 
+# Takes what an operator writes, so that autograd notices if it had kept one of them: nothing else does below custom_op.
+_written = torch.autograd.graph.increment_version
+
+
 def _inner_contiguous(t: torch.Tensor) -> bool:
     """Whether t[0] is contiguous."""
     want = 1
@@ -556,12 +561,15 @@ def page_tables(tables, held, free_pages, n_free, length, n_new, row_off, start,
     if page < 32 or page % 32 != 0 or prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
         raise ValueError("page_tables: page a multiple of 32, prefix_len >= 0, positions below 2^31")
     ts = (tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots)
-    i32 = torch.int32
-    for i, (t, n) in enumerate(zip(ts, (B * W, B, F, 1, B, B, B + 1, B, T, T, T))):
-        if t.dtype is not i32 or t.numel() != n or not t.is_contiguous():
-            _index("page_tables", ("tables", "held", "free_pages", "n_free", "length", "n_new", "row_off", "start",
-                                   "tok_row", "tok_pos", "slots")[i], t, n)
-    d = _on_gpu("page_tables", *ts)
+    sizes = (B * W, B, F, 1, B, B, B + 1, B, T, T, T)
+    i32, d = torch.int32, tables.get_device()
+    for t, n in zip(ts, sizes):  # (one walk over the arrays: their checks are most of a call's time)
+        if t.dtype is not i32 or t.numel() != n or not t.is_contiguous() or t.get_device() != d or d < 0:
+            for what, t, n in zip(("tables", "held", "free_pages", "n_free", "length", "n_new", "row_off", "start",
+                                   "tok_row", "tok_pos", "slots"), ts, sizes):
+                _index("page_tables", what, t, n)
+            _on_gpu("page_tables", *ts)
+    _written((tables, held, free_pages, n_free, row_off, start, tok_row, tok_pos, slots))
     _launch("fc_page_tables", d, lib().fc_page_tables, *[t.data_ptr() for t in ts], B, W, F, T, page, prefix_len)
 
 
@@ -572,11 +580,15 @@ def page_append(k, v, slots, k_pages, v_pages):
         raise ValueError(f"page_append: k and v [tokens][{G}][{hd}] (got {tuple(k.shape)} and {tuple(v.shape)})")
     if k.dtype != v.dtype or (k.dtype != k_pages.dtype and k.dtype != torch.float32):
         raise ValueError(f"page_append: k and v in the pages' dtype or fp32 (got {k.dtype} and {v.dtype})")
+    if (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and \
+            torch.is_grad_enabled():
+        raise ValueError("page_append has no backward pass")
     M = k.shape[0]
     _index("page_append", "slots", slots, M)
     d = _on_gpu("page_append", k_pages, v_pages, k, v, slots)
     if M == 0:
         return
+    _written((k_pages, v_pages))
     kt, kh, kd = k.stride()
     vt, vh, vd = v.stride()
     if hd != 1 and (kd != 1 or vd != 1):
@@ -640,12 +652,12 @@ def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, wi
 
 @torch.library.register_fake(f"{NS}::page_tables", lib=_PAGED)
 def _(tables, held, free_pages, n_free, length, n_new, row_off, start, tok_row, tok_pos, slots, page, prefix_len=0):
-    return None
+    _written((tables, held, free_pages, n_free, row_off, start, tok_row, tok_pos, slots))
 
 
 @torch.library.register_fake(f"{NS}::page_append", lib=_PAGED)
 def _(k, v, slots, k_pages, v_pages):
-    return None
+    _written((k_pages, v_pages))
 
 
 @torch.library.register_fake(f"{NS}::paged_attention", lib=_PAGED)

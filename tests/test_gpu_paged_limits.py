@@ -56,3 +56,26 @@ def test_longest_prefix(dtype, B, n, inside, window):
     keep = np.arange(len(q)) % n < (n - 1 if inside else n)
     _check(got[keep], ref[keep], tol[keep])
     assert not torch.isfinite(got[~keep]).any()
+
+
+def test_written_tensors_are_seen_by_autograd():
+    """A pool that autograd keeps for a backward pass and that page_append then
+    writes to is noticed there, as are the tables that page_tables writes."""
+    _say("page_append, page_tables: versions")
+    f = dict(device=dev(), dtype=torch.float32)
+    kp, vp = torch.ones(2, 1, 32, 128, **f), torch.ones(2, 1, 1, 128, 32, **f)
+    x = torch.ones_like(kp, requires_grad=True)
+    y = (x * kp).sum()
+    k = torch.ones(1, 1, 128, **f)
+    OPS.page_append(k, k, up([3]), kp, vp)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="backward"):
+        OPS.page_append(k, k.clone().requires_grad_(), up([3]), kp, vp)
+    s = [up(a) for a in ([[-1, -1]], [0], [0, 1], [2], [0], [1], [0, 0], [0], [0], [0], [0])]
+    OPS.page_tables(*s, 32, 0)
+    assert [t._version for t in s] == [1, 1, 1, 1, 0, 0, 1, 1, 1, 1, 1]
+    with torch.inference_mode():  # tensors made here have no version
+        kp, vp, k = torch.ones(2, 1, 32, 128, **f), torch.ones(2, 1, 1, 128, 32, **f), torch.zeros(1, 1, 128, **f)
+        OPS.page_append(k, k, up([3]), kp, vp)
+        assert int((kp == 0).sum()) == 128 and int((vp == 0).sum()) == 128

@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import flaxchat_amd.torch_ops  # noqa: E402,F401
 from flaxchat_amd import _lib  # noqa: E402
 
 P_MOST = 2 ** 31 - 1 - 32  # with a table of one page of 32 positions: the longest prefix accepted
@@ -43,3 +44,41 @@ def test_workspace_refuses_what_the_call_does():
     for bad in (dict(P=P_MOST + 1), dict(W=2 ** 26), dict(B=4097), dict(H=65536), dict(T=1 << 24), dict(window=-1),
                 dict(T=1 << 22, H=60000)):
         assert workspace(p, **{**dict(B=1, T=1, most=1, H=1, W=1, P=0), **bad}) < 0, bad
+
+
+# ---------------------------------------------------------------- autograd
+OPS = torch.ops.flaxchat_mi355x
+
+
+def append_args(**kw):
+    a = dict(k=torch.zeros(5, 3, 128), v=torch.zeros(5, 3, 128), slots=torch.zeros(5, dtype=torch.int32),
+             k_pages=torch.zeros(4, 3, 64, 128), v_pages=torch.zeros(4, 3, 2, 128, 32))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_pages", "v_pages"])
+def test_append_refuses_gradients(name):
+    """There is no backward pass, so a gradient is refused, not dropped; where
+    none is recorded the call goes on (here to the check of the device)."""
+    a = append_args()
+    a[name] = a[name].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        OPS.page_append(*a.values())
+    for off in (torch.no_grad, torch.inference_mode):
+        with off(), pytest.raises(ValueError, match="CUDA"):
+            OPS.page_append(*a.values())
+
+
+def test_versions_of_what_is_written():
+    """Autograd finds a tensor that it kept and that the operators then wrote to."""
+    m = lambda *s: torch.zeros(*s, dtype=torch.int32, device="meta")  # noqa: E731
+    a = {k: t.to("meta") for k, t in append_args().items()}
+    OPS.page_append(*a.values())
+    assert {k: t._version for k, t in a.items()} == dict(k=0, v=0, slots=0, k_pages=1, v_pages=1)
+    t = [m(3, 4), m(3), m(9), m(1), m(3), m(3), m(4), m(3), m(6), m(6), m(6)]
+    OPS.page_tables(*t, 64, 0)
+    assert [x._version for x in t] == [1, 1, 1, 1, 0, 0, 1, 1, 1, 1, 1]
+    with torch.inference_mode():  # which has no versions
+        a = {k: t.to("meta") for k, t in append_args().items()}
+        OPS.page_append(*a.values())

@@ -768,10 +768,10 @@ __device__ __forceinline__ int chunk_length(const PagedChunk& c, float total, in
   const uint32_t len = (max((uint32_t)fminf(share, (float)(CB == 128 ? CHUNK_WIDE : CHUNK_MAX)), least) + 63) & ~63u;
   return __builtin_amdgcn_readfirstlane((int)min(len, 0x7fffffe0u));
 }
-// pieces of a row: its keys / chunk, at least one
+// pieces of a row: its keys / chunk, at least one (past 2^24 keys it may be one too few, never too many)
 __device__ __forceinline__ int row_pieces(const RowKeys& r, int chunk) {
   const uint32_t len = max(r.len, 0), by = chunk;
-  uint32_t ns = (uint32_t)((float)len * (1.f / (float)chunk));  // one off at most
+  uint32_t ns = (uint32_t)((float)len * (1.f / (float)chunk));
   ns += ns * by < len;
   return max(1, (int)(ns - (ns > 1 && (ns - 1) * by >= len)));
 }
@@ -789,8 +789,9 @@ __device__ __forceinline__ bool item_of(const PagedChunk& c, int& at, int r0, co
   // (the walk's addresses are scalar: said so here, since the compiler loses track of it where the ways here meet)
   it.b = __builtin_amdgcn_readfirstlane(r0 + l);
   it.nsplit = __builtin_amdgcn_readlane(ns, l);
-  // pieces of one length (no longer than the chunk, so none is empty)
-  it.len = it.nsplit > 1 ? ((__builtin_amdgcn_readlane(r.len, l) - 1) / it.nsplit + 64) & ~63 : chunk;
+  // pieces of one length, that of the row's keys and not of the chunk (about no longer than it, so none is empty); a
+  // row's only piece takes all
+  it.len = it.nsplit > 1 ? ((__builtin_amdgcn_readlane(r.len, l) - 1) / it.nsplit + 64) & ~63 : 0x7fffffe0;
   const int unit = __builtin_amdgcn_readfirstlane(at) / c.pv.G;
   it.g = __builtin_amdgcn_readfirstlane(at) - unit * c.pv.G;
   it.blk = __builtin_amdgcn_readlane(r.blocks, l) - 1 - unit / it.nsplit;  // (later queries see more keys: first)

@@ -79,3 +79,20 @@ def test_written_tensors_are_seen_by_autograd():
         kp, vp, k = torch.ones(2, 1, 32, 128, **f), torch.ones(2, 1, 1, 128, 32, **f), torch.zeros(1, 1, 128, **f)
         OPS.page_append(k, k, up([3]), kp, vp)
         assert int((kp == 0).sum()) == 128 and int((vp == 0).sum()) == 128
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [1, 30])
+def test_a_row_of_one_key_more_than_a_piece(dtype, n):
+    """Beside a row of 1.69e9 positions, of which a 64th is a piece, one of one
+    key more than that: float has no room for the one, the sums have to."""
+    piece = 26433600
+    _say(f"paged_attention {dtype}: {n} tokens up to key {piece}")
+    c = Paged(61, [0, 97 - n], [1, n], 0, 2, 128, 32, DT[dtype])
+    q = c.queries(4)
+    ref, tol = c.reference(q, 0, gone=[(0, 0)])  # the long row holds no page at all
+    a = c.device(dev())
+    tables = torch.full((2, piece * 64 // 32), -1, dtype=torch.int32, device=dev())
+    tables[1, piece // 32 - 3:piece // 32 + 1] = a["tables"][1, :4]
+    got = _run(c, q, 0, dict(a, tables=tables, start=up([64 * piece - 1, piece + 1 - n])))
+    _check(got, ref, tol)

@@ -1780,7 +1780,7 @@ struct PagedPlan {
   bool mfma;
   int own_qb, own_blk, pre_qb, pre_blk;
   int S_own, S_pre, pre_chunk, target, joint;
-  int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short
+  int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short, none has more than S_own
   int64_t part_bytes, ml_bytes, item_bytes;
 };
 // Key splits of the prefix. With S of them, in us: the time that their workgroups
@@ -1845,7 +1845,7 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   if (P == 0 && longest <= 1024) a.S_own = 1;
   a.target = a.own_qb ? 768 : 256;
   const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;
-  a.items = a.S_own == 1 ? units : units + std::max<int64_t>(a.target, cut);
+  a.items = std::min(units * a.S_own, units + std::max<int64_t>(a.target, cut));
   if (P > 0 && a.joint == 0) {
     // The splits are counted from the first key that a column block sees: all of the prefix, or, by tokens behind it,
     // the window's end. The last one takes what is left, for rows that begin within the prefix. (7 rows of 9 tokens, 8

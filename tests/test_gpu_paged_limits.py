@@ -96,3 +96,20 @@ def test_a_row_of_one_key_more_than_a_piece(dtype, n):
     tables[1, piece // 32 - 3:piece // 32 + 1] = a["tables"][1, :4]
     got = _run(c, q, 0, dict(a, tables=tables, start=up([64 * piece - 1, piece + 1 - n])))
     _check(got, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,W,most", [(64, 2 ** 22, 1), (64, 2 ** 22, 20), (300, 2 ** 20, 1)])
+def test_short_rows_in_wide_tables(dtype, B, W, most):
+    """Rows of up to a few hundred positions in tables of 2^25 and 2^27, in
+    front of which the table's own length would ask for 2^24 workgroups."""
+    _say(f"paged_attention {dtype}: {B} rows of up to {most} tokens, tables of {W} pages")
+    r = np.random.default_rng(B)
+    n = r.integers(0, most + 1, B) if most > 1 else np.ones(B, int)
+    c = Paged(67, r.integers(0, 200, B), n, 0, 8, 64, 32, DT[dtype])
+    q = c.queries(8)
+    ref, tol = c.reference(q, 0)
+    a = c.device(dev())
+    tables = torch.full((B, W), -1, dtype=torch.int32, device=dev())
+    tables[:, :c.W] = a["tables"]
+    _check(_run(c, q, 0, dict(a, tables=tables)), ref, tol)

@@ -82,3 +82,20 @@ def test_versions_of_what_is_written():
     with torch.inference_mode():  # which has no versions
         a = {k: t.to("meta") for k, t in append_args().items()}
         OPS.page_append(*a.values())
+
+
+# ---------------------------------------------------------------- wide tables
+@pytest.mark.parametrize("B,G,H,W,P,most", [
+    (64, 8, 8, 2 ** 26 - 2, 0, 1), (64, 8, 64, 2 ** 26 - 2, 0, 4), (4096, 8, 8, 2 ** 26 - 1, 0, 1),
+    (300, 32, 32, 2 ** 25, 2 ** 30 - 64, 1), (64, 8, 8, 2 ** 26 - 2, 0, 40),
+])
+@pytest.mark.parametrize("dtype", [_lib.FC_BF16, _lib.FC_F32])
+def test_wide_tables_are_taken(dtype, B, G, H, W, P, most):
+    """Positions up to 2^31 are accepted whatever the number of rows: how many
+    workgroups a call takes is bounded by its pieces, not by the table. (With
+    no workspace the call ends at that check, the one behind the sizes'.)"""
+    p, L = pages(G, dtype=dtype), _lib.lib()
+    T, x = B * most, 0x1000
+    assert workspace(p, B, T, most, H, W, P) > 0
+    rc = L.fc_paged_attention(p, x, H * 128, 128, x, B, T, most, H, x, W, x, x, x, P, 0, 0, None, 0, None)
+    assert rc == -1 and b"workspace" in L.fc_last_error()

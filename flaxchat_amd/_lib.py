@@ -80,7 +80,8 @@ EXPORTS = ["fc_last_error", "fc_version", "fc_forward_workspace_bytes", "fc_forw
            "fc_spec_workspace_bytes",
            "fc_spec_round", "fc_spec_accept", "fc_spec_part_bytes", "fc_fast_sample", "fc_engine_sample",
            "fc_cross_entropy", "fc_page_tables", "fc_page_append", "fc_paged_attention",
-           "fc_paged_attention_workspace_bytes", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe", "fc_gemm_walk_probe",
+           "fc_paged_attention_workspace_bytes", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe",
+           "fc_gemm_walk_probe",
            "fc_gemm_walk_probe_words", "fc_graph_begin", "fc_graph_end", "fc_graph_launch", "fc_graph_destroy"]
 
 _lib = None

@@ -459,15 +459,15 @@ extern "C" int32_t fc_page_append(const fc_pages* pages, const void* k, const vo
   const int per = src_dtype == FC_BF16 ? 8 : 4, per_page = pages->dtype == FC_BF16 ? 8 : 4;
   const uintptr_t at = (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)k | (uintptr_t)v;
   const int64_t strides = k_token_stride | k_head_stride | v_token_stride | v_head_stride;
+  const int64_t tiles = ((int64_t)M + PA_TILE - 1) / PA_TILE;
   const bool vec = (at & 15) == 0 && strides % per == 0 && (pages->k_stride | pages->v_stride) % per_page == 0 &&
-                   pv.hd % 8 == 0 && pv.G <= 65535;
-  const int tiles = (M + PA_TILE - 1) / PA_TILE;
+                   pv.hd % 8 == 0 && pv.G <= 65535 && tiles < 1 << 24;  // (a launch's threads are counted in 32 bits)
   const int64_t n = (int64_t)M * pv.G * pv.hd;
 #define APPEND(T, S, KBLK)                                                                                           \
   if (vec)                                                                                                           \
-    hipLaunchKernelGGL((k_page_append<T, S, KBLK>), dim3(tiles, pv.G), dim3(256), PA_MOST * (pv.hd + 2) * sizeof(T), \
-                       s, pv, (T*)pages->k, (T*)pages->v, (const S*)k, (const S*)v, k_token_stride, k_head_stride,   \
-                       v_token_stride, v_head_stride, slots, M);                                                     \
+    hipLaunchKernelGGL((k_page_append<T, S, KBLK>), dim3((int)tiles, pv.G), dim3(256),                               \
+                       PA_MOST * (pv.hd + 2) * sizeof(T), s, pv, (T*)pages->k, (T*)pages->v, (const S*)k, (const S*)v,\
+                       k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, M);                      \
   else                                                                                                               \
     hipLaunchKernelGGL((k_page_append_any<T, S>), dim3((unsigned)std::min<int64_t>((n + 255) / 256, 65536)),         \
                        dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, (const S*)k, (const S*)v, k_token_stride,    \

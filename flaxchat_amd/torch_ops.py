@@ -524,8 +524,8 @@ def _pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
     N, G, page, hd = k_pages.shape
     if page == 0 or page % 32 != 0:
         raise ValueError(f"{name}: page must be a multiple of 32 (got {page})")
-    if N < 1 or G < 1 or not 1 <= hd <= 256:
-        raise ValueError(f"{name}: n_pages, n_kv_head and head_dim (at most 256) must be positive")
+    if N < 1 or G < 1 or not 1 <= hd <= 256 or max(N, G, page) > 0x7fffffff:
+        raise ValueError(f"{name}: n_pages, n_kv_head and head_dim (at most 256) must be positive, and below 2^31")
     if v_pages.shape != (N, G, page // 32, hd, 32):
         raise ValueError(f"{name}: v_pages {[N, G, page // 32, hd, 32]} (got {tuple(v_pages.shape)})")
     dt = k_pages.dtype
@@ -584,6 +584,8 @@ def page_append(k, v, slots, k_pages, v_pages):
             torch.is_grad_enabled():
         raise ValueError("page_append has no backward pass")
     M = k.shape[0]
+    if M > 0x7fffffff:
+        raise ValueError("page_append: tokens below 2^31")
     _index("page_append", "slots", slots, M)
     d = _on_gpu("page_append", k_pages, v_pages, k, v, slots)
     if M == 0:
@@ -616,8 +618,8 @@ def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, wi
     T, H, _ = q.shape
     if not 1 <= B <= 4096 or W < 1 or H > 65535 or not 1 <= max_per_row <= 0x7fffffff:
         raise ValueError("paged_attention: batch in [1, 4096], width and max_per_row at least 1 and below 2^31")
-    if not 0 <= window <= 0x7fffffff:
-        raise ValueError("paged_attention: window in [0, 2^31)")
+    if not 0 <= window <= 0x7fffffff or T > 0x7fffffff:
+        raise ValueError("paged_attention: window in [0, 2^31), tokens below 2^31")
     if prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
         raise ValueError("paged_attention: prefix_len >= 0, positions below 2^31")
     _index("paged_attention", "tables", tables, B * W)

@@ -113,3 +113,21 @@ def test_short_rows_in_wide_tables(dtype, B, W, most):
     tables = torch.full((B, W), -1, dtype=torch.int32, device=dev())
     tables[:, :c.W] = a["tables"]
     _check(_run(c, q, 0, dict(a, tables=tables)), ref, tol)
+
+
+def test_append_of_very_many_tokens():
+    """More tokens than a launch has room for at 32 a workgroup, nearly all of
+    them without a slot."""
+    M = 2 ** 29 + 5
+    _say(f"page_append: {M} tokens")
+    one = torch.arange(1, 9, device=dev(), dtype=torch.bfloat16).view(1, 1, 8)
+    k = one.expand(M, 1, 8)
+    slots = torch.full((M,), -1, dtype=torch.int32, device=dev())
+    slots[[0, 2 ** 28, M - 1]] = up([5, 40, 63])
+    kp = torch.zeros(2, 1, 32, 8, device=dev(), dtype=torch.bfloat16)
+    vp = torch.zeros(2, 1, 1, 8, 32, device=dev(), dtype=torch.bfloat16)
+    OPS.page_append(k, k, slots, kp, vp)
+    rows = torch.zeros(64, 8)
+    rows[[5, 40, 63]] = torch.arange(1.0, 9.0)
+    assert torch.equal(kp.float().cpu().view(64, 8), rows)
+    assert torch.equal(vp.float().cpu().view(2, 8, 32).transpose(1, 2).reshape(64, 8), rows)

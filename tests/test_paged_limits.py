@@ -30,8 +30,8 @@ def test_workspace_of_long_prefixes(dtype, B, T, most, G, H, window):
     whatever the prefix's length, up to the last one accepted."""
     p = pages(G, dtype=dtype)
     two = 2 * T * H * (128 + 2) * 4
-    lengths = [1, 127, 128, 129, 10 ** 6, 1908874305, 2130836481, 2 ** 31 - 200, 2 ** 31 - 129, 2 ** 31 - 97, P_MOST - 1,
-               P_MOST]
+    lengths = [1, 127, 128, 129, 10 ** 6, 1908874305, 2130836481, 2 ** 31 - 200, 2 ** 31 - 129, 2 ** 31 - 97,
+               P_MOST - 1, P_MOST]
     lengths += range(2 ** 31 - 40 * 10 ** 6, P_MOST, 1234567)
     for P in lengths:
         nb = workspace(p, B, T, most, H, 1, P, window)
@@ -99,3 +99,25 @@ def test_wide_tables_are_taken(dtype, B, G, H, W, P, most):
     assert workspace(p, B, T, most, H, W, P) > 0
     rc = L.fc_paged_attention(p, x, H * 128, 128, x, B, T, most, H, x, W, x, x, x, P, 0, 0, None, 0, None)
     assert rc == -1 and b"workspace" in L.fc_last_error()
+
+
+# ---------------------------------------------------------------- counts past 31 bits
+def test_counts_past_31_bits_are_refused():
+    """The C entries count in 32 bits: what does not fit is refused, not cut
+    off. (Shapes alone: tensors without memory, given to the operators' own
+    functions.)"""
+    def m(*s, dtype=torch.bfloat16):
+        return torch.empty(s, dtype=dtype, device="meta")
+
+    def i(*s):
+        return m(*s, dtype=torch.int32)
+
+    ops, T = flaxchat_amd.torch_ops, 2 ** 32 + 1
+    kp, vp = m(4, 1, 32, 8), m(4, 1, 1, 8, 32)
+    with pytest.raises(ValueError, match="tokens below"):
+        ops.page_append(m(T, 1, 8), m(T, 1, 8), i(T), kp, vp)
+    with pytest.raises(ValueError, match="tokens below"):
+        ops.paged_attention(m(T, 1, 8), kp, vp, i(1, 1), i(2), i(1), 1, 0)
+    for N, page in ((2 ** 32 + 1, 32), (1, 2 ** 32 + 32)):
+        with pytest.raises(ValueError, match="below 2\\^31"):
+            ops.page_append(m(1, 1, 1), m(1, 1, 1), i(1), m(N, 1, page, 1), m(N, 1, page // 32, 1, 32))

@@ -518,7 +518,8 @@ struct PagedChunk {
 // kept from earlier. What is kept of it through a whole walk, with the constants
 // that the compiler makes of it for its divisions, is more than the scalar
 // registers hold, and a spill of theirs is not to be had here: a part of one came
-// back wrong (the lower half of a pointer), so the walks' kernels are to have none.
+// back wrong (the lower half of a pointer), so the kernels here are to have none: the
+// build fails if one has.
 template <typename P>
 __device__ __forceinline__ P* in_global(P* p) {
   return (P*)(__attribute__((address_space(1))) P*)p;

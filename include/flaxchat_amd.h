@@ -346,7 +346,11 @@ typedef struct fc_pages {
  * (a stack; entries at n_free and above are scratch; free_cap may be 0). Per row: length[b]
  * positions held (counted behind the shared prefix of prefix_len positions),
  * n_new[b] to be added; n_new < 0 ends the row: its pages go onto the stack,
- * in row order, and held[b] becomes 0. A row with n_new > 0 asks if
+ * in row order, and held[b] becomes 0. (The stack has to have room for every
+ * page that may be free at once, free_cap >= the pages it hands out and takes
+ * back: a page given back past free_cap is dropped, and nothing says so. The
+ * table keeps the ended row's entries, so a caller that reads them can still
+ * put such pages back.) A row with n_new > 0 asks if
  * ceil(length / page) <= held <= width and length + n_new <= width * page; it
  * needs the pages past held that its new positions reach. It is taken in if
  * it needs none, or if its pages and those of all rows before it that ask fit

@@ -131,3 +131,19 @@ def test_append_of_very_many_tokens():
     rows[[5, 40, 63]] = torch.arange(1.0, 9.0)
     assert torch.equal(kp.float().cpu().view(64, 8), rows)
     assert torch.equal(vp.float().cpu().view(2, 8, 32).transpose(1, 2).reshape(64, 8), rows)
+
+
+def test_pages_given_back_past_the_stack():
+    """Pages that the stack has no room for are not on it, and the ended row's
+    table still names them: put back by the caller, they are handed out."""
+    _say("page_tables: a stack of two for three pages")
+    s = [up(a) for a in ([[4, 5, 6], [-1] * 3], [3, 0], [-1, -1], [0], [70, 0], [-1, 0], [0] * 3, [0] * 2, [0] * 70,
+                         [0] * 70, [0] * 70)]
+    OPS.page_tables(*s, 32, 0)
+    assert s[2].tolist() == [4, 5] and s[3].item() == 2 and s[1].tolist() == [0, 0]
+    assert s[0][0].tolist() == [4, 5, 6]
+    s[2] = up([4, 5, 6])  # a stack with room
+    s[3].fill_(3)
+    s[4:6] = up([0, 0]), up([0, 70])
+    OPS.page_tables(*s, 32, 0)
+    assert s[0][1].tolist() == [6, 5, 4] and s[1].tolist() == [0, 3] and s[3].item() == 0

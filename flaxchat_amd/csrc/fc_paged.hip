@@ -1773,7 +1773,10 @@ __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2)
 // Host side
 // ---------------------------------------------------------------------------
 namespace {
-constexpr int64_t kPartMax = 256ll << 20;  // bytes of partials a call may ask for
+// Bytes of partials that the own keys' splits are cut down to, and those of the prefix for themselves: together up to
+// twice that. One split of each there is whatever its size. (16000 tokens of 12 heads of 128 behind 4000 keys ask for up
+// to 381 MiB, two splits of either, 95 MiB each; 100000 such tokens in 4000 rows for 1.2 GiB, one of either.)
+constexpr int64_t kPartMax = 256ll << 20;
 // How a call is cut: the kernels of the rows' own keys and of the prefix (query
 // blocks of 16 columns in a workgroup of the streaming kernel, 0: the wide one),
 // their column blocks, and the key splits.

@@ -147,3 +147,121 @@ def test_pages_given_back_past_the_stack():
     s[4:6] = up([0, 0]), up([0, 70])
     OPS.page_tables(*s, 32, 0)
     assert s[0][1].tolist() == [6, 5, 4] and s[1].tolist() == [0, 3] and s[3].item() == 0
+
+
+# ---------------------------------------------------------------- every key counted once
+def _counted(c, H, window, div, gone=()):
+    """With queries of 0 every visible key weighs 1, and with V of one 1 at dim (position // div + 17 head) % head_dim
+    the output times the number of keys is how many visible keys have that dim: whole numbers, exact in the
+    sums, and off by at most 2^-8 of themselves in a bf16 result, so by less than a half up to 127. Writes those V
+    into c; returns (counts [T][H][hd], keys [T])."""
+    P, page, hd, G = c.P, c.page, c.hd, c.G
+    counts, keys = np.zeros((int(c.off[-1]), H, hd), np.int64), np.zeros(int(c.off[-1]), np.int64)
+    for b in range(c.B):
+        L = P + int(c.ctx[b] + c.n[b])
+        at, there = np.arange(L), np.ones(L, bool)
+        for r, j in gone:
+            if r == b:
+                there[P + j * page:P + (j + 1) * page] = False
+            elif r == -1:
+                there[j * page:min(P, (j + 1) * page)] = False
+        for first, last, table in ((0, P, c.pre_ids), (P, L, c.tables[b])):
+            i = np.arange(first, last) - first
+            pid = np.asarray(table)[i // page]
+            for g in range(G):
+                c.V[pid, g, i % page] = (at[first:last, None] // div + 17 * g) % hd == np.arange(hd)
+        hot = ((at[:, None, None] // div + 17 * np.arange(G)[:, None]) % hd == np.arange(hd)) & there[:, None, None]
+        upto = np.concatenate([np.zeros((1, G, hd), np.int64), hot.cumsum(0)])
+        n_upto = np.concatenate([[0], there.cumsum()])
+        pos = c.start[b] + np.arange(c.n[b])
+        lo = np.maximum(0, pos - window) if window > 0 else 0 * pos
+        seen = np.s_[c.off[b]:c.off[b] + c.n[b]]
+        counts[seen] = (upto[pos + 1] - upto[lo]).repeat(H // G, 1)
+        keys[seen] = n_upto[pos + 1] - n_upto[lo]
+    assert counts.max() < 128
+    return counts, keys
+
+
+COUNTED = [
+    # ctx, n, prefix, start (None: behind the prefix), H, G, hd, page, window
+    ([5, 700, 0, 64, 131], [3, 0, 1, 9, 5], 7003, None, 12, 4, 128, 64, 0),     # a long prefix, few tokens
+    ([10, 450, 90], [33, 2, 60], 6001, None, 6, 2, 128, 96, 0),                 # and many
+    ([10, 450, 90], [33, 2, 60], 6001, None, 6, 2, 128, 32, 3000),
+    ([10, 450, 90], [33, 2, 60], 5000, None, 4, 4, 64, 64, 0),
+    ([300, 0, 17], [140, 200, 130], 250, None, 6, 6, 128, 64, 0),               # prompts that walk a short prefix
+    ([300, 0, 17], [140, 200, 130], 999, None, 4, 2, 64, 32, 700),              # themselves
+    ([300, 0, 17, 0], [140, 200, 130, 20], 1023, [1323, 900, 500, 1010], 4, 2, 128, 32, 0),  # rows that begin in it
+    ([300, 0, 17, 0], [140, 200, 130, 20], 1023, [1323, 900, 500, 1010], 4, 2, 128, 64, 300),
+    ([7000, 3, 2500], [1, 1, 1], 0, None, 6, 6, 128, 64, 0),                    # long rows, cut into pieces
+    ([7000, 3, 2500], [1, 1, 1], 2000, None, 16, 2, 128, 32, 0),
+    ([7000, 3, 2500], [12, 1, 7], 0, None, 4, 2, 128, 256, 0),
+    ([7000, 3, 2500], [90, 120, 7], 0, None, 4, 2, 128, 96, 0),
+    ([7000, 3, 2500], [90, 120, 7], 0, None, 4, 2, 64, 32, 4000),
+    ([5000, 40, 3000], [200, 129, 64], 500, None, 4, 2, 128, 64, 0),            # pieces that begin in the prefix
+    ([50 * (i % 40) for i in range(300)], [i % 3 for i in range(300)], 777, None, 2, 2, 128, 32, 0),
+    ([50 * (i % 40) for i in range(300)], [i % 3 for i in range(300)], 0, None, 2, 1, 64, 32, 900),
+    ([7 * i % 50 for i in range(97)], [16] * 97, 1100, None, 128, 16, 128, 32, 0),  # rounds of blocks behind 1100 keys
+    ([9 * i % 70 for i in range(30)], [40] * 30, 1500, [1500 - 40 * (i % 9) for i in range(30)], 4, 4, 128, 32, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("case", range(len(COUNTED)))
+def test_every_key_counts_once(dtype, case):
+    """No key left out or taken twice at a border of tiles, pages, pieces,
+    splits or of the prefix, however many keys there are."""
+    ctx, n, P, start, H, G, hd, page, window = COUNTED[case]
+    _say(f"paged_attention {dtype} counted case {case}: {len(n)} rows, prefix {P}, window {window}")
+    c = Paged(case, ctx, n, P, G, hd, page, DT[dtype])
+    if start is not None:
+        c.start = np.array(start, np.int32)
+    q = np.zeros((int(c.off[-1]), H, hd), np.float32)
+    for div in (1, 32):
+        counts, keys = _counted(c, H, window, div)
+        got = _run(c, q, window).double().cpu().numpy().reshape(counts.shape) * keys[:, None, None]
+        assert np.abs(got - counts).max() < 0.5, f"div {div}: {np.argwhere(np.abs(got - counts) >= 0.5)[:4].tolist()}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [128, 64, 96])
+@pytest.mark.parametrize("n", [[3, 5, 2], [45, 20, 9], [150, 130, 3]])
+def test_counted_keys_without_pages(dtype, hd, n):
+    """The same where entries of the tables and of the prefix are no page, and
+    where a position that only a row's last two queries see holds an infinity."""
+    _say(f"paged_attention {dtype} hd={hd}: rows of {n} tokens, entries that are no page, an infinity")
+    c = Paged(71, [170, 10, 600], n, 290, 2, hd, 32, DT[dtype])
+    gone = [(0, 1), (2, 0), (2, 18), (-1, 3), (-1, 9)]
+    q = np.zeros((int(c.off[-1]), 4, hd), np.float32)
+    for window in (0, 250):
+        counts, keys = _counted(c, 4, window, 1, gone)
+        at = 170 + n[0] - 2
+        assert at // 32 != 1
+        c.V[c.tables[0, at // 32], :, at % 32] = INF
+        a = c.device(dev())
+        a["tables"][0, 1], a["tables"][2, 0], a["tables"][2, 18] = -1, c.N, 2 ** 31 - 1
+        a["pre"][3], a["pre"][9] = -2 ** 31, c.N + 1
+        got = _run(c, q, window, a).double().cpu().numpy().reshape(counts.shape) * keys[:, None, None]
+        keep = np.ones(len(q), bool)
+        keep[n[0] - 2:n[0]] = False
+        assert np.abs(got - counts)[keep].max() < 0.5, f"window {window}"
+        assert not np.isfinite(got[~keep]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("window", [0, 60])
+def test_contiguous_and_paged_within_the_bound(dtype, window):
+    """attention on a contiguous cache and paged_attention on the same cache as
+    a pool of one page a row: both as near the softmax as the bound of each
+    output says."""
+    _say(f"attention and paged_attention {dtype}, window {window}")
+    c = Paged(73, [90, 3, 151, 0], [5, 1, 9, 40], 0, 2, 128, 160, DT[dtype], junk=0.0)
+    q = c.queries(4)
+    ref, tol = c.reference(q, window)
+    a = c.device(dev())
+    _check(_run(c, q, window, a), ref, tol, "paged")
+    ids = a["tables"][:, 0].long()
+    qt = torch.from_numpy(q).to(dev(), c.dtype)
+    got = OPS.attention(qt, a["k"][ids], a["v"][ids], a["row_off"], a["start"], 40, window)
+    _check(got, ref, tol, "contiguous")
+    as_pool = dict(a, k=a["k"][ids], v=a["v"][ids], tables=up(np.arange(4)[:, None]))
+    _check(_run(c, q, window, as_pool), ref, tol, "the cache as a pool")

@@ -391,7 +391,8 @@ int32_t fc_page_append(const fc_pages* pages, const void* k, const void* v, int6
  * row whose tokens run past max_tokens or number more than max_per_row is
  * treated as empty (its tokens' outputs are not written). row_off does not
  * decrease. batch <= 4096. Calls that may run at the same time, captured
- * graphs included, each need a workspace of their own. */
+ * graphs included, each need a workspace of their own; the query says how
+ * large (0: none), or a negative status for sizes that the call refuses. */
 #define FC_PAGED_ZERO_TAIL 1
 int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
                                            int32_t max_per_row, int32_t n_head, int32_t width, int32_t prefix_len,

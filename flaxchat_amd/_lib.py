@@ -54,6 +54,7 @@ class FcPages(Structure):
                 ("dtype", c_int32)]
 
 
+FC_TREE_MOST = 512  # nodes of a row's tree
 FC_PAGED_ZERO_TAIL = 1  # fc_paged_attention flags: tokens past the last row become 0
 
 
@@ -80,7 +81,8 @@ EXPORTS = ["fc_last_error", "fc_version", "fc_forward_workspace_bytes", "fc_forw
            "fc_spec_workspace_bytes",
            "fc_spec_round", "fc_spec_accept", "fc_spec_part_bytes", "fc_fast_sample", "fc_engine_sample",
            "fc_cross_entropy", "fc_page_tables", "fc_page_append", "fc_paged_attention",
-           "fc_paged_attention_workspace_bytes", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe",
+           "fc_paged_attention_workspace_bytes", "fc_tree_tables", "fc_tree_attention_workspace_bytes",
+           "fc_tree_attention", "fc_tree_accept", "fc_tree_commit", "fc_rope_append", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe",
            "fc_gemm_walk_probe",
            "fc_gemm_walk_probe_words", "fc_graph_begin", "fc_graph_end", "fc_graph_launch", "fc_graph_destroy"]
 
@@ -143,6 +145,20 @@ def _declare(L):
     L.fc_paged_attention.argtypes = [POINTER(FcPages), vp, i64, i64, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, i32,
                                      i32, i32, vp, i64, vp]
     L.fc_paged_attention.restype = i32
+    L.fc_tree_tables.argtypes = [vp] * 5 + [i32] * 3 + [vp]
+    L.fc_tree_tables.restype = i32
+    L.fc_tree_attention_workspace_bytes.argtypes = L.fc_paged_attention_workspace_bytes.argtypes
+    L.fc_tree_attention_workspace_bytes.restype = i64
+    L.fc_tree_attention.argtypes = [POINTER(FcPages), vp, i64, i64, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp,
+                                    vp, i32, i32, i32, vp, i64, vp]
+    L.fc_tree_attention.restype = i32
+    L.fc_tree_accept.argtypes = [vp] * 7 + [i32] * 3 + [vp]
+    L.fc_tree_accept.restype = i32
+    L.fc_tree_commit.argtypes = [POINTER(FcPages), i32, i64, i64, vp, vp, vp, i32, i32, i32, vp]
+    L.fc_tree_commit.restype = i32
+    L.fc_rope_append.argtypes = [POINTER(FcPages), vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp, i32,
+                                 i32, i32, f32, vp, i32, i32, vp]
+    L.fc_rope_append.restype = i32
     L.fc_read_probe.argtypes = [vp, i64, vp, i32, vp]
     L.fc_read_probe.restype = i32
     L.fc_l2_read_probe.argtypes = [vp, i64, i64, vp, i32, vp]

@@ -11,25 +11,13 @@
 // p / page of prefix_pages; from there on entry (p - prefix_len) / page of the
 // row's table. An entry outside [0, n_pages) holds no keys.
 #include "fc_common.h"
-#include "fc_internal.h"
+#include "fc_paged.h"
 #include <type_traits>
 
 // K and V of a row's own pages are read once a call: non-temporal loads keep
 // them from displacing lines that are read again.
 typedef uint32_t kv_u32x4 __attribute__((ext_vector_type(4)));
 #define KV_LD(p) __builtin_bit_cast(uint4, __builtin_nontemporal_load((const kv_u32x4*)(p)))
-
-// Smallest b in [0, n) with off[b + 1] > t; n if there is none. Ends for any
-// contents of off.
-__device__ __forceinline__ int row_of(const int* off, int n, int t) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (off[mid + 1] > t) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
 
 // ---------------------------------------------------------------------------
 // Page tables
@@ -53,7 +41,6 @@ __device__ __forceinline__ void stage_offsets(int* off, const int* __restrict__ 
 // associative and in 32 bits whatever the arrays hold. Bound by latency: four
 // dependent passes over global memory and two scans, hence no more waves than
 // there are rows or tokens for (64 rows with 16 waves: 7.8 us, with one: 6.5).
-#define PT_ROWS 4096     // rows a call may have: 4 per thread
 #define PT_SAT (1u << 30)
 __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, PT_SAT); }
 
@@ -277,34 +264,6 @@ extern "C" int32_t fc_page_tables(int32_t* tables, int32_t* held, int32_t* free_
 // ---------------------------------------------------------------------------
 // Append
 // ---------------------------------------------------------------------------
-// What the kernels need of an fc_pages.
-struct PageView {
-  int64_t ks, vs;  // elements between pages
-  int N, G, page, hd;
-  int kblk;        // K blocks in the matrix-core order
-};
-static PageView page_view(const fc_pages* p) {
-  return PageView{p->k_stride, p->v_stride, p->n_pages, p->n_kv_head, p->page, p->head_dim,
-                  p->dtype == FC_BF16 && p->head_dim == 128};
-}
-static int check_pages(const fc_pages* p) {
-  FC_CHECK_ARG(p && p->k && p->v, "null pointer");
-  FC_CHECK_ARG(p->dtype == FC_F32 || p->dtype == FC_BF16, "dtype");
-  FC_CHECK_ARG(p->n_pages > 0 && p->n_kv_head > 0 && p->head_dim > 0 && p->head_dim <= 256,
-               "n_pages, n_kv_head and head_dim (at most 256) must be positive");
-  FC_CHECK_ARG(p->page > 0 && p->page % 32 == 0, "page must be a multiple of 32");
-  const int64_t elems = (int64_t)p->n_kv_head * p->page * p->head_dim;
-  FC_CHECK_ARG(p->k_stride >= elems && p->v_stride >= elems, "page strides below a page's elements");
-  return FC_OK;
-}
-__device__ __forceinline__ int64_t k_elem(const PageView& pv, int id, int g, int at, int d) {
-  const int64_t base = (int64_t)id * pv.ks + (int64_t)g * pv.page * pv.hd;
-  return base + (pv.kblk ? kblk_idx(at, d) : (int64_t)at * pv.hd + d);
-}
-__device__ __forceinline__ int64_t v_elem(const PageView& pv, int id, int g, int at, int d) {
-  return (int64_t)id * pv.vs + (int64_t)g * pv.page * pv.hd + (int64_t)(at >> 5) * 32 * pv.hd + d * 32 + (at & 31);
-}
-
 // Any head size and alignment: an element per thread.
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void k_page_append_any(PageView pv, T* __restrict__ kp, T* __restrict__ vp,
@@ -320,30 +279,6 @@ __global__ __launch_bounds__(256) void k_page_append_any(PageView pv, T* __restr
     st<T>(kp, k_elem(pv, id, g, at, d), ld<S>(k, m * kst + g * ksh + d));
     st<T>(vp, v_elem(pv, id, g, at, d), ld<S>(v, m * vst + g * vsh + d));
   }
-}
-
-// 8 consecutive values as fp32, and back (rounded to nearest even)
-__device__ __forceinline__ void load8(const bf16_t* p, float (&x)[8]) {
-  const uint4 u = *(const uint4*)p;
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-// 8 results of a row, times f
-__device__ __forceinline__ void store8(bf16_t* y, const float (&o)[8], float f) {
-  *(uint4*)y = uint4{pack2bf(o[0] * f, o[1] * f), pack2bf(o[2] * f, o[3] * f), pack2bf(o[4] * f, o[5] * f),
-                     pack2bf(o[6] * f, o[7] * f)};
-}
-__device__ __forceinline__ void store8(float* y, const float (&o)[8], float f) {
-  ((float4*)y)[0] = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
-  ((float4*)y)[1] = make_float4(o[4] * f, o[5] * f, o[6] * f, o[7] * f);
 }
 
 // About 32 tokens of one KV head per workgroup, 16 bytes per load and store.
@@ -512,6 +447,10 @@ struct PagedChunk {
   int* items;  // of more than ROWS_SCAN rows: the chunk's length, and every 64 rows' first item
   const void *q, *kp, *vp;
   void* y;
+  // a tree's chunk: each token's row of bits (`words` of them) and its position
+  const uint64_t* mask;
+  const int* tok_pos;
+  int words;
 };
 
 // The chunk, read from the kernel's arguments (its first) at this point and not
@@ -547,6 +486,8 @@ __device__ __forceinline__ PagedChunk chunk_args() {
   c.kp = in_global(c.kp);
   c.vp = in_global(c.vp);
   c.y = in_global(c.y);
+  c.mask = in_global(c.mask);
+  c.tok_pos = in_global(c.tok_pos);
   return c;
 }
 
@@ -555,7 +496,10 @@ __device__ __forceinline__ PagedChunk chunk_args() {
 // running maximum and sum of the softmax. Without matrix instructions and with keys
 // read once per query head, it is for shapes that no model here has: 64 rows of 300
 // keys, 12 heads of 96, 175 us (12 of 128: 25).
-template <typename T>
+//
+// tree: a key before the row's start is seen by the window that ends at the token's
+// position, one of the chunk's own if the token's row of bits says so.
+template <typename T, bool tree>
 __global__ __launch_bounds__(256) void k_paged_any(PagedChunk c) {
   const T *q = (const T*)c.q, *kp = (const T*)c.kp, *vp = (const T*)c.vp;
   T* y = (T*)c.y;
@@ -572,16 +516,20 @@ __global__ __launch_bounds__(256) void k_paged_any(PagedChunk c) {
   }
   const int g = h / (c.H / c.pv.G);
   // keys [lo, hi]: the prefix's positions, then the table's
-  const int64_t pos = (int64_t)c.start[b] + (t - sp.base);
-  const int64_t lo = c.window > 0 ? max((int64_t)0, pos - c.window) : 0;
-  const int64_t hi = min(pos, (int64_t)c.P + (int64_t)c.W * c.pv.page - 1);
+  const int64_t first = c.start[b], last = (int64_t)c.P + (int64_t)c.W * c.pv.page - 1;
+  const int64_t pos = tree ? max(first, (int64_t)c.tok_pos[t]) : first + (t - sp.base);
+  const int64_t from = tree ? min(pos - c.window, first) : pos - c.window;
+  const int64_t lo = c.window > 0 ? max((int64_t)0, from) : 0;
+  const int64_t hi = min(tree ? first + sp.n - 1 : pos, last);
+  const uint64_t* bits = c.mask + (int64_t)t * c.words;
   for (int d = tid; d < hd; d += 256) qs[d] = ld<T>(q, t * c.qst + h * c.qsh + d);
   __syncthreads();
   float m = -INFINITY, l = 0.f, o = 0.f;
   for (int64_t k0 = lo; k0 <= hi; k0 += 256) {
     const int64_t key = k0 + tid;
     int id = -1, at = 0;
-    if (key <= hi) {
+    if (key <= hi && (!tree || key < first ||
+                      (key >= c.P && (bits[(key - first) >> 6] >> ((key - first) & 63) & 1)))) {
       const int w = (int)(key < c.P ? key : key - c.P);
       id = key < c.P ? c.pre[w / c.pv.page] : c.tables[(int64_t)b * c.W + w / c.pv.page];
       at = w % c.pv.page;
@@ -1920,6 +1868,14 @@ int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
 }
 }  // namespace
 
+namespace {
+// A tree's nodes as bits; none: a chunk's tokens follow one another.
+struct TreeBits {
+  const uint64_t* mask;
+  const int32_t* tok_pos;
+};
+}  // namespace
+
 // What the plan's arithmetic and the launches are made for. (A launch's threads are counted in 32 bits along x, its
 // workgroups in 16 along y.)
 static constexpr int64_t kMostGroups = (1 << 24) - 1024;
@@ -1946,12 +1902,11 @@ extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int
   return a.part_bytes + a.ml_bytes + a.item_bytes;
 }
 
-extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,
-                                      int64_t q_head_stride, void* y, int32_t batch, int32_t max_tokens,
-                                      int32_t max_per_row, int32_t n_head, const int32_t* tables, int32_t width,
-                                      const int32_t* row_off, const int32_t* start, const int32_t* prefix_pages,
-                                      int32_t prefix_len, int32_t window, int32_t flags, void* work,
-                                      int64_t work_bytes, void* stream) {
+static int attention(const fc_pages* pages, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* y,
+                     int32_t batch, int32_t max_tokens, int32_t max_per_row, int32_t n_head, const int32_t* tables,
+                     int32_t width, const int32_t* row_off, const int32_t* start, const int32_t* prefix_pages,
+                     int32_t prefix_len, int32_t window, int32_t flags, void* work, int64_t work_bytes, void* stream,
+                     const TreeBits* tree) {
   int rc = check_pages(pages);
   if (rc != FC_OK) return rc;
   FC_CHECK_ARG(q && y && tables && row_off && start, "null pointer");
@@ -1966,23 +1921,64 @@ extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int6
                max_per_row, max_tokens, flags, q_token_stride, q_head_stride,
                1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, a.joint, (float*)work,
                (float2*)((char*)work + a.part_bytes), (int*)((char*)work + a.part_bytes + a.ml_bytes),
-               q, pages->k, pages->v, y};
+               q, pages->k, pages->v, y, tree ? tree->mask : nullptr, tree ? tree->tok_pos : nullptr,
+               (max_per_row + 63) / 64};
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;
   const bool vec = (((uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)y | (uintptr_t)work) & 15) ==
                        0 && (strides & (pages->dtype == FC_BF16 ? 7 : 3)) == 0;
-  if (a.mfma && vec) {
+  if (a.mfma && vec && !tree) {
     if (pages->dtype == FC_BF16)
       return pages->head_dim == 128 ? launch_mfma<bf16_t, 128>(c, a, s)
                                     : launch_mfma<bf16_t, 64>(c, a, s);
     return pages->head_dim == 128 ? launch_mfma<float, 128>(c, a, s)
                                   : launch_mfma<float, 64>(c, a, s);
   }
-  if (pages->dtype == FC_BF16)
-    hipLaunchKernelGGL(k_paged_any<bf16_t>, dim3(max_tokens, n_head), dim3(256), 0, s, c);
-  else
-    hipLaunchKernelGGL(k_paged_any<float>, dim3(max_tokens, n_head), dim3(256), 0, s, c);
+  const dim3 grid(max_tokens, n_head);
+  if (tree) {
+    if (pages->dtype == FC_BF16) hipLaunchKernelGGL((k_paged_any<bf16_t, true>), grid, dim3(256), 0, s, c);
+    else hipLaunchKernelGGL((k_paged_any<float, true>), grid, dim3(256), 0, s, c);
+  } else {
+    if (pages->dtype == FC_BF16) hipLaunchKernelGGL((k_paged_any<bf16_t, false>), grid, dim3(256), 0, s, c);
+    else hipLaunchKernelGGL((k_paged_any<float, false>), grid, dim3(256), 0, s, c);
+  }
   FC_LAUNCH_CHECK();
   return FC_OK;
+}
+
+extern "C" int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,
+                                      int64_t q_head_stride, void* y, int32_t batch, int32_t max_tokens,
+                                      int32_t max_per_row, int32_t n_head, const int32_t* tables, int32_t width,
+                                      const int32_t* row_off, const int32_t* start, const int32_t* prefix_pages,
+                                      int32_t prefix_len, int32_t window, int32_t flags, void* work,
+                                      int64_t work_bytes, void* stream) {
+  return attention(pages, q, q_token_stride, q_head_stride, y, batch, max_tokens, max_per_row, n_head, tables, width,
+                   row_off, start, prefix_pages, prefix_len, window, flags, work, work_bytes, stream, nullptr);
+}
+
+static int check_tree_sizes(int32_t max_per_row) {
+  FC_CHECK_ARG(max_per_row <= FC_TREE_MOST, "max_per_row must be in [1, 512]");
+  return FC_OK;
+}
+
+extern "C" int64_t fc_tree_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
+                                                     int32_t max_per_row, int32_t n_head, int32_t width,
+                                                     int32_t prefix_len, int32_t window) {
+  if (check_tree_sizes(max_per_row) != FC_OK) return FC_ERR_ARG;
+  return fc_paged_attention_workspace_bytes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+}
+
+extern "C" int32_t fc_tree_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,
+                                     int64_t q_head_stride, void* y, int32_t batch, int32_t max_tokens,
+                                     int32_t max_per_row, int32_t n_head, const int32_t* tables, int32_t width,
+                                     const int32_t* row_off, const int32_t* start, const uint64_t* mask,
+                                     const int32_t* tok_pos, const int32_t* prefix_pages, int32_t prefix_len,
+                                     int32_t window, int32_t flags, void* work, int64_t work_bytes, void* stream) {
+  FC_CHECK_ARG(mask && tok_pos, "null pointer");
+  const int rc = check_tree_sizes(max_per_row);
+  if (rc != FC_OK) return rc;
+  const TreeBits t{mask, tok_pos};
+  return attention(pages, q, q_token_stride, q_head_stride, y, batch, max_tokens, max_per_row, n_head, tables, width,
+                   row_off, start, prefix_pages, prefix_len, window, flags, work, work_bytes, stream, &t);
 }

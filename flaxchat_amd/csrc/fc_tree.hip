@@ -1,0 +1,445 @@
+// Decoding with trees of drafted tokens over the paged KV cache: the trees'
+// bookkeeping, the append with rotation, the accepted path and its way back
+// to consecutive positions. (The attention is fc_paged.hip's.) No counterpart
+// in the reference, which verifies one drafted chain, token by token
+// (flaxchat/engine.py:484-606); rotation and norm are those of
+// flaxchat/gpt.py:52-71 and flaxchat/engine.py:108-126.
+//
+// Row b's chunk is tokens row_off[b] .. row_off[b+1]-1, its nodes; node i's
+// parent is an earlier node of the row, anything else makes it a root. Node i
+// sits in the cache at position start[b] + i, whatever its depth.
+#include "fc_paged.h"
+
+// ---------------------------------------------------------------------------
+// Ancestors
+// ---------------------------------------------------------------------------
+// Node i and the nodes above it, as bits: word w holds nodes 64 w .. 64 w + 63.
+// Within a block of 64 nodes, a lane each, by doubling: with the ancestors up
+// to 2^r steps above in m and the 2^r-th in p, m |= m[p] and p = p[p] give
+// 2^(r+1) steps. Six rounds at most, whatever the tree's shape.
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int from) {
+  const uint32_t lo = __shfl((uint32_t)v, from, WAVE), hi = __shfl((uint32_t)(v >> 32), from, WAVE);
+  return (uint64_t)hi << 32 | lo;
+}
+// p: the lane's parent within the block, -1: none there
+__device__ __forceinline__ uint64_t block_ancestors(int p) {
+  uint64_t m = 1ull << (threadIdx.x & 63);
+  for (int r = 0; r < 6 && __any(p >= 0); ++r) {
+    const uint64_t mo = shfl64(m, max(p, 0));
+    const int po = __shfl(p, max(p, 0), WAVE);
+    if (p >= 0) {
+      m |= mo;
+      p = po;
+    }
+  }
+  return m;
+}
+__device__ __forceinline__ int parent_of(const int* __restrict__ parent, int base, int i, int n) {
+  const int p = i < n ? parent[base + i] : -1;
+  return p >= 0 && p < i ? p : -1;
+}
+
+// All of a row's nodes, by a workgroup, into LDS: mask[node][W]. First every
+// block of 64 for itself, with the node by which each lane's chain leaves it;
+// then, block by block, the words of that node. Bits of nodes past n: only
+// their own.
+struct RowTree {
+  uint64_t* mask;  // [64 W][W]
+  int* up;         // [64 W] the first ancestor in an earlier block, -1: none
+};
+__device__ __forceinline__ RowTree row_tree(char* lds, int W) {
+  return RowTree{(uint64_t*)lds, (int*)(lds + (size_t)64 * W * W * 8)};
+}
+static size_t row_tree_bytes(int W) { return (size_t)64 * W * (W * 8 + 4); }
+__device__ __forceinline__ void row_ancestors(const RowTree& t, const int* __restrict__ parent, int base, int n,
+                                              int W) {
+  const int lane = threadIdx.x & 63, nb = (n + 63) >> 6;
+  for (int k = threadIdx.x >> 6; k < nb; k += blockDim.x >> 6) {
+    const int i = 64 * k + lane, p = parent_of(parent, base, i, n);
+    const uint64_t m = block_ancestors(p >= 64 * k ? p - 64 * k : -1);
+    t.mask[i * W + k] = m;
+    const int above = __shfl(p, __builtin_ctzll(m), WAVE);  // the chain's topmost node here has the lowest index
+    t.up[i] = above;
+    for (int w = k + 1; w < W; ++w) t.mask[i * W + w] = 0;
+  }
+  __syncthreads();
+  for (int k = 1; k < nb; ++k) {
+    for (int x = threadIdx.x; x < 64 * k; x += blockDim.x) {
+      const int i = 64 * k + x / k, w = x % k, u = t.up[i];
+      t.mask[i * W + w] = u >= 0 ? t.mask[u * W + w] : 0;
+    }
+    __syncthreads();
+  }
+}
+
+// Tokens of no row: behind the last one, before the first, or of a row that is treated as empty.
+template <typename F>
+__device__ __forceinline__ void each_unowned(const int* __restrict__ row_off, int b, int B, int max_tokens, int n,
+                                             F f) {
+  const int lo = max(row_off[b], 0), hi = min(row_off[b + 1], max_tokens);
+  if (n == 0)
+    for (int t = lo + threadIdx.x; t < hi; t += blockDim.x) f(t);
+  if (b == 0)
+    for (int t = threadIdx.x; t < min(lo, max_tokens); t += blockDim.x) f(t);
+  for (int64_t t = max(row_off[B], 0) + (int64_t)b * blockDim.x + threadIdx.x; t < max_tokens;
+       t += (int64_t)B * blockDim.x)
+    f((int)t);
+}
+
+// A row per workgroup; rows of up to 64 nodes in one wave's registers. Bound by
+// latency: offsets, parents, six rounds of shuffles.
+template <bool ONE>
+__global__ __launch_bounds__(256) void k_tree_tables(const int* __restrict__ parent, const int* __restrict__ row_off,
+                                                     const int* __restrict__ start, uint64_t* __restrict__ mask,
+                                                     int* __restrict__ tok_pos, int B, int max_tokens,
+                                                     int max_per_row, int W) {
+  extern __shared__ char lds[];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int at = start[b];
+  const RowSpan sp = row_span(row_off, b, max_per_row, max_tokens);
+  each_unowned(row_off, b, B, max_tokens, sp.n, [&](int t) {
+    for (int w = 0; w < W; ++w) mask[(int64_t)t * W + w] = 0;
+    tok_pos[t] = -1;
+  });
+  if (sp.n == 0) return;
+  if constexpr (ONE) {
+    const uint64_t m = block_ancestors(parent_of(parent, sp.base, tid, sp.n));
+    if (tid < sp.n) {
+      mask[sp.base + tid] = m;
+      tok_pos[sp.base + tid] = at + __popcll(m) - 1;
+    }
+  } else {
+    const RowTree t = row_tree(lds, W);
+    row_ancestors(t, parent, sp.base, sp.n, W);
+    for (int x = tid; x < sp.n * W; x += blockDim.x) mask[(int64_t)sp.base * W + x] = t.mask[x];
+    for (int i = tid; i < sp.n; i += blockDim.x) {
+      int deep = -1;
+      for (int w = 0; w <= i >> 6; ++w) deep += __popcll(t.mask[i * W + w]);
+      tok_pos[sp.base + i] = at + deep;
+    }
+  }
+}
+
+static int check_tree(int32_t batch, int32_t max_tokens, int32_t max_per_row) {
+  FC_CHECK_ARG(batch > 0 && batch <= PT_ROWS, "batch must be in [1, 4096]");
+  FC_CHECK_ARG(max_tokens > 0 && max_tokens < 1 << 30, "max_tokens must be in [1, 2^30)");
+  FC_CHECK_ARG(max_per_row > 0 && max_per_row <= FC_TREE_MOST, "max_per_row must be in [1, 512]");
+  return FC_OK;
+}
+
+extern "C" int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
+                                  int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row,
+                                  void* stream) {
+  FC_CHECK_ARG(parent && row_off && start && mask && tok_pos, "null pointer");
+  const int rc = check_tree(batch, max_tokens, max_per_row);
+  if (rc != FC_OK) return rc;
+  const int W = (max_per_row + 63) / 64;
+  const hipStream_t s = (hipStream_t)stream;
+  if (W == 1)
+    hipLaunchKernelGGL(k_tree_tables<true>, dim3(batch), dim3(64), 0, s, parent, row_off, start, mask, tok_pos, batch,
+                       max_tokens, max_per_row, W);
+  else
+    hipLaunchKernelGGL(k_tree_tables<false>, dim3(batch), dim3(256), row_tree_bytes(W), s, parent, row_off, start,
+                       mask, tok_pos, batch, max_tokens, max_per_row, W);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Accept
+// ---------------------------------------------------------------------------
+// A node agrees if it is a root or its token is the target's choice at its
+// parent; it is accepted if it and all nodes above it agree, that is, if none of
+// its mask's bits is outside the agreeing nodes' set. The accepted node with the
+// most nodes above it, the lowest index among equals, ends the path.
+template <bool ONE>
+__global__ __launch_bounds__(256) void k_tree_accept(const int* __restrict__ parent, const int* __restrict__ tokens,
+                                                     const int* __restrict__ target, const int* __restrict__ row_off,
+                                                     int* __restrict__ n_accepted, int* __restrict__ next_token,
+                                                     int* __restrict__ path, int B, int max_tokens, int max_per_row,
+                                                     int W) {
+  extern __shared__ char lds[];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const RowSpan sp = row_span(row_off, b, max_per_row, max_tokens);
+  each_unowned(row_off, b, B, max_tokens, sp.n, [&](int t) { path[t] = -1; });
+  if (sp.n == 0) {
+    if (tid == 0) {
+      n_accepted[b] = 0;
+      next_token[b] = -1;
+    }
+    return;
+  }
+  const int *tok = tokens + sp.base, *tgt = target + sp.base;
+  int* out = path + sp.base;
+  // (count of the path, 511 - index): the larger is better, and one bit at least is set
+  if constexpr (ONE) {
+    const int p = parent_of(parent, sp.base, lane, sp.n);
+    const int mine = lane < sp.n ? tok[lane] : 0, chosen = lane < sp.n ? tgt[lane] : 0;
+    const int above = __shfl(chosen, max(p, 0), WAVE);
+    const uint64_t agree = __ballot(lane < sp.n && (p < 0 || mine == above)), m = block_ancestors(p);
+    const int count = (m & ~agree) == 0 ? __popcll(m) : 0;
+    int key = count > 0 ? count << 9 | (511 - lane) : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) key = max(key, __shfl_xor(key, o, WAVE));
+    const int best = 511 - (key & 511), most = key >> 9;  // (node 0 is a root: most > 0)
+    const uint64_t line = shfl64(m, best);
+    if ((line >> lane) & 1) out[__popcll(line & ((1ull << lane) - 1))] = lane;
+    if (lane >= most && lane < sp.n) out[lane] = -1;
+    if (lane == best) {
+      n_accepted[b] = most;
+      next_token[b] = chosen;
+    }
+  } else {
+    __shared__ uint64_t agree[FC_TREE_MOST / 64];
+    __shared__ int keys[4];
+    const RowTree t = row_tree(lds, W);
+    row_ancestors(t, parent, sp.base, sp.n, W);
+    const int nb = (sp.n + 63) >> 6;
+    for (int k = tid >> 6; k < nb; k += blockDim.x >> 6) {
+      const int i = 64 * k + lane, p = parent_of(parent, sp.base, i, sp.n);
+      const uint64_t a = __ballot(i < sp.n && (p < 0 || tok[i] == tgt[p]));
+      if (lane == 0) agree[k] = a;
+    }
+    __syncthreads();
+    int key = 0;
+    for (int i = tid; i < sp.n; i += blockDim.x) {
+      int count = 0;
+      bool ok = true;
+      for (int w = 0; w <= i >> 6; ++w) {
+        const uint64_t m = t.mask[i * W + w];
+        ok = ok && (m & ~agree[w]) == 0;
+        count += __popcll(m);
+      }
+      if (ok) key = max(key, count << 9 | (511 - i));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) key = max(key, __shfl_xor(key, o, WAVE));
+    if (lane == 0) keys[tid >> 6] = key;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) key = max(key, keys[w]);
+    const int best = 511 - (key & 511), most = key >> 9;
+    const uint64_t* line = t.mask + best * W;
+    for (int i = tid; i < sp.n; i += blockDim.x) {
+      if ((line[i >> 6] >> (i & 63)) & 1) {
+        int place = __popcll(line[i >> 6] & ((1ull << (i & 63)) - 1));
+        for (int w = 0; w < i >> 6; ++w) place += __popcll(line[w]);
+        out[place] = i;
+      }
+      if (i >= most) out[i] = -1;
+    }
+    if (tid == 0) {
+      n_accepted[b] = most;
+      next_token[b] = tgt[best];
+    }
+  }
+}
+
+extern "C" int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, const int32_t* target,
+                                  const int32_t* row_off, int32_t* n_accepted, int32_t* next_token, int32_t* path,
+                                  int32_t batch, int32_t max_tokens, int32_t max_per_row, void* stream) {
+  FC_CHECK_ARG(parent && tokens && target && row_off && n_accepted && next_token && path, "null pointer");
+  const int rc = check_tree(batch, max_tokens, max_per_row);
+  if (rc != FC_OK) return rc;
+  const int W = (max_per_row + 63) / 64;
+  const hipStream_t s = (hipStream_t)stream;
+  if (W == 1)
+    hipLaunchKernelGGL(k_tree_accept<true>, dim3(batch), dim3(64), 0, s, parent, tokens, target, row_off, n_accepted,
+                       next_token, path, batch, max_tokens, max_per_row, W);
+  else
+    hipLaunchKernelGGL(k_tree_accept<false>, dim3(batch), dim3(256), row_tree_bytes(W), s, parent, tokens, target,
+                       row_off, n_accepted, next_token, path, batch, max_tokens, max_per_row, W);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Commit
+// ---------------------------------------------------------------------------
+// Place j of a row's chunk takes K and V of node path[j] > j; an entry that is not
+// behind its place moves nothing. In ascending order no move reads what an earlier one
+// wrote (its source lies behind every place before it), so the places are done in
+// batches, each read before it is written: the result is that of reading all first.
+// A workgroup takes one row, KV head and layer.
+#define MOVES 16  // places a batch
+template <typename T>
+__global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, int64_t kls, int64_t vls,
+                                                     const int* __restrict__ path, const int* __restrict__ slots,
+                                                     const int* __restrict__ row_off, int max_tokens,
+                                                     int max_per_row) {
+  __shared__ int s_src[FC_TREE_MOST], s_dst[FC_TREE_MOST], s_n[FC_TREE_MOST / 64 + 1];
+  const int b = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const RowSpan sp = row_span(row_off, b, max_per_row, max_tokens);
+  if (sp.n == 0) return;
+  const int pool = (int)min((int64_t)pv.N * pv.page, (int64_t)0x7fffffff);
+  int total = 0;  // the moves so far, in order of their places; the first wave lists them
+  if (tid < 64) {
+    for (int j0 = 0; j0 < sp.n; j0 += 64) {
+      const int j = j0 + lane, p = j < sp.n ? path[sp.base + j] : -1;
+      bool is = p > j && p < sp.n;
+      const int src = is ? slots[sp.base + p] : -1, dst = is ? slots[sp.base + j] : -1;
+      is = src >= 0 && src < pool && dst >= 0 && dst < pool;
+      const uint64_t who = __ballot(is);
+      if (is) {
+        const int at = total + __popcll(who & ((1ull << lane) - 1));
+        s_src[at] = src;
+        s_dst[at] = dst;
+      }
+      total += __popcll(who);
+    }
+    if (lane == 0) s_n[0] = total;
+  }
+  __syncthreads();
+  total = s_n[0];
+  kp += blockIdx.z * kls;
+  vp += blockIdx.z * vls;
+  constexpr int E = MOVES;  // elements of a batch per thread, of K and of V (hd <= 256)
+  for (int m0 = 0; m0 < total; m0 += MOVES) {
+    T kx[E], vx[E];
+    const int n = min(MOVES, total - m0) * pv.hd;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int x = tid + 256 * e;
+      if (x < n) {
+        const int src = s_src[m0 + x / pv.hd], id = src / pv.page, at = src - id * pv.page, d = x % pv.hd;
+        kx[e] = kp[k_elem(pv, id, g, at, d)];
+        vx[e] = vp[v_elem(pv, id, g, at, d)];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int x = tid + 256 * e;
+      if (x < n) {
+        const int dst = s_dst[m0 + x / pv.hd], id = dst / pv.page, at = dst - id * pv.page, d = x % pv.hd;
+        kp[k_elem(pv, id, g, at, d)] = kx[e];
+        vp[v_elem(pv, id, g, at, d)] = vx[e];
+      }
+    }
+  }
+}
+
+extern "C" int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_t k_layer_stride,
+                                  int64_t v_layer_stride, const int32_t* path, const int32_t* slots,
+                                  const int32_t* row_off, int32_t batch, int32_t max_tokens, int32_t max_per_row,
+                                  void* stream) {
+  int rc = check_pages(pages);
+  if (rc != FC_OK) return rc;
+  FC_CHECK_ARG(path && slots && row_off, "null pointer");
+  rc = check_tree(batch, max_tokens, max_per_row);
+  if (rc != FC_OK) return rc;
+  FC_CHECK_ARG(n_layer > 0 && n_layer <= 65535 && pages->n_kv_head <= 65535, "n_layer and n_kv_head in [1, 65535]");
+  const PageView pv = page_view(pages);
+  const hipStream_t s = (hipStream_t)stream;
+  const dim3 grid(batch, pv.G, n_layer);
+#define COMMIT(T)                                                                                                 \
+  hipLaunchKernelGGL(k_tree_commit<T>, grid, dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, k_layer_stride,      \
+                     v_layer_stride, path, slots, row_off, max_tokens, max_per_row)
+  if (pages->dtype == FC_BF16) COMMIT(bf16_t);
+  else COMMIT(float);
+#undef COMMIT
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Append with rotation
+// ---------------------------------------------------------------------------
+struct RopeArgs {
+  PageView pv;
+  void *kp, *vp, *out;
+  const void *q, *k, *v;
+  int64_t qst, qsh, kst, ksh, vst, vsh;
+  const int *tok_pos, *slots;
+  const float *cos, *sin;
+  int M, H, len, rot, interleaved;
+  float norm;
+};
+
+// Any head size and alignment: a wave per token and head of q, k or v, a pair of dims per lane and step.
+template <typename T, typename S>
+__global__ __launch_bounds__(256) void k_rope_append_any(RopeArgs a) {
+  const PageView& pv = a.pv;
+  const int lane = threadIdx.x & 63, hd = pv.hd, half = a.rot >> 1, jobs = a.H + 2 * pv.G;
+  const int64_t all = (int64_t)a.M * jobs, nw = (int64_t)gridDim.x * 4;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < all; i += nw) {
+    const int m = (int)(i / jobs), job = (int)(i - (int64_t)m * jobs);
+    const int pos = a.tok_pos[m], slot = a.slots[m];
+    const bool there = pos >= 0 && pos < a.len;
+    const int id = slot >= 0 && slot / pv.page < pv.N ? slot / pv.page : -1, at = slot - id * pv.page;
+    if (job >= a.H && (id < 0 || !there)) continue;
+    if (job >= a.H + pv.G) {
+      const int g = job - a.H - pv.G;
+      for (int d = lane; d < hd; d += 64)
+        st<T>((T*)a.vp, v_elem(pv, id, g, at, d), ld<S>((const S*)a.v, m * a.vst + g * a.vsh + d));
+      continue;
+    }
+    const int g = job < a.H ? job : job - a.H;
+    const S* x = job < a.H ? (const S*)a.q + m * a.qst + g * a.qsh : (const S*)a.k + m * a.kst + g * a.ksh;
+    // pairs lane and lane + 64, then the dims that stay
+    float y1[2], y2[2], y0[4], ss = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int p = lane + 64 * t;
+      y1[t] = y2[t] = 0.f;
+      if (p < half && there) {
+        const float c = a.cos[(int64_t)pos * half + p], s = a.sin[(int64_t)pos * half + p];
+        const float x1 = ld<S>(x, a.interleaved ? 2 * p : p), x2 = ld<S>(x, a.interleaved ? 2 * p + 1 : p + half);
+        y1[t] = x1 * c + x2 * s;
+        y2[t] = x2 * c - x1 * s;
+        ss += y1[t] * y1[t] + y2[t] * y2[t];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int d = a.rot + lane + 64 * t;
+      y0[t] = d < hd && there ? ld<S>(x, d) : 0.f;
+      ss += y0[t] * y0[t];
+    }
+    const float f = a.norm > 0.f ? a.norm / sqrtf(wave_sum(ss) / (float)hd + 1e-6f) : 1.f;
+    auto put = [&](int d, float v) {
+      if (job < a.H) st<T>((T*)a.out, ((int64_t)m * a.H + g) * hd + d, v * f);
+      else st<T>((T*)a.kp, k_elem(pv, id, g, at, d), v * f);
+    };
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int p = lane + 64 * t;
+      if (p < half) {
+        put(a.interleaved ? 2 * p : p, y1[t]);
+        put(a.interleaved ? 2 * p + 1 : p + half, y2[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (a.rot + lane + 64 * t < hd) put(a.rot + lane + 64 * t, y0[t]);
+  }
+}
+
+extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const void* k, const void* v,
+                                  int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                  int32_t src_dtype, const int32_t* tok_pos, const int32_t* slots, const float* cos,
+                                  const float* sin, int32_t rope_len, int32_t rot, int32_t interleaved, float norm,
+                                  void* q_out, int32_t n_head, int32_t M, void* stream) {
+  const int rc = check_pages(pages);
+  if (rc != FC_OK) return rc;
+  FC_CHECK_ARG(M >= 0 && n_head > 0 && n_head <= 65535 && pages->n_kv_head <= 65535,
+               "M, n_head and n_kv_head in [1, 65535]");
+  FC_CHECK_ARG(src_dtype == FC_F32 || src_dtype == FC_BF16, "src_dtype");
+  FC_CHECK_ARG(src_dtype == pages->dtype || src_dtype == FC_F32, "bf16 values into fp32 pages");
+  FC_CHECK_ARG(rot > 0 && rot % 2 == 0 && rot <= pages->head_dim, "rot must be even, in [2, head_dim]");
+  FC_CHECK_ARG(rope_len > 0, "rope_len");
+  FC_CHECK_ARG(norm >= 0.f && norm <= 3.0e38f, "norm must be finite and not negative");
+  if (M == 0) return FC_OK;
+  FC_CHECK_ARG(q && k && v && tok_pos && slots && cos && sin && q_out, "null pointer");
+  const RopeArgs a{page_view(pages), pages->k, pages->v, q_out, q, k, v, q_token_stride, q_head_stride,
+                   k_token_stride, k_head_stride, v_token_stride, v_head_stride, tok_pos, slots, cos, sin,
+                   M, n_head, rope_len, rot, interleaved != 0, norm};
+  const hipStream_t s = (hipStream_t)stream;
+  const int64_t waves = (int64_t)M * (n_head + 2 * pages->n_kv_head);
+  const dim3 grid((unsigned)std::min<int64_t>((waves + 3) / 4, 65536));
+  if (pages->dtype == FC_F32) hipLaunchKernelGGL((k_rope_append_any<float, float>), grid, dim3(256), 0, s, a);
+  else if (src_dtype == FC_F32) hipLaunchKernelGGL((k_rope_append_any<bf16_t, float>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_rope_append_any<bf16_t, bf16_t>), grid, dim3(256), 0, s, a);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}

@@ -37,7 +37,7 @@ DeviceModel) and everything they write as tensors, declared mutated:
              gen_cap, vocab, temperature, top_k, seed, workspace)
                                      one whole speculative round (engine.py:484-606)
 
-The paged KV cache (one layer; k_pages [n_pages][n_kv_head][page][head_dim]
+The paged KV cache (one layer unless said; k_pages [n_pages][n_kv_head][page][head_dim]
 and v_pages [n_pages][n_kv_head][page / 32][head_dim][32] in the caches' block
 order, whose pages may be strided, as those of one layer of a pool of all
 layers are; every index tensor int32). None has a backward pass: tensors that require a gradient are refused
@@ -52,6 +52,23 @@ where gradients are recorded, and what a call writes counts as modified in place
   paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None,
                   prefix_len=0)      attention over the pages, the shared prefix computed once for all rows
                                      (engine.py:128-156) -> [tokens][n_head * head_dim]; inference only
+Decoding with trees of drafted tokens over that cache: row b's chunk is a tree or a forest whose node i, token
+row_off[b] + i, continues node parent[row_off[b] + i] < i of its row (any other value: a root), lies in the cache at
+start[b] + i and counts as position start[b] + its depth; at most 512 nodes a row (max_per_row):
+  tree_tables(parent, row_off, start, max_per_row) -> (mask, tok_pos)
+                                     each node's ancestors and itself as bits, int64 [tokens][words of 64], and its
+                                     position (fc_tree_tables)
+  rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved=False, norm=0.0) -> q
+                                     page_append with the rotation of q and k at tok_pos and the QK norm
+                                     (gpt.py:52-71, engine.py:108-126); trees or not
+  tree_attention(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, max_per_row, window,
+                 prefix_pages=None, prefix_len=0)
+                                     paged_attention where a node sees what its row holds and the nodes of its mask
+  tree_accept(parent, tokens, target, row_off, max_per_row) -> (n_accepted, next_token, path)
+                                     the deepest path on which the target's choices are the drafted tokens
+  tree_commit(path, slots, row_off, max_per_row, k_pages, v_pages)
+                                     that path's K and V to the front of its row's chunk, in one layer, or in all of
+                                     [n_layer] of them
 `buffers` is the speculative state's device arrays in fc_spec_state order
 (`SPEC_BUFFERS`: t_len .. p_stats, then the partials buffer `part`).
 """
@@ -65,7 +82,7 @@ from ._lib import check, lib
 
 __all__ = ["pack_operand", "linear", "attention", "cross_entropy", "frag_to_rows", "forward", "attn_prologue",
            "attn_qkv", "row_stats", "spec_accept", "spec_round", "SPEC_BUFFERS", "page_tables", "page_append",
-           "paged_attention"]
+           "paged_attention", "tree_tables", "tree_attention", "tree_accept", "tree_commit", "rope_append"]
 
 NS = "flaxchat_mi355x"
 
@@ -604,36 +621,50 @@ def page_append(k, v, slots, k_pages, v_pages):
      "int max_per_row, int window, Tensor? prefix_pages=None, int prefix_len=0) -> Tensor")
 def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None,
                     prefix_len=0):
-    p, G, page, hd = _pages("paged_attention", k_pages, v_pages)
+    return _attend("paged_attention", q, k_pages, v_pages, tables, row_off, start, (), max_per_row, window,
+                   prefix_pages, prefix_len)
+
+
+def _attend(name, q, k_pages, v_pages, tables, row_off, start, tree, max_per_row, window, prefix_pages, prefix_len):
+    """paged_attention, or with tree = (mask, tok_pos) tree_attention."""
+    p, G, page, hd = _pages(name, k_pages, v_pages)
     if q.dim() != 3 or q.shape[2] != hd or q.shape[1] == 0 or q.shape[1] % G != 0:
-        raise ValueError(f"paged_attention: q [tokens][n_head][{hd}], n_head a multiple of {G} "
+        raise ValueError(f"{name}: q [tokens][n_head][{hd}], n_head a multiple of {G} "
                          f"(got {tuple(q.shape)})")
     if q.dtype != k_pages.dtype:
-        raise ValueError("paged_attention: q and the pages share one dtype")
+        raise ValueError(f"{name}: q and the pages share one dtype")
     if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
-        raise ValueError("paged_attention has no backward pass")
+        raise ValueError(f"{name} has no backward pass")
     if tables.dim() != 2:
-        raise ValueError(f"paged_attention: tables [batch][width] (got {tuple(tables.shape)})")
+        raise ValueError(f"{name}: tables [batch][width] (got {tuple(tables.shape)})")
     B, W = tables.shape
     T, H, _ = q.shape
     if not 1 <= B <= 4096 or W < 1 or H > 65535 or not 1 <= max_per_row <= 0x7fffffff:
-        raise ValueError("paged_attention: batch in [1, 4096], width and max_per_row at least 1 and below 2^31")
+        raise ValueError(f"{name}: batch in [1, 4096], width and max_per_row at least 1 and below 2^31")
     if not 0 <= window <= 0x7fffffff or T > 0x7fffffff:
-        raise ValueError("paged_attention: window in [0, 2^31), tokens below 2^31")
+        raise ValueError(f"{name}: window in [0, 2^31), tokens below 2^31")
     if prefix_len < 0 or W * page + prefix_len > 0x7fffffff:
-        raise ValueError("paged_attention: prefix_len >= 0, positions below 2^31")
-    _index("paged_attention", "tables", tables, B * W)
-    _index("paged_attention", "row_off", row_off, B + 1)
-    _index("paged_attention", "start", start, B)
+        raise ValueError(f"{name}: prefix_len >= 0, positions below 2^31")
+    _index(name, "tables", tables, B * W)
+    _index(name, "row_off", row_off, B + 1)
+    _index(name, "start", start, B)
+    if tree:
+        _tree_rows(name, max_per_row)
+        mask, tok_pos = tree
+        words = (max_per_row + 63) // 64
+        if mask.dtype != torch.int64 or mask.shape != (T, words) or not mask.is_contiguous():
+            raise ValueError(f"{name}: mask is a contiguous int64 tensor [{T}][{words}] "
+                             f"(got {mask.dtype}, {tuple(mask.shape)})")
+        _index(name, "tok_pos", tok_pos, T)
     pre = 0
     if prefix_len > 0:
         if prefix_pages is None or prefix_pages.numel() * page < prefix_len:
-            raise ValueError(f"paged_attention: prefix_pages holds the pages of {prefix_len} positions")
-        _index("paged_attention", "prefix_pages", prefix_pages, prefix_pages.numel())
+            raise ValueError(f"{name}: prefix_pages holds the pages of {prefix_len} positions")
+        _index(name, "prefix_pages", prefix_pages, prefix_pages.numel())
         pre = prefix_pages.data_ptr()
-        d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start, prefix_pages)
+        d = _on_gpu(name, q, k_pages, v_pages, tables, row_off, start, prefix_pages, *tree)
     else:
-        d = _on_gpu("paged_attention", q, k_pages, v_pages, tables, row_off, start)
+        d = _on_gpu(name, q, k_pages, v_pages, tables, row_off, start, *tree)
     y = q.new_empty((T, H * hd))
     if T == 0:
         return y
@@ -642,12 +673,14 @@ def paged_attention(q, k_pages, v_pages, tables, row_off, start, max_per_row, wi
         q = q.contiguous()
         qt, qh, _ = q.stride()
     L = lib()
-    nb = L.fc_paged_attention_workspace_bytes(p, B, T, max_per_row, H, W, prefix_len, window)
+    query, call = (L.fc_tree_attention_workspace_bytes, L.fc_tree_attention) if tree else \
+        (L.fc_paged_attention_workspace_bytes, L.fc_paged_attention)
+    nb = query(p, B, T, max_per_row, H, W, prefix_len, window)
     if nb < 0:
-        check(nb, "fc_paged_attention_workspace_bytes")
+        check(nb, f"fc_{name}_workspace_bytes")
     ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None  # held until the launch is queued
-    _launch("fc_paged_attention", d, L.fc_paged_attention, p, q.data_ptr(), qt, qh, y.data_ptr(), B, T, max_per_row, H,
-            tables.data_ptr(), W, row_off.data_ptr(), start.data_ptr(), pre, prefix_len, window,
+    _launch(f"fc_{name}", d, call, p, q.data_ptr(), qt, qh, y.data_ptr(), B, T, max_per_row, H, tables.data_ptr(), W,
+            row_off.data_ptr(), start.data_ptr(), *[t.data_ptr() for t in tree], pre, prefix_len, window,
             _lib.FC_PAGED_ZERO_TAIL, ws.data_ptr() if nb else 0, nb)
     return y
 
@@ -665,3 +698,165 @@ def _(k, v, slots, k_pages, v_pages):
 @torch.library.register_fake(f"{NS}::paged_attention", lib=_PAGED)
 def _(q, k_pages, v_pages, tables, row_off, start, max_per_row, window, prefix_pages=None, prefix_len=0):
     return q.new_empty((q.shape[0], q.shape[1] * q.shape[2]))
+
+
+# ---------------------------------------------------------------- trees of drafted tokens
+def _tree_rows(name: str, max_per_row: int):
+    if not 1 <= max_per_row <= _lib.FC_TREE_MOST:
+        raise ValueError(f"{name}: max_per_row in [1, {_lib.FC_TREE_MOST}]")
+
+
+def _tree_chunk(name: str, row_off: torch.Tensor, max_per_row: int, **per_token):
+    """(batch, tokens) of a chunk, its arrays checked."""
+    _tree_rows(name, max_per_row)
+    B = row_off.numel() - 1
+    T = next(iter(per_token.values())).numel()
+    if not 1 <= B <= 4096 or T >= 1 << 30:
+        raise ValueError(f"{name}: row_off of 2 to 4097 entries, tokens below 2^30")
+    _index(name, "row_off", row_off, B + 1)
+    for what, t in per_token.items():
+        _index(name, what, t, T)
+    return B, T
+
+
+@_op("tree_tables(Tensor parent, Tensor row_off, Tensor start, int max_per_row) -> (Tensor, Tensor)")
+def tree_tables(parent, row_off, start, max_per_row):
+    B, T = _tree_chunk("tree_tables", row_off, max_per_row, parent=parent)
+    _index("tree_tables", "start", start, B)
+    d = _on_gpu("tree_tables", parent, row_off, start)
+    mask = parent.new_empty((T, (max_per_row + 63) // 64), dtype=torch.int64)
+    tok_pos = parent.new_empty((T,))
+    if T > 0:
+        _launch("fc_tree_tables", d, lib().fc_tree_tables, parent.data_ptr(), row_off.data_ptr(), start.data_ptr(),
+                mask.data_ptr(), tok_pos.data_ptr(), B, T, max_per_row)
+    return mask, tok_pos
+
+
+@_op("tree_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor tables, Tensor row_off, Tensor start, "
+     "Tensor mask, Tensor tok_pos, int max_per_row, int window, Tensor? prefix_pages=None, int prefix_len=0) "
+     "-> Tensor")
+def tree_attention(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, max_per_row, window,
+                   prefix_pages=None, prefix_len=0):
+    return _attend("tree_attention", q, k_pages, v_pages, tables, row_off, start, (mask, tok_pos), max_per_row, window,
+                   prefix_pages, prefix_len)
+
+
+@_op("tree_accept(Tensor parent, Tensor tokens, Tensor target, Tensor row_off, int max_per_row) "
+     "-> (Tensor, Tensor, Tensor)")
+def tree_accept(parent, tokens, target, row_off, max_per_row):
+    B, T = _tree_chunk("tree_accept", row_off, max_per_row, parent=parent, tokens=tokens, target=target)
+    d = _on_gpu("tree_accept", parent, tokens, target, row_off)
+    n_accepted, next_token, path = (parent.new_empty((n,)) for n in (B, B, T))
+    if T == 0:
+        n_accepted.fill_(0)
+        next_token.fill_(-1)
+    else:
+        _launch("fc_tree_accept", d, lib().fc_tree_accept, parent.data_ptr(), tokens.data_ptr(), target.data_ptr(),
+                row_off.data_ptr(), n_accepted.data_ptr(), next_token.data_ptr(), path.data_ptr(), B, T, max_per_row)
+    return n_accepted, next_token, path
+
+
+@_op("tree_commit(Tensor path, Tensor slots, Tensor row_off, int max_per_row, Tensor(a!) k_pages, "
+     "Tensor(b!) v_pages) -> ()")
+def tree_commit(path, slots, row_off, max_per_row, k_pages, v_pages):
+    L, ks, vs = 1, 0, 0
+    if k_pages.dim() == 5:  # all layers
+        if v_pages.dim() != 6 or v_pages.shape[0] != k_pages.shape[0] or not 1 <= k_pages.shape[0] <= 65535:
+            raise ValueError(f"tree_commit: k_pages and v_pages of as many layers, 1 to 65535 (got "
+                             f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)})")
+        L = k_pages.shape[0]
+        kl, vl = k_pages[0], v_pages[0]
+        if L > 1:
+            ks, vs = k_pages.stride(0), v_pages.stride(0)
+    else:
+        kl, vl = k_pages, v_pages
+    p, G, page, hd = _pages("tree_commit", kl, vl)
+    if L > 1 and not (_layers_apart(k_pages) and _layers_apart(v_pages)):
+        raise ValueError("tree_commit: layers must not overlap")
+    if G > 65535:
+        raise ValueError("tree_commit: n_kv_head at most 65535")
+    if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("tree_commit has no backward pass")
+    B, T = _tree_chunk("tree_commit", row_off, max_per_row, path=path, slots=slots)
+    d = _on_gpu("tree_commit", k_pages, v_pages, path, slots, row_off)
+    if T == 0:
+        return
+    _written((k_pages, v_pages))
+    _launch("fc_tree_commit", d, lib().fc_tree_commit, p, L, ks, vs, path.data_ptr(), slots.data_ptr(),
+            row_off.data_ptr(), B, T, max_per_row)
+
+
+def _layers_apart(t: torch.Tensor) -> bool:
+    """Whether layers [n_layer][n_pages].. share no element: one behind the other, or page by page."""
+    one = t[0, 0].numel()
+    ls, ps, L, N = t.stride(0), t.stride(1) if t.shape[1] > 1 else one, t.shape[0], t.shape[1]
+    return ls >= ps * (N - 1) + one or (ls >= one and ps >= ls * (L - 1) + one)
+
+
+@_op("rope_append(Tensor q, Tensor k, Tensor v, Tensor tok_pos, Tensor slots, Tensor cos, Tensor sin, "
+     "Tensor(a!) k_pages, Tensor(b!) v_pages, bool interleaved=False, float norm=0.0) -> Tensor")
+def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved=False, norm=0.0):
+    p, G, _, hd = _pages("rope_append", k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != hd or not 1 <= q.shape[1] <= 65535 or G > 65535:
+        raise ValueError(f"rope_append: q [tokens][n_head][{hd}], at most 65535 heads (got {tuple(q.shape)})")
+    M, H, _ = q.shape
+    if k.shape != (M, G, hd) or v.shape != k.shape:
+        raise ValueError(f"rope_append: k and v [{M}][{G}][{hd}] (got {tuple(k.shape)} and {tuple(v.shape)})")
+    if q.dtype != k.dtype or v.dtype != k.dtype or (k.dtype != k_pages.dtype and k.dtype != torch.float32):
+        raise ValueError(f"rope_append: q, k and v in the pages' dtype or fp32 (got {q.dtype}, {k.dtype} and "
+                         f"{v.dtype})")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, cos, sin, k_pages, v_pages)):
+        raise ValueError("rope_append has no backward pass")
+    if cos.dim() != 2 or cos.shape != sin.shape or not 1 <= cos.shape[1] <= hd // 2 or \
+            not 1 <= cos.shape[0] <= 0x7fffffff:
+        raise ValueError(f"rope_append: cos and sin [positions][pairs], up to {hd // 2} pairs of a head (got "
+                         f"{tuple(cos.shape)} and {tuple(sin.shape)})")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("rope_append: cos and sin are contiguous fp32 tensors")
+    if not 0.0 <= norm <= 3e38:
+        raise ValueError(f"rope_append: norm is finite and not negative (got {norm})")
+    if M > 0x7fffffff:
+        raise ValueError("rope_append: tokens below 2^31")
+    _index("rope_append", "tok_pos", tok_pos, M)
+    _index("rope_append", "slots", slots, M)
+    d = _on_gpu("rope_append", q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages)
+    out = q.new_empty((M, H, hd), dtype=k_pages.dtype)
+    if M == 0:
+        return out
+    _written((k_pages, v_pages))
+    if hd != 1 and (q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    _launch("fc_rope_append", d, lib().fc_rope_append, p, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0),
+            q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _dtype_code(k), tok_pos.data_ptr(),
+            slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], interleaved, norm,
+            out.data_ptr(), H, M)
+    return out
+
+
+@torch.library.register_fake(f"{NS}::tree_tables", lib=_PAGED)
+def _(parent, row_off, start, max_per_row):
+    return (parent.new_empty((parent.shape[0], (max_per_row + 63) // 64), dtype=torch.int64),
+            parent.new_empty((parent.shape[0],)))
+
+
+@torch.library.register_fake(f"{NS}::tree_attention", lib=_PAGED)
+def _(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, max_per_row, window, prefix_pages=None,
+      prefix_len=0):
+    return q.new_empty((q.shape[0], q.shape[1] * q.shape[2]))
+
+
+@torch.library.register_fake(f"{NS}::tree_accept", lib=_PAGED)
+def _(parent, tokens, target, row_off, max_per_row):
+    B, T = row_off.shape[0] - 1, parent.shape[0]
+    return parent.new_empty((B,)), parent.new_empty((B,)), parent.new_empty((T,))
+
+
+@torch.library.register_fake(f"{NS}::tree_commit", lib=_PAGED)
+def _(path, slots, row_off, max_per_row, k_pages, v_pages):
+    _written((k_pages, v_pages))
+
+
+@torch.library.register_fake(f"{NS}::rope_append", lib=_PAGED)
+def _(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved=False, norm=0.0):
+    _written((k_pages, v_pages))
+    return q.new_empty(q.shape, dtype=k_pages.dtype)

@@ -403,6 +403,84 @@ int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token
                            const int32_t* prefix_pages, int32_t prefix_len, int32_t window, int32_t flags,
                            void* work, int64_t work_bytes, void* stream);
 
+/* Decoding with trees of drafted tokens. Row b's chunk (packed, as above) is a
+ * tree or a forest: node i of the row is token row_off[b] + i, its parent is
+ * parent[row_off[b] + i], the index in the row of an earlier node; any other
+ * value makes it a root, which continues what the row holds. Node i sits in
+ * the cache at position start[b] + i and is, for rotation and windows, at
+ * position start[b] + its depth (a root's is 0). A row has at most
+ * max_per_row <= FC_TREE_MOST nodes; one of more, or that runs past max_tokens, is
+ * treated as empty. batch <= 4096; row_off does not decrease. No counterpart
+ * in the reference, which drafts and verifies one chain
+ * (flaxchat/engine.py:484-606).
+ *
+ * fc_tree_tables: of each token the set of its ancestors and itself, bit
+ * j % 64 of mask[token][j / 64] for node j of its row, in
+ * ceil(max_per_row / 64) words, and its position; 0 and -1 for tokens of no
+ * row. */
+#define FC_TREE_MOST 512
+int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
+                       int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row, void* stream);
+
+/* fc_paged_attention for such chunks: a token of row b at tok_pos (taken to
+ * be start[b] at least) sees the key at position p < start[b] if window is 0
+ * or tok_pos - p <= window, and the key of node j of its row, at position
+ * start[b] + j in the row's own pages, if bit j of its mask is set, whatever
+ * the window and whatever node j is (masks need not be those of a tree; a
+ * token may have no bit). Bits past the row's nodes mean nothing, and a node whose
+ * position lies in the prefix holds no key. mask: [max_tokens]
+ * [ceil(max_per_row / 64)]. The rest as in fc_paged_attention. */
+int64_t fc_tree_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
+                                          int32_t max_per_row, int32_t n_head, int32_t width, int32_t prefix_len,
+                                          int32_t window);
+int32_t fc_tree_attention(const fc_pages* pages, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          void* y, int32_t batch, int32_t max_tokens, int32_t max_per_row, int32_t n_head,
+                          const int32_t* tables, int32_t width, const int32_t* row_off, const int32_t* start,
+                          const uint64_t* mask, const int32_t* tok_pos, const int32_t* prefix_pages,
+                          int32_t prefix_len, int32_t window, int32_t flags, void* work, int64_t work_bytes,
+                          void* stream);
+
+/* What a step accepts: tokens[max_tokens] are the drafted tokens, target
+ * [max_tokens] the target model's choice behind each node (its argmax, or its
+ * sample). A root is accepted (it is what was decided before); another node
+ * is if its parent is and its token is the parent's target. The deepest
+ * accepted node, the lowest index among equals, ends row b's path:
+ * n_accepted[b] nodes, next_token[b] its target (0 and -1: a row without
+ * nodes), path[row_off[b] + j] the j-th of them from the root, -1 behind
+ * them and for tokens of no row. */
+int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, const int32_t* target, const int32_t* row_off,
+                       int32_t* n_accepted, int32_t* next_token, int32_t* path, int32_t batch, int32_t max_tokens,
+                       int32_t max_per_row, void* stream);
+
+/* The accepted path to the front of its row's chunk, in n_layer layers'
+ * pages, layer l's at pages->k + l * k_layer_stride and pages->v + l *
+ * v_layer_stride elements: K and V of slot slots[row_off[b] + path[j]] go
+ * into slot slots[row_off[b] + j], for every entry path[j] = path
+ * [row_off[b] + j] in (j, nodes of row b), as if all were read before the first is
+ * written. Other entries, and slots outside the pool, move nothing. The
+ * slots of a call's tokens differ. */
+int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_t k_layer_stride, int64_t v_layer_stride,
+                       const int32_t* path, const int32_t* slots, const int32_t* row_off, int32_t batch,
+                       int32_t max_tokens, int32_t max_per_row, void* stream);
+
+/* fc_page_append with the rotation and the norm that q and k take on the way
+ * (flaxchat/gpt.py:52-71, flaxchat/engine.py:108-126), for M tokens. Of each
+ * q and k head the first `rot` dims (even) are rotated in pairs, (i, i + rot
+ * / 2), or (2 i, 2 i + 1) if `interleaved`: (x1 c + x2 s, x2 c - x1 s) with
+ * c = cos[tok_pos][i], s = sin[tok_pos][i] (both [rope_len][rot / 2]; the
+ * other direction is a table of -sin, positions stretched for a long context
+ * are in the tables too). Then, if norm > 0, the head is scaled by norm /
+ * sqrt(mean of its squares + 1e-6). q goes to q_out [M][n_head][head_dim] in
+ * the pages' dtype, K and V into their slots; slots outside the pool keep
+ * nothing, a slot may occur once. A token whose position is outside
+ * [0, rope_len) keeps nothing, and its q is 0. q, k and v: strides in
+ * elements, in the pages' dtype or fp32. */
+int32_t fc_rope_append(const fc_pages* pages, const void* q, const void* k, const void* v, int64_t q_token_stride,
+                       int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                       int64_t v_head_stride, int32_t src_dtype, const int32_t* tok_pos, const int32_t* slots,
+                       const float* cos, const float* sin, int32_t rope_len, int32_t rot, int32_t interleaved,
+                       float norm, void* q_out, int32_t n_head, int32_t M, void* stream);
+
 /* Streaming read of `bytes` (a multiple of 16) from device memory by
  * `workgroups` workgroups of 256 threads, each streaming one contiguous
  * share with 16-byte non-temporal loads; out receives 4 * workgroups

@@ -642,23 +642,51 @@ __device__ __forceinline__ int lanes_scan(int v) {
 
 // Keys of a job are counted from 0: the prefix's positions, or a row's own
 // ones (position - P, which is their place in the row's table).
-// The keys [lo, hi] that a query at position `pos` sees; hi < lo: none.
-__device__ __forceinline__ void key_range(const PagedChunk& c, int64_t pos, bool pre, int& lo, int& hi) {
+// A query: its position, and, of a tree, its row's start and nodes.
+struct Query {
+  int64_t pos, first;
+  int n;
+};
+// Query j of a row of n that starts at `first`; t: its token.
+template <bool tree>
+__device__ __forceinline__ Query query_at(const PagedChunk& c, int64_t first, int n, int j, int t) {
+  return Query{tree ? max(first, (int64_t)c.tok_pos[t]) : first + j, first, n};
+}
+// The keys [lo, hi] that a query sees; hi < lo: none. Of a tree: what the row
+// holds before its start, as far as the window reaches, and all of its nodes'
+// keys, of which the query's bits say more.
+template <bool tree>
+__device__ __forceinline__ void key_range(const PagedChunk& c, const Query& q, bool pre, int& lo, int& hi) {
   const int64_t off = pre ? 0 : c.P, last = pre ? (int64_t)c.P - 1 : (int64_t)c.W * c.pv.page - 1;
-  hi = (int)max((int64_t)-1, min(pos - off, last));
-  lo = c.window > 0 ? (int)max((int64_t)0, min(pos - c.window - off, (int64_t)0x7fffffff)) : 0;
+  const int64_t end = !tree ? q.pos : pre ? q.first - 1 : q.first + q.n - 1;
+  const int64_t from = tree ? min(q.pos - c.window, q.first) : q.pos - c.window;
+  hi = (int)max((int64_t)-1, min(end - off, last));
+  lo = c.window > 0 ? (int)max((int64_t)0, min(from - off, (int64_t)0x7fffffff)) : 0;
+}
+// Where the nodes' keys begin in a walk whose keys are counted from `off`. (Below -FC_TREE_MOST no node has one.)
+__device__ __forceinline__ int nodes_from(int64_t first, int64_t off) {
+  return (int)max(first - off, (int64_t)-2 * FC_TREE_MOST);
+}
+// Bits j0 .. j0 + 7 of a token's row of `words` words; those before 0, for what the row holds before its nodes, are
+// set, those behind the words are not.
+__device__ __forceinline__ uint32_t bits8(const uint64_t* row, int words, int j0) {
+  const int w = j0 >> 6, sh = j0 & 63;
+  const uint64_t a = w < 0 ? ~0ull : w < words ? row[w] : 0ull;
+  uint64_t x = a >> sh;
+  if (sh > 56) x |= (w + 1 < 0 ? ~0ull : w + 1 < words ? row[w + 1] : 0ull) << (64 - sh);
+  return (uint32_t)x & 0xffu;
 }
 
 // How a workgroup walks: over a row's own keys, over the prefix for all rows, or
 // over a row's keys and, if c.joint, the prefix ahead of them. In the last, keys are
 // counted from the prefix's first, and own ones from c.joint: no key lies between.
 enum Walk { OWN_KEYS, PREFIX_KEYS, ROW_KEYS };
-template <int walk>
-__device__ __forceinline__ void walk_range(const PagedChunk& c, int64_t pos, int& lo, int& hi) {
-  key_range(c, pos, walk == PREFIX_KEYS, lo, hi);
+template <int walk, bool tree>
+__device__ __forceinline__ void walk_range(const PagedChunk& c, const Query& q, int& lo, int& hi) {
+  key_range<tree>(c, q, walk == PREFIX_KEYS, lo, hi);
   if constexpr (walk == ROW_KEYS) {
     int plo, phi;
-    key_range(c, pos, true, plo, phi);
+    key_range<tree>(c, q, true, plo, phi);
     if (c.joint > 0) {
       lo = plo < c.P ? plo : (int)min((int64_t)lo + c.joint, (int64_t)0x7fffffff);
       hi = hi >= 0 ? hi + c.joint : phi;
@@ -677,13 +705,13 @@ struct Item {
 struct RowKeys {
   int len, blocks;
 };
-template <int CB, int walk>
+template <int CB, int walk, bool tree>
 __device__ __forceinline__ RowKeys row_keys(const PagedChunk& c, int r) {
   const int64_t at = c.start[min(r, c.B - 1)];  // (its load goes beside those of the offsets)
   const RowSpan sp = row_span(c.row_off, min(r, c.B - 1), c.max_per_row, c.Mcap);
-  int lo, hi, lo1, hi1;
-  walk_range<walk>(c, at, lo, hi);
-  walk_range<walk>(c, at + sp.n - 1, lo1, hi1);
+  int lo, hi, lo1, hi1;  // (no node of a tree is before its row's start, and all reach its last node's key)
+  walk_range<walk, tree>(c, Query{at, at, sp.n}, lo, hi);
+  walk_range<walk, tree>(c, Query{at + sp.n - 1, at, sp.n}, lo1, hi1);
   if (r >= c.B || sp.n == 0) return {-1, 0};
   return {hi1 < lo ? 0 : hi1 + 1 - (lo & ~31), (sp.n * (c.H / c.pv.G) + CB - 1) / CB};
 }
@@ -748,7 +776,7 @@ __device__ __forceinline__ bool item_of(const PagedChunk& c, int& at, int r0, co
   it.skip = (int64_t)it.split * it.len;
   return true;
 }
-template <int CB, int walk, int N>
+template <int CB, int walk, bool tree, int N>
 __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it) {
   const int lane = threadIdx.x & 63;
   RowKeys r[N];
@@ -756,7 +784,7 @@ __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it
   int longest = 1;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    r[i] = row_keys<CB, walk>(c, 64 * i + lane);
+    r[i] = row_keys<CB, walk, tree>(c, 64 * i + lane);
     total += (float)max(r[i].len, 0) * (float)r[i].blocks;
     longest = max(longest, r[i].len);
   }
@@ -766,17 +794,17 @@ __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it
     if (item_of(c, at, 64 * i, r[i], chunk, it)) return true;
   return false;
 }
-template <int CB, int walk>
+template <int CB, int walk, bool tree>
 __device__ __forceinline__ bool find_item(const PagedChunk& c, int at, Item& it) {
-  if (c.B <= 64) return find_among<CB, walk, 1>(c, at, it);
-  if (c.B <= ROWS_SCAN) return find_among<CB, walk, ROWS_SCAN / 64>(c, at, it);
+  if (c.B <= 64) return find_among<CB, walk, tree, 1>(c, at, it);
+  if (c.B <= ROWS_SCAN) return find_among<CB, walk, tree, ROWS_SCAN / 64>(c, at, it);
   const int lane = threadIdx.x & 63, n = (c.B + 63) >> 6;
   const int chunk = __builtin_amdgcn_readfirstlane(c.items[0]), first = c.items[1 + min(lane, n)];
   const int k = __builtin_popcountll(__ballot(lane < n && first <= at)) - 1;
   at -= __builtin_amdgcn_readlane(first, k);
-  return item_of(c, at, 64 * k, row_keys<CB, walk>(c, 64 * k + lane), chunk, it);
+  return item_of(c, at, 64 * k, row_keys<CB, walk, tree>(c, 64 * k + lane), chunk, it);
 }
-template <int CB, int walk>
+template <int CB, int walk, bool tree>
 __global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
   constexpr int N = PT_ROWS / 1024;
   __shared__ float s_total[16];
@@ -787,7 +815,7 @@ __global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
   int longest = 1;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    r[i] = row_keys<CB, walk>(c, 64 * (wave + 16 * i) + lane);
+    r[i] = row_keys<CB, walk, tree>(c, 64 * (wave + 16 * i) + lane);
     total += (float)max(r[i].len, 0) * (float)r[i].blocks;
     longest = max(longest, r[i].len);
   }
@@ -841,7 +869,7 @@ __device__ __forceinline__ void zero_tail(int wg, int nwg) {
 // [c_lo, c_hi) over to this plain form, one wave per column, over the keys
 // [kbeg, kend). (Anything done about them in the walk itself costs every call
 // registers, and spills.)
-template <typename T, int HD>
+template <typename T, int HD, bool tree>
 __device__ __forceinline__ void redo_columns(int walk, const Item& it, int base, int c_lo, int c_hi, int kbeg, int kend,
                                              int wave) {
   const PagedChunk c = chunk_args();
@@ -852,17 +880,18 @@ __device__ __forceinline__ void redo_columns(int walk, const Item& it, int base,
   const int lane = threadIdx.x & 63, rep = c.H / c.pv.G, b = it.b, g = it.g;
   for (int col = c_lo + wave; col < c_hi; col += 4) {
     const int j = col / rep, head = g * rep + col - j * rep;
-    int64_t pos = pre ? 0 : (int64_t)c.start[b] + j;
+    int r = b;
     if (pre) {
-      const int r = row_of(c.row_off, c.B, j);
+      r = row_of(c.row_off, c.B, j);
       if (r >= c.B) continue;
-      const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
-      if (j < sp.base || j >= sp.base + sp.n) continue;
-      pos = (int64_t)c.start[r] + (j - sp.base);
     }
+    const RowSpan sp = row_span(c.row_off, r, c.max_per_row, c.Mcap);
+    if (pre && (j < sp.base || j >= sp.base + sp.n)) continue;
+    const Query qy = query_at<tree>(c, c.start[r], sp.n, pre ? j - sp.base : j, base + j);
+    const uint64_t* bits = c.mask + (int64_t)(base + j) * c.words;
     int v_lo, v_hi;
-    if (walk == ROW_KEYS) walk_range<ROW_KEYS>(c, pos, v_lo, v_hi);
-    else key_range(c, pos, pre, v_lo, v_hi);
+    if (walk == ROW_KEYS) walk_range<ROW_KEYS, tree>(c, qy, v_lo, v_hi);
+    else key_range<tree>(c, qy, pre, v_lo, v_hi);
     v_lo = max(v_lo, kbeg);
     v_hi = min(v_hi, kend - 1);
     const T* qr = q + (base + j) * c.qst + head * c.qsh;
@@ -876,7 +905,12 @@ __device__ __forceinline__ void redo_columns(int walk, const Item& it, int base,
       for (int left = hi - lo + 1; left > 0; left -= 64) {
         const int key = hi + 1 - left + min(lane, left - 1), pg = key / c.pv.page, at = key - pg * c.pv.page;
         const int id = list[pg];
-        const bool ok = lane < left && (unsigned)id < (unsigned)c.pv.N;
+        bool ok = lane < left && (unsigned)id < (unsigned)c.pv.N;
+        if constexpr (tree) {
+          const bool own = !pre && part == 1;  // (of the prefix, what is before the start)
+          const int node = key - nodes_from(qy.first, own ? c.P : 0);
+          ok = ok && (node < 0 || (own && node < qy.n && (bits[node >> 6] >> (node & 63) & 1)));
+        }
         if (!__any(ok)) continue;
         float s = -INFINITY;
         if (ok) {
@@ -1033,17 +1067,19 @@ struct Tile<float, HD> {
 };
 
 // One tile of one wave for 16 query columns: S^T = K Q^T, the running softmax,
-// O^T += V^T P^T. lo, hi: the keys that this lane's column sees; the tile's V is
-// 0 for those that none sees.
-template <typename T, int HD>
+// O^T += V^T P^T. lo, hi: the keys that this lane's column sees, and, of a tree,
+// the bits of the lane's 8; the tile's V is 0 for those that none sees.
+template <bool tree, typename T, int HD>
 __device__ __forceinline__ void tile16(const Tile<T, HD>& t, const typename Tile<T, HD>::Q& q, int kb, int g4, int lo,
-                                       int hi, float scale_log2, float& m_run, float& l_run, f32x4 (&O)[HD / 16]) {
+                                       int hi, uint32_t bits, float scale_log2, float& m_run, float& l_run,
+                                       f32x4 (&O)[HD / 16]) {
   f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
   t.scores(q, sc);
   float p[8], mt = -INFINITY;
 #pragma unroll
   for (int jj = 0; jj < 8; ++jj) {
-    p[jj] = jj >= lo - kb - 8 * g4 && jj <= hi - kb - 8 * g4 ? sc[jj >> 2][jj & 3] * scale_log2 : -INFINITY;
+    const bool seen = jj >= lo - kb - 8 * g4 && jj <= hi - kb - 8 * g4 && (!tree || (bits >> jj & 1));
+    p[jj] = seen ? sc[jj >> 2][jj & 3] * scale_log2 : -INFINITY;
     mt = fmaxf(mt, p[jj]);
   }
   const float m_new = fmaxf(m_run, rows_max(mt));
@@ -1080,7 +1116,7 @@ struct StreamLds {
   float o[4][16][HD + 4];
   float m[4][16], l[4][16];
 };
-template <typename T, int HD, int QB, bool pre>
+template <typename T, int HD, int QB, bool pre, bool tree>
 __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& lds, const Item& it, int base,
                                             int ncol) {
   constexpr int NW = 4, NT = 2 * HD;  // threads that own 8 dims of a column after the merge
@@ -1088,8 +1124,8 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
   const int cl = lane & 15, g4 = lane >> 4;
   const int b = it.b, g = it.g, col0 = it.blk * 16 * QB;
   typename Tile<T, HD>::Q qf[QB];
-  int lo[QB], hi[QB];
-  int w_lo = 0x7fffffff, w_hi = -1, f_lo = 0, f_hi = 0x7fffffff;
+  int lo[QB], hi[QB], tok[QB];
+  int w_lo = 0x7fffffff, w_hi = -1, f_lo = 0, f_hi = 0x7fffffff, nodes = 0x7fffffff;
   int64_t kbeg, kend;
   {
     const PagedChunk& c = w;
@@ -1100,18 +1136,19 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
       const int col = col0 + 16 * u + cl;
       bool ok = col < ncol;
       const int j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
-      int64_t pos = 0;
+      Query qy{0, 0, 0};
       if (pre) {
         const int* off = (const int*)&lds;
         const int r = row_of(off, c.B, j);
         RowSpan sp{0, 0};
         if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
         ok = ok && j >= sp.base && j < sp.base + sp.n;
-        pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+        if (ok) qy = query_at<tree>(c, c.start[r], sp.n, j - sp.base, j);
       } else {
-        pos = (int64_t)c.start[b] + j;
+        qy = query_at<tree>(c, c.start[b], ncol / rep, j, base + j);
       }
-      key_range(c, pos, pre, lo[u], hi[u]);
+      tok[u] = base + j;
+      key_range<tree>(c, qy, pre, lo[u], hi[u]);
       if (!ok) lo[u] = 0x7fffffff, hi[u] = -1;
       const bool some = lo[u] <= hi[u];  // columns that see nothing do not widen the range
       w_lo = min(w_lo, some ? lo[u] : 0x7fffffff);
@@ -1124,9 +1161,13 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
     w_hi = lanes_max<16>(w_hi);
     f_lo = lanes_max<16>(f_lo);
     f_hi = lanes_min<16>(f_hi);
+    if constexpr (tree && !pre) {
+      nodes = nodes_from(c.start[b], c.P);
+      f_hi = min(f_hi, nodes - 1);
+    }
     // (a row's splits are counted from its first column's first key in every one of its blocks)
     int from = w_lo, unused;
-    if (!pre && c.window > 0) key_range(c, c.start[b], false, from, unused);
+    if (!pre && c.window > 0) key_range<tree>(c, Query{c.start[b], c.start[b], 1}, false, from, unused);
     const int64_t s_beg = (int64_t)(from & ~31) + it.skip;
     kbeg = max(s_beg, (int64_t)(w_lo & ~31));
     kend = min((int64_t)w_hi + 1, s_beg + it.len);
@@ -1169,13 +1210,20 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
     Tile<T, HD> t;
     const int64_t in = gofs + r0 * (32 * HD);
     t.load((const T*)w.kp + (int64_t)id0 * w.pv.ks + in, (const T*)w.vp + (int64_t)id0 * w.pv.vs + in, lane);
+    uint32_t bits[QB];
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+      bits[u] = 0xff;
+      if (tree && !pre && kb + 31 >= nodes)
+        bits[u] = bits8(w.mask + (int64_t)tok[u] * w.words, w.words, kb + 8 * g4 - nodes);
+    }
     if (!(kb >= f_lo && kb + 31 <= f_hi)) odd |= t.clear(w_lo - kb - 8 * g4, w_hi - kb - 8 * g4);
 #pragma unroll
     for (int u = 0; u < QB; ++u)
-      tile16<T, HD>(t, qf[u], kb, g4, lo[u], hi[u], scale_log2, m_run[u], l_run[u], O[u]);
+      tile16<tree && !pre, T, HD>(t, qf[u], kb, g4, lo[u], hi[u], bits[u], scale_log2, m_run[u], l_run[u], O[u]);
   }
   if (__syncthreads_or(odd)) {  // (also: the readers of the LDS are done with it)
-    redo_columns<T, HD>(pre ? PREFIX_KEYS : OWN_KEYS, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend),
+    redo_columns<T, HD, tree>(pre ? PREFIX_KEYS : OWN_KEYS, it, base, col0, min(col0 + 16 * QB, ncol), (int)min(kbeg, kend),
                         (int)kend, wave);
     return;
   }
@@ -1227,7 +1275,7 @@ __device__ __forceinline__ void stream_item(const PagedChunk& w, StreamLds<HD>& 
 }
 
 // The workgroup numbered `at`: an item of the list, or a split of the prefix.
-template <typename T, int HD, int QB, bool pre>
+template <typename T, int HD, int QB, bool pre, bool tree>
 __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& lds, int at) {
   Item it;
   int base = 0, ncol;
@@ -1245,12 +1293,12 @@ __device__ __forceinline__ void stream_keys(const PagedChunk& c, StreamLds<HD>& 
     stage_offsets(off, c.row_off, c.B);
     __syncthreads();
   } else {
-    if (!find_item<16 * QB, OWN_KEYS>(c, at, it)) return;
+    if (!find_item<16 * QB, OWN_KEYS, tree>(c, at, it)) return;
     const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
     base = sp.base;
     ncol = sp.n * (c.H / c.pv.G);
   }
-  stream_item<T, HD, QB, pre>(c, lds, it, base, ncol);
+  stream_item<T, HD, QB, pre, tree>(c, lds, it, base, ncol);
 }
 
 // Merge of the key splits of one (token, head), HD / 8 threads with 8
@@ -1353,7 +1401,7 @@ struct WideLds {
   WideStage<HD> stg[2];
   int rng[4][2];
 };
-template <int HD, int walk>
+template <int HD, int walk, bool tree>
 __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
   constexpr bool pre = walk == PREFIX_KEYS;
@@ -1362,7 +1410,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, kk = lane & 31;
   Item it;
-  int base = 0, ncol, lo_c, hi_c, w_lo, w_hi;
+  int base = 0, ncol, lo_c, hi_c, w_lo, w_hi, tok = 0;
   int64_t kbeg64, kend64;
   bool ok;
   v4u qf[DS];  // dims 16 h + 8 hl .. +7 of this lane's query
@@ -1385,7 +1433,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       stage_offsets(off, c.row_off, c.B);
       __syncthreads();
     } else {
-      if (!find_item<128, walk>(c, at, it)) return;
+      if (!find_item<128, walk, tree>(c, at, it)) return;
       const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
       base = sp.base;
       ncol = sp.n * rep;
@@ -1395,16 +1443,17 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     const int col = c0 + 32 * wave + kk;
     ok = col < ncol;
     const int j = ok ? col / rep : 0, head = it.g * rep + (ok ? col - j * rep : 0);
-    int64_t pos = 0;
+    Query qy{0, 0, 0};
     if (pre) {
       const int* off = (const int*)stg;
       const int r = row_of(off, c.B, j);
       RowSpan sp{0, 0};
       if (r < c.B) sp = row_span(off, r, c.max_per_row, c.Mcap);
       ok = ok && j >= sp.base && j < sp.base + sp.n;
-      pos = ok ? (int64_t)c.start[r] + (j - sp.base) : 0;
+      if (ok) qy = query_at<tree>(c, c.start[r], sp.n, j - sp.base, j);
     } else {
-      pos = (int64_t)c.start[it.b] + j;
+      tok = base + j;
+      qy = query_at<tree>(c, c.start[it.b], ncol / rep, j, tok);
     }
     {
       const bf16_t* qr = (const bf16_t*)c.q + (base + j) * c.qst + head * c.qsh + 8 * hl;
@@ -1412,7 +1461,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 #pragma unroll
       for (int h = 0; h < DS; ++h) qf[h] = *(const v4u*)(qr + 16 * h) & keep;
     }
-    walk_range<walk>(c, pos, lo_c, hi_c);
+    walk_range<walk, tree>(c, qy, lo_c, hi_c);
     if (!ok) lo_c = 0x7fffffff, hi_c = -1;
     // the keys that some column of the workgroup sees
     w_lo = lanes_min<32>(lo_c <= hi_c ? lo_c : 0x7fffffff);
@@ -1432,7 +1481,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     g_hi = __builtin_amdgcn_readfirstlane(g_hi);
     // (a row's splits are counted from its first column's first key in every one of its blocks)
     int row_lo = g_lo, unused;
-    if (!pre && c.window > 0) walk_range<walk>(c, c.start[it.b], row_lo, unused);
+    if (!pre && c.window > 0) walk_range<walk, tree>(c, Query{c.start[it.b], c.start[it.b], 1}, row_lo, unused);
     const int64_t s_beg = (int64_t)(row_lo & ~31) + it.skip;
     kend64 = min((int64_t)g_hi + 1, s_beg + it.len);
     kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
@@ -1518,7 +1567,10 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     const const_ints list = CONST_INTS(pre || part == 0 ? w.pre : w.tables + (int64_t)b * w.W);
     // keys that the column sees, that one of the wave does, that all of them do; behind t1 a step repeats its last tile
     const int lo = lo_c - from, hi = min(hi_c - from, t1 - 1), a_lo = w_lo - from, a_hi = min(w_hi - from, t1 - 1);
-    const int f_lo = lanes_max<32>(ok ? lo : 0), f_hi = lanes_min<32>(ok ? hi : 0x7fffffff);
+    const int f_lo = lanes_max<32>(ok ? lo : 0), h_hi = lanes_min<32>(ok ? hi : 0x7fffffff);
+    // a tree's nodes: their keys' first, and the words of bits that say who sees which (in the prefix, none)
+    const int nodes = tree && !pre ? nodes_from(w.start[b], part == 0 ? 0 : w.P) : 0x7fffffff;
+    const int f_hi = tree && !pre ? min(h_hi, nodes - 1) : h_hi;
     // the walk over the pages, one tile at a time; the next page's entry is under way a page ahead
     int tile = t0 >> 5, pg = pg0, tr = tile - pg * tpp;
     int id = list[pg], id_next = list[min(pg + 1, pg_last)];
@@ -1526,6 +1578,13 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     auto step = [&](const WideStage<HD>& S_, int in, int i) {
       const int kb = t0 + 64 * i;
       if (!(kb <= a_hi && kb + 63 >= a_lo)) return;
+      uint32_t bits = 0xffffffffu;  // which of the lane's keys a tree's node may see, 16 of either tile
+      if (tree && !pre && kb + 63 >= nodes) {
+        const uint64_t* row = w.mask + (int64_t)tok * w.words;
+        const int words = part == 0 ? 0 : w.words, k0 = kb + 8 * hl - nodes;
+        bits = bits8(row, words, k0) | bits8(row, words, k0 + 16) << 8 | bits8(row, words, k0 + 32) << 16 |
+               bits8(row, words, k0 + 48) << 24;
+      }
       f32x16 sc[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -1557,7 +1616,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const int kx = 16 * (x >> 3) + (x & 7);
-            if (!(kx >= lr && kx <= hr)) sc[u][x] = -INFINITY;
+            if (!(kx >= lr && kx <= hr && (!tree || pre || (bits >> (16 * u + x) & 1)))) sc[u][x] = -INFINITY;
           }
           // keys that no column of the wave sees: their weights are 0, and so have their V to be, which may be
           // anything; then whether any is left that is not finite
@@ -1626,7 +1685,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 #undef WIDE_SYNC
 #undef WIDE_ISSUE
   if (__syncthreads_or(odd)) {
-    redo_columns<bf16_t, HD>(walk, it, base, c0, min(c0 + 128, ncol), kbeg, kend, wave);
+    redo_columns<bf16_t, HD, tree>(walk, it, base, c0, min(c0 + 128, ncol), kbeg, kend, wave);
     return;
   }
   const PagedChunk c = chunk_args();
@@ -1684,7 +1743,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 // keys alone 29, the prefix alone 15.) Without a prefix the streaming kernel runs
 // three to a CU, which hides more of the waits at an item's start (64 rows of 300 keys
 // 25 us, two to a CU 30; rows of 100000 keys 1262 us, and 1243).
-template <typename T, int HD, int PRE, int OWN>
+template <typename T, int HD, int PRE, int OWN, bool tree>
 __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2) void k_paged_attn(PagedChunk c,
                                                                                                 int npre, int nown) {
   union Lds {
@@ -1706,15 +1765,15 @@ __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2)
     }
     if (pre) {
       if (at >= npre) return;
-      if constexpr (PRE == 0) wide_keys<HD, PREFIX_KEYS>(c, lds.w, at);
-      else stream_keys<T, HD, PRE, true>(c, lds.s, at);
+      if constexpr (PRE == 0) wide_keys<HD, PREFIX_KEYS, tree>(c, lds.w, at);
+      else stream_keys<T, HD, PRE, true, tree>(c, lds.s, at);
       return;
     }
     if (at >= nown) return;
   }
   const PagedChunk o = PRE >= 0 ? chunk_args() : c;
-  if constexpr (OWN == 0) wide_keys<HD, PRE < 0 ? ROW_KEYS : OWN_KEYS>(o, lds.w, at);
-  else stream_keys<T, HD, OWN, false>(o, lds.s, at);
+  if constexpr (OWN == 0) wide_keys<HD, PRE < 0 ? ROW_KEYS : OWN_KEYS, tree>(o, lds.w, at);
+  else stream_keys<T, HD, OWN, false, tree>(o, lds.s, at);
 }
 
 // ---------------------------------------------------------------------------
@@ -1824,18 +1883,18 @@ int64_t prefix_groups(const PagedPlan& a, int G) {
   return (int64_t)(a.pre_qb ? units : (units + 7) / 8 * 8) * a.pre_blk;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool tree>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   const int nown = (int)a.items, npre = (int)prefix_groups(a, c.pv.G);
   if (c.B > ROWS_SCAN) {
-    if (a.own_qb == 0) hipLaunchKernelGGL((k_paged_items<128, ROW_KEYS>), dim3(1), dim3(1024), 0, s, c);
-    else if (a.own_qb == 2) hipLaunchKernelGGL((k_paged_items<32, OWN_KEYS>), dim3(1), dim3(1024), 0, s, c);
-    else hipLaunchKernelGGL((k_paged_items<16, OWN_KEYS>), dim3(1), dim3(1024), 0, s, c);
+    if (a.own_qb == 0) hipLaunchKernelGGL((k_paged_items<128, ROW_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
+    else if (a.own_qb == 2) hipLaunchKernelGGL((k_paged_items<32, OWN_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
+    else hipLaunchKernelGGL((k_paged_items<16, OWN_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
     FC_LAUNCH_CHECK();
   }
   const dim3 grid(npre == 0 ? nown : 256 * ((npre + 255) / 256 + (nown + 255) / 256));
 #define PAGED(PRE, OWN)                                                                                             \
-  hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN>), grid, dim3(256), 0, s, c, npre, nown)
+  hipLaunchKernelGGL((k_paged_attn<T, HD, PRE, OWN, tree>), grid, dim3(256), 0, s, c, npre, nown)
   if constexpr (sizeof(T) == 4) {
     if (npre == 0) PAGED(-1, 1);
     else PAGED(1, 1);
@@ -1928,12 +1987,13 @@ static int attention(const fc_pages* pages, const void* q, int64_t q_token_strid
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;
   const bool vec = (((uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v | (uintptr_t)y | (uintptr_t)work) & 15) ==
                        0 && (strides & (pages->dtype == FC_BF16 ? 7 : 3)) == 0;
-  if (a.mfma && vec && !tree) {
-    if (pages->dtype == FC_BF16)
-      return pages->head_dim == 128 ? launch_mfma<bf16_t, 128>(c, a, s)
-                                    : launch_mfma<bf16_t, 64>(c, a, s);
-    return pages->head_dim == 128 ? launch_mfma<float, 128>(c, a, s)
-                                  : launch_mfma<float, 64>(c, a, s);
+  if (a.mfma && vec) {
+    const bool bf = pages->dtype == FC_BF16, wide = pages->head_dim == 128;
+    if (tree)
+      return bf ? wide ? launch_mfma<bf16_t, 128, true>(c, a, s) : launch_mfma<bf16_t, 64, true>(c, a, s)
+                : wide ? launch_mfma<float, 128, true>(c, a, s) : launch_mfma<float, 64, true>(c, a, s);
+    return bf ? wide ? launch_mfma<bf16_t, 128, false>(c, a, s) : launch_mfma<bf16_t, 64, false>(c, a, s)
+              : wide ? launch_mfma<float, 128, false>(c, a, s) : launch_mfma<float, 64, false>(c, a, s);
   }
   const dim3 grid(max_tokens, n_head);
   if (tree) {

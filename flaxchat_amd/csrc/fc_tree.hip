@@ -414,6 +414,145 @@ __global__ __launch_bounds__(256) void k_rope_append_any(RopeArgs a) {
   }
 }
 
+// Heads of 64 and 128, rotated in multiples of 16 dims, arrays aligned to 16
+// bytes. A workgroup takes 4096 / HD tokens and either `per` heads of q and k
+// or one head of v.
+//
+// q and k: HD / 16 lanes a token, 16 dims each: with the halves of `rot` paired,
+// 8 of either half; cos and sin stay in registers for all of the workgroup's
+// heads. K goes out as it comes, 16 bytes a lane: in the matrix-core order four
+// positions' pieces are 64 bytes next to each other. V is stored dim by dim: it is
+// turned through LDS and written with the positions along the lanes, so that a
+// wave's 2-byte stores fill the 64-byte rows that they lie in, whatever the slots'
+// alignment (with the dims along the lanes each store is a line of its own).
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {  // over groups of L = 4 or 8 lanes, in every lane
+#define ROPE_STEP(CTRL) \
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, false))
+  ROPE_STEP(0xb1);                            // lanes l ^ 1
+  ROPE_STEP(0x4e);                            // l ^ 2
+  if constexpr (L == 8) ROPE_STEP(0x141);     // 7 - l: the other four
+#undef ROPE_STEP
+  return v;
+}
+__device__ __forceinline__ void load4(const float* p, float (&x)[8], int at) {
+  const float4 a = *(const float4*)p;
+  x[at] = a.x; x[at + 1] = a.y; x[at + 2] = a.z; x[at + 3] = a.w;
+}
+template <typename T, typename S, int HD>
+__device__ __forceinline__ void rope_rows(const RopeArgs& a, int t0, int h0, int h1) {
+  constexpr int L = HD / 16, U = sizeof(S) == 2 ? 4 : 2;  // heads whose loads are under way at once
+  const int tid = threadIdx.x, l = tid % L, m = t0 + tid / L, half = a.rot >> 1;
+  if (m >= a.M) return;
+  const int pos = a.tok_pos[m], slot = a.slots[m];
+  const bool there = pos >= 0 && pos < a.len, turns = 16 * l < a.rot;
+  const int da = turns && !a.interleaved ? 8 * l : 16 * l, db = turns && !a.interleaved ? half + 8 * l : 16 * l + 8;
+  float c[8], s[8];
+  if (there && turns) {
+    const int64_t at = (int64_t)pos * half + 8 * l;
+    load4(a.cos + at, c, 0);
+    load4(a.cos + at + 4, c, 4);
+    load4(a.sin + at, s, 0);
+    load4(a.sin + at + 4, s, 4);
+  }
+  const int id = slot >= 0 && slot / a.pv.page < a.pv.N ? slot / a.pv.page : -1, in = slot - id * a.pv.page;
+  const bool keeps = there && id >= 0;
+  const int64_t ka = keeps ? k_elem(a.pv, id, 0, in, da) : 0, kb = keeps ? k_elem(a.pv, id, 0, in, db) : 0;
+  for (int h = h0; h < h1; h += U) {
+    float x[U][8], y[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int hu = min(h + u, h1 - 1);
+      const S* p = hu < a.H ? (const S*)a.q + m * a.qst + hu * a.qsh : (const S*)a.k + m * a.kst + (hu - a.H) * a.ksh;
+      load8(p + da, x[u]);
+      load8(p + db, y[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;
+      if (turns) {
+        if (a.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x1 = x[u][2 * i], x2 = x[u][2 * i + 1], y1 = y[u][2 * i], y2 = y[u][2 * i + 1];
+            x[u][2 * i] = x1 * c[i] + x2 * s[i];
+            x[u][2 * i + 1] = x2 * c[i] - x1 * s[i];
+            y[u][2 * i] = y1 * c[4 + i] + y2 * s[4 + i];
+            y[u][2 * i + 1] = y2 * c[4 + i] - y1 * s[4 + i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x1 = x[u][i], x2 = y[u][i];
+            x[u][i] = x1 * c[i] + x2 * s[i];
+            y[u][i] = x2 * c[i] - x1 * s[i];
+          }
+        }
+      }
+      float f = 1.f;
+      if (a.norm > 0.f) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x[u][i] * x[u][i] + y[u][i] * y[u][i];
+        f = a.norm / sqrtf(group_sum<L>(ss) * (1.f / HD) + 1e-6f);
+      }
+      if (h + u < a.H) {
+        T* o = (T*)a.out + ((int64_t)m * a.H + h + u) * HD;
+        if (!there) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[u][i] = y[u][i] = 0.f;
+          f = 1.f;
+        }
+        store8(o + da, x[u], f);
+        store8(o + db, y[u], f);
+      } else if (keeps) {
+        T* o = (T*)a.kp + (int64_t)(h + u - a.H) * a.pv.page * HD;
+        store8(o + ka, x[u], f);
+        store8(o + kb, y[u], f);
+      }
+    }
+  }
+}
+template <typename T, typename S, int HD>
+__device__ __forceinline__ void append_v(const RopeArgs& a, T* lds, int t0, int g) {
+  constexpr int TT = 4096 / HD, LD = HD + (sizeof(T) == 2 ? 2 : 1), C = HD / 8;
+  const int tid = threadIdx.x, t = tid % TT, m = t0 + t;
+  int slot = m < a.M ? a.slots[m] : -1;
+  const int pos = m < a.M ? a.tok_pos[m] : -1;
+  float x[2][8];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = tid + 256 * e, tok = min(t0 + i / C, a.M - 1);
+    load8((const S*)a.v + tok * a.vst + g * a.vsh + 8 * (i % C), x[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = tid + 256 * e;
+    T* w = lds + i / C * LD + 8 * (i % C);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *(uint32_t*)(w + 2 * k) = pack2bf(x[e][2 * k], x[e][2 * k + 1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = x[e][k];
+    }
+  }
+  __syncthreads();
+  const int id = slot >= 0 ? slot / a.pv.page : a.pv.N;
+  if (id >= a.pv.N || pos < 0 || pos >= a.len) return;
+  T* o = (T*)a.vp + v_elem(a.pv, id, g, slot - id * a.pv.page, tid / TT);
+  const T* r = lds + t * LD + tid / TT;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) o[e * (256 / TT) * 32] = r[e * (256 / TT)];
+}
+template <typename T, typename S, int HD>
+__global__ __launch_bounds__(256) void k_rope_append(RopeArgs a, int per, int groups) {
+  __shared__ T lds[(4096 / HD) * (HD + (sizeof(T) == 2 ? 2 : 1))];
+  const int jobs = groups + a.pv.G, job = blockIdx.x % jobs, t0 = (blockIdx.x / jobs) * (4096 / HD);
+  if (job < groups) rope_rows<T, S, HD>(a, t0, job * per, min((job + 1) * per, a.H + a.pv.G));
+  else append_v<T, S, HD>(a, lds, t0, job - groups);
+}
+
 extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const void* k, const void* v,
                                   int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
                                   int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
@@ -435,7 +574,38 @@ extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const vo
                    k_token_stride, k_head_stride, v_token_stride, v_head_stride, tok_pos, slots, cos, sin,
                    M, n_head, rope_len, rot, interleaved != 0, norm};
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t waves = (int64_t)M * (n_head + 2 * pages->n_kv_head);
+  const int G = pages->n_kv_head, hd = pages->head_dim;
+  // 16 bytes at a time: everything aligned to them
+  const int src = src_dtype == FC_BF16 ? 8 : 4, dst = pages->dtype == FC_BF16 ? 8 : 4;
+  const uintptr_t at = (uintptr_t)pages->k | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out |
+                       (uintptr_t)cos | (uintptr_t)sin;
+  const int64_t strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
+                          v_head_stride;
+  if ((hd == 64 || hd == 128) && rot % 16 == 0 && (at & 15) == 0 && strides % src == 0 && pages->k_stride % dst == 0) {
+    // as many heads of q and k a workgroup as leave a few for every CU, up to 8
+    const int64_t tiles = ((int64_t)M * hd + 4095) / 4096, heads = n_head + G;
+    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * heads / 2048));
+    const int64_t groups = (heads + per - 1) / per, all = tiles * (groups + G);
+    if (all < 1 << 24) {  // (a launch's threads are counted in 32 bits)
+#define ROPE(T, S, HD) \
+  hipLaunchKernelGGL((k_rope_append<T, S, HD>), dim3((int)all), dim3(256), 0, s, a, per, (int)groups)
+#define ROPE_HD(T, S)          \
+  if (hd == 64) ROPE(T, S, 64); \
+  else ROPE(T, S, 128)
+      if (pages->dtype == FC_F32) {
+        ROPE_HD(float, float);
+      } else if (src_dtype == FC_F32) {
+        ROPE_HD(bf16_t, float);
+      } else {
+        ROPE_HD(bf16_t, bf16_t);
+      }
+#undef ROPE_HD
+#undef ROPE
+      FC_LAUNCH_CHECK();
+      return FC_OK;
+    }
+  }
+  const int64_t waves = (int64_t)M * (n_head + 2 * G);
   const dim3 grid((unsigned)std::min<int64_t>((waves + 3) / 4, 65536));
   if (pages->dtype == FC_F32) hipLaunchKernelGGL((k_rope_append_any<float, float>), grid, dim3(256), 0, s, a);
   else if (src_dtype == FC_F32) hipLaunchKernelGGL((k_rope_append_any<bf16_t, float>), grid, dim3(256), 0, s, a);

@@ -9,6 +9,7 @@
 // parent is an earlier node of the row, anything else makes it a root. Node i
 // sits in the cache at position start[b] + i, whatever its depth.
 #include "fc_paged.h"
+#include <type_traits>
 
 // ---------------------------------------------------------------------------
 // Ancestors
@@ -259,24 +260,31 @@ extern "C" int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, 
 // behind its place moves nothing. In ascending order no move reads what an earlier one
 // wrote (its source lies behind every place before it), so the places are done in
 // batches, each read before it is written: the result is that of reading all first.
-// A workgroup takes one row, KV head and layer.
-#define MOVES 16  // places a batch
-template <typename T>
+//
+// A workgroup lists a row's moves once and makes them for some of the layers' KV
+// heads, U at a time. The moves lie along the lanes: V is stored dim by dim, and those
+// of one 32-position block then share the 64-byte rows of a load or store; of K,
+// 8 dims of a position are 16 bytes of its block (VEC).
+#define MOVES 16  // a batch
+template <typename T, bool VEC, int E>  // E: V's elements of a batch per thread, head_dim <= 16 E
 __global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, int64_t kls, int64_t vls,
                                                      const int* __restrict__ path, const int* __restrict__ slots,
                                                      const int* __restrict__ row_off, int max_tokens,
-                                                     int max_per_row) {
-  __shared__ int s_src[FC_TREE_MOST], s_dst[FC_TREE_MOST], s_n[FC_TREE_MOST / 64 + 1];
-  const int b = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+                                                     int max_per_row, int units) {
+  constexpr int U = E <= 8 ? 2 : 1, KE = VEC ? (sizeof(T) == 2 ? (E + 7) / 8 : (E + 3) / 4) : E;
+  constexpr int KD = VEC ? 16 / (int)sizeof(T) : 1;  // dims of a piece of K
+  using Piece = std::conditional_t<VEC, uint4, T>;
+  __shared__ int s_src[FC_TREE_MOST], s_dst[FC_TREE_MOST], s_n;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, hd = pv.hd;
   const RowSpan sp = row_span(row_off, b, max_per_row, max_tokens);
   if (sp.n == 0) return;
-  const int pool = (int)min((int64_t)pv.N * pv.page, (int64_t)0x7fffffff);
-  int total = 0;  // the moves so far, in order of their places; the first wave lists them
-  if (tid < 64) {
+  if (tid < 64) {  // the moves, in order of their places
+    const int pool = (int)min((int64_t)pv.N * pv.page, (int64_t)0x7fffffff);
+    int total = 0;
     for (int j0 = 0; j0 < sp.n; j0 += 64) {
-      const int j = j0 + lane, p = j < sp.n ? path[sp.base + j] : -1;
+      const int j = j0 + lane, p = j < sp.n ? path[sp.base + j] : -1, dst = j < sp.n ? slots[sp.base + j] : -1;
       bool is = p > j && p < sp.n;
-      const int src = is ? slots[sp.base + p] : -1, dst = is ? slots[sp.base + j] : -1;
+      const int src = is ? slots[sp.base + p] : -1;
       is = src >= 0 && src < pool && dst >= 0 && dst < pool;
       const uint64_t who = __ballot(is);
       if (is) {
@@ -286,33 +294,45 @@ __global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, 
       }
       total += __popcll(who);
     }
-    if (lane == 0) s_n[0] = total;
+    if (lane == 0) s_n = total;
   }
   __syncthreads();
-  total = s_n[0];
-  kp += blockIdx.z * kls;
-  vp += blockIdx.z * vls;
-  constexpr int E = MOVES;  // elements of a batch per thread, of K and of V (hd <= 256)
+  const int total = s_n, jm = tid % MOVES, d0 = tid / MOVES;
   for (int m0 = 0; m0 < total; m0 += MOVES) {
-    T kx[E], vx[E];
-    const int n = min(MOVES, total - m0) * pv.hd;
+    const bool is = m0 + jm < total;
+    const int src = is ? s_src[m0 + jm] : 0, dst = is ? s_dst[m0 + jm] : 0;
+    const int si = src / pv.page, sa = src - si * pv.page, di = dst / pv.page, da = dst - di * pv.page;
+    const int64_t vs = v_elem(pv, si, 0, sa, d0), vd = v_elem(pv, di, 0, da, d0);
+    for (int u0 = blockIdx.y; u0 < units; u0 += U * gridDim.y) {
+      Piece k[U][KE];
+      T v[U][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int x = tid + 256 * e;
-      if (x < n) {
-        const int src = s_src[m0 + x / pv.hd], id = src / pv.page, at = src - id * pv.page, d = x % pv.hd;
-        kx[e] = kp[k_elem(pv, id, g, at, d)];
-        vx[e] = vp[v_elem(pv, id, g, at, d)];
+      for (int u = 0; u < U; ++u) {
+        const int unit = u0 + u * gridDim.y, layer = unit / pv.G, g = unit - layer * pv.G;
+        if (!is || unit >= units) continue;
+        const int64_t head = (int64_t)g * pv.page * hd;
+        const T *kl = kp + layer * kls + head, *vl = vp + layer * vls + head;
+#pragma unroll
+        for (int e = 0; e < KE; ++e)
+          if ((d0 + 16 * e) * KD < hd) k[u][e] = *(const Piece*)(kl + k_elem(pv, si, 0, sa, (d0 + 16 * e) * KD));
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (d0 + 16 * e < hd) v[u][e] = vl[vs + 16 * e * 32];
       }
-    }
-    __syncthreads();
+      __builtin_amdgcn_s_waitcnt(0);  // all is read ...
+      __syncthreads();                // ... before any is written
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int x = tid + 256 * e;
-      if (x < n) {
-        const int dst = s_dst[m0 + x / pv.hd], id = dst / pv.page, at = dst - id * pv.page, d = x % pv.hd;
-        kp[k_elem(pv, id, g, at, d)] = kx[e];
-        vp[v_elem(pv, id, g, at, d)] = vx[e];
+      for (int u = 0; u < U; ++u) {
+        const int unit = u0 + u * gridDim.y, layer = unit / pv.G, g = unit - layer * pv.G;
+        if (!is || unit >= units) continue;
+        const int64_t head = (int64_t)g * pv.page * hd;
+        T *kl = kp + layer * kls + head, *vl = vp + layer * vls + head;
+#pragma unroll
+        for (int e = 0; e < KE; ++e)
+          if ((d0 + 16 * e) * KD < hd) *(Piece*)(kl + k_elem(pv, di, 0, da, (d0 + 16 * e) * KD)) = k[u][e];
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (d0 + 16 * e < hd) vl[vd + 16 * e * 32] = v[u][e];
       }
     }
   }
@@ -330,13 +350,27 @@ extern "C" int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_
   FC_CHECK_ARG(n_layer > 0 && n_layer <= 65535 && pages->n_kv_head <= 65535, "n_layer and n_kv_head in [1, 65535]");
   const PageView pv = page_view(pages);
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 grid(batch, pv.G, n_layer);
-#define COMMIT(T)                                                                                                 \
-  hipLaunchKernelGGL(k_tree_commit<T>, grid, dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, k_layer_stride,      \
-                     v_layer_stride, path, slots, row_off, max_tokens, max_per_row)
-  if (pages->dtype == FC_BF16) COMMIT(bf16_t);
-  else COMMIT(float);
+  // a few workgroups for every CU, rows first; each takes every grid.y-th KV head of all layers
+  const int64_t units = (int64_t)n_layer * pv.G;
+  FC_CHECK_ARG(units < 1 << 30, "too many layers and heads");
+  const dim3 grid(batch, (unsigned)std::max<int64_t>(1, std::min<int64_t>({units, 4096 / batch, 65535})));
+  const int per = pages->dtype == FC_BF16 ? 8 : 4;
+  const bool vec = ((uintptr_t)pages->k & 15) == 0 && (k_layer_stride | pages->k_stride) % per == 0 && pv.hd % per == 0;
+#define COMMIT_E(T, VEC, E)                                                                                           \
+  hipLaunchKernelGGL((k_tree_commit<T, VEC, E>), grid, dim3(256), 0, s, pv, (T*)pages->k, (T*)pages->v, k_layer_stride,\
+                     v_layer_stride, path, slots, row_off, max_tokens, max_per_row, (int)units)
+#define COMMIT(T)                            \
+  if (!vec) COMMIT_E(T, false, 16);          \
+  else if (pv.hd <= 64) COMMIT_E(T, true, 4);  \
+  else if (pv.hd <= 128) COMMIT_E(T, true, 8); \
+  else COMMIT_E(T, true, 16)
+  if (pages->dtype == FC_BF16) {
+    COMMIT(bf16_t);
+  } else {
+    COMMIT(float);
+  }
 #undef COMMIT
+#undef COMMIT_E
   FC_LAUNCH_CHECK();
   return FC_OK;
 }

@@ -1813,7 +1813,7 @@ int pre_splits(int64_t P, int G, int blk, int64_t part_bytes, int most, bool fp3
   }
   return best;
 }
-PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, int W, int P, int window) {
+PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, int W, int P, int window, bool tree) {
   PagedPlan a{};
   a.mfma = p->head_dim == 64 || p->head_dim == 128;
   if (!a.mfma) return a;
@@ -1855,6 +1855,15 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   // and 3.4 with the gap between them; 17 us or 21 from one call to the next)
   if (P == 0 && longest <= 1024) a.S_own = 1;
   a.target = a.own_qb ? 768 : 256;
+  if (tree) {
+    // Rows of trees that alone are a workgroup for every CU are not cut up to 4096 keys, as a cut costs the merge and a
+    // start (32 rows of 1280 keys, 12 heads, cut in two or not: trees of 16 53 and 47 us, of 32 64 and 52, of 64 65 and
+    // 61; 128 rows of 50 to 2000 keys, 10 nodes of 12 heads on 4 65 and 59). Behind a prefix there is a merge all the
+    // same, and in the wide kernel long rows are cut to the mean's length (those 128 rows, 25 nodes, behind 6144 keys:
+    // 148 us, 158 uncut).
+    if (P == 0 && units >= 256 && longest <= 4096) a.S_own = 1;
+    if (P > 0 && !a.own_qb) a.target = 512;
+  }
   const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;
   a.items = std::min(units * a.S_own, units + std::max<int64_t>(a.target, cut));
   if (P > 0 && a.joint == 0) {
@@ -1951,14 +1960,19 @@ static int check_sizes(const fc_pages* p, int32_t batch, int32_t max_tokens, int
   return FC_OK;
 }
 
-extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
-                                                      int32_t max_per_row, int32_t n_head, int32_t width,
-                                                      int32_t prefix_len, int32_t window) {
+static int64_t workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens, int32_t max_per_row,
+                               int32_t n_head, int32_t width, int32_t prefix_len, int32_t window, bool tree) {
   if (check_pages(pages) != FC_OK ||
       check_sizes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window) != FC_OK)
     return FC_ERR_ARG;
-  const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window, tree);
   return a.part_bytes + a.ml_bytes + a.item_bytes;
+}
+
+extern "C" int64_t fc_paged_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,
+                                                      int32_t max_per_row, int32_t n_head, int32_t width,
+                                                      int32_t prefix_len, int32_t window) {
+  return workspace_bytes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window, false);
 }
 
 static int attention(const fc_pages* pages, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* y,
@@ -1972,7 +1986,8 @@ static int attention(const fc_pages* pages, const void* q, int64_t q_token_strid
   rc = check_sizes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
   if (rc != FC_OK) return rc;
   FC_CHECK_ARG(prefix_len == 0 || prefix_pages, "window, prefix");
-  const PagedPlan a = paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  const PagedPlan a =
+      paged_plan(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window, tree != nullptr);
   FC_CHECK_ARG(a.items + prefix_groups(a, pages->n_kv_head) < kMostGroups, "too many tokens, rows or heads");
   const int64_t need = a.part_bytes + a.ml_bytes + a.item_bytes;
   FC_CHECK_ARG(need == 0 || (work && work_bytes >= need), "workspace too small");
@@ -2026,7 +2041,7 @@ extern "C" int64_t fc_tree_attention_workspace_bytes(const fc_pages* pages, int3
                                                      int32_t max_per_row, int32_t n_head, int32_t width,
                                                      int32_t prefix_len, int32_t window) {
   if (check_tree_sizes(max_per_row) != FC_OK) return FC_ERR_ARG;
-  return fc_paged_attention_workspace_bytes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window);
+  return workspace_bytes(pages, batch, max_tokens, max_per_row, n_head, width, prefix_len, window, true);
 }
 
 extern "C" int32_t fc_tree_attention(const fc_pages* pages, const void* q, int64_t q_token_stride,

@@ -742,7 +742,7 @@ __device__ __forceinline__ int chunk_length(const PagedChunk& c, float total, in
   const float share = ceilf(total * (float)c.pv.G / (float)c.target);
   // (unsigned: a row may have up to 2^31 - 32 keys)
   const uint32_t least = max(128u, ((uint32_t)longest + c.S_own - 1) / c.S_own);
-  const uint32_t len = (max((uint32_t)fminf(share, (float)(CB == 128 ? CHUNK_WIDE : CHUNK_MAX)), least) + 63) & ~63u;
+  const uint32_t len = (max((uint32_t)fminf(share, (float)(CB >= 64 ? CHUNK_WIDE : CHUNK_MAX)), least) + 63) & ~63u;
   return __builtin_amdgcn_readfirstlane((int)min(len, 0x7fffffe0u));
 }
 // pieces of a row: its keys / chunk, at least one (past 2^24 keys it may be one too few, never too many)
@@ -1401,14 +1401,21 @@ struct WideLds {
   WideStage<HD> stg[2];
   int rng[4][2];
 };
-template <int HD, int walk, bool tree>
+//
+// CB = 64: blocks of 64 columns, two waves on each of a step's two tiles, joined at
+// the end: a step is then half as long, and the next one's loads go out the sooner.
+template <int HD, int walk, bool tree, int CB = 128>
 __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
+  constexpr bool halves = CB == 64;
+  constexpr int NU = halves ? 1 : 2;  // tiles of a step that a wave takes
+  static_assert(!halves || walk == OWN_KEYS, "a row's own keys");
   constexpr bool pre = walk == PREFIX_KEYS;
   WideStage<HD>(&stg)[2] = lds.stg;
   static_assert(sizeof(lds.stg) >= (PT_ROWS + 1) * 4, "the rows' offsets");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, kk = lane & 31;
+  const int cw = halves ? wave & 1 : wave, u0 = halves ? wave >> 1 : 0;  // its 32 columns, its first tile
   Item it;
   int base = 0, ncol, lo_c, hi_c, w_lo, w_hi, tok = 0;
   int64_t kbeg64, kend64;
@@ -1433,14 +1440,14 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       stage_offsets(off, c.row_off, c.B);
       __syncthreads();
     } else {
-      if (!find_item<128, walk, tree>(c, at, it)) return;
+      if (!find_item<CB, walk, tree>(c, at, it)) return;
       const RowSpan sp = row_span(c.row_off, it.b, c.max_per_row, c.Mcap);
       base = sp.base;
       ncol = sp.n * rep;
     }
-    const int c0 = it.blk * 128;
+    const int c0 = it.blk * CB;
     // this lane's column
-    const int col = c0 + 32 * wave + kk;
+    const int col = c0 + 32 * cw + kk;
     ok = col < ncol;
     const int j = ok ? col / rep : 0, head = it.g * rep + (ok ? col - j * rep : 0);
     Query qy{0, 0, 0};
@@ -1486,11 +1493,11 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     kend64 = min((int64_t)g_hi + 1, s_beg + it.len);
     kbeg64 = max(s_beg, (int64_t)(g_lo & ~31));
   }
-  const int b = it.b, g = it.g, c0 = it.blk * 128;
+  const int b = it.b, g = it.g, c0 = it.blk * CB;
   const bool none = kbeg64 >= kend64;
   if (none && w.S_own + w.S_pre > 1) {
     const int cx = c0 + threadIdx.x, rep = w.H / w.pv.G;
-    if (threadIdx.x < 128 && cx < ncol) {
+    if (threadIdx.x < CB && cx < ncol) {
       const int jx = cx / rep;
       const int64_t pair = (int64_t)(base + jx) * w.H + g * rep + cx - jx * rep;
       w.pml[(int64_t)(pre ? w.S_own + it.split : it.split) * w.Mcap * w.H + pair] = make_float2(-INFINITY, 0.f);
@@ -1581,37 +1588,37 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       uint32_t bits = 0xffffffffu;  // which of the lane's keys a tree's node may see, 16 of either tile
       if (tree && !pre && kb + 63 >= nodes) {
         const uint64_t* row = w.mask + (int64_t)tok * w.words;
-        const int words = part == 0 ? 0 : w.words, k0 = kb + 8 * hl - nodes;
-        bits = bits8(row, words, k0) | bits8(row, words, k0 + 16) << 8 | bits8(row, words, k0 + 32) << 16 |
-               bits8(row, words, k0 + 48) << 24;
+        const int words = part == 0 ? 0 : w.words, k0 = kb + 32 * u0 + 8 * hl - nodes;
+        bits = bits8(row, words, k0) | bits8(row, words, k0 + 16) << 8;
+        if (!halves) bits |= bits8(row, words, k0 + 32) << 16 | bits8(row, words, k0 + 48) << 24;
       }
-      f32x16 sc[2];
+      f32x16 sc[NU];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
-      v4u kf[DS][2], vf[2][DS];
+      v4u kf[DS][NU], vf[NU][DS];
 #pragma unroll
       for (int h = 0; h < DS; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) kf[h][u] = __builtin_bit_cast(v4u, S_.k[u][h][lane]);
+        for (int u = 0; u < NU; ++u) kf[h][u] = __builtin_bit_cast(v4u, S_.k[u0 + u][h][lane]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < DS; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) sc[u] = mfma32(kf[h][u], qf[h], sc[u]);
+        for (int u = 0; u < NU; ++u) sc[u] = mfma32(kf[h][u], qf[h], sc[u]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u][f][lane]);
+        for (int f = 0; f < DS; ++f) vf[u][f] = __builtin_bit_cast(v4u, S_.v[u0 + u][f][lane]);
       __builtin_amdgcn_sched_barrier(0);
       if (!(kb >= f_lo && kb + 63 <= f_hi && in == 3)) {
         u16x2 mag = {0, 0};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bool there = (in >> u) & 1;
-          const int k0 = kb + 32 * u + 8 * hl;
+        for (int u = 0; u < NU; ++u) {
+          const bool there = (in >> (u0 + u)) & 1;
+          const int k0 = kb + 32 * (u0 + u) + 8 * hl;
           const int lr = there ? lo - k0 : 64, hr = hi - k0;
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
@@ -1638,9 +1645,9 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       }
       float m4[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) m4[x] = fmaxf(sc[0][x], sc[1][x]);
+      for (int x = 0; x < 4; ++x) m4[x] = fmaxf(sc[0][x], sc[NU - 1][x]);
 #pragma unroll
-      for (int x = 4; x < 16; ++x) m4[x & 3] = fmaxf(m4[x & 3], fmaxf(sc[0][x], sc[1][x]));
+      for (int x = 4; x < 16; ++x) m4[x & 3] = fmaxf(m4[x & 3], fmaxf(sc[0][x], sc[NU - 1][x]));
       float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       {
         const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
@@ -1657,7 +1664,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
       const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key yet: every term exp2(-inf) = 0
       float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh) {
           float pv[8];  // rounded to bf16 for the product, not in the sum
@@ -1685,12 +1692,37 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 #undef WIDE_SYNC
 #undef WIDE_ISSUE
   if (__syncthreads_or(odd)) {
-    redo_columns<bf16_t, HD, tree>(walk, it, base, c0, min(c0 + 128, ncol), kbeg, kend, wave);
+    redo_columns<bf16_t, HD, tree>(walk, it, base, c0, min(c0 + CB, ncol), kbeg, kend, wave);
     return;
+  }
+  if constexpr (halves) {
+    // the second tiles' waves hand over: the sums through the second stage, maximum and sum through what the taking wave
+    // writes its outputs through later
+    float* sums = (float*)&stg[1] + cw * (DD * 16 * 64) + lane;
+    float2* ml = (float2*)((bf16_t*)&stg[0] + cw * 32 * (HD + 8)) + lane;
+    static_assert(sizeof(WideStage<HD>) >= 2 * DD * 16 * 64 * 4, "two waves' sums");
+    if (u0 == 1) {
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sums[(16 * dd + x) * 64] = O[dd][x];
+      *ml = make_float2(m_run, l_run);
+    }
+    __syncthreads();
+    if (u0 == 1) return;
+    const float2 e = *ml;
+    const float m_new = fmaxf(m_run, e.x), mu = m_new == -INFINITY ? 0.f : m_new;
+    const float a0 = exp2a(m_run - mu), a1 = exp2a(e.x - mu);
+    l_run = l_run * a0 + e.y * a1;
+    m_run = m_new;
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) O[dd][x] = O[dd][x] * a0 + sums[(16 * dd + x) * 64] * a1;
   }
   const PagedChunk c = chunk_args();
   const int rep = c.H / c.pv.G, sg = pre ? c.S_own + it.split : it.split;
-  const int col = c0 + 32 * wave + kk, j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
+  const int col = c0 + 32 * cw + kk, j = ok ? col / rep : 0, head = g * rep + (ok ? col - j * rep : 0);
   const float l_tot = l_run + __shfl_xor(l_run, 32, WAVE);
   // lane: column kk; register 4 i4 + x of O[dd] is dim 32 dd + 8 i4 + 4 hl + x
   if (pre || !whole(c, it)) {
@@ -1728,7 +1760,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     constexpr int TP = HD / 8, CP = 64 / TP;  // lanes per column, columns per pass
 #pragma unroll
     for (int it = 0; it < 32 / CP; ++it) {
-      const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * wave + cc, jo = co / rep;
+      const int cc = CP * it + lane / TP, d0 = 8 * (lane % TP), co = c0 + 32 * cw + cc, jo = co / rep;
       const uint4 val = *(const uint4*)(T + cc * LD + d0);
       if (co < ncol) *(uint4*)((bf16_t*)c.y + ((int64_t)(base + jo) * c.H + g * rep + co - jo * rep) * HD + d0) = val;
     }
@@ -1736,7 +1768,7 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
 }
 
 // The prefix (PRE: 16-column blocks of the streaming kernel, 0: the wide one,
-// -1: no prefix) and the rows' own keys in one launch: the first is bound by
+// -1: no prefix) and the rows' own keys (OWN likewise, 64: the wide one with 64 columns) in one launch: the first is bound by
 // the matrix cores where many rows share it, the second by memory, and each
 // hides the other's start and end. 256 workgroups of either in turn, so that a CU
 // holds one of each. (64 samples behind 5000 keys: 41 us with the merge, the rows' own
@@ -1748,7 +1780,7 @@ __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2)
                                                                                                 int npre, int nown) {
   union Lds {
     StreamLds<HD> s;
-    std::conditional_t<PRE == 0 || OWN == 0, WideLds<HD>, char> w;
+    std::conditional_t<PRE == 0 || OWN == 0 || OWN == 64, WideLds<HD>, char> w;
   };
   __shared__ Lds lds;
   int at = blockIdx.x;
@@ -1772,7 +1804,8 @@ __global__ __launch_bounds__(256, PRE < 0 && OWN == 1 && sizeof(T) == 2 ? 3 : 2)
     if (at >= nown) return;
   }
   const PagedChunk o = PRE >= 0 ? chunk_args() : c;
-  if constexpr (OWN == 0) wide_keys<HD, PRE < 0 ? ROW_KEYS : OWN_KEYS, tree>(o, lds.w, at);
+  if constexpr (OWN == 64) wide_keys<HD, OWN_KEYS, tree, 64>(o, lds.w, at);
+  else if constexpr (OWN == 0) wide_keys<HD, PRE < 0 ? ROW_KEYS : OWN_KEYS, tree>(o, lds.w, at);
   else stream_keys<T, HD, OWN, false, tree>(o, lds.s, at);
 }
 
@@ -1789,7 +1822,7 @@ constexpr int64_t kPartMax = 256ll << 20;
 // their column blocks, and the key splits.
 struct PagedPlan {
   bool mfma;
-  int own_qb, own_blk, pre_qb, pre_blk;
+  int own_qb, own_cb, own_blk, pre_qb, pre_blk;
   int S_own, S_pre, pre_chunk, target, joint;
   int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short, none has more than S_own
   int64_t part_bytes, ml_bytes, item_bytes;
@@ -1822,21 +1855,22 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
     qb = ncol <= 16 || p->dtype == FC_F32 ? 1 : ncol <= 32 ? 2 : 0;
     blk = (int)(qb ? (ncol + 16 * qb - 1) / (16 * qb) : (ncol + 127) / 128);
   };
-  kernel((int64_t)std::min(max_per_row, T) * rep, a.own_qb, a.own_blk);
+  const int64_t cols = (int64_t)std::min(max_per_row, T) * rep;
+  kernel(cols, a.own_qb, a.own_blk);
+  a.own_cb = a.own_qb ? 16 * a.own_qb : tree && cols <= 64 ? 64 : 128;
   kernel((int64_t)T * rep, a.pre_qb, a.pre_blk);
   a.mfma = (!a.own_qb || a.own_blk <= 65535) && (!a.pre_qb || a.pre_blk <= 65535);
   if (!a.mfma) return a;
   const int64_t width = (int64_t)W * p->page, pad = ((int64_t)P + 31) / 32 * 32;
   // (a row's last block may be short, so the tokens make up to one more block a row than they would side by side)
-  const int cb = a.own_qb ? 16 * a.own_qb : 128;
-  const int64_t units = G * std::min((int64_t)B * a.own_blk, (int64_t)T * rep / cb + B);
+  const int64_t units = G * std::min((int64_t)B * a.own_blk, (int64_t)T * rep / a.own_cb + B);
   // Rows that fill column blocks of the wide kernel may walk the prefix themselves, which saves its partials and the
   // merge, but cuts the work coarser and leaves the rows' last blocks part empty: done where they see little of it, or
   // the blocks are several rounds of the card's 512 workgroups and not many more than the tokens fill. (92 rows of 490
   // tokens, 8 heads on one, behind 7 keys: 167 us so, and 726 with the prefix walked for itself; 64 rows of up to 512,
   // 12 heads, behind 2000: 441 and 542; but 16 such rows behind 4001, 516 blocks, 264 and 205, and 100 rows of up to
   // 130 behind 8000 627 and 422.)
-  const int64_t cols = (int64_t)std::min(max_per_row, T) * rep, full = G * ((int64_t)T * rep / 128);
+  const int64_t full = G * ((int64_t)T * rep / 128);
   const bool rounds = units >= 3 * 512 && units <= full + full * 3 / 5;
   const int seen = window > 0 ? std::min(P, window) : P;  // by tokens behind the prefix
   if (P > 0 && !a.own_qb && cols >= 128 && (seen <= 1024 || rounds) && pad + width <= 0x7fffffff) a.joint = (int)pad;
@@ -1896,7 +1930,8 @@ template <typename T, int HD, bool tree>
 int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   const int nown = (int)a.items, npre = (int)prefix_groups(a, c.pv.G);
   if (c.B > ROWS_SCAN) {
-    if (a.own_qb == 0) hipLaunchKernelGGL((k_paged_items<128, ROW_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
+    if (tree && a.own_cb == 64) hipLaunchKernelGGL((k_paged_items<64, OWN_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
+    else if (a.own_qb == 0) hipLaunchKernelGGL((k_paged_items<128, ROW_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
     else if (a.own_qb == 2) hipLaunchKernelGGL((k_paged_items<32, OWN_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
     else hipLaunchKernelGGL((k_paged_items<16, OWN_KEYS, tree>), dim3(1), dim3(1024), 0, s, c);
     FC_LAUNCH_CHECK();
@@ -1910,9 +1945,11 @@ int launch_mfma(const PagedChunk& c, const PagedPlan& a, hipStream_t s) {
   } else if (npre == 0) {
     if (a.own_qb == 1) PAGED(-1, 1);
     else if (a.own_qb == 2) PAGED(-1, 2);
+    else if (tree && a.own_cb == 64) PAGED(-1, tree ? 64 : 0);
     else PAGED(-1, 0);
   } else if (a.own_qb == 0) {
-    PAGED(0, 0);
+    if (tree && a.own_cb == 64) PAGED(0, tree ? 64 : 0);
+    else PAGED(0, 0);
   } else if (a.own_qb == 2) {
     if (a.pre_qb == 2) PAGED(2, 2);
     else PAGED(0, 2);

@@ -350,10 +350,11 @@ extern "C" int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_
   FC_CHECK_ARG(n_layer > 0 && n_layer <= 65535 && pages->n_kv_head <= 65535, "n_layer and n_kv_head in [1, 65535]");
   const PageView pv = page_view(pages);
   const hipStream_t s = (hipStream_t)stream;
-  // a few workgroups for every CU, rows first; each takes every grid.y-th KV head of all layers
-  const int64_t units = (int64_t)n_layer * pv.G;
+  // each takes every grid.y-th KV head of all layers; two or more if few workgroups are enough, as listing the moves
+  // weighs more then (32 rows of 12 heads in one layer 10.5 us, 11.1 with one each; one row in 24 layers of 12 8.1, 9.9)
+  const int64_t units = (int64_t)n_layer * pv.G, each = units * batch > 4096 ? 1 : 2;
   FC_CHECK_ARG(units < 1 << 30, "too many layers and heads");
-  const dim3 grid(batch, (unsigned)std::max<int64_t>(1, std::min<int64_t>({units, 4096 / batch, 65535})));
+  const dim3 grid(batch, (unsigned)std::max<int64_t>(1, std::min<int64_t>({(units + each - 1) / each, 8192 / batch, 65535})));
   const int per = pages->dtype == FC_BF16 ? 8 : 4;
   const bool vec = ((uintptr_t)pages->k & 15) == 0 && (k_layer_stride | pages->k_stride) % per == 0 && pv.hd % per == 0;
 #define COMMIT_E(T, VEC, E)                                                                                           \
@@ -582,9 +583,10 @@ __device__ __forceinline__ void append_v(const RopeArgs& a, T* lds, int t0, int 
 template <typename T, typename S, int HD>
 __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a, int per, int groups) {
   __shared__ T lds[(4096 / HD) * (HD + (sizeof(T) == 2 ? 2 : 1))];
-  const int jobs = groups + a.pv.G, job = blockIdx.x % jobs, t0 = (blockIdx.x / jobs) * (4096 / HD);
-  if (job < groups) rope_rows<T, S, HD>(a, t0, job * per, min((job + 1) * per, a.H + a.pv.G));
-  else append_v<T, S, HD>(a, lds, t0, job - groups);
+  // v's jobs, then q's and k's: dealt out in turn, each kind would come to the same XCDs again and again
+  const int G = a.pv.G, nv = G * ((a.M + 4096 / HD - 1) / (4096 / HD)), r = (int)blockIdx.x - nv;
+  if (r >= 0) rope_rows<T, S, HD>(a, r / groups * (4096 / HD), r % groups * per, min((r % groups + 1) * per, a.H + G));
+  else append_v<T, S, HD>(a, lds, (int)blockIdx.x / G * (4096 / HD), (int)blockIdx.x % G);
 }
 
 extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const void* k, const void* v,
@@ -616,9 +618,10 @@ extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const vo
   const int64_t strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
                           v_head_stride;
   if ((hd == 64 || hd == 128) && rot % 16 == 0 && (at & 15) == 0 && strides % src == 0 && pages->k_stride % dst == 0) {
-    // as many heads of q and k a workgroup as leave a few for every CU, up to 8
+    // as many heads of q and k a workgroup as leave six for every CU, up to 4 (16000 tokens of 12 + 4 heads: one each 50
+    // us, two 44, four 42.5, eight 43.5, all 60)
     const int64_t tiles = ((int64_t)M * hd + 4095) / 4096, heads = n_head + G;
-    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * heads / 2048));
+    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(4, tiles * heads / 1536));
     const int64_t groups = (heads + per - 1) / per, all = tiles * (groups + G);
     if (all < 1 << 24) {  // (a launch's threads are counted in 32 bits)
 #define ROPE(T, S, HD) \

@@ -651,9 +651,8 @@ def _attend(name, q, k_pages, v_pages, tables, row_off, start, tree, max_per_row
     if tree:
         _tree_rows(name, max_per_row)
         mask, tok_pos = tree
-        words = (max_per_row + 63) // 64
-        if mask.dtype != torch.int64 or mask.shape != (T, words) or not mask.is_contiguous():
-            raise ValueError(f"{name}: mask is a contiguous int64 tensor [{T}][{words}] "
+        if mask.dtype is not torch.int64 or mask.shape != (T, (max_per_row + 63) // 64) or not mask.is_contiguous():
+            raise ValueError(f"{name}: mask is a contiguous int64 tensor [{T}][{(max_per_row + 63) // 64}] "
                              f"(got {mask.dtype}, {tuple(mask.shape)})")
         _index(name, "tok_pos", tok_pos, T)
     pre = 0
@@ -706,24 +705,28 @@ def _tree_rows(name: str, max_per_row: int):
         raise ValueError(f"{name}: max_per_row in [1, {_lib.FC_TREE_MOST}]")
 
 
-def _tree_chunk(name: str, row_off: torch.Tensor, max_per_row: int, **per_token):
-    """(batch, tokens) of a chunk, its arrays checked."""
+def _tree_chunk(name: str, names: str, row_off: torch.Tensor, max_per_row: int, per_token, per_row=()):
+    """(batch, tokens, device) of a chunk, its arrays checked; `names`: those of the arrays."""
     _tree_rows(name, max_per_row)
-    B = row_off.numel() - 1
-    T = next(iter(per_token.values())).numel()
-    if not 1 <= B <= 4096 or T >= 1 << 30:
+    n, T, i32, d = row_off.numel(), per_token[0].numel(), torch.int32, row_off.get_device()
+    if not 2 <= n <= 4097 or T >= 1 << 30:
         raise ValueError(f"{name}: row_off of 2 to 4097 entries, tokens below 2^30")
-    _index(name, "row_off", row_off, B + 1)
-    for what, t in per_token.items():
-        _index(name, what, t, T)
-    return B, T
+    ok = row_off.dtype is i32 and row_off.is_contiguous() and d >= 0
+    for t in per_token:  # (one walk over the arrays: their checks are most of a call's time)
+        ok = ok and t.dtype is i32 and t.numel() == T and t.is_contiguous() and t.get_device() == d
+    for t in per_row:
+        ok = ok and t.dtype is i32 and t.numel() == n - 1 and t.is_contiguous() and t.get_device() == d
+    if not ok:
+        sizes = [n] + [T] * len(per_token) + [n - 1] * len(per_row)
+        for what, t, k in zip(names.split(), (row_off, *per_token, *per_row), sizes):
+            _index(name, what, t, k)
+        _on_gpu(name, row_off, *per_token, *per_row)
+    return n - 1, T, d
 
 
 @_op("tree_tables(Tensor parent, Tensor row_off, Tensor start, int max_per_row) -> (Tensor, Tensor)")
 def tree_tables(parent, row_off, start, max_per_row):
-    B, T = _tree_chunk("tree_tables", row_off, max_per_row, parent=parent)
-    _index("tree_tables", "start", start, B)
-    d = _on_gpu("tree_tables", parent, row_off, start)
+    B, T, d = _tree_chunk("tree_tables", "row_off parent start", row_off, max_per_row, (parent,), (start,))
     mask = parent.new_empty((T, (max_per_row + 63) // 64), dtype=torch.int64)
     tok_pos = parent.new_empty((T,))
     if T > 0:
@@ -744,8 +747,8 @@ def tree_attention(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, m
 @_op("tree_accept(Tensor parent, Tensor tokens, Tensor target, Tensor row_off, int max_per_row) "
      "-> (Tensor, Tensor, Tensor)")
 def tree_accept(parent, tokens, target, row_off, max_per_row):
-    B, T = _tree_chunk("tree_accept", row_off, max_per_row, parent=parent, tokens=tokens, target=target)
-    d = _on_gpu("tree_accept", parent, tokens, target, row_off)
+    B, T, d = _tree_chunk("tree_accept", "row_off parent tokens target", row_off, max_per_row,
+                          (parent, tokens, target))
     n_accepted, next_token, path = (parent.new_empty((n,)) for n in (B, B, T))
     if T == 0:
         n_accepted.fill_(0)
@@ -777,8 +780,9 @@ def tree_commit(path, slots, row_off, max_per_row, k_pages, v_pages):
         raise ValueError("tree_commit: n_kv_head at most 65535")
     if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise ValueError("tree_commit has no backward pass")
-    B, T = _tree_chunk("tree_commit", row_off, max_per_row, path=path, slots=slots)
-    d = _on_gpu("tree_commit", k_pages, v_pages, path, slots, row_off)
+    B, T, d = _tree_chunk("tree_commit", "row_off path slots", row_off, max_per_row, (path, slots))
+    if k_pages.get_device() != d or v_pages.get_device() != d:
+        _on_gpu("tree_commit", path, k_pages, v_pages)
     if T == 0:
         return
     _written((k_pages, v_pages))
@@ -797,21 +801,22 @@ def _layers_apart(t: torch.Tensor) -> bool:
      "Tensor(a!) k_pages, Tensor(b!) v_pages, bool interleaved=False, float norm=0.0) -> Tensor")
 def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved=False, norm=0.0):
     p, G, _, hd = _pages("rope_append", k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != hd or not 1 <= q.shape[1] <= 65535 or G > 65535:
-        raise ValueError(f"rope_append: q [tokens][n_head][{hd}], at most 65535 heads (got {tuple(q.shape)})")
-    M, H, _ = q.shape
-    if k.shape != (M, G, hd) or v.shape != k.shape:
+    qs, cs, dt = q.shape, cos.shape, k.dtype
+    if len(qs) != 3 or qs[2] != hd or not 1 <= qs[1] <= 65535 or G > 65535:
+        raise ValueError(f"rope_append: q [tokens][n_head][{hd}], at most 65535 heads (got {tuple(qs)})")
+    M, H, _ = qs
+    if k.shape != (M, G, hd) or v.shape != (M, G, hd):
         raise ValueError(f"rope_append: k and v [{M}][{G}][{hd}] (got {tuple(k.shape)} and {tuple(v.shape)})")
-    if q.dtype != k.dtype or v.dtype != k.dtype or (k.dtype != k_pages.dtype and k.dtype != torch.float32):
-        raise ValueError(f"rope_append: q, k and v in the pages' dtype or fp32 (got {q.dtype}, {k.dtype} and "
-                         f"{v.dtype})")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, cos, sin, k_pages, v_pages)):
+    if q.dtype is not dt or v.dtype is not dt or (dt is not k_pages.dtype and dt is not torch.float32):
+        raise ValueError(f"rope_append: q, k and v in the pages' dtype or fp32 (got {q.dtype}, {dt} and {v.dtype})")
+    if (q.requires_grad or k.requires_grad or v.requires_grad or cos.requires_grad or sin.requires_grad or
+            k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise ValueError("rope_append has no backward pass")
-    if cos.dim() != 2 or cos.shape != sin.shape or not 1 <= cos.shape[1] <= hd // 2 or \
-            not 1 <= cos.shape[0] <= 0x7fffffff:
+    if len(cs) != 2 or sin.shape != cs or not 1 <= cs[1] <= hd // 2 or not 1 <= cs[0] <= 0x7fffffff:
         raise ValueError(f"rope_append: cos and sin [positions][pairs], up to {hd // 2} pairs of a head (got "
-                         f"{tuple(cos.shape)} and {tuple(sin.shape)})")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+                         f"{tuple(cs)} and {tuple(sin.shape)})")
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
+            not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("rope_append: cos and sin are contiguous fp32 tensors")
     if not 0.0 <= norm <= 3e38:
         raise ValueError(f"rope_append: norm is finite and not negative (got {norm})")
@@ -820,16 +825,17 @@ def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved
     _index("rope_append", "tok_pos", tok_pos, M)
     _index("rope_append", "slots", slots, M)
     d = _on_gpu("rope_append", q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages)
-    out = q.new_empty((M, H, hd), dtype=k_pages.dtype)
+    out = q.new_empty(qs) if dt is k_pages.dtype else q.new_empty(qs, dtype=k_pages.dtype)
     if M == 0:
         return out
     _written((k_pages, v_pages))
-    if hd != 1 and (q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1):
+    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride()
+    if hd != 1 and (qd != 1 or kd != 1 or vd != 1):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    _launch("fc_rope_append", d, lib().fc_rope_append, p, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0),
-            q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _dtype_code(k), tok_pos.data_ptr(),
-            slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], interleaved, norm,
-            out.data_ptr(), H, M)
+        (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+    _launch("fc_rope_append", d, lib().fc_rope_append, p, q.data_ptr(), k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt,
+            vh, _dtype_code(k), tok_pos.data_ptr(), slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cs[0], 2 * cs[1],
+            interleaved, norm, out.data_ptr(), H, M)
     return out
 
 

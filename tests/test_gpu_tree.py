@@ -339,6 +339,14 @@ SHAPES = [
     ([3000, 5], [60, 64], 0, 2, 2, 128, 32, 0),
     ([40] * 70, [4] * 70, 600, 2, 2, 128, 32, 0),              # many rows
     ([0, 0], [0, 0], 10, 2, 2, 128, 32, 0),                    # no node at all
+    ([300, 0, 17, 64], [45, 64, 0, 33], 0, 2, 2, 128, 64, 0),  # 33 to 64 columns: two waves on either tile of a step
+    ([300, 0, 17, 96], [20, 9, 0, 16], 0, 6, 2, 128, 32, 100),
+    ([300, 0, 17, 95], [45, 64, 1, 33], 333, 2, 2, 128, 96, 0),
+    ([300, 0, 17, 64], [45, 64, 0, 33], 0, 2, 2, 64, 32, 0),
+    ([300, 0, 17, 64], [20, 30, 2, 9], 70, 4, 2, 64, 64, 50),
+    ([3000, 40], [40, 64], 100, 2, 2, 128, 32, 0),             # such rows, cut
+    ([5000, 40], [40, 64], 0, 1, 1, 64, 32, 1500),
+    ([200] * 64, [40] * 64, 0, 4, 4, 128, 32, 0),              # rows that fill the card
     ([700], [512], 0, 1, 1, 128, 64, 0),
 ]
 
@@ -499,7 +507,8 @@ def test_strided_and_unaligned(dtype, hd):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-@pytest.mark.parametrize("B,most,P,window", [(300, 3, 0, 0), (300, 20, 40, 50), (1000, 2, 10, 0), (257, 40, 0, 0)])
+@pytest.mark.parametrize("B,most,P,window", [(300, 3, 0, 0), (300, 20, 40, 50), (1000, 2, 10, 0), (257, 40, 0, 0),
+                                             (260, 25, 0, 0), (260, 25, 33, 70)])
 def test_many_rows(dtype, B, most, P, window):
     _say(f"tree_attention {dtype}: {B} rows")
     rng = np.random.default_rng(B)

@@ -12,6 +12,7 @@
 // row's table. An entry outside [0, n_pages) holds no keys.
 #include "fc_common.h"
 #include "fc_paged.h"
+#include <cmath>
 #include <type_traits>
 
 // K and V of a row's own pages are read once a call: non-temporal loads keep
@@ -450,7 +451,7 @@ struct PagedChunk {
   // a tree's chunk: each token's row of bits (`words` of them) and its position
   const uint64_t* mask;
   const int* tok_pos;
-  int words;
+  int words, pre_blk;
 };
 
 // The chunk, read from the kernel's arguments (its first) at this point and not
@@ -1426,10 +1427,21 @@ __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds,
     const int rep = c.H / c.pv.G;
     it = Item{0, 0, 0, 0, 1, c.pre_chunk, 0};
     if constexpr (pre) {
-      const int nunit = c.pv.G * c.S_pre, nul = (nunit + 7) >> 3, jj = at >> 3;
-      const int unit = (jj % nul) * 8 + (at & 7);
-      if (unit >= nunit) return;
-      it.blk = jj / nul;
+      const int nunit = c.pv.G * c.S_pre;
+      int unit;
+      // a tree's chunk: the blocks unit by unit, an eighth of them on each XCD. (By whole units one XCD may get two and
+      // the next one: 37 blocks of 4 groups against 6144 keys in 3 splits 140 us so, 99 in equal numbers.)
+      if constexpr (tree) {
+        const int nb = c.pre_blk, per = (nunit * nb + 7) >> 3, idx = (at & 7) * per + (at >> 3);
+        unit = idx / nb;
+        if ((at >> 3) >= per || unit >= nunit) return;
+        it.blk = idx - unit * nb;
+      } else {
+        const int nul = (nunit + 7) >> 3, jj = at >> 3;
+        unit = (jj % nul) * 8 + (at & 7);
+        if (unit >= nunit) return;
+        it.blk = jj / nul;
+      }
       it.g = unit / c.S_pre;
       it.split = unit - it.g * c.S_pre;
       it.skip = (int64_t)it.split * it.len;
@@ -1821,7 +1833,7 @@ constexpr int64_t kPartMax = 256ll << 20;
 // blocks of 16 columns in a workgroup of the streaming kernel, 0: the wide one),
 // their column blocks, and the key splits.
 struct PagedPlan {
-  bool mfma;
+  bool mfma, even;  // even: the prefix's workgroups go to the XCDs in equal numbers, not by units
   int own_qb, own_cb, own_blk, pre_qb, pre_blk;
   int S_own, S_pre, pre_chunk, target, joint;
   int64_t items;  // of the rows' own keys, at most: every row's last chunk may be short, none has more than S_own
@@ -1842,6 +1854,27 @@ int pre_splits(int64_t P, int G, int blk, int64_t part_bytes, int most, bool fp3
     const int64_t on = (int64_t)((G * S + 7) / 8) * blk;
     const double steps = (double)(((P + S - 1) / S + 63) / 64 * (fp32 ? 2 : 1) + 6);
     const double t = on * steps * 2.0 / 64 + steps * 0.6 + S * (0.2 + (double)part_bytes * 2 / 5e6);
+    if (t < least) least = t, best = S;
+  }
+  return best;
+}
+// The same where the workgroups go to the XCDs in equal numbers (`even`), beside `items` of the rows' own keys. A step of
+// a workgroup alone on its CU is 1.5 us, of one of two 2.4, and with more than two for every CU the last ones are a
+// round of their own, or fill the gaps of others, half and half; a start and an end are four steps. As far as the own
+// keys' items fill the card, the prefix's time counts half, and the sum of its steps for the rest. Its choice costs 4% or
+// less against the best of S = 1 .. 10 in 9 of 10 measured shapes, 17% in the other (prefixes of 500 to 16000 keys under
+// 40 to 1600 nodes, 17 to 148 us).
+int pre_splits_even(int64_t P, int G, int blk, int64_t part_bytes, int most, int64_t items) {
+  const double fill = std::min(1.0, (double)items / 512);
+  int best = 1;
+  double least = 1e30;
+  for (int S = 1; S <= std::min<int64_t>(most, (P + 127) / 128); ++S) {
+    const int64_t on = ((int64_t)G * S * blk + 7) / 8;
+    const double steps = (double)(((P + S - 1) / S + 63) / 64), rounds = (double)on / 64;
+    const double step = on <= 24 ? 1.5 : on <= 40 ? 1.5 + 0.9 * (double)(on - 24) / 16
+                        : on <= 64 ? 2.4 : 2.4 * (rounds + std::ceil(rounds)) / 2;
+    const double t = (steps + 4) * step * (1 - fill / 2) + (double)on * (steps + 6) * 2.0 / 64 * fill +
+                     S * (0.2 + (double)part_bytes * 2 / 5e6);
     if (t < least) least = t, best = S;
   }
   return best;
@@ -1900,13 +1933,16 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   }
   const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;
   a.items = std::min(units * a.S_own, units + std::max<int64_t>(a.target, cut));
+  a.even = tree && !a.pre_qb;
   if (P > 0 && a.joint == 0) {
     // The splits are counted from the first key that a column block sees: all of the prefix, or, by tokens behind it,
     // the window's end. The last one takes what is left, for rows that begin within the prefix. (7 rows of 9 tokens, 8
     // heads on one, fp32, a window of 1024 over 12268 keys: 85 us with splits of the whole prefix, 25 so.)
     // (in 64 bits: a prefix may have up to 2^31 - 33 positions)
     const int64_t over = window > 0 ? std::min<int64_t>(P, (int64_t)window + 32) : P;
-    const int S = pre_splits(over, G, a.pre_blk, one, (int)std::min<int64_t>(room, 128), p->dtype == FC_F32);
+    const int most = (int)std::min<int64_t>(room, 128);
+    const int S = a.even ? pre_splits_even(over, G, a.pre_blk, one, most, a.items)
+                         : pre_splits(over, G, a.pre_blk, one, most, p->dtype == FC_F32);
     const int64_t chunk = ((over + S - 1) / S + 63) / 64 * 64;
     a.S_pre = (int)((over + chunk - 1) / chunk);
     a.pre_chunk = (int)std::min<int64_t>(chunk, 0x7fffffc0);  // (below the chunk with one split alone, which takes all)
@@ -1923,6 +1959,7 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
 // workgroups of the prefix: in the wide kernel's order its units go to the XCDs in turn
 int64_t prefix_groups(const PagedPlan& a, int G) {
   const int units = G * a.S_pre;
+  if (a.even) return ((int64_t)units * a.pre_blk + 7) / 8 * 8;
   return (int64_t)(a.pre_qb ? units : (units + 7) / 8 * 8) * a.pre_blk;
 }
 
@@ -2033,7 +2070,7 @@ static int attention(const fc_pages* pages, const void* q, int64_t q_token_strid
                1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, a.joint, (float*)work,
                (float2*)((char*)work + a.part_bytes), (int*)((char*)work + a.part_bytes + a.ml_bytes),
                q, pages->k, pages->v, y, tree ? tree->mask : nullptr, tree ? tree->tok_pos : nullptr,
-               (max_per_row + 63) / 64};
+               (max_per_row + 63) / 64, a.pre_blk};
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;

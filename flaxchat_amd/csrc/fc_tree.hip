@@ -87,8 +87,10 @@ __device__ __forceinline__ void each_unowned(const int* __restrict__ row_off, in
     f((int)t);
 }
 
-// A row per workgroup; rows of up to 64 nodes in one wave's registers. Bound by
-// latency: offsets, parents, six rounds of shuffles.
+// A row per workgroup; rows of up to 64 nodes in one wave's registers (ONE). Bound
+// by latency: offsets, parents, at most six rounds of shuffles, the stores; 64 rows
+// of 64 nodes 3.0 us. Longer rows, four waves a row: a round of LDS and a barrier
+// for each block of 64 nodes; 500 rows of up to 300 nodes 6.2 us, 3.7 MB at 0.6 TB/s.
 template <bool ONE>
 __global__ __launch_bounds__(256) void k_tree_tables(const int* __restrict__ parent, const int* __restrict__ row_off,
                                                      const int* __restrict__ start, uint64_t* __restrict__ mask,
@@ -152,7 +154,10 @@ extern "C" int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off,
 // A node agrees if it is a root or its token is the target's choice at its
 // parent; it is accepted if it and all nodes above it agree, that is, if none of
 // its mask's bits is outside the agreeing nodes' set. The accepted node with the
-// most nodes above it, the lowest index among equals, ends the path.
+// most nodes above it, the lowest index among equals, ends the path. The masks are
+// made again (six shuffles) and not read: they would be the call's longest array, and
+// a caller that only wants the path need not have them. Latency, as above: 64 rows of
+// 64 nodes 3.2 us, 500 of up to 300 6.9.
 template <bool ONE>
 __global__ __launch_bounds__(256) void k_tree_accept(const int* __restrict__ parent, const int* __restrict__ tokens,
                                                      const int* __restrict__ target, const int* __restrict__ row_off,
@@ -264,7 +269,11 @@ extern "C" int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, 
 // A workgroup lists a row's moves once and makes them for some of the layers' KV
 // heads, U at a time. The moves lie along the lanes: V is stored dim by dim, and those
 // of one 32-position block then share the 64-byte rows of a load or store; of K,
-// 8 dims of a position are 16 bytes of its block (VEC).
+// 8 dims of a position are 16 bytes of its block (VEC). With the dims along the lanes
+// each value of V was a request of its own: 24 layers, 64 rows, 4 heads of 128 in bf16
+// 126 us, and 50 so. What is left there are the lines of V: a place and its source are
+// 2 bytes in each of hd rows of 64, and about 170 MB move for 59 of keys and values.
+// One layer (32 rows, 12 heads): 10 us, path, slots, values and stores in turn.
 #define MOVES 16  // a batch
 template <typename T, bool VEC, int E>  // E: V's elements of a batch per thread, head_dim <= 16 E
 __global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, int64_t kls, int64_t vls,
@@ -390,7 +399,8 @@ struct RopeArgs {
   float norm;
 };
 
-// Any head size and alignment: a wave per token and head of q, k or v, a pair of dims per lane and step.
+// Any head size and alignment: a wave per token and head of q, k or v, up to two pairs of dims per lane, and the dims
+// that are not rotated beside them. V's values are stored one by one, a line each. For shapes that no model here has.
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void k_rope_append_any(RopeArgs a) {
   const PageView& pv = a.pv;
@@ -460,6 +470,11 @@ __global__ __launch_bounds__(256) void k_rope_append_any(RopeArgs a) {
 // turned through LDS and written with the positions along the lanes, so that a
 // wave's 2-byte stores fill the 64-byte rows that they lie in, whatever the slots'
 // alignment (with the dims along the lanes each store is a line of its own).
+//
+// Bound by memory, and a workgroup's loads and stores do not overlap, several on a CU
+// do: 16000 tokens of 12 + 4 + 4 heads in bf16 43 us, 168 MB at 3.9 TB/s (a copy: 4.9).
+// Tokens in runs of 8 fill 16 bytes of V's rows of 64 at a time: 4000 tokens of
+// 12 + 12 + 12 heads, fp32 to bf16, 83 us for 110 MB.
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {  // over groups of L = 4 or 8 lanes, in every lane
 #define ROPE_STEP(CTRL) \

@@ -841,8 +841,8 @@ def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved
 
 @torch.library.register_fake(f"{NS}::tree_tables", lib=_PAGED)
 def _(parent, row_off, start, max_per_row):
-    return (parent.new_empty((parent.shape[0], (max_per_row + 63) // 64), dtype=torch.int64),
-            parent.new_empty((parent.shape[0],)))
+    T = parent.numel()
+    return parent.new_empty((T, (max_per_row + 63) // 64), dtype=torch.int64), parent.new_empty((T,))
 
 
 @torch.library.register_fake(f"{NS}::tree_attention", lib=_PAGED)
@@ -853,7 +853,7 @@ def _(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, max_per_row, w
 
 @torch.library.register_fake(f"{NS}::tree_accept", lib=_PAGED)
 def _(parent, tokens, target, row_off, max_per_row):
-    B, T = row_off.shape[0] - 1, parent.shape[0]
+    B, T = row_off.numel() - 1, parent.numel()
     return parent.new_empty((B,)), parent.new_empty((B,)), parent.new_empty((T,))
 
 

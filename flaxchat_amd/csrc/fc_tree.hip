@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) void k_rope_append_any(RopeArgs a) {
 // alignment (with the dims along the lanes each store is a line of its own).
 //
 // Bound by memory, and a workgroup's loads and stores do not overlap, several on a CU
-// do: 16000 tokens of 12 + 4 + 4 heads in bf16 43 us, 168 MB at 3.9 TB/s (a copy: 4.9).
+// do: 16000 tokens of 12 + 4 + 4 heads in bf16 39 us, 168 MB at 4.3 TB/s (a copy: 4.9).
 // Tokens in runs of 8 fill 16 bytes of V's rows of 64 at a time: 4000 tokens of
 // 12 + 12 + 12 heads, fp32 to bf16, 83 us for 110 MB.
 template <int L>
@@ -598,10 +598,19 @@ __device__ __forceinline__ void append_v(const RopeArgs& a, T* lds, int t0, int 
 template <typename T, typename S, int HD>
 __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a, int per, int groups) {
   __shared__ T lds[(4096 / HD) * (HD + (sizeof(T) == 2 ? 2 : 1))];
-  // v's jobs, then q's and k's: dealt out in turn, each kind would come to the same XCDs again and again
-  const int G = a.pv.G, nv = G * ((a.M + 4096 / HD - 1) / (4096 / HD)), r = (int)blockIdx.x - nv;
-  if (r >= 0) rope_rows<T, S, HD>(a, r / groups * (4096 / HD), r % groups * per, min((r % groups + 1) * per, a.H + G));
-  else append_v<T, S, HD>(a, lds, (int)blockIdx.x / G * (4096 / HD), (int)blockIdx.x % G);
+  // v's jobs, then q's and k's, an eighth of either kind on each XCD, next to each other: of V, a head's tiles one behind
+  // the other, since the 64-byte rows in which two tiles meet are put together in the XCD's L2; of q and k, a tile's
+  // heads, which read the same rows of cos and sin. (16000 tokens of 12 + 4 + 4 heads, half rotated, dealt out in turn:
+  // 42 us; V's so 41, both 39. All of each head rotated: 43, 42, 38.)
+  const int G = a.pv.G, tiles = (a.M + 4096 / HD - 1) / (4096 / HD), each = (G * tiles + 7) >> 3;
+  const int r = (int)blockIdx.x - 8 * each;
+  if (r >= 0) {
+    const int each_qk = (tiles * groups + 7) >> 3, job = (r & 7) * each_qk + (r >> 3), at = job % groups * per;
+    if (job < tiles * groups) rope_rows<T, S, HD>(a, job / groups * (4096 / HD), at, min(at + per, a.H + G));
+  } else {
+    const int job = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if (job < G * tiles) append_v<T, S, HD>(a, lds, job % tiles * (4096 / HD), job / tiles);
+  }
 }
 
 extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const void* k, const void* v,
@@ -633,11 +642,11 @@ extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const vo
   const int64_t strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
                           v_head_stride;
   if ((hd == 64 || hd == 128) && rot % 16 == 0 && (at & 15) == 0 && strides % src == 0 && pages->k_stride % dst == 0) {
-    // as many heads of q and k a workgroup as leave six for every CU, up to 4 (16000 tokens of 12 + 4 heads: one each 50
-    // us, two 44, four 42.5, eight 43.5, all 60)
+    // as many heads of q and k a workgroup as leave six for every CU, up to 4 (16000 tokens of 12 + 4 heads: one each 49
+    // us, two 41, four 39, eight 41, all 57)
     const int64_t tiles = ((int64_t)M * hd + 4095) / 4096, heads = n_head + G;
     const int per = (int)std::max<int64_t>(1, std::min<int64_t>(4, tiles * heads / 1536));
-    const int64_t groups = (heads + per - 1) / per, all = tiles * (groups + G);
+    const int64_t groups = (heads + per - 1) / per, all = (tiles * groups + 7) / 8 * 8 + (tiles * G + 7) / 8 * 8;
     if (all < 1 << 24) {  // (a launch's threads are counted in 32 bits)
 #define ROPE(T, S, HD) \
   hipLaunchKernelGGL((k_rope_append<T, S, HD>), dim3((int)all), dim3(256), 0, s, a, per, (int)groups)

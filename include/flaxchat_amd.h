@@ -458,7 +458,8 @@ int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, const int32
  * into slot slots[row_off[b] + j], for every entry path[j] = path
  * [row_off[b] + j] in (j, nodes of row b), as if all were read before the first is
  * written. Other entries, and slots outside the pool, move nothing. The
- * slots of a call's tokens differ. */
+ * slots of a call's tokens differ. A second call moves again, from what the
+ * first has left. */
 int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_t k_layer_stride, int64_t v_layer_stride,
                        const int32_t* path, const int32_t* slots, const int32_t* row_off, int32_t batch,
                        int32_t max_tokens, int32_t max_per_row, void* stream);

@@ -273,7 +273,7 @@ extern "C" int32_t fc_tree_accept(const int32_t* parent, const int32_t* tokens, 
 // each value of V was a request of its own: 24 layers, 64 rows, 4 heads of 128 in bf16
 // 126 us, and 50 so. What is left there are the lines of V: a place and its source are
 // 2 bytes in each of hd rows of 64, and about 170 MB move for 59 of keys and values.
-// One layer (32 rows, 12 heads): 10 us, path, slots, values and stores in turn.
+// One layer (32 rows, 12 heads): 10.3 us, path and slots, values, stores in turn.
 #define MOVES 16  // a batch
 template <typename T, bool VEC, int E>  // E: V's elements of a batch per thread, head_dim <= 16 E
 __global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, int64_t kls, int64_t vls,
@@ -283,17 +283,22 @@ __global__ __launch_bounds__(256) void k_tree_commit(PageView pv, T* kp, T* vp, 
   constexpr int U = E <= 8 ? 2 : 1, KE = VEC ? (sizeof(T) == 2 ? (E + 7) / 8 : (E + 3) / 4) : E;
   constexpr int KD = VEC ? 16 / (int)sizeof(T) : 1;  // dims of a piece of K
   using Piece = std::conditional_t<VEC, uint4, T>;
-  __shared__ int s_src[FC_TREE_MOST], s_dst[FC_TREE_MOST], s_n;
+  __shared__ int s_path[FC_TREE_MOST], s_slot[FC_TREE_MOST], s_src[FC_TREE_MOST], s_dst[FC_TREE_MOST], s_n;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, hd = pv.hd;
   const RowSpan sp = row_span(row_off, b, max_per_row, max_tokens);
   if (sp.n == 0) return;
+  for (int j = tid; j < sp.n; j += 256) {  // (so that the sources' slots are not a trip to memory behind the path's)
+    s_path[j] = path[sp.base + j];
+    s_slot[j] = slots[sp.base + j];
+  }
+  __syncthreads();
   if (tid < 64) {  // the moves, in order of their places
     const int pool = (int)min((int64_t)pv.N * pv.page, (int64_t)0x7fffffff);
     int total = 0;
     for (int j0 = 0; j0 < sp.n; j0 += 64) {
-      const int j = j0 + lane, p = j < sp.n ? path[sp.base + j] : -1, dst = j < sp.n ? slots[sp.base + j] : -1;
+      const int j = j0 + lane, p = j < sp.n ? s_path[j] : -1, dst = j < sp.n ? s_slot[j] : -1;
       bool is = p > j && p < sp.n;
-      const int src = is ? slots[sp.base + p] : -1;
+      const int src = is ? s_slot[p] : -1;
       is = src >= 0 && src < pool && dst >= 0 && dst < pool;
       const uint64_t who = __ballot(is);
       if (is) {
@@ -360,7 +365,7 @@ extern "C" int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_
   const PageView pv = page_view(pages);
   const hipStream_t s = (hipStream_t)stream;
   // each takes every grid.y-th KV head of all layers; two or more if few workgroups are enough, as listing the moves
-  // weighs more then (32 rows of 12 heads in one layer 10.5 us, 11.1 with one each; one row in 24 layers of 12 8.1, 9.9)
+  // weighs more then (32 rows of 12 heads in one layer 10.5 us, 11.1 with one each; one row in 24 layers of 12 heads 8.1, 9.9)
   const int64_t units = (int64_t)n_layer * pv.G, each = units * batch > 4096 ? 1 : 2;
   FC_CHECK_ARG(units < 1 << 30, "too many layers and heads");
   const dim3 grid(batch, (unsigned)std::max<int64_t>(1, std::min<int64_t>({(units + each - 1) / each, 8192 / batch, 65535})));

@@ -267,6 +267,31 @@ def test_rope_append(case, dtype, src, interleaved, norm):
         assert torch.equal(kp[:, 0].cpu(), pools[0][0]) and torch.equal(vp[:, 0].cpu(), pools[0][1])
 
 
+@pytest.mark.parametrize("dtype,src", [("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp32")])
+@pytest.mark.parametrize("M,H,G,hd", [(7000, 10, 5, 128), (10001, 10, 5, 128), (14000, 10, 5, 128), (13999, 20, 10, 64),
+                                      (4000, 1, 1, 128)])
+def test_rope_append_of_many_tokens(M, H, G, hd, dtype, src):
+    """A chunk whose workgroups take several heads each, 2 to 4 of 15 or 30, gives what the same tokens give in calls of
+    300, where they take one: a token's arithmetic is the same whoever does it, so the results are equal."""
+    _say(f"rope_append {src} -> {dtype}: {M} tokens of {H} and {G} heads of {hd}")
+    rng = np.random.default_rng(M)
+    page, length = 64, 9000
+    N = -(-M // page) + 3
+    slots = up(np.where(rng.random(M) < 0.01, -1, rng.permutation(N * page)[:M] if M % 2 else np.arange(M) + 70))
+    pos = up(rng.integers(-1, length + 1, M))
+    cos, sin = (torch.randn(length, hd // 4, device=dev()) for _ in range(2))
+    qkv = torch.randn(M, H + 2 * G, hd, device=dev()).to(DT[src])
+    pools = [[torch.zeros(N, G, *z, dtype=DT[dtype], device=dev()) for z in ((page, hd), (page // 32, hd, 32))]
+             for _ in range(2)]
+    call = lambda a, b, p: OPS.rope_append(qkv[a:b, :H], qkv[a:b, H:H + G], qkv[a:b, H + G:], pos[a:b], slots[a:b],  # noqa: E731
+                                           cos, sin, *p, False, 1.2)
+    whole = call(0, M, pools[0])
+    parts = torch.cat([call(a, min(a + 300, M), pools[1]) for a in range(0, M, 300)])
+    assert torch.equal(whole, parts)
+    assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(pools[0][1], pools[1][1])
+    assert pools[0][0].abs().amax((1, 2, 3)).gt(0).any() and torch.isfinite(whole).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_rope_is_the_prologue(dtype):
     """On this model's own tables rope_append does what attn_prologue does to q and k, value by value in bf16 steps."""

@@ -172,6 +172,28 @@ def test_commit(case, dtype, order):
 
 
 # ---------------------------------------------------------------- rope_append
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,layers,G,hd", [(40, 24, 12, 64), (300, 7, 9, 128), (2, 700, 12, 64)])
+def test_commit_of_many_heads(B, layers, G, hd, dtype):
+    """All layers at once, more KV heads than the launch has workgroups for, and layer by layer: the same."""
+    _say(f"tree_commit {dtype}: {B} rows, {layers} layers of {G} heads of {hd}")
+    rng = np.random.default_rng(B)
+    ns = rng.integers(0, 24, B)
+    off, par, _ = packed(rng, ns, ["3", "chain", "star"])
+    T, page = int(off[-1]), 32
+    N = -(-T // page) + 2
+    slots = up(rng.permutation(N * page)[:T])
+    _, _, path = OPS.tree_accept(up(par), up(np.zeros(T)), up(np.zeros(T)), up(off), 24)
+    k = torch.randn(layers, N, G, page, hd, device=dev()).to(DT[dtype])
+    v = torch.randn(layers, N, G, 1, hd, 32, device=dev()).to(DT[dtype])
+    k0, v0, k1, v1 = k.clone(), v.clone(), k.clone(), v.clone()
+    OPS.tree_commit(path, slots, up(off), 24, k, v)
+    for i in range(layers):
+        OPS.tree_commit(path, slots, up(off), 24, k1[i], v1[i])
+    assert torch.equal(k, k1) and torch.equal(v, v1)
+    assert all((k[i] != k0[i]).any() and (v[i] != v0[i]).any() for i in range(layers))
+
+
 ROPES = [
     # heads, KV heads, head_dim, rot, page, runs, strided
     (1, 1, 128, 128, 32, [1], False),

@@ -437,7 +437,8 @@ extern "C" int32_t fc_page_append(const fc_pages* pages, const void* k, const vo
 // first node's, and only tiles and steps behind that ask for bits: a lane's 8 keys of
 // a tile are 8 bits next to each other, a load of one word or two. The bound is the
 // one of plain chunks (128 trees of up to 25 nodes, 12 heads on 4, behind 6144 keys,
-// 50-2000 of their own: 144 us with the merge, 69 GFLOP in 56).
+// 50-2000 of their own: 144 us with the merge; a library product does the 69 GFLOP
+// in 56).
 //
 // One chunk's attention as the kernels see it.
 struct PagedChunk {

@@ -81,7 +81,7 @@ EXPORTS = ["fc_last_error", "fc_version", "fc_forward_workspace_bytes", "fc_forw
            "fc_spec_workspace_bytes",
            "fc_spec_round", "fc_spec_accept", "fc_spec_part_bytes", "fc_fast_sample", "fc_engine_sample",
            "fc_cross_entropy", "fc_page_tables", "fc_page_append", "fc_paged_attention",
-           "fc_paged_attention_workspace_bytes", "fc_tree_tables", "fc_tree_attention_workspace_bytes",
+           "fc_paged_attention_workspace_bytes", "fc_tree_tables", "fc_tree_tables_window", "fc_tree_attention_workspace_bytes",
            "fc_tree_attention", "fc_tree_accept", "fc_tree_commit", "fc_rope_append", "fc_read_probe", "fc_l2_read_probe", "fc_walk_probe",
            "fc_gemm_walk_probe",
            "fc_gemm_walk_probe_words", "fc_graph_begin", "fc_graph_end", "fc_graph_launch", "fc_graph_destroy"]
@@ -147,6 +147,8 @@ def _declare(L):
     L.fc_paged_attention.restype = i32
     L.fc_tree_tables.argtypes = [vp] * 5 + [i32] * 3 + [vp]
     L.fc_tree_tables.restype = i32
+    L.fc_tree_tables_window.argtypes = [vp] * 5 + [i32] * 4 + [vp]
+    L.fc_tree_tables_window.restype = i32
     L.fc_tree_attention_workspace_bytes.argtypes = L.fc_paged_attention_workspace_bytes.argtypes
     L.fc_tree_attention_workspace_bytes.restype = i64
     L.fc_tree_attention.argtypes = [POINTER(FcPages), vp, i64, i64, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp,

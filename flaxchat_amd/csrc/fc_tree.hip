@@ -87,6 +87,20 @@ __device__ __forceinline__ void each_unowned(const int* __restrict__ row_off, in
     f((int)t);
 }
 
+// m without its lowest k bits that are set: above the position below which there are k of them, found in six halvings.
+__device__ __forceinline__ uint64_t without_lowest(uint64_t m, int k) {
+  if (k >= __popcll(m)) return 0;
+  int at = 0;
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)
+    if (__popcll(m & ((1ull << (at + step)) - 1)) <= k) at += step;
+  return m >> at << at;
+}
+
+// window > 0: of a node's ancestors those at most `window` positions above it. Parents
+// come before their children, so a node's bits lie in the order of its ancestors'
+// depths, and the ones that are too far are its lowest.
+//
 // A row per workgroup; rows of up to 64 nodes in one wave's registers (ONE). Bound
 // by latency: offsets, parents, at most six rounds of shuffles, the stores; 64 rows
 // of 64 nodes 3.0 us. Longer rows, four waves a row: a round of LDS and a barrier
@@ -95,7 +109,7 @@ template <bool ONE>
 __global__ __launch_bounds__(256) void k_tree_tables(const int* __restrict__ parent, const int* __restrict__ row_off,
                                                      const int* __restrict__ start, uint64_t* __restrict__ mask,
                                                      int* __restrict__ tok_pos, int B, int max_tokens,
-                                                     int max_per_row, int W) {
+                                                     int max_per_row, int W, int window) {
   extern __shared__ char lds[];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int at = start[b];
@@ -108,18 +122,26 @@ __global__ __launch_bounds__(256) void k_tree_tables(const int* __restrict__ par
   if constexpr (ONE) {
     const uint64_t m = block_ancestors(parent_of(parent, sp.base, tid, sp.n));
     if (tid < sp.n) {
-      mask[sp.base + tid] = m;
-      tok_pos[sp.base + tid] = at + __popcll(m) - 1;
+      const int deep = __popcll(m) - 1;
+      mask[sp.base + tid] = window > 0 && deep > window ? without_lowest(m, deep - window) : m;
+      tok_pos[sp.base + tid] = at + deep;
     }
   } else {
     const RowTree t = row_tree(lds, W);
     row_ancestors(t, parent, sp.base, sp.n, W);
-    for (int x = tid; x < sp.n * W; x += blockDim.x) mask[(int64_t)sp.base * W + x] = t.mask[x];
     for (int i = tid; i < sp.n; i += blockDim.x) {
       int deep = -1;
       for (int w = 0; w <= i >> 6; ++w) deep += __popcll(t.mask[i * W + w]);
       tok_pos[sp.base + i] = at + deep;
+      if (window > 0)
+        for (int w = 0, far = deep - window; far > 0; ++w) {  // (far <= deep: it ends before the node's own word does)
+          const uint64_t m = t.mask[i * W + w];
+          t.mask[i * W + w] = without_lowest(m, far);
+          far -= __popcll(m);
+        }
     }
+    if (window > 0) __syncthreads();
+    for (int x = tid; x < sp.n * W; x += blockDim.x) mask[(int64_t)sp.base * W + x] = t.mask[x];
   }
 }
 
@@ -130,22 +152,28 @@ static int check_tree(int32_t batch, int32_t max_tokens, int32_t max_per_row) {
   return FC_OK;
 }
 
-extern "C" int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
-                                  int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row,
-                                  void* stream) {
+extern "C" int32_t fc_tree_tables_window(const int32_t* parent, const int32_t* row_off, const int32_t* start,
+                                         uint64_t* mask, int32_t* tok_pos, int32_t batch, int32_t max_tokens,
+                                         int32_t max_per_row, int32_t window, void* stream) {
   FC_CHECK_ARG(parent && row_off && start && mask && tok_pos, "null pointer");
   const int rc = check_tree(batch, max_tokens, max_per_row);
   if (rc != FC_OK) return rc;
+  FC_CHECK_ARG(window >= 0, "window");
   const int W = (max_per_row + 63) / 64;
   const hipStream_t s = (hipStream_t)stream;
   if (W == 1)
     hipLaunchKernelGGL(k_tree_tables<true>, dim3(batch), dim3(64), 0, s, parent, row_off, start, mask, tok_pos, batch,
-                       max_tokens, max_per_row, W);
+                       max_tokens, max_per_row, W, window);
   else
     hipLaunchKernelGGL(k_tree_tables<false>, dim3(batch), dim3(256), row_tree_bytes(W), s, parent, row_off, start,
-                       mask, tok_pos, batch, max_tokens, max_per_row, W);
+                       mask, tok_pos, batch, max_tokens, max_per_row, W, window);
   FC_LAUNCH_CHECK();
   return FC_OK;
+}
+extern "C" int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
+                                  int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row,
+                                  void* stream) {
+  return fc_tree_tables_window(parent, row_off, start, mask, tok_pos, batch, max_tokens, max_per_row, 0, stream);
 }
 
 // ---------------------------------------------------------------------------

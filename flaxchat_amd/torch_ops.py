@@ -55,15 +55,17 @@ where gradients are recorded, and what a call writes counts as modified in place
 Decoding with trees of drafted tokens over that cache: row b's chunk is a tree or a forest whose node i, token
 row_off[b] + i, continues node parent[row_off[b] + i] < i of its row (any other value: a root), lies in the cache at
 start[b] + i and counts as position start[b] + its depth; at most 512 nodes a row (max_per_row):
-  tree_tables(parent, row_off, start, max_per_row) -> (mask, tok_pos)
+  tree_tables(parent, row_off, start, max_per_row, window=0) -> (mask, tok_pos)
                                      each node's ancestors and itself as bits, int64 [tokens][words of 64], and its
-                                     position (fc_tree_tables)
+                                     position (fc_tree_tables_window); of the ancestors those at most `window`
+                                     positions above: the mask of the layers with that window
   rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved=False, norm=0.0) -> q
                                      page_append with the rotation of q and k at tok_pos and the QK norm
                                      (gpt.py:52-71, engine.py:108-126); trees or not
   tree_attention(q, k_pages, v_pages, tables, row_off, start, mask, tok_pos, max_per_row, window,
                  prefix_pages=None, prefix_len=0)
-                                     paged_attention where a node sees what its row holds and the nodes of its mask
+                                     paged_attention where a node sees what its row holds, as far as the window
+                                     reaches, and the nodes of its mask, whatever the window
   tree_accept(parent, tokens, target, row_off, max_per_row) -> (n_accepted, next_token, path)
                                      the deepest path on which the target's choices are the drafted tokens
   tree_commit(path, slots, row_off, max_per_row, k_pages, v_pages)
@@ -724,14 +726,16 @@ def _tree_chunk(name: str, names: str, row_off: torch.Tensor, max_per_row: int, 
     return n - 1, T, d
 
 
-@_op("tree_tables(Tensor parent, Tensor row_off, Tensor start, int max_per_row) -> (Tensor, Tensor)")
-def tree_tables(parent, row_off, start, max_per_row):
+@_op("tree_tables(Tensor parent, Tensor row_off, Tensor start, int max_per_row, int window=0) -> (Tensor, Tensor)")
+def tree_tables(parent, row_off, start, max_per_row, window=0):
+    if not 0 <= window <= 0x7fffffff:
+        raise ValueError("tree_tables: window in [0, 2^31)")
     B, T, d = _tree_chunk("tree_tables", "row_off parent start", row_off, max_per_row, (parent,), (start,))
     mask = parent.new_empty((T, (max_per_row + 63) // 64), dtype=torch.int64)
     tok_pos = parent.new_empty((T,))
     if T > 0:
-        _launch("fc_tree_tables", d, lib().fc_tree_tables, parent.data_ptr(), row_off.data_ptr(), start.data_ptr(),
-                mask.data_ptr(), tok_pos.data_ptr(), B, T, max_per_row)
+        _launch("fc_tree_tables_window", d, lib().fc_tree_tables_window, parent.data_ptr(), row_off.data_ptr(),
+                start.data_ptr(), mask.data_ptr(), tok_pos.data_ptr(), B, T, max_per_row, window)
     return mask, tok_pos
 
 
@@ -840,7 +844,7 @@ def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved
 
 
 @torch.library.register_fake(f"{NS}::tree_tables", lib=_PAGED)
-def _(parent, row_off, start, max_per_row):
+def _(parent, row_off, start, max_per_row, window=0):
     T = parent.numel()
     return parent.new_empty((T, (max_per_row + 63) // 64), dtype=torch.int64), parent.new_empty((T,))
 

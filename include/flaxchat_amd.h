@@ -417,17 +417,24 @@ int32_t fc_paged_attention(const fc_pages* pages, const void* q, int64_t q_token
  * fc_tree_tables: of each token the set of its ancestors and itself, bit
  * j % 64 of mask[token][j / 64] for node j of its row, in
  * ceil(max_per_row / 64) words, and its position; 0 and -1 for tokens of no
- * row. */
+ * row. fc_tree_tables_window: the ancestors at most `window` positions above
+ * the token (0: all), which are those that a sliding-window layer's token
+ * sees; the same for rows no deeper than window + 1 nodes. */
 #define FC_TREE_MOST 512
 int32_t fc_tree_tables(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
                        int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row, void* stream);
+int32_t fc_tree_tables_window(const int32_t* parent, const int32_t* row_off, const int32_t* start, uint64_t* mask,
+                              int32_t* tok_pos, int32_t batch, int32_t max_tokens, int32_t max_per_row,
+                              int32_t window, void* stream);
 
 /* fc_paged_attention for such chunks: a token of row b at tok_pos (taken to
  * be start[b] at least) sees the key at position p < start[b] if window is 0
  * or tok_pos - p <= window, and the key of node j of its row, at position
- * start[b] + j in the row's own pages, if bit j of its mask is set, whatever
- * the window and whatever node j is (masks need not be those of a tree; a
- * token may have no bit). Bits past the row's nodes mean nothing, and a node whose
+ * start[b] + j in the row's own pages, if bit j of its mask is set. Among the
+ * nodes the mask alone decides: a key's place does not tell its node's depth,
+ * so `window` does not reach them, and a layer with a window takes the mask
+ * that fc_tree_tables_window makes for it (masks need not be those of a tree;
+ * a token may have no bit). Bits past the row's nodes mean nothing, and a node whose
  * position lies in the prefix holds no key. mask: [max_tokens]
  * [ceil(max_per_row / 64)]. The rest as in fc_paged_attention. */
 int64_t fc_tree_attention_workspace_bytes(const fc_pages* pages, int32_t batch, int32_t max_tokens,

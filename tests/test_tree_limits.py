@@ -1,0 +1,70 @@
+"""Trees of drafted tokens at their limits, without a GPU: windows shorter than a tree is deep."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import flaxchat_amd.torch_ops  # noqa: E402,F401
+from flaxchat_amd import _lib  # noqa: E402
+from tests.test_tree import OPS, tables_args  # noqa: E402
+from tests.tree_cases import Tree, line_of, trees  # noqa: E402
+
+
+def within(seen, depth, window):
+    """Of the nodes that each of a row's nodes sees ([n][n]) those at most `window` positions above it (0: all)."""
+    d = np.asarray(depth)
+    return seen & (d[:, None] - d[None] <= window) if window > 0 else seen
+
+
+def narrowed(c, window):
+    """The rows, keys and nodes of c; its nodes see their ancestors as far as the window reaches."""
+    c.seen = [within(s, d, window) for s, d in zip(c.seen, c.depth)]
+    return c
+
+
+@pytest.mark.parametrize("n,ctx,window", [(200, 40, 128), (40, 40, 16), (9, 0, 1), (5, 100, 4), (5, 100, 3)])
+def test_a_chain_behind_a_window_is_plain_decoding(n, ctx, window):
+    """Two 64-bit references of one thing: a chain of nodes with the windowed mask, and a plain chunk."""
+    c = Tree(3, [ctx, 7], [n, 3], 10, 1, 8, 32, torch.float32, kinds=["chain"])
+    q = c.queries(1)
+    want = c.reference(q, window)[0]
+    deeper = np.abs(c.tree_reference(q, window)[0] - want).max()
+    assert (deeper > 1e-3) == (n > window + 1)  # the mask of all ancestors is another one exactly there
+    np.testing.assert_allclose(narrowed(c, window).tree_reference(q, window)[0], want, atol=1e-12)
+
+
+def test_each_node_is_its_path_decoded_token_by_token():
+    """The same for trees: every node against a row that holds its path and nothing else."""
+    rng = np.random.default_rng(8)
+    n, ctx, window = 40, 6, 4
+    par = trees(rng, n, "4")
+    seen = np.zeros((n, n), bool)
+    for i in range(n):
+        seen[i, line_of(par, i)] = True
+    depth = seen.sum(1) - 1
+    assert depth.max() > window + 2
+    c = narrowed(Tree(4, [ctx], [n], 0, 1, 8, 32, torch.float32, seen=[seen], depth=[depth]), window)
+    q = c.queries(1)
+    got = c.tree_reference(q, window)[0]
+    for i in range(n):
+        on = line_of(par, i)
+        one = Tree(4, [ctx + len(on) - 1], [1], 0, 1, 8, 32, torch.float32)
+        one.rows = [tuple(x[list(range(ctx)) + [ctx + j for j in on]] for x in c.rows[0])]
+        np.testing.assert_allclose(got[i], one.reference(q[i:i + 1], window)[0][0], atol=1e-12)
+
+
+def test_tree_tables_takes_a_window():
+    mask, pos = OPS.tree_tables(*[t.to("meta") if torch.is_tensor(t) else t for t in tables_args(max_per_row=65)], 7)
+    assert mask.shape == (7, 2) and pos.shape == (7,)
+    for window in (-1, 1 << 31):
+        with pytest.raises(ValueError, match="window"):
+            OPS.tree_tables(*tables_args(), window)
+    with pytest.raises(ValueError, match="CUDA"):
+        OPS.tree_tables(*tables_args(), 7)
+    L, p = _lib.lib(), 0x1000
+    good = [p] * 5 + [2, 7, 5, 3, None]
+    for at, value in [(i, None) for i in range(5)] + [(5, 0), (6, 0), (7, 513), (8, -1)]:
+        a = list(good)
+        a[at] = value
+        assert L.fc_tree_tables_window(*a) == -1, (at, value)

@@ -1,4 +1,6 @@
-"""Trees of drafted tokens at their limits, on the GPU: windows shorter than a tree is deep."""
+"""Trees of drafted tokens at their limits, on the GPU: windows shorter than a tree is deep; rows of 17 to 32 and of 33
+to 64 query columns (nodes times heads a KV head), which have kernels of their own, where masks, pages or values go
+wrong; rotation by workgroups of several heads."""
 
 import numpy as np
 import pytest
@@ -157,3 +159,148 @@ def test_decode_with_windowed_layers(pattern):
             length[b] = min(length[b], len(out[b]))
         steps += 1
     assert steps < want_n / 3
+
+
+# ---------------------------------------------------------------- 24 and 50 columns a row
+COLUMNS = [[12, 3], [25, 8]]  # two heads a KV head
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("P", [0, 50])
+@pytest.mark.parametrize("n", COLUMNS)
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_values_of_unseen_nodes(dtype, hd, P, n, junk):
+    """What is not finite at a node that only its descendants see does not reach the others; it reaches those that see
+    it (every weight is positive)."""
+    _say(f"tree_attention {dtype} hd={hd} n={n} prefix={P}: {junk} at a node")
+    c = Tree(7, [37, 3], n, P, 2, hd, 32, DT[dtype], kinds=["4", "chain"])
+    q = c.queries(4)
+    ref, tol = c.tree_reference(q, 0)
+    for node in (n[0] // 2, 1, n[0] - 1):
+        hit = np.concatenate([c.seen[0][:, node], np.zeros(n[1], bool)])
+        assert hit.any() and not hit.all()
+        at = 37 + node
+        K, V = c.K.copy(), c.V.copy()
+        for both in (False, True):
+            c.V[c.tables[0, at // 32], :, at % 32] = junk
+            if both:
+                c.K[c.tables[0, at // 32], :, at % 32] = junk
+            got = _run(c, q, 0)
+            _check(got[torch.from_numpy(~hit)], ref[~hit], tol[~hit], f"node {node}, K too: {both}")
+            assert both or not torch.isfinite(got[torch.from_numpy(hit)]).any()
+        c.K, c.V = K, V
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("n,P,window", [([12, 3], 40, 0), ([12, 3], 0, 9), ([25, 20], 0, 0), ([25, 20], 40, 0),
+                                        ([25, 32], 70, 25), ([32, 9], 0, 8)])
+def test_any_mask(dtype, hd, n, P, window):
+    """Masks that are no tree's: nodes that see none, later nodes, all of them; columns of one wave that see nothing."""
+    _say(f"tree_attention {dtype} hd={hd} n={n} prefix={P} window={window}: any mask")
+    rng = np.random.default_rng(sum(n))
+    seen = [rng.random((m, m)) < 0.4 for m in n]
+    depth = [rng.integers(0, 30, m) for m in n]
+    for s, d in zip(seen, depth):
+        s[1], s[2] = False, True
+        d[0], d[1] = -40, 10 ** 6
+    seen[0][:16] = False  # (32 columns, all of a wave's)
+    c = Tree(3, [0, 50], n, P, 2, hd, 32, DT[dtype], seen=seen, depth=depth)
+    q = c.queries(4)
+    got = _run(c, q, window, junk=True)
+    ref, tol = c.tree_reference(q, window)
+    _check(got, ref, tol)
+    if P == 0 and window == 0:
+        assert torch.all(got[:min(16, n[0])] == 0)  # row 0 holds nothing before its nodes
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("P", [0, 90])
+@pytest.mark.parametrize("n", [[12, 9, 16, 10], [25, 17, 32, 20]])
+def test_rows_without_pages(dtype, hd, P, n):
+    """Entries that are no page: of one of a step's two tiles, of all of a row's, of the tree's own nodes."""
+    _say(f"tree_attention {dtype} hd={hd} n={n} prefix={P}: entries that are no page")
+    c = Tree(5, [70, 10, 0, 126], n, P, 2, hd, 32, DT[dtype])
+    gone = [(0, 1), (1, 0), (2, 0), (3, 4)] + ([(-1, 1)] if P else [])
+    a = c.tree_device(dev(), int(c.off[-1]))
+    a["tables"][0, 1], a["tables"][1, 0], a["tables"][2, 0], a["tables"][3, 4] = -1, c.N, 2 ** 31 - 1, -2 ** 31
+    if P:
+        a["pre"][1] = c.N + 1
+    q = c.queries(4)
+    for window in (0, 8):
+        got = _run(c, q, window, a)
+        ref, tol = c.tree_reference(q, window, gone)
+        _check(got, ref, tol, f"window {window}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [[12, 3, 16], [25, 17, 32]])
+def test_rows_that_start_inside_the_prefix(dtype, n):
+    _say(f"tree_attention {dtype} n={n}: positions inside the prefix")
+    c = Tree(9, [40, 0, 3], n, 100, 2, 128, 32, DT[dtype])
+    c.start = np.array([140, 37, 98], np.int32)
+    c.tok_pos = np.concatenate([c.start[b] + c.depth[b] for b in range(3)])
+    q = c.queries(4)
+    for window in (0, 30):
+        got = _run(c, q, window)
+        ref, tol = c.tree_reference(q, window)
+        _check(got, ref, tol, f"window={window}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [[12, 16, 3], [25, 32, 17]])
+def test_rows_of_too_many_nodes(dtype, n):
+    """A row of more nodes than max_per_row is treated as empty, and the others are as they are without it."""
+    _say(f"tree_attention {dtype} n={n}: bad rows")
+    c = Tree(11, [40, 7, 90], n, 50, 2, 128, 32, DT[dtype])
+    q = c.queries(4)
+    ref, tol = c.tree_reference(q, 0)
+    got = _run(c, q, 0, most=n[0])
+    for s in (slice(0, n[0]), slice(n[0] + n[1], sum(n))):
+        _check(got[s], ref[s], tol[s])
+
+
+# ---------------------------------------------------------------- rope_append, several heads a workgroup
+@pytest.mark.parametrize("dtype,src", [("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp32")])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [0.0, 1.2])
+@pytest.mark.parametrize("M,H,G,hd,rot", [(14000, 10, 5, 128, 128), (10001, 10, 5, 128, 32), (13999, 20, 10, 64, 64)])
+def test_rope_append_of_many_tokens(M, H, G, hd, rot, interleaved, norm, dtype, src):
+    """Workgroups of 2 to 4 heads, q's and K's in one of them: a sample of the tokens, those at the tiles' borders and at
+    both ends among them, against the formula in 64 bits."""
+    _say(f"rope_append {src} -> {dtype}: {M} tokens of {H} and {G} heads of {hd}, {rot} rotated, interleaved="
+         f"{interleaved}, norm={norm}")
+    rng = np.random.default_rng(M + rot)
+    page, length = 64, 3000
+    N = -(-M // page) + 1
+    slots, pos = rng.permutation(N * page)[:M], rng.integers(0, length, M)
+    angle = np.outer(np.arange(length) * 25.0, 100000.0 ** (-np.arange(rot // 2) / (rot // 2)))
+    cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+    g = torch.Generator(device=dev()).manual_seed(M)
+    qkv = (2 * torch.randn(M, H + 2 * G, hd, device=dev(), generator=g)).to(DT[src])
+    k = torch.zeros(N, G, page, hd, device=dev(), dtype=DT[dtype])
+    v = torch.zeros(N, G, page // 32, hd, 32, device=dev(), dtype=DT[dtype])
+    q = OPS.rope_append(qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:], up(pos), up(slots), torch.from_numpy(cos).to(dev()),
+                        torch.from_numpy(sin).to(dev()), k, v, interleaved, norm)
+    some = np.unique(np.concatenate([np.arange(70), np.arange(M - 70, M), rng.integers(0, M, 300)]))
+    x = qkv[torch.from_numpy(some).to(dev())].float().cpu().numpy()
+    blk, at = slots[some] // page, slots[some] % page
+    if dtype == "bf16" and hd == 128:  # positions' order: see the block layout
+        from tests.paged_cases import k_blocks
+        number = k_blocks(np.arange(32 * hd).reshape(32, hd)).reshape(-1)
+        kk = k.view(N, G, page // 32, 32 * hd)[..., torch.from_numpy(np.argsort(number)).to(dev())]
+        kk = kk.view(N, G, page, hd)
+    else:
+        kk = k
+    sel = [torch.from_numpy(z).to(dev()) for z in (blk, at, at // 32, at % 32)]
+    got = [("q", q[torch.from_numpy(some).to(dev())], x[:, :H]), ("K", kk[sel[0], :, sel[1]], x[:, H:H + G])]
+    for what, t, heads in got:
+        y, tol = rope_plain(heads, pos[some], cos, sin, interleaved, norm)
+        if dtype == "bf16":  # half a step of the result's rounding: 2^-8 of it
+            tol = tol + 2.0 ** -8 * (abs(y) + tol)
+        bad = ~(abs(t.double().cpu().numpy() - y) <= tol)
+        assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, first at {np.argwhere(bad)[0]}"
+    vv = v[sel[0], :, sel[2], :, sel[3]]
+    assert torch.equal(vv, qkv[torch.from_numpy(some).to(dev()), H + G:].to(DT[dtype]))

@@ -660,7 +660,8 @@ extern "C" int32_t fc_rope_append(const fc_pages* pages, const void* q, const vo
   FC_CHECK_ARG(src_dtype == pages->dtype || src_dtype == FC_F32, "bf16 values into fp32 pages");
   FC_CHECK_ARG(rot > 0 && rot % 2 == 0 && rot <= pages->head_dim, "rot must be even, in [2, head_dim]");
   FC_CHECK_ARG(rope_len > 0, "rope_len");
-  FC_CHECK_ARG(norm >= 0.f && norm <= 3.0e38f, "norm must be finite and not negative");
+  // (norm / sqrt(0 + 1e-6) is finite, so that a head of zeros stays one)
+  FC_CHECK_ARG(norm >= 0.f && norm <= 3.0e35f, "norm must be in [0, 3e35]");
   if (M == 0) return FC_OK;
   FC_CHECK_ARG(q && k && v && tok_pos && slots && cos && sin && q_out, "null pointer");
   const RopeArgs a{page_view(pages), pages->k, pages->v, q_out, q, k, v, q_token_stride, q_head_stride,

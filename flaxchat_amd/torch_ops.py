@@ -822,8 +822,8 @@ def rope_append(q, k, v, tok_pos, slots, cos, sin, k_pages, v_pages, interleaved
     if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
             not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("rope_append: cos and sin are contiguous fp32 tensors")
-    if not 0.0 <= norm <= 3e38:
-        raise ValueError(f"rope_append: norm is finite and not negative (got {norm})")
+    if not 0.0 <= norm <= 3e35:
+        raise ValueError(f"rope_append: norm in [0, 3e35] (got {norm})")
     if M > 0x7fffffff:
         raise ValueError("rope_append: tokens below 2^31")
     _index("rope_append", "tok_pos", tok_pos, M)

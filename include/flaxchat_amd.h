@@ -478,7 +478,7 @@ int32_t fc_tree_commit(const fc_pages* pages, int32_t n_layer, int64_t k_layer_s
  * c = cos[tok_pos][i], s = sin[tok_pos][i] (both [rope_len][rot / 2]; the
  * other direction is a table of -sin, positions stretched for a long context
  * are in the tables too). Then, if norm > 0, the head is scaled by norm /
- * sqrt(mean of its squares + 1e-6). q goes to q_out [M][n_head][head_dim] in
+ * sqrt(mean of its squares + 1e-6); norm <= 3e35. q goes to q_out [M][n_head][head_dim] in
  * the pages' dtype, K and V into their slots; slots outside the pool keep
  * nothing, a slot may occur once. A token whose position is outside
  * [0, rope_len) keeps nothing, and its q is 0. q, k and v: strides in

@@ -304,3 +304,15 @@ def test_rope_append_of_many_tokens(M, H, G, hd, rot, interleaved, norm, dtype, 
         assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, first at {np.argwhere(bad)[0]}"
     vv = v[sel[0], :, sel[2], :, sel[3]]
     assert torch.equal(vv, qkv[torch.from_numpy(some).to(dev()), H + G:].to(DT[dtype]))
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 128), (64, 32), (96, 40)])
+def test_rope_append_of_zeros(hd, rot):
+    """Heads of zeros, and tokens without a position, stay 0 under the largest norm."""
+    _say(f"rope_append: zeros, heads of {hd}")
+    x = torch.zeros(5, 3, hd, device=dev())
+    x[0] = 1.0
+    cos, sin = torch.ones(9, rot // 2, device=dev()), torch.ones(9, rot // 2, device=dev())
+    k, v = torch.full((1, 1, 32, hd), 7.0, device=dev()), torch.full((1, 1, 1, hd, 32), 7.0, device=dev())
+    q = OPS.rope_append(x[:, :1], x[:, 1:2], x[:, 2:], up([-1, 0, 8, 9, 3]), up([0, 1, 2, 3, 4]), cos, sin, k, v, False, 3e35)
+    assert torch.all(q == 0) and torch.all(k[0, 0, [1, 2, 4]] == 0) and torch.all(k[0, 0, [0, 3, 5]] == 7)

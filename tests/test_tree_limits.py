@@ -1,4 +1,4 @@
-"""Trees of drafted tokens at their limits, without a GPU: windows shorter than a tree is deep."""
+"""Trees of drafted tokens at their limits, without a GPU: windows shorter than a tree is deep, norms past fp32."""
 
 import numpy as np
 import pytest
@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 
 import flaxchat_amd.torch_ops  # noqa: E402,F401
 from flaxchat_amd import _lib  # noqa: E402
-from tests.test_tree import OPS, tables_args  # noqa: E402
+from tests.test_tree import OPS, rope_args, tables_args  # noqa: E402
 from tests.tree_cases import Tree, line_of, trees  # noqa: E402
 
 
@@ -68,3 +68,19 @@ def test_tree_tables_takes_a_window():
         a = list(good)
         a[at] = value
         assert L.fc_tree_tables_window(*a) == -1, (at, value)
+
+
+def test_norms_whose_quotient_is_no_fp32_value():
+    """norm / sqrt(1e-6) is what a head of zeros is multiplied by: past fp32's largest value it would come back as NaN."""
+    assert np.float32(3e35) / np.sqrt(np.float32(1e-6)) < np.float32(np.inf)
+    for norm in (4e35, 3e38):
+        with pytest.raises(ValueError, match="norm"):
+            OPS.rope_append(*rope_args(norm=norm))
+    with pytest.raises(ValueError, match="CUDA"):
+        OPS.rope_append(*rope_args(norm=3e35))
+    L, p = _lib.lib(), 0x1000
+    pages = _lib.FcPages(k=p, v=p, k_stride=64 * 3 * 128, v_stride=64 * 3 * 128, n_pages=4, n_kv_head=3, page=64,
+                         head_dim=128, dtype=1)
+    for norm, rc in ((4e35, -1), (3e35, 0)):  # (no token: nothing is launched)
+        assert L.fc_rope_append(pages, p, p, p, 768, 128, 384, 128, 384, 128, 1, p, p, p, p, 9, 128, 0, norm, p, 6, 0,
+                                None) == rc

@@ -2080,7 +2080,7 @@ static int attention(const fc_pages* pages, const void* q, int64_t q_token_strid
                1.f / sqrtf((float)pages->head_dim), a.S_own, a.S_pre, a.pre_chunk, a.target, a.joint, (float*)work,
                (float2*)((char*)work + a.part_bytes), (int*)((char*)work + a.part_bytes + a.ml_bytes),
                q, pages->k, pages->v, y, tree ? tree->mask : nullptr, tree ? tree->tok_pos : nullptr,
-               (max_per_row + 63) / 64, a.pre_blk};
+               tree ? (max_per_row + 63) / 64 : 0, a.pre_blk};  // (of plain chunks max_per_row may be 2^31 - 1)
   const hipStream_t s = (hipStream_t)stream;
   // the matrix-core kernels load 16 bytes at a time
   const int64_t strides = q_token_stride | q_head_stride | pages->k_stride | pages->v_stride;

@@ -316,3 +316,18 @@ def test_rope_append_of_zeros(hd, rot):
     k, v = torch.full((1, 1, 32, hd), 7.0, device=dev()), torch.full((1, 1, 1, hd, 32), 7.0, device=dev())
     q = OPS.rope_append(x[:, :1], x[:, 1:2], x[:, 2:], up([-1, 0, 8, 9, 3]), up([0, 1, 2, 3, 4]), cos, sin, k, v, False, 3e35)
     assert torch.all(q == 0) and torch.all(k[0, 0, [1, 2, 4]] == 0) and torch.all(k[0, 0, [0, 3, 5]] == 7)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [128, 96])
+def test_paged_attention_of_any_max_per_row(dtype, hd):
+    """A plain chunk's max_per_row may be as large as its type: no word of bits is counted from it."""
+    _say(f"paged_attention {dtype} hd={hd}: max_per_row up to 2^31 - 1")
+    c = Tree(2, [70, 3], [5, 2], 40, 2, hd, 32, DT[dtype])
+    q = c.queries(4)
+    a = c.device(dev())
+    qt = torch.from_numpy(q).to(dev(), DT[dtype])
+    ref, tol = c.reference(q, 9)
+    for most in (2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64, 7):
+        y = OPS.paged_attention(qt, a["k"], a["v"], a["tables"], a["row_off"], a["start"], most, 9, a["pre"], 40)
+        _check(y, ref, tol, f"max_per_row {most}")

@@ -747,9 +747,15 @@ __device__ __forceinline__ RowKeys row_keys(const PagedChunk& c, int r) {
 #define CHUNK_MAX 4096
 #define CHUNK_WIDE 1000000000
 #define ROWS_SCAN 256
-template <int CB>
+// A tree's rows without a prefix, in the streaming kernel: none is cut if the longest is no longer than a share of 256
+// items, a workgroup for every CU, as a cut costs a start (32 rows at 1280 keys, 12 heads, not cut and in two: trees of 16
+// 49 and 52 us, of 32 54 and 64; 22 rows at 8000 keys, cut to c.target all the same, 190, and 199 with CHUNK_MAX). Where
+// rows are cut it is to c.target and not to 256 (32 rows of 100 to 4000 keys 81 and 86 us, 8 rows at 8000 73 and 88).
+template <int CB, bool tree>
 __device__ __forceinline__ int chunk_length(const PagedChunk& c, float total, int longest) {
-  const float share = ceilf(total * (float)c.pv.G / (float)c.target);
+  const float all = total * (float)c.pv.G;
+  float share = ceilf(all / (float)c.target);
+  if (tree && CB < 64 && c.P == 0 && longest <= CHUNK_MAX && (float)longest * 256.f <= all) share = (float)longest;
   // (unsigned: a row may have up to 2^31 - 32 keys)
   const uint32_t least = max(128u, ((uint32_t)longest + c.S_own - 1) / c.S_own);
   const uint32_t len = (max((uint32_t)fminf(share, (float)(CB >= 64 ? CHUNK_WIDE : CHUNK_MAX)), least) + 63) & ~63u;
@@ -798,7 +804,7 @@ __device__ __forceinline__ bool find_among(const PagedChunk& c, int at, Item& it
     total += (float)max(r[i].len, 0) * (float)r[i].blocks;
     longest = max(longest, r[i].len);
   }
-  const int chunk = chunk_length<CB>(c, lanes_sum(total), lanes_max<64>(longest));
+  const int chunk = chunk_length<CB, tree>(c, lanes_sum(total), lanes_max<64>(longest));
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (item_of(c, at, 64 * i, r[i], chunk, it)) return true;
@@ -835,7 +841,7 @@ __global__ __launch_bounds__(1024) void k_paged_items(PagedChunk c) {
   __syncthreads();
   total = 0.f;
   for (int i = 0; i < 16; ++i) total += s_total[i], longest = max(longest, s_longest[i]);
-  const int chunk = chunk_length<CB>(c, total, longest);
+  const int chunk = chunk_length<CB, tree>(c, total, longest);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int upto = lanes_scan(row_pieces(r[i], chunk) * r[i].blocks * c.pv.G);
@@ -1413,8 +1419,8 @@ struct WideLds {
 };
 // CB = 64: blocks of 64 columns, two waves on each of a step's two tiles, joined at
 // the end: a step is then half as long, and the next one's loads go out the sooner.
-// (32 trees of 64 nodes at 1024-1536 keys, 12 heads, 60 us and 4.6 TB/s, 67 in blocks
-// of 128; at 300 keys 25 and 29.)
+// (32 trees of 64 nodes at 1024-1536 keys, 12 heads, 60 us and 4.6 TB/s without the merge,
+// 67 in blocks of 128; at 300 keys 25 and 29.)
 template <int HD, int walk, bool tree, int CB = 128>
 __device__ __forceinline__ void wide_keys(const PagedChunk& w, WideLds<HD>& lds, int at) {
   constexpr int DS = HD / 16, DD = HD / 32;  // 16-dim slices, 32-dim output blocks
@@ -1933,12 +1939,12 @@ PagedPlan paged_plan(const fc_pages* p, int B, int T, int max_per_row, int H, in
   if (P == 0 && longest <= 1024) a.S_own = 1;
   a.target = a.own_qb ? 768 : 256;
   if (tree) {
-    // Rows of trees that alone are a workgroup for every CU are not cut up to 4096 keys, as a cut costs the merge and a
-    // start (32 rows of 1280 keys, 12 heads, cut in two or not: trees of 16 53 and 47 us, of 32 64 and 52, of 64 65 and
-    // 61; 128 rows of 50 to 2000 keys, 10 nodes of 12 heads on 4 65 and 59). Behind a prefix there is a merge all the
-    // same, and in the wide kernel long rows are cut to the mean's length (those 128 rows, 25 nodes, behind 6144 keys:
-    // 148 us, 158 uncut).
-    if (P == 0 && units >= 256 && longest <= 4096) a.S_own = 1;
+    // Without a prefix chunk_length decides, by the rows' lengths, whether any is cut. A rule here could only go by the
+    // slots for rows and the tables' width: it would save rows of one length the merge (32 rows of 64 nodes at 1280 keys,
+    // 12 heads, 60 us, 63 with it) and leave one live row of 64 at 3900 keys, or one among 31 of 100-300, to a workgroup
+    // a head (70 and 28 us; 73 and 32).
+    // Behind a prefix in the wide kernel long rows are cut to the mean's length (128 rows of 50 to 2000 keys, up to 25
+    // nodes of 12 heads on 4, behind 6144 keys: 148 us, 158 uncut).
     if (P > 0 && !a.own_qb) a.target = 512;
   }
   const int64_t cut = units * longest / (a.own_qb ? CHUNK_MAX : CHUNK_WIDE) + 1;

@@ -331,3 +331,37 @@ def test_paged_attention_of_any_max_per_row(dtype, hd):
     for most in (2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64, 7):
         y = OPS.paged_attention(qt, a["k"], a["v"], a["tables"], a["row_off"], a["start"], most, 9, a["pre"], 40)
         _check(y, ref, tol, f"max_per_row {most}")
+
+
+# ---------------------------------------------------------------- one long row among finished or short ones
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [5, 25, 64])
+@pytest.mark.parametrize("others", [0, 2])
+def test_a_long_row_among_others(dtype, n, others):
+    """A row of 3000 keys and 63 slots whose rows have ended, or hold a few keys."""
+    _say(f"tree_attention {dtype}: one row of {n} nodes at 3000 keys, 63 of {others}")
+    ctx = np.zeros(64, np.int64)
+    ctx[40], ctx[3::7] = 3000, 50 * others
+    ns = np.full(64, others)
+    ns[40] = n
+    c = Tree(4, ctx, ns, 0, 4, 128, 64, DT[dtype])
+    q = c.queries(4, tail=3)
+    got = _run(c, q, 0, most=n)
+    ref, tol = c.tree_reference(q, 0)
+    _check(got, ref, tol)
+    assert torch.all(got[int(c.off[-1]):] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 25, 40])
+@pytest.mark.parametrize("last", [1100, 20, 4200])
+def test_rows_of_one_length(dtype, n, last):
+    """As many rows as leave a workgroup for every CU, longer than those that no call cuts: whole beside a place for
+    partials, and with a last row that is shorter, or cut."""
+    _say(f"tree_attention {dtype}: 29 rows of {n} nodes at 1100 keys, one at {last}")
+    c = Tree(6, [1100] * 29 + [last], [n] * 30, 0, 9, 64, 64, DT[dtype])
+    q = c.queries(9, tail=1)
+    got = _run(c, q, 0)
+    ref, tol = c.tree_reference(q, 0)
+    _check(got, ref, tol)
+    assert torch.all(got[int(c.off[-1]):] == 0)

@@ -84,3 +84,16 @@ def test_norms_whose_quotient_is_no_fp32_value():
     for norm, rc in ((4e35, -1), (3e35, 0)):  # (no token: nothing is launched)
         assert L.fc_rope_append(pages, p, p, p, 768, 128, 384, 128, 384, 128, 1, p, p, p, p, 9, 128, 0, norm, p, 6, 0,
                                 None) == rc
+
+
+@pytest.mark.parametrize("slots,most,G", [(64, 8, 12), (64, 64, 12), (128, 25, 4), (32, 32, 12)])
+@pytest.mark.parametrize("width", [20, 33, 64])
+def test_rows_may_be_cut_whatever_the_batch_has_room_for(slots, most, G, width):
+    """How many key splits a row may have does not hang on how many rows the call has slots for: a batch whose other rows
+    have ended, or are short, cuts its long one (tables of 1280 to 4096 keys; partials of two splits at least)."""
+    L, p = _lib.lib(), 0x1000
+    pages = _lib.FcPages(k=p, v=p, k_stride=64 * G * 128, v_stride=64 * G * 128, n_pages=4, n_kv_head=G, page=64,
+                         head_dim=128, dtype=1)
+    T = slots * most
+    nb = L.fc_tree_attention_workspace_bytes(pages, slots, T, most, 12, width, 0, 0)
+    assert nb >= 2 * T * 12 * (128 + 2) * 4
